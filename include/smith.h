@@ -367,6 +367,84 @@ int smith_set_i32(void* ctx, int32_t* p, int32_t v);
 /* seeded N(mean, std) f32 stream (SplitMix64 + Box-Muller), offset even. */
 int smith_randn(void* ctx, float* out, uint64_t n, uint64_t seed, uint64_t offset, float stdv, float mean);
 
+/* ---- paged KV cache: several requests at once ----
+ * No counterpart in the reference, whose cache belongs to one request.  A
+ * layer's keys and values live in two pools of pages,
+ * [n_pages][n_kv_heads][page_size][head_dim] of kv_type, 16-byte aligned;
+ * page_size is a power of two and n_pages * page_size < 2^31.  Row b of
+ * `tables` ([n_req][max_pages] int32) names the pages of request b in the order
+ * of its keys; a key's slot is page * page_size + its place in the page.  A step
+ * of n_req <= 4096 requests, any of them with any number of rows, is one
+ * smith_paged_plan, then smith_paged_append and smith_paged_attention per layer.
+ * Any device memory of the context's device serves as a buffer (these three read
+ * nothing past its end); all three are enqueued, and can be captured once each
+ * has run with the same sizes.
+ *
+ * Lengths, slots, positions and pages live in device memory and are checked
+ * there: what does not fit is left out as stated for each call, and the next
+ * synchronising call (smith_sync, smith_copy_d2h) returns -1 with the first such
+ * finding in smith_last_error. */
+#define SMITH_KV_F32 0
+#define SMITH_KV_F16 1
+#define SMITH_KV_BF16 2
+/* Rotary positions of smith_paged_append: none; the whole-row indexing of
+ * smith_attention (element i of a row of width W pairs with i + W/2, table entry
+ * pos * (W/2) + i, q and k rows each by their own width); or head by head
+ * (element i pairs with i + head_dim/2, entry pos * (head_dim/2) + i). */
+#define SMITH_ROPE_NONE 0
+#define SMITH_ROPE_ROW 1
+#define SMITH_ROPE_HEAD 2
+/* Block tables, slots and positions of a step from its lengths.  Request b has
+ * cached[b] keys and brings added[b] rows (0: it sits the step out).  Rows are
+ * numbered request by request: row_start[b] is b's first ([n_req + 1], the last
+ * entry the number of rows), lens[b] = cached[b] + added[b]; row r gets
+ * slots[r] and positions[r], and rows behind the last one up to max_rows get -1
+ * in both.  A page that a request starts to need is taken off the end of
+ * free_pages[0 .. *free_count - 1], requests in order, and entered into tables;
+ * other entries stay as they are.  *free_left is what remains of the list.
+ * Outputs overlap no input (tables is both): the next step's cached and
+ * free_count are this one's lens and free_left in buffers of their own.  A
+ * length that is negative or longer than max_pages pages, more than max_rows
+ * rows or too few free pages fail the step: no page is taken, row_start is all 0,
+ * every slot -1 and lens = cached.  A page outside the pool fails the rows in it
+ * (slot -1). */
+int smith_paged_plan(void* ctx, const int32_t* cached, const int32_t* added, uint32_t n_req,
+                     const int32_t* free_pages, const int32_t* free_count, uint32_t n_pages, uint32_t page_size,
+                     uint32_t max_pages, uint32_t max_rows, int32_t* tables, int32_t* row_start, int32_t* lens,
+                     int32_t* slots, int32_t* positions, int32_t* free_left);
+/* Rows of [q | k | v] (row stride ld floats) into the cache: k after its rotary
+ * position, and v, rounded to the nearest value of kv_type (ties to even), into
+ * the row's slot of kpages and vpages; q after its rotary position into q_out
+ * (row stride ld_q; qkv itself with ld_q = ld rotates in place, else the two do
+ * not overlap; may be NULL without rotary positions, where it would be a copy).
+ * Rows of slot -1 are padding: nothing of them is read or written.  The other
+ * slots of a call are distinct.  rope_len: entries of each table.  A slot outside
+ * the pool, or a position outside the tables, fails its row. */
+int smith_paged_append(void* ctx, uint32_t kv_type, const float* qkv, uint32_t ld, uint32_t rows,
+                       const int32_t* slots, const int32_t* positions, uint32_t n_heads, uint32_t n_kv_heads,
+                       uint32_t head_dim, uint32_t rope, const float* rope_cos, const float* rope_sin,
+                       uint32_t rope_len, void* kpages, void* vpages, uint32_t n_pages, uint32_t page_size,
+                       float* q_out, uint32_t ld_q);
+/* Softmax attention of the step's rows over the cached keys and values, causal:
+ * row i of request b's n = row_start[b+1] - row_start[b] sits at position
+ * lens[b] - n + i and sees the keys up to and with its own.  row_start NULL: row
+ * b is request b's one new row (max_rows = n_req); with lens[b] = 0 it has no key
+ * and its output is 0.  Head h reads KV head h / (n_heads / n_kv_heads); scale 0
+ * is 1 / sqrt(head_dim).  q and out are f32 with row strides ld_q and ld_out and
+ * room for max_rows rows; they do not overlap.  Rows of out behind the last row
+ * stay as they are.  f32 accuracy for every kv_type.  Keys that a row does not
+ * see may hold anything; among those that it sees an entry that is not finite
+ * makes that row's head not finite.  head_dim <= 128 and % 8 == 0.  A row_start
+ * past max_rows fails the call; starts that do not ascend, and a len below the
+ * request's rows or past max_pages pages, fail the request (nothing of it is
+ * written); a page outside the pool leaves its
+ * request's rows undefined. */
+int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
+                          const int32_t* row_start, const int32_t* lens, const int32_t* tables, uint32_t n_req,
+                          uint32_t max_pages, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,
+                          const void* kpages, const void* vpages, uint32_t n_pages, uint32_t page_size, float* out,
+                          uint32_t ld_out);
+
 /* ---- HIP graphs: capture the context stream, replay it ----
  * Ops enqueued between begin and end are recorded, not run; their scratch
  * must already be allocated (run the same ops once before capturing).

@@ -3,6 +3,7 @@
   smith_amd/lib/smith_kernels.hsaco   hipcc --offload-device-only --offload-arch=gfx950
   smith_amd/lib/smith_llama.hsaco     (the GGUF decode-path kernels, same flags)
   smith_amd/lib/smith_gemm.hsaco      (the prefill MFMA GEMM, same flags)
+  smith_amd/lib/smith_paged.hsaco     (the paged KV cache's kernels, same flags)
   smith_amd/lib/libsmith.so           hipcc -x hip: host code against libamdhip64 (+ static device scratch)
   smith_amd/lib/smith_bench.hsaco     bench-only floor kernels (bench_floor.hip)
   smith_amd/lib/libsmith_bench.so     bench-only host helper that times them (bench_floor_host.cpp)
@@ -20,6 +21,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HSACO = os.path.join(LIBDIR, "smith_kernels.hsaco")
 HSACO_LLAMA = os.path.join(LIBDIR, "smith_llama.hsaco")
 HSACO_GEMM = os.path.join(LIBDIR, "smith_gemm.hsaco")
+HSACO_PAGED = os.path.join(LIBDIR, "smith_paged.hsaco")
 LIBSMITH = os.path.join(LIBDIR, "libsmith.so")
 # bench-only: the floor kernels bench.py times beside the product's steps
 HSACO_BENCH = os.path.join(LIBDIR, "smith_bench.hsaco")
@@ -42,7 +44,8 @@ def _kernel_cmds():
     return [[os.path.join(ROCM, "bin", "hipcc"), *HIP_FLAGS, "--offload-device-only", "--no-gpu-bundle-output",
              "-c", os.path.join(CSRC, src), "-o", dst]
             for src, dst in (("smith_kernels.hip", HSACO), ("llama_kernels.hip", HSACO_LLAMA),
-                             ("gemm_kernels.hip", HSACO_GEMM), ("bench_floor.hip", HSACO_BENCH))]
+                             ("gemm_kernels.hip", HSACO_GEMM), ("paged_kernels.hip", HSACO_PAGED),
+                             ("bench_floor.hip", HSACO_BENCH))]
 
 
 def _bridge_cmd():

@@ -18,6 +18,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <atomic>
+#include <cmath>
 #include <condition_variable>
 #include <cstring>
 #include <map>
@@ -30,6 +31,7 @@
 
 #include "../../include/smith.h"
 #include "gguf_tiles.h"
+#include "paged.h"
 
 namespace {
 
@@ -87,6 +89,10 @@ struct Ctx {
   // call (pos_err_host) and passed to kernels as pos_err_dev
   uint32_t* pos_err_host = nullptr;
   uint32_t* pos_err_dev = nullptr;
+  // what the paged cache's kernels found wrong: one {code, argument} word
+  // further on in the same memory
+  uint64_t* paged_err_dev() const { return (uint64_t*)(pos_err_dev + PAGED_ERR_WORD); }
+  static constexpr uint32_t PAGED_ERR_WORD = 16;
   // pinned staging of large device -> host copies (large_d2h)
   std::mutex stage_mu;
   uint8_t* stage = nullptr;
@@ -258,11 +264,34 @@ int ensure(Ctx* c, void** p, size_t* have, size_t need) {
   return 0;
 }
 
+// The paged cache's finding since the last check, reported once.
+int check_paged_err(Ctx* c) {
+  volatile uint64_t* e = (volatile uint64_t*)(c->pos_err_host + Ctx::PAGED_ERR_WORD);
+  const uint64_t v = *e;
+  if (v == 0) return 0;
+  *e = 0;
+  const uint32_t code = (uint32_t)v, arg = (uint32_t)(v >> 32);
+  static const char* const what[] = {
+      "?",
+      "smith_paged_plan: request %u: a length is negative or longer than its block table; the step has no rows",
+      "smith_paged_plan: the requests bring more than max_rows = %u rows; the step has no rows",
+      "smith_paged_plan: the requests need more than the %u free pages; the step has no rows",
+      "smith_paged_plan: request %u: a page outside the pool",
+      "smith_paged_append: row %u: its slot lies outside the pool",
+      "smith_paged_append: row %u: its position lies outside the rotary tables",
+      "smith_paged_attention: row_start ends at %d, outside 0 .. max_rows",
+      "smith_paged_attention: request %u: its length does not hold its rows, or is longer than its block table, or row_start does not ascend",
+      "smith_paged_attention: request %u: a page outside the pool",
+  };
+  return fail(c, what[code < sizeof what / sizeof what[0] ? code : 0], arg);
+}
+
 // Called after the stream has drained: reports (once) a position bound
 // failure that a kernel recorded on the device since the last check.
 int check_pos_err(Ctx* c) {
   volatile uint32_t* e = c->pos_err_host;
-  if (!e || e[0] == 0) return 0;
+  if (!e) return 0;
+  if (e[0] == 0) return check_paged_err(c);
   static const char* who[] = {"?", "smith_kv_append", "smith_attention", "smith_attention (prefill)",
                               "smith_attention_parts"};
   const uint32_t code = e[0], p0 = e[1], S = e[2];
@@ -2248,6 +2277,158 @@ int smith_argmax_embed(void* ctx, const float* logits, uint32_t N, const float* 
   void* args[] = {&logits, &N, &E, &dim, &x, &tokens, &count, &pos, &act_out, &gamma_out,
                   &rope_cos, &rope_sin, &rope_len, &wq, &wk, &rope_row};
   return launch(c, "smith_argmax_embed", dim3(1), dim3(1024), args);
+}
+
+// ---------------- paged KV cache ----------------
+static const char* kv_name(uint32_t t) {
+  return t == SMITH_KV_F32 ? "f32" : t == SMITH_KV_F16 ? "f16" : t == SMITH_KV_BF16 ? "bf16" : nullptr;
+}
+
+// log2 of a page size, and the bounds of the pool
+static int pool_shift(Ctx* c, const char* fn, uint32_t n_pages, uint32_t page_size, uint32_t* shift) {
+  if (!page_size || (page_size & (page_size - 1))) return fail(c, "%s: page size %u is no power of two", fn, page_size);
+  if (!n_pages || (uint64_t)n_pages * page_size > 0x7FFFFFFFull)
+    return fail(c, "%s: a pool of %u pages of %u keys (at least one page, less than 2^31 keys)", fn, n_pages, page_size);
+  *shift = (uint32_t)__builtin_ctz(page_size);
+  return 0;
+}
+
+static bool overlap(const void* a, uint64_t an, const void* b, uint64_t bn) {
+  return (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
+
+// what append and attention ask of a cache and its heads
+static int check_paged(Ctx* c, const char* fn, uint32_t kv_type, uint32_t n_heads, uint32_t n_kv_heads,
+                       uint32_t head_dim, const void* kpages, const void* vpages, uint32_t n_pages,
+                       uint32_t page_size, uint32_t* shift) {
+  if (!kv_name(kv_type)) return fail(c, "%s: unknown page type %u", fn, kv_type);
+  if (!n_heads || !n_kv_heads || n_heads % n_kv_heads)
+    return fail(c, "%s: %u heads not a multiple of %u kv heads", fn, n_heads, n_kv_heads);
+  if (!head_dim || head_dim > 128 || head_dim % 8)
+    return fail(c, "%s: head_dim %u unsupported (<= 128, %% 8)", fn, head_dim);
+  if (n_heads > 65535) return fail(c, "%s: %u heads", fn, n_heads);
+  if (!kpages || !vpages || ((uintptr_t)kpages | (uintptr_t)vpages) % 16)
+    return fail(c, "%s: the page pools must be 16-byte aligned device memory", fn);
+  return pool_shift(c, fn, n_pages, page_size, shift);
+}
+
+int smith_paged_plan(void* ctx, const int32_t* cached, const int32_t* added, uint32_t n_req,
+                     const int32_t* free_pages, const int32_t* free_count, uint32_t n_pages, uint32_t page_size,
+                     uint32_t max_pages, uint32_t max_rows, int32_t* tables, int32_t* row_start, int32_t* lens,
+                     int32_t* slots, int32_t* positions, int32_t* free_left) {
+  Ctx* c = (Ctx*)ctx;
+  if (!c) return -1;
+  static const char fn[] = "smith_paged_plan";
+  if (!n_req || n_req > PAGED_MAX_REQ) return fail(c, "%s: %u requests (1 .. %u)", fn, n_req, PAGED_MAX_REQ);
+  if (!cached || !added || !free_pages || !free_count || !tables || !row_start || !lens || !free_left ||
+      (max_rows && (!slots || !positions)))
+    return fail(c, "%s: null buffer", fn);
+  if (!max_pages || max_rows > 0x7FFFFFFFu) return fail(c, "%s: max_pages %u, max_rows %u", fn, max_pages, max_rows);
+  uint32_t shift;
+  if (pool_shift(c, fn, n_pages, page_size, &shift)) return -1;
+  if (((uint64_t)max_pages << shift) > 0x7FFFFFFFull)
+    return fail(c, "%s: block tables of %u pages of %u keys (less than 2^31 keys)", fn, max_pages, page_size);
+  {
+    // every workgroup reads all the lengths: a step in place would change them under it
+    struct Range {
+      const void* p;
+      uint64_t n;
+    };
+    const uint64_t nb = 4ull * n_req, rb = 4ull * max_rows;
+    const Range in[] = {{cached, nb}, {added, nb}, {free_pages, 4}, {free_count, 4}};
+    const Range io[] = {{tables, nb * max_pages}, {row_start, nb + 4}, {lens, nb}, {slots, rb}, {positions, rb}, {free_left, 4}};
+    for (size_t i = 0; i < sizeof io / sizeof io[0]; i++) {
+      for (const Range& r : in)
+        if (overlap(io[i].p, io[i].n, r.p, r.n)) return fail(c, "%s: an output overlaps an input", fn);
+      for (size_t k = 0; k < i; k++)
+        if (overlap(io[i].p, io[i].n, io[k].p, io[k].n)) return fail(c, "%s: two outputs overlap", fn);
+    }
+  }
+  if (set_device(c)) return -1;
+  uint64_t* perr = c->paged_err_dev();
+  void* args[] = {&cached, &added, &n_req, &free_pages, &free_count, &n_pages, &shift, &max_pages, &max_rows,
+                  &tables, &row_start, &lens, &slots, &positions, &free_left, &perr};
+  const uint32_t groups = std::max<uint32_t>(1, (max_rows + 255) / 256);  // PLAN_THREADS rows each
+  return launch(c, "smith_paged_plan", dim3(groups), dim3(256), args);
+}
+
+int smith_paged_append(void* ctx, uint32_t kv_type, const float* qkv, uint32_t ld, uint32_t rows,
+                       const int32_t* slots, const int32_t* positions, uint32_t n_heads, uint32_t n_kv_heads,
+                       uint32_t head_dim, uint32_t rope, const float* rope_cos, const float* rope_sin,
+                       uint32_t rope_len, void* kpages, void* vpages, uint32_t n_pages, uint32_t page_size,
+                       float* q_out, uint32_t ld_q) {
+  Ctx* c = (Ctx*)ctx;
+  if (!c) return -1;
+  static const char fn[] = "smith_paged_append";
+  uint32_t shift;
+  if (check_paged(c, fn, kv_type, n_heads, n_kv_heads, head_dim, kpages, vpages, n_pages, page_size, &shift)) return -1;
+  const uint64_t Wq = (uint64_t)n_heads * head_dim, Wk = (uint64_t)n_kv_heads * head_dim;
+  if (rope > SMITH_ROPE_HEAD) return fail(c, "%s: unknown rotary indexing %u", fn, rope);
+  if (rope && (!rope_cos || !rope_sin || !q_out)) return fail(c, "%s: rotary positions need both tables and q_out", fn);
+  if (ld < Wq + 2 * Wk || (q_out && ld_q < Wq))
+    return fail(c, "%s: row strides %u and %u for rows of %llu and %llu floats", fn, ld, ld_q,
+                (unsigned long long)(Wq + 2 * Wk), (unsigned long long)Wq);
+  if (rows > 0x7FFFFFFFu) return fail(c, "%s: %u rows", fn, rows);
+  if (!rows) return 0;
+  if (!qkv || !slots || !positions) return fail(c, "%s: null buffer", fn);
+  if (q_out && !(q_out == qkv && ld_q == ld) &&
+      overlap(q_out, 4 * ((uint64_t)(rows - 1) * ld_q + Wq), qkv, 4 * ((uint64_t)(rows - 1) * ld + Wq + 2 * Wk)))
+    return fail(c, "%s: q_out overlaps qkv and is not it", fn);
+  if (set_device(c)) return -1;
+  uint32_t n_slots = n_pages << shift;
+  uint64_t* perr = c->paged_err_dev();
+  // 16-byte accesses where every row and table starts on 16 bytes
+  const bool vec = (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)rope_cos | (uintptr_t)rope_sin) % 16) == 0 &&
+                   ld % 4 == 0 && ld_q % 4 == 0;
+  char name[48];
+  snprintf(name, sizeof name, "smith_paged_append_%s%s", kv_name(kv_type), vec ? "" : "_u");
+  const uint32_t items = (uint32_t)((Wq + 2 * Wk) / 8);
+  // rows along the grid's second axis, which ends at 65535
+  for (uint32_t r0 = 0; r0 < rows; r0 += 65535) {
+    const uint32_t n = std::min<uint32_t>(65535, rows - r0);
+    const float* x = qkv + (size_t)r0 * ld;
+    const int32_t *sl = slots + r0, *po = positions + r0;
+    float* qo = q_out ? q_out + (size_t)r0 * ld_q : nullptr;
+    void* args[] = {&x, &ld, &sl, &po, &n_heads, &n_kv_heads, &head_dim, &rope, &rope_cos, &rope_sin,
+                    &rope_len, &kpages, &vpages, &n_slots, &shift, &qo, &ld_q, &perr};
+    if (launch(c, name, dim3((items + 255) / 256, n), dim3(256), args)) return -1;
+  }
+  return 0;
+}
+
+int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
+                          const int32_t* row_start, const int32_t* lens, const int32_t* tables, uint32_t n_req,
+                          uint32_t max_pages, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,
+                          const void* kpages, const void* vpages, uint32_t n_pages, uint32_t page_size, float* out,
+                          uint32_t ld_out) {
+  Ctx* c = (Ctx*)ctx;
+  if (!c) return -1;
+  static const char fn[] = "smith_paged_attention";
+  uint32_t shift;
+  if (check_paged(c, fn, kv_type, n_heads, n_kv_heads, head_dim, kpages, vpages, n_pages, page_size, &shift)) return -1;
+  const uint64_t Wq = (uint64_t)n_heads * head_dim;
+  if (!n_req || n_req > PAGED_MAX_REQ) return fail(c, "%s: %u requests (1 .. %u)", fn, n_req, PAGED_MAX_REQ);
+  if (!max_pages || ((uint64_t)max_pages << shift) > 0x7FFFFFFFull)
+    return fail(c, "%s: block tables of %u pages of %u keys (at least one page, less than 2^31 keys)", fn, max_pages,
+                page_size);
+  if (!row_start && max_rows != n_req)
+    return fail(c, "%s: max_rows %u for one row of each of %u requests", fn, max_rows, n_req);
+  if (ld_q < Wq || ld_out < Wq)
+    return fail(c, "%s: row strides %u and %u for rows of %llu floats", fn, ld_q, ld_out, (unsigned long long)Wq);
+  if (max_rows > 0x7FFFFFFFu) return fail(c, "%s: max_rows %u", fn, max_rows);
+  if (!std::isfinite(scale)) return fail(c, "%s: scale %g", fn, (double)scale);
+  if (!max_rows) return 0;
+  if (!q || !lens || !tables || !out) return fail(c, "%s: null buffer", fn);
+  if (overlap(out, 4 * ((uint64_t)(max_rows - 1) * ld_out + Wq), q, 4 * ((uint64_t)(max_rows - 1) * ld_q + Wq)))
+    return fail(c, "%s: out overlaps q", fn);
+  if (set_device(c)) return -1;
+  if (scale == 0.f) scale = 1.0f / sqrtf((float)head_dim);
+  uint64_t* perr = c->paged_err_dev();
+  char name[48];
+  snprintf(name, sizeof name, "smith_paged_attention_%s", kv_name(kv_type));
+  void* args[] = {&q, &ld_q, &max_rows, &row_start, &lens, &tables, &n_req, &max_pages, &n_heads, &n_kv_heads,
+                  &head_dim, &scale, &kpages, &vpages, &n_pages, &shift, &out, &ld_out, &perr};
+  return launch(c, name, dim3(max_rows, n_heads), dim3(256), args);
 }
 
 int smith_set_i32(void* ctx, int32_t* p, int32_t v) {

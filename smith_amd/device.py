@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libsmith.so")
 CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_kernels.hsaco")
 LLAMA_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_llama.hsaco")
 GEMM_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_gemm.hsaco")
+PAGED_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_paged.hsaco")
 
 SHARED = 0
 PRIVATE = 1
@@ -117,6 +118,11 @@ SYMBOLS = {
     "smith_argmax_embed": (_INT, [_P, _P, _U32, _P, _U32, _P, _P, _P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _P]),
     "smith_set_i32": (_INT, [_P, _P, ctypes.c_int32]),
     "smith_randn": (_INT, [_P, _P, _U64, _U64, _U64, ctypes.c_float, ctypes.c_float]),
+    "smith_paged_plan": (_INT, [_P, _P, _P, _U32, _P, _P, _U32, _U32, _U32, _U32, _P, _P, _P, _P, _P, _P]),
+    "smith_paged_append": (_INT, [_P, _U32, _P, _U32, _U32, _P, _P, _U32, _U32, _U32, _U32, _P, _P, _U32, _P, _P,
+                                  _U32, _U32, _P, _U32]),
+    "smith_paged_attention": (_INT, [_P, _U32, _P, _U32, _U32, _P, _P, _P, _U32, _U32, _U32, _U32, _U32,
+                                     ctypes.c_float, _P, _P, _U32, _U32, _P, _U32]),
     "smith_graph_begin": (_INT, [_P]),
     "smith_graph_end": (_P, [_P]),
     "smith_graph_launch": (_INT, [_P, _P]),
@@ -187,7 +193,7 @@ def shader_lib():
             raise RuntimeError("smith: failed to load code object at %s: %s"
                                % (CODE_OBJECT_PATH, lib.smith_last_error(c).decode()))
         _library = lp
-        for path in (LLAMA_CODE_OBJECT_PATH, GEMM_CODE_OBJECT_PATH):
+        for path in (LLAMA_CODE_OBJECT_PATH, GEMM_CODE_OBJECT_PATH, PAGED_CODE_OBJECT_PATH):
             if not lib.smith_load_library(c, path.encode()):
                 raise RuntimeError("smith: failed to load code object at %s: %s"
                                    % (path, lib.smith_last_error(c).decode()))

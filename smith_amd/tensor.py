@@ -10,7 +10,8 @@ import numpy as np
 
 from . import device, prng
 
-_DTYPES = {"f32": np.float32, "i32": np.int32, "u8": np.uint8}
+# bf16: the upper halves of f32 words
+_DTYPES = {"f32": np.float32, "i32": np.int32, "u8": np.uint8, "f16": np.float16, "bf16": np.uint16}
 
 
 class Tensor:
