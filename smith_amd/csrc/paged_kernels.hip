@@ -281,113 +281,735 @@ DEF_APPEND(smith_paged_append_bf16_u, KvBf16, false)
 
 // ---------------------------------------------------------------------------
 // Attention over the pages: row i of request b's n rows is position p = len -
-// n + i and sees its keys 0 .. p; head h reads KV head h / (nH / nKV):
+// n + i and sees its keys 0 .. p; head h reads KV head h / G, G = nH / nKV:
 //   s_t = scale q.k_t,  out = sum_t e^(s_t - m) v_t / sum_t e^(s_t - m).
-// A row without keys gives zeros.  One workgroup to a row and head, 256 keys
-// a step with a running maximum and sum.
+// A row without keys gives zeros.
+//
+// The (row, head) pairs that read one KV head are the columns of a product:
+// S^T = K Q^T and O^T = V^T P^T on the matrix cores, 16 columns to a tile and
+// NT tiles to a workgroup (its block).  Its four waves take the block's keys in
+// turn, TK at a time, straight from the pages into the operands' registers, and
+// keep their own running maximum m, sum l and O^T; at the end they are joined
+// through LDS.  In this form nothing moves between lanes: a lane's four (or
+// eight) scores of S^T are one column's, so they become the P operand where they
+// are, and m, l and the rescaling of O^T are the lane's own.
+//   MFMA 16x16: lane (n = lane % 16, g = lane / 16) holds row n of A and column n
+//   of B at the k's of group g, and rows 4g .. 4g+3 of column n of D.
+//   K: A rows are keys, lane n its key's dims.  V: lane n holds dims n*DPL ..
+//   +DPL-1 of the keys 4g .. 4g+3 (of each 16), row n of the d-th A operand being
+//   dim n*DPL + d; so D's row 4g+i is dim (4g+i)*DPL + d.
+//
+// f16 and bf16 pages are exact in the matrix cores' operands; q and P are split
+// into parts of the pages' type that add up to 22 (two f16) or 24 (three bf16)
+// bits, the products are exact and summed in f32.  q is brought to [2^14, 2^15)
+// by a power of two first and P to at most 2^14 (P_EXP + the slack of the lazy
+// maximum), so that the small parts stay clear of f16's subnormals.  f32 pages
+// go through the f32 matrix cores.
+//
+// Work is cut on the device, where the lengths are: an item is (request, block
+// of columns, KV head, split of the block's keys).  With W = sum over blocks of
+// their request's length, a request of more than 1.5 C keys, C = max(SPLIT_MIN,
+// W / target), has its keys cut into about len / C splits, so that target items
+// or so of about C keys each fill the chip whatever the lengths are.  Every
+// workgroup forms the prefix sums of the items by itself.  The last of a block's
+// splits to finish (agent-scope counter) joins their partials in split order:
+// the same sums whichever finishes last.
 // ---------------------------------------------------------------------------
-template <class KV>
-__device__ __forceinline__ void attention_body(const float* __restrict__ q, uint32_t ld_q, uint32_t max_rows,
-                                               const int32_t* __restrict__ row_start, const int32_t* __restrict__ lens,
-                                               const int32_t* __restrict__ tables, uint32_t n_req, uint32_t max_pages,
-                                               uint32_t nH, uint32_t nKV, uint32_t hd, float scale,
-                                               const typename KV::T* __restrict__ kpages,
-                                               const typename KV::T* __restrict__ vpages, uint32_t n_pages,
-                                               uint32_t shift, float* __restrict__ out, uint32_t ld_out,
-                                               uint64_t* __restrict__ err) {
-  __shared__ float s_q[128], s_p[256], s_red[8], s_o[2][128];
-  __shared__ uint32_t s_slot[256];
-  const uint32_t r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const uint32_t P = 1u << shift, kvh = h / (nH / nKV);
-  uint32_t b = r, i = 0, n = 1;
-  if (row_start) {
-    const int32_t total = row_start[n_req];
-    if (total < 0 || (uint32_t)total > max_rows) {
-      if (r == 0 && h == 0 && tid == 0) paged_err(err, PAGED_ERR_ATT_ROWS, (uint32_t)total);
-      return;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+#define P_EXP 6.0f   // P = 2^(score - m + P_EXP)
+#define M_SLACK 8.0f // m follows a new maximum only when it is this far (log2) above
+
+// the parts of eight f32 values in the pages' type, and the product of parts
+struct MmF16 {
+  typedef _Float16 T;
+  static constexpr int TERMS = 2;
+  static constexpr uint32_t EXPONENT = 0x7C00u;
+  static __device__ __forceinline__ void split(const float (&x)[8], u32x4 (&t)[TERMS]) {
+    f16x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      hi[e] = (_Float16)x[e];
+      lo[e] = (_Float16)(x[e] - (float)hi[e]);
     }
-    if (r >= (uint32_t)total) return;
-    uint32_t lo = 0, hi = n_req;
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) >> 1;
-      if ((uint32_t)row_start[mid] <= r) lo = mid;
-      else hi = mid;
-    }
-    b = lo;
-    const int32_t r0 = row_start[b], r1 = row_start[b + 1];
-    if (r0 < 0 || (uint32_t)r0 > r || (uint32_t)r1 <= r || r1 > total) {  // starts that do not ascend
-      if (h == 0 && tid == 0) paged_err(err, PAGED_ERR_ATT_LENGTH, b);
-      return;
-    }
-    i = r - (uint32_t)r0;
-    n = (uint32_t)(r1 - r0);
+    t[0] = __builtin_bit_cast(u32x4, hi);
+    t[1] = __builtin_bit_cast(u32x4, lo);
   }
-  const int32_t len = lens[b];
-  if (len < 0 || (row_start && (uint32_t)len < n) || (uint64_t)len > ((uint64_t)max_pages << shift)) {
-    if (i == 0 && h == 0 && tid == 0) paged_err(err, PAGED_ERR_ATT_LENGTH, b);
-    return;
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
-  const uint32_t keys = row_start ? (uint32_t)len - n + i + 1 : (uint32_t)len;
-  if (tid < hd) s_q[tid] = q[(size_t)r * ld_q + h * hd + tid] * scale;
-  float m = -__builtin_inff(), l = 0.f, o = 0.f;
-  const uint32_t d = tid & 127, part = tid >> 7;
-  __syncthreads();
-  for (uint32_t t0 = 0; t0 < keys; t0 += 256) {
-    const uint32_t t = t0 + tid, nt = keys - t0 < 256 ? keys - t0 : 256;
-    float s = -__builtin_inff();
-    if (t < keys) {
-      uint32_t page = (uint32_t)tables[(size_t)b * max_pages + (t >> shift)];
-      if (page >= n_pages) {
-        paged_err(err, PAGED_ERR_ATT_PAGE, b);
-        page = 0;
+};
+struct MmBf16 {
+  typedef __bf16 T;
+  static constexpr int TERMS = 3;
+  static constexpr uint32_t EXPONENT = 0x7F80u;
+  static __device__ __forceinline__ void split(const float (&x)[8], u32x4 (&t)[TERMS]) {
+    bf16x8 a, b, c;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      a[e] = (__bf16)x[e];
+      const float r = x[e] - (float)a[e];
+      b[e] = (__bf16)r;
+      c[e] = (__bf16)(r - (float)b[e]);
+    }
+    t[0] = __builtin_bit_cast(u32x4, a);
+    t[1] = __builtin_bit_cast(u32x4, b);
+    t[2] = __builtin_bit_cast(u32x4, c);
+  }
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+  }
+};
+
+// One wave's tile of 32 keys of f16 or bf16: K and V operands in registers.
+template <class MM, int DPL>
+struct Tile16 {
+  typedef typename MM::T T;
+  static constexpr int NJ = 2, KS = DPL / 2, TERMS = MM::TERMS, QREG = KS * TERMS;
+  u32x4 K[NJ][KS];
+  uint32_t V[8][DPL / 2];  // a key's dims of this lane
+  u32x4 D[DPL];            // a dim's keys
+  // Q: parts of the lane's column, dims s*32 + 8g .. +7
+  static __device__ __forceinline__ void load_q(const float* q, bool there, uint32_t g, uint32_t hd, float sign, int& e2,
+                                                u32x4 (&Q)[QREG]) {
+    float x[KS][8];
+    float big = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        x[s][e] = there && s * 32 + 8 * g < hd ? q[s * 32 + 8 * g + e] * sign : 0.f;
+        big = fmaxf(big, fabsf(x[s][e]));
       }
-      s_slot[tid] = (page << shift) + (t & (P - 1));
-      const typename KV::T* k = kpages + (((size_t)page * nKV + kvh) * P + (t & (P - 1))) * hd;
-      s = 0.f;
-      for (uint32_t e = 0; e < hd; e++) s = __builtin_fmaf(s_q[e], KV::up(k[e]), s);
+    big = fmaxf(big, __shfl_xor(big, 16));
+    big = fmaxf(big, __shfl_xor(big, 32));
+    // largest element to [2^14, 2^15); what is not finite stays as it is
+    int ex;
+    (void)frexpf(big, &ex);
+    e2 = big > 0.f && big < __builtin_inff() ? 15 - ex : 0;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[s][e] = ldexpf(x[s][e], e2);
+      u32x4 t[TERMS];
+      MM::split(x[s], t);
+#pragma unroll
+      for (int k = 0; k < TERMS; k++) Q[s * TERMS + k] = t[k];
     }
-    float x = s;
-    for (int k = 32; k >= 1; k >>= 1) {
-      const float y = __shfl_xor(x, k);
-      x = y > x ? y : x;
-    }
-    if (lane == 0) s_red[wave] = x;
-    __syncthreads();
-    float mn = m;
-    for (int w = 0; w < 4; w++) mn = s_red[w] > mn ? s_red[w] : mn;
-    const float base = mn == -__builtin_inff() ? 0.f : mn;
-    const float alpha = __expf(m - base), p = t < keys ? __expf(s - base) : 0.f;
-    s_p[tid] = p;
-    float y = p;
-    for (int k = 32; k >= 1; k >>= 1) y += __shfl_xor(y, k);
-    if (lane == 0) s_red[4 + wave] = y;
-    __syncthreads();
-    l = l * alpha + (s_red[4] + s_red[5] + s_red[6] + s_red[7]);
-    o *= alpha;
-    m = mn;
-    if (d < hd)
-      for (uint32_t k = part; k < nt; k += 2) {
-        const uint32_t sl = s_slot[k];
-        const size_t a = (((size_t)(sl >> shift) * nKV + kvh) * P + (sl & (P - 1))) * hd + d;
-        o = __builtin_fmaf(s_p[k], KV::up(vpages[a]), o);
-      }
-    __syncthreads();
   }
-  s_o[part][d] = o;
-  __syncthreads();
-  if (tid < hd) out[(size_t)r * ld_out + h * hd + tid] = keys ? (s_o[0][tid] + s_o[1][tid]) / l : 0.f;
+  __device__ __forceinline__ void load_k(int j, const T* key, uint32_t g, uint32_t hd) {
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      K[j][s] = (u32x4){0u, 0u, 0u, 0u};
+      if (s * 32 + 8 * g < hd) K[j][s] = *(const u32x4*)(key + s * 32 + 8 * g);
+    }
+  }
+  // key 4g + i of the j-th 16
+  __device__ __forceinline__ void load_v(int j, int i, const T* key, uint32_t n, uint32_t hd) {
+    uint32_t(&r)[DPL / 2] = V[4 * j + i];
+#pragma unroll
+    for (int k = 0; k < DPL / 2; k++) r[k] = 0u;
+    if (n * DPL < hd) {
+      if constexpr (DPL == 8) {
+        const u32x4 v = *(const u32x4*)(key + 8 * n);
+#pragma unroll
+        for (int k = 0; k < 4; k++) r[k] = v[k];
+      } else {
+        const u32x2 v = *(const u32x2*)(key + 4 * n);
+        r[0] = v[0];
+        r[1] = v[1];
+      }
+    }
+  }
+  __device__ __forceinline__ void zero_v(int j, int i) {
+#pragma unroll
+    for (int k = 0; k < DPL / 2; k++) V[4 * j + i][k] = 0u;
+  }
+  // V's rows of dims into rows of keys: word k of dim d is keys 2k, 2k+1
+  __device__ __forceinline__ void turn() {
+#pragma unroll
+    for (int d = 0; d < DPL; d++)
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        D[d][k] = __builtin_amdgcn_perm(V[2 * k + 1][d / 2], V[2 * k][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
+  }
+  __device__ __forceinline__ bool all_finite() const {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int d = 0; d < DPL; d++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const uint32_t x = D[d][k];
+        bad |= (uint32_t)((x & MM::EXPONENT) == MM::EXPONENT) |
+               (uint32_t)((x & (MM::EXPONENT << 16)) == (MM::EXPONENT << 16));
+      }
+    return !bad;
+  }
+  template <class QF>
+  __device__ __forceinline__ void scores(QF q, f32x4 (&S)[NJ]) const {
+#pragma unroll
+    for (int j = 0; j < NJ; j++) S[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int k = 0; k < TERMS; k++) {
+        const u32x4 x = q(s * TERMS + k);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) S[j] = MM::mfma(K[j][s], x, S[j]);
+      }
+  }
+  static __device__ __forceinline__ void weights(const f32x4 (&S)[NJ], u32x4 (&t)[TERMS]) {
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) p[e] = S[e / 4][e % 4];
+    MM::split(p, t);
+  }
+  __device__ __forceinline__ void add_pv(const f32x4 (&S)[NJ], f32x4 (&O)[DPL]) const {
+    u32x4 t[TERMS];
+    weights(S, t);
+#pragma unroll
+    for (int d = 0; d < DPL; d++)
+#pragma unroll
+      for (int k = 0; k < TERMS; k++) O[d] = MM::mfma(D[d], t[k], O[d]);
+  }
+  // only the values that seen(j, i) says, and only into the columns of `mine`
+  template <class SEEN>
+  __device__ __forceinline__ void add_pv_seen(const f32x4 (&S)[NJ], f32x4 (&O)[DPL], SEEN seen, bool mine) const {
+    u32x4 t[TERMS], mask;
+    weights(S, t);
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      mask[k] = (seen(k / 2, 2 * (k % 2)) ? 0x0000FFFFu : 0u) | (seen(k / 2, 2 * (k % 2) + 1) ? 0xFFFF0000u : 0u);
+#pragma unroll
+    for (int d = 0; d < DPL; d++) {
+      f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < TERMS; k++) o = MM::mfma(D[d] & mask, t[k], o);
+      if (mine) O[d] += o;
+    }
+  }
+};
+
+// One wave's tile of 16 keys of f32.
+template <int DPL>
+struct Tile32 {
+  typedef float T;
+  static constexpr int NJ = 1, KS = DPL, QREG = KS;
+  f32x4 K[KS];  // dims s*16 + 4g .. +3
+  float V[4][DPL];
+  static __device__ __forceinline__ void load_q(const float* q, bool there, uint32_t g, uint32_t hd, float sign, int& e2,
+                                                u32x4 (&Q)[QREG]) {
+    e2 = 0;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      f32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = there && s * 16 + 4 * g < hd ? q[s * 16 + 4 * g + e] * sign : 0.f;
+      Q[s] = __builtin_bit_cast(u32x4, x);
+    }
+  }
+  __device__ __forceinline__ void load_k(int, const float* key, uint32_t g, uint32_t hd) {
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      K[s] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      if (s * 16 + 4 * g < hd) K[s] = *(const f32x4*)(key + s * 16 + 4 * g);
+    }
+  }
+  __device__ __forceinline__ void load_v(int, int i, const float* key, uint32_t n, uint32_t hd) {
+#pragma unroll
+    for (int k = 0; k < DPL; k++) V[i][k] = 0.f;
+    if (n * DPL < hd) {
+#pragma unroll
+      for (int k = 0; k < DPL; k += 4) {
+        const f32x4 v = *(const f32x4*)(key + n * DPL + k);
+#pragma unroll
+        for (int e = 0; e < 4; e++) V[i][k + e] = v[e];
+      }
+    }
+  }
+  __device__ __forceinline__ void zero_v(int, int i) {
+#pragma unroll
+    for (int k = 0; k < DPL; k++) V[i][k] = 0.f;
+  }
+  __device__ __forceinline__ bool all_finite() const {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+      for (int d = 0; d < DPL; d++) bad |= (uint32_t)((__float_as_uint(V[k][d]) & 0x7F800000u) == 0x7F800000u);
+    return !bad;
+  }
+  __device__ __forceinline__ void turn() {}
+  template <class QF>
+  __device__ __forceinline__ void scores(QF q, f32x4 (&S)[NJ]) const {
+    // two independent chains, summed at the end
+    f32x4 a = (f32x4){0.f, 0.f, 0.f, 0.f}, b = a;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const f32x4 x = __builtin_bit_cast(f32x4, q(s));
+      a = __builtin_amdgcn_mfma_f32_16x16x4f32(K[s][0], x[0], a, 0, 0, 0);
+      b = __builtin_amdgcn_mfma_f32_16x16x4f32(K[s][1], x[1], b, 0, 0, 0);
+      a = __builtin_amdgcn_mfma_f32_16x16x4f32(K[s][2], x[2], a, 0, 0, 0);
+      b = __builtin_amdgcn_mfma_f32_16x16x4f32(K[s][3], x[3], b, 0, 0, 0);
+    }
+    S[0] = a + b;
+  }
+  __device__ __forceinline__ void add_pv(const f32x4 (&S)[NJ], f32x4 (&O)[DPL]) const {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int d = 0; d < DPL; d++) O[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[i][d], S[0][i], O[d], 0, 0, 0);
+  }
+  template <class SEEN>
+  __device__ __forceinline__ void add_pv_seen(const f32x4 (&S)[NJ], f32x4 (&O)[DPL], SEEN seen, bool mine) const {
+#pragma unroll
+    for (int d = 0; d < DPL; d++) {
+      f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        o = __builtin_amdgcn_mfma_f32_16x16x4f32(seen(0, i) ? V[i][d] : 0.f, S[0][i], o, 0, 0, 0);
+      if (mine) O[d] += o;
+    }
+  }
+};
+
+struct AttArgs {
+  const float* q;
+  const int32_t* row_start;
+  const int32_t* lens;
+  const int32_t* tables;
+  const void* kpages;
+  const void* vpages;
+  float* out;
+  float* parts;        // a split's partial: O [columns][head dim], then (m, l) of each column
+  uint32_t* counters;  // splits of a block that are done, by the index of its first partial; zero between calls
+  uint64_t* err;
+  uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift, target;
+  float scale;
+};
+
+__device__ __forceinline__ uint32_t div_up(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
+
+// a partial's words cross from one XCD's L2 to another's: written and read
+// through to the agent's coherence point
+__device__ __forceinline__ void put2(float* p, float a, float b) {
+  __hip_atomic_store((uint64_t*)p, ((uint64_t)__float_as_uint(b) << 32) | __float_as_uint(a), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float* p) {
+  const uint64_t v = __hip_atomic_load((uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-#define DEF_ATTENTION(NAME, KV)                                                                                     \
-  extern "C" __global__ __launch_bounds__(256) void NAME(                                                          \
-      const float* __restrict__ q, uint32_t ld_q, uint32_t max_rows, const int32_t* __restrict__ row_start,         \
-      const int32_t* __restrict__ lens, const int32_t* __restrict__ tables, uint32_t n_req, uint32_t max_pages,     \
-      uint32_t nH, uint32_t nKV, uint32_t hd, float scale, const KV::T* __restrict__ kpages,                        \
-      const KV::T* __restrict__ vpages, uint32_t n_pages, uint32_t shift, float* __restrict__ out, uint32_t ld_out, \
-      uint64_t* __restrict__ err) {                                                                                \
-    attention_body<KV>(q, ld_q, max_rows, row_start, lens, tables, n_req, max_pages, nH, nKV, hd, scale, kpages,    \
-                       vpages, n_pages, shift, out, ld_out, err);                                                   \
+// Request b's first row, rows and length; no rows if they do not fit.
+__device__ __forceinline__ void request(const AttArgs& a, uint32_t b, bool tell, uint32_t& r0, uint32_t& n, uint32_t& len) {
+  int32_t s = (int32_t)b, e = s + 1;
+  if (a.row_start) {
+    s = a.row_start[b];
+    e = a.row_start[b + 1];
   }
-DEF_ATTENTION(smith_paged_attention_f32, KvF32)
-DEF_ATTENTION(smith_paged_attention_f16, KvF16)
-DEF_ATTENTION(smith_paged_attention_bf16, KvBf16)
+  const int32_t l = a.lens[b];
+  r0 = (uint32_t)s;
+  n = (uint32_t)(e - s);
+  len = (uint32_t)l;
+  const bool fits = s >= 0 && e >= s && (uint32_t)e <= a.max_rows &&
+                    (s == e || (l >= 0 && (!a.row_start || len >= n) && (uint64_t)len <= ((uint64_t)a.max_pages << a.shift)));
+  if (!fits) {
+    if (tell) paged_err(a.err, PAGED_ERR_ATT_LENGTH, b);
+    n = 0;
+    len = 0;
+  }
+}
+
+#define MERGE_PAD 4  // floats between the columns of a wave's O in LDS
+
+template <class TILE, int DPL, int NT>
+__device__ __forceinline__ void attention_body(const AttArgs& a) {
+  typedef typename TILE::T T;
+  constexpr int NJ = TILE::NJ, QREG = TILE::QREG;
+  constexpr uint32_t TK = 16 * NJ, HDP = 16 * DPL, CB = 16 * NT;
+  constexpr uint32_t OS = HDP + MERGE_PAD;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  float* s_o = (float*)lds;                 // [4 waves][16 columns][OS], or the splits' weights
+  float* s_ml = s_o + 4 * 16 * OS;          // [4 waves][16 columns][m, l]
+  u32x4* s_q = (u32x4*)(s_ml + 4 * 16 * 2);  // NT > 1: [NT][QREG][64 lanes]
+  uint32_t* s_item = (uint32_t*)(s_q + (NT > 1 ? NT * QREG * 64 : 0));  // [n_req + 1] first item of a request
+  uint32_t* s_part = s_item + a.n_req + 1;                              // [n_req] its first partial
+  __shared__ uint64_t s_sum[4];
+  __shared__ uint32_t s_wave[4][2];
+  __shared__ uint32_t s_last;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  const uint32_t ln = lane & 15, lg = lane >> 4;
+  const uint32_t P = 1u << a.shift, G = a.G, hd = a.hd;
+  const uint32_t gcols = G < CB ? G : CB, groups = div_up(G, CB), RB = CB / gcols;  // rows to a block
+  const bool first_wg = blockIdx.x == 0;
+
+  // ---- the items of the call ----
+  if (a.row_start) {
+    const int32_t total = a.row_start[a.n_req];
+    if (total < 0 || (uint32_t)total > a.max_rows) {
+      if (first_wg && tid == 0) paged_err(a.err, PAGED_ERR_ATT_ROWS, (uint32_t)total);
+      return;
+    }
+  }
+  const uint32_t per = div_up(a.n_req, 256);
+  uint64_t work = 0;
+  for (uint32_t k = 0; k < per; k++) {
+    const uint32_t b = tid * per + k;
+    if (b >= a.n_req) break;
+    uint32_t r0, n, len;
+    request(a, b, first_wg, r0, n, len);
+    work += (uint64_t)(div_up(n, RB) * groups) * len;
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) work += __shfl_xor(work, d);
+  if (lane == 0) s_sum[w] = work;
+  __syncthreads();
+  work = (s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) * a.nKV;
+  const uint64_t c64 = (work + a.target - 1) / a.target;
+  const uint32_t C = c64 < PAGED_SPLIT_MIN ? PAGED_SPLIT_MIN : c64 > 0x40000000u ? 0x40000000u : (uint32_t)c64;
+  auto splits = [&](uint32_t len) {
+    const uint32_t s = (len + C / 2) / C;
+    return s < 1 ? 1u : s > PAGED_SPLIT_MAX ? PAGED_SPLIT_MAX : s;
+  };
+  uint32_t items = 0, parts = 0;
+  for (uint32_t k = 0; k < per; k++) {
+    const uint32_t b = tid * per + k;
+    if (b >= a.n_req) break;
+    uint32_t r0, n, len;
+    request(a, b, false, r0, n, len);
+    const uint32_t ns = splits(len), it = div_up(n, RB) * groups * a.nKV * ns;
+    items += it;
+    parts += ns > 1 ? it : 0;
+  }
+  uint32_t ii = items, ip = parts;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t x = __shfl_up(ii, d), y = __shfl_up(ip, d);
+    if (lane >= (uint32_t)d) {
+      ii += x;
+      ip += y;
+    }
+  }
+  if (lane == 63) {
+    s_wave[w][0] = ii;
+    s_wave[w][1] = ip;
+  }
+  __syncthreads();
+  uint32_t n_items = 0;
+  ii -= items;
+  ip -= parts;
+#pragma unroll
+  for (uint32_t k = 0; k < 4; k++) {
+    if (k < w) {
+      ii += s_wave[k][0];
+      ip += s_wave[k][1];
+    }
+    n_items += s_wave[k][0];
+  }
+  for (uint32_t k = 0; k < per; k++) {
+    const uint32_t b = tid * per + k;
+    if (b >= a.n_req) break;
+    uint32_t r0, n, len;
+    request(a, b, false, r0, n, len);
+    const uint32_t ns = splits(len), it = div_up(n, RB) * groups * a.nKV * ns;
+    s_item[b] = ii;
+    s_part[b] = ip;
+    ii += it;
+    ip += ns > 1 ? it : 0;
+  }
+  if (tid == 0) s_item[a.n_req] = n_items;
+  __syncthreads();
+
+  for (uint32_t item = blockIdx.x; item < n_items; item += gridDim.x) {
+    uint32_t b = 0, top = a.n_req;
+    while (top - b > 1) {
+      const uint32_t mid = (b + top) >> 1;
+      if (s_item[mid] <= item) b = mid;
+      else top = mid;
+    }
+    b = (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
+    uint32_t r0, n, len;
+    request(a, b, false, r0, n, len);
+    const uint32_t ns = splits(len), nblk = div_up(n, RB) * groups;
+    const uint32_t local = item - s_item[b];
+    // the KV head first (neighbouring blocks of a head meet in one XCD's L2 when
+    // there are 8 of them), the blocks with the most keys before the others
+    const uint32_t kvh = local % a.nKV, rest = local / a.nKV, split = rest % ns, blk = nblk - 1 - rest / ns;
+    const uint32_t hg = blk % groups, row0 = blk / groups * RB;
+    const uint32_t rows = n - row0 < RB ? n - row0 : RB;
+    const uint32_t gc = G - hg * CB < gcols ? G - hg * CB : gcols;  // heads of this block
+    const uint32_t ncols = rows * gc;
+    // keys: row i of the request sees base + i + 1 of them
+    const uint32_t base = len - n;  // a lone row without keys: -1
+    const uint32_t keys = base + row0 + rows;
+    const uint32_t least = base + row0 + 1;  // what the block's first row sees
+    const uint32_t chunk = ns > 1 ? div_up(div_up(keys, ns), TK) * TK : keys;
+    const uint64_t at0 = (uint64_t)split * chunk;
+    const uint32_t k0 = at0 < keys ? (uint32_t)at0 : keys, k1 = keys - k0 < chunk ? keys : k0 + chunk;
+
+    // ---- this lane's columns ----
+    u32x4 Q[QREG];
+    float c[NT];
+    uint32_t limit[NT];
+    const float sign = a.scale < 0.f ? -1.f : 1.f, mul = fabsf(a.scale) * 1.44269504088896340736f;
+    auto column = [&](uint32_t col, uint32_t& row, uint32_t& head) {
+      row = col / gc;
+      head = kvh * G + hg * CB + col % gc;
+    };
+    if (NT == 1) {
+      uint32_t row, head;
+      column(ln, row, head);
+      int e2;
+      TILE::load_q(a.q + (size_t)(r0 + row0 + row) * a.ld_q + head * hd, ln < ncols, lg, hd, sign, e2, Q);
+      c[0] = fmaxf(ldexpf(mul, -e2), 1.17549435e-38f);
+      limit[0] = least + row;
+    } else {
+      // tile w is this wave's to prepare
+      uint32_t row, head;
+      column(w * 16 + ln, row, head);
+      int e2;
+      TILE::load_q(a.q + (size_t)(r0 + row0 + row) * a.ld_q + head * hd, w * 16 + ln < ncols, lg, hd, sign, e2, Q);
+#pragma unroll
+      for (int k = 0; k < QREG; k++) s_q[(w * QREG + k) * 64 + lane] = Q[k];
+      if (lg == 0) s_ml[w * 16 + ln] = fmaxf(ldexpf(mul, -e2), 1.17549435e-38f);
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        c[t] = s_ml[t * 16 + ln];
+        limit[t] = least + (t * 16 + ln) / gc;
+      }
+    }
+    f32x4 O[NT][DPL];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      m[t] = -__builtin_inff();
+      l[t] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DPL; d++) O[t][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+
+    // ---- this wave's keys ----
+    const int32_t* table = a.tables + (size_t)b * a.max_pages;
+    const size_t head_len = (size_t)hd << a.shift;  // values of a page's KV head
+    auto page_of = [&](uint32_t t) {
+      uint32_t p = (uint32_t)table[t >> a.shift];
+      if (p >= a.n_pages) {
+        paged_err(a.err, PAGED_ERR_ATT_PAGE, b);
+        p = 0;
+      }
+      return p;
+    };
+    for (uint32_t t0 = k0 + w * TK; t0 < k1; t0 += 4 * TK) {
+      TILE tile;
+      if (a.shift >= 4) {
+        // 16 keys lie in one page: its address is the wave's
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+          const uint32_t tj = t0 + 16 * j < k1 ? t0 + 16 * j : t0;
+          const size_t at = ((size_t)page_of(tj) * a.nKV + kvh) * head_len + (size_t)(tj & (P - 1)) * hd;
+          const T *kp = (const T*)a.kpages + at, *vp = (const T*)a.vpages + at;
+          tile.load_k(j, kp + ln * hd, lg, hd);
+#pragma unroll
+          for (int i = 0; i < 4; i++) tile.load_v(j, i, vp + (4 * lg + i) * hd, ln, hd);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+          auto at = [&](uint32_t t) {
+            t = t < k1 ? t : k1 - 1;
+            return ((size_t)page_of(t) * a.nKV + kvh) * head_len + (size_t)(t & (P - 1)) * hd;
+          };
+          tile.load_k(j, (const T*)a.kpages + at(t0 + 16 * j + ln), lg, hd);
+#pragma unroll
+          for (int i = 0; i < 4; i++) tile.load_v(j, i, (const T*)a.vpages + at(t0 + 16 * j + 4 * lg + i), ln, hd);
+        }
+      }
+      const bool masked = t0 + TK > least || t0 + TK > k1;
+      bool apart = false;  // values that some columns must not touch, not even with a weight of 0
+      if (masked) {
+        // values behind the block's keys may be anything: their weight is 0, they must be finite
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (t0 + 16 * j + 4 * lg + i >= k1) tile.zero_v(j, i);
+      }
+      tile.turn();
+      if (masked && rows > 1) apart = __any(!tile.all_finite());
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        if (t * 16 >= ncols) break;
+        f32x4 S[NJ];
+        tile.scores([&](int k) { return NT > 1 ? s_q[(t * QREG + k) * 64 + lane] : Q[k]; }, S);
+        if (masked) {
+          const uint32_t end = limit[t] < k1 ? limit[t] : k1;
+#pragma unroll
+          for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              if (t0 + 16 * j + 4 * lg + i >= end) S[j][i] = -__builtin_inff();
+        }
+        float x = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) x = fmaxf(x, S[j][i]);
+        x = fmaxf(x, __shfl_xor(x, 16));
+        x = fmaxf(x, __shfl_xor(x, 32)) * c[t];
+        if (__any(x > m[t] + M_SLACK)) {
+          const float mn = fmaxf(x, m[t]);
+          const float f = mn == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[t] - mn);
+          m[t] = mn;
+          l[t] *= f;
+#pragma unroll
+          for (int d = 0; d < DPL; d++) O[t][d] *= f;
+        }
+        const float shift = m[t] == -__builtin_inff() ? 0.f : P_EXP - m[t];
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            S[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[j][i], c[t], shift));
+            l[t] += S[j][i];
+          }
+        if (!apart) {
+          tile.add_pv(S, O[t]);
+        } else {
+          // row by row, with the values that the row does not see at 0
+          const uint32_t last = t * 16 + 15 < ncols ? t * 16 + 15 : ncols - 1;
+          for (uint32_t row = t * 16 / gc; row <= last / gc; row++)
+            tile.add_pv_seen(S, O[t], [&](int j, int i) { return t0 + 16 * j + 4 * lg + i < least + row; },
+                             limit[t] == least + row);
+        }
+      }
+    }
+
+    // ---- join the waves, 16 columns at a time ----
+    const uint32_t part = s_part[b] + local;  // of ns > 1; a split's are nKV apart
+    float* mine = a.parts + (size_t)part * CB * (hd + 2);
+    const uint32_t col = tid >> 4, d0 = (tid & 15) * DPL;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      if (t * 16 >= ncols) break;
+      l[t] = add_xor32(add_xor16(l[t]));
+      __syncthreads();  // s_ml and s_o are free
+      if (lg == 0) {
+        s_ml[(w * 16 + ln) * 2] = m[t];
+        s_ml[(w * 16 + ln) * 2 + 1] = l[t];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int d = 0; d < DPL; d += 4)
+          *(f32x4*)&s_o[(w * 16 + ln) * OS + (4 * lg + i) * DPL + d] =
+              (f32x4){O[t][d][i], O[t][d + 1][i], O[t][d + 2][i], O[t][d + 3][i]};
+      __syncthreads();
+      float mx = s_ml[col * 2];
+#pragma unroll
+      for (int k = 1; k < 4; k++) mx = fmaxf(mx, s_ml[(k * 16 + col) * 2]);
+      float sum = 0.f, o[DPL];
+#pragma unroll
+      for (int d = 0; d < DPL; d++) o[d] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float mk = s_ml[(k * 16 + col) * 2];
+        const float f = mk == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mk - mx);
+        sum = __builtin_fmaf(f, s_ml[(k * 16 + col) * 2 + 1], sum);
+#pragma unroll
+        for (int d = 0; d < DPL; d++) o[d] = __builtin_fmaf(f, s_o[(k * 16 + col) * OS + d0 + d], o[d]);
+      }
+      const uint32_t at = t * 16 + col;
+      if (at < ncols && d0 < hd) {
+        if (ns == 1) {
+          uint32_t row, head;
+          column(at, row, head);
+          float* y = a.out + (size_t)(r0 + row0 + row) * a.ld_out + head * hd + d0;
+#pragma unroll
+          for (int d = 0; d < DPL; d++) y[d] = keys ? o[d] / sum : 0.f;
+        } else {
+#pragma unroll
+          for (int d = 0; d < DPL; d += 2) put2(mine + at * hd + d0 + d, o[d], o[d + 1]);
+          if (d0 == 0) put2(mine + CB * hd + at * 2, mx, sum);
+        }
+      }
+    }
+    if (ns > 1) {
+      const size_t stride = (size_t)a.nKV * CB * (hd + 2);
+      const uint32_t first = part - split * a.nKV;
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      if (tid == 0)
+        s_last = __hip_atomic_fetch_add(a.counters + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ns - 1;
+      __syncthreads();
+      if (s_last) {
+        const float* all = a.parts + (size_t)first * CB * (hd + 2);
+        if (tid == 0) __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (uint32_t c0 = 0; c0 < ncols; c0 += 16) {
+          // weights 2^(m - max) of the splits, 16 threads to a column
+          const uint32_t cc = c0 + (tid & 15), sp0 = tid >> 4;
+          float mx = -__builtin_inff(), sum = 0.f;
+          if (cc < ncols)
+            for (uint32_t s = sp0; s < ns; s += 16) mx = fmaxf(mx, get2(all + s * stride + CB * hd + cc * 2).x);
+          mx = fmaxf(mx, __shfl_xor(mx, 16));
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          __syncthreads();
+          if (lg == 0) s_ml[w * 16 + ln] = mx;
+          __syncthreads();
+          mx = fmaxf(fmaxf(s_ml[ln], s_ml[16 + ln]), fmaxf(s_ml[32 + ln], s_ml[48 + ln]));
+          if (cc < ncols)
+            for (uint32_t s = sp0; s < ns; s += 16) {
+              const float2 v = get2(all + s * stride + CB * hd + cc * 2);
+              const float f = v.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(v.x - mx);
+              s_o[s * 16 + ln] = f;
+              sum = __builtin_fmaf(f, v.y, sum);
+            }
+          sum = add_xor32(add_xor16(sum));
+          __syncthreads();
+          if (lg == 0) s_ml[64 + w * 16 + ln] = sum;
+          __syncthreads();
+          const uint32_t nc = ncols - c0 < 16 ? ncols - c0 : 16;
+          for (uint32_t e = 2 * tid; e < nc * hd; e += 512) {
+            const uint32_t k = e / hd, d = e % hd;
+            float2 o = make_float2(0.f, 0.f);
+#pragma unroll 8
+            for (uint32_t s = 0; s < ns; s++) {
+              const float2 v = get2(all + s * stride + c0 * hd + e);
+              o.x = __builtin_fmaf(s_o[s * 16 + k], v.x, o.x);
+              o.y = __builtin_fmaf(s_o[s * 16 + k], v.y, o.y);
+            }
+            const float tot = s_ml[64 + k] + s_ml[80 + k] + s_ml[96 + k] + s_ml[112 + k];
+            uint32_t row, head;
+            column(c0 + k, row, head);
+            float* y = a.out + (size_t)(r0 + row0 + row) * a.ld_out + head * hd + d;
+            y[0] = o.x / tot;
+            y[1] = o.y / tot;
+          }
+        }
+      }
+    }
+    __syncthreads();  // LDS is free for the next item
+  }
+}
+
+#define DEF_ATTENTION(NAME, TILE, DPL, NT)                                                         \
+  extern "C" __global__ __launch_bounds__(256, 2) void NAME(AttArgs a) {                           \
+    attention_body<TILE, DPL, NT>(a);                                                              \
+  }
+#define COMMA ,
+// named by page type, head dims held (64 or 128) and tiles of 16 columns to a workgroup
+DEF_ATTENTION(smith_paged_attention_f32_d64_t1, Tile32<4>, 4, 1)
+DEF_ATTENTION(smith_paged_attention_f32_d128_t1, Tile32<8>, 8, 1)
+DEF_ATTENTION(smith_paged_attention_f16_d64_t1, Tile16<MmF16 COMMA 4>, 4, 1)
+DEF_ATTENTION(smith_paged_attention_f16_d128_t1, Tile16<MmF16 COMMA 8>, 8, 1)
+DEF_ATTENTION(smith_paged_attention_f16_d64_t4, Tile16<MmF16 COMMA 4>, 4, 4)
+DEF_ATTENTION(smith_paged_attention_f16_d128_t4, Tile16<MmF16 COMMA 8>, 8, 4)
+DEF_ATTENTION(smith_paged_attention_bf16_d64_t1, Tile16<MmBf16 COMMA 4>, 4, 1)
+DEF_ATTENTION(smith_paged_attention_bf16_d128_t1, Tile16<MmBf16 COMMA 8>, 8, 1)
+DEF_ATTENTION(smith_paged_attention_bf16_d64_t4, Tile16<MmBf16 COMMA 4>, 4, 4)
+DEF_ATTENTION(smith_paged_attention_bf16_d128_t4, Tile16<MmBf16 COMMA 8>, 8, 4)

@@ -80,6 +80,9 @@ struct Ctx {
   size_t att_ws_bytes = 0;
   uint32_t* att_cnt = nullptr;
   size_t att_cnt_n = 0;
+  void* paged_ws = nullptr;  // partials of smith_paged_attention
+  size_t paged_ws_bytes = 0;
+  uint32_t* paged_cnt = nullptr;  // and the splits of a block that are done
   bool capturing = false;
   // set while an entry point that must not allocate runs on the static
   // scratch (its name, for the error when a region is too small)
@@ -327,6 +330,18 @@ int ensure_amx(Ctx* c) {
   c->allocated += 2 * sizeof(uint64_t);
   if (zero_now(c, c->amx, 2 * sizeof(uint64_t))) return -1;
   return 0;
+}
+
+// One counter to a partial of smith_paged_attention, whatever the call.
+constexpr uint32_t PAGED_COUNTERS = 4096;
+
+int ensure_paged_counters(Ctx* c) {
+  if (c->paged_cnt) return 0;
+  if (c->capturing)
+    return fail(c, "smith_paged_attention: counters needed while capturing a graph; run the op once first");
+  HIPCHK(c, hipMalloc((void**)&c->paged_cnt, PAGED_COUNTERS * sizeof(uint32_t)));
+  c->allocated += PAGED_COUNTERS * sizeof(uint32_t);
+  return zero_now(c, c->paged_cnt, PAGED_COUNTERS * sizeof(uint32_t));
 }
 
 // Kernel argument of smith_lmhead_q4_0_nb (same layout as the device struct).
@@ -1005,6 +1020,8 @@ void smith_destroy(void* ctx) {
   if (c->ws) (void)hipFree(c->ws);
   if (c->counters) (void)hipFree(c->counters);
   if (c->amx) (void)hipFree(c->amx);
+  if (c->paged_ws) (void)hipFree(c->paged_ws);
+  if (c->paged_cnt) (void)hipFree(c->paged_cnt);
   for (void* r : c->retired) (void)hipFree(r);
   for (auto& r : c->recs) {
     (void)hipEventDestroy(r.a);
@@ -2423,12 +2440,39 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
     return fail(c, "%s: out overlaps q", fn);
   if (set_device(c)) return -1;
   if (scale == 0.f) scale = 1.0f / sqrtf((float)head_dim);
-  uint64_t* perr = c->paged_err_dev();
-  char name[48];
-  snprintf(name, sizeof name, "smith_paged_attention_%s", kv_name(kv_type));
-  void* args[] = {&q, &ld_q, &max_rows, &row_start, &lens, &tables, &n_req, &max_pages, &n_heads, &n_kv_heads,
-                  &head_dim, &scale, &kpages, &vpages, &n_pages, &shift, &out, &ld_out, &perr};
-  return launch(c, name, dim3(max_rows, n_heads), dim3(256), args);
+  // tiles of 16 columns (row, head) to a workgroup: one where requests bring a
+  // row or so each (the keys are read once, columns hardly matter), four where
+  // they fill more than two; the f32 matrix cores are the bound at one already
+  const uint32_t G = n_heads / n_kv_heads;
+  const uint32_t tiles = row_start && kv_type != SMITH_KV_F32 && (uint64_t)max_rows * G > 32ull * n_req ? 4 : 1;
+  const uint32_t CB = 16 * tiles, dims = head_dim <= 64 ? 64 : 128;
+  const uint32_t target = tiles == 1 ? 1024 : 512;
+  // splits have at least 1.5 C keys between two of them, so there are fewer
+  // than 4/3 W / C of those that leave a partial
+  const uint32_t max_parts = target + target / 3 + 1;
+  if (ensure(c, &c->paged_ws, &c->paged_ws_bytes, (size_t)max_parts * CB * (head_dim + 2) * sizeof(float))) return -1;
+  if (ensure_paged_counters(c)) return -1;
+  const uint64_t RB = CB / std::min(G, CB), groups = (G + CB - 1) / CB;
+  const uint64_t blocks = groups * n_kv_heads * (row_start ? n_req + max_rows / RB : n_req);
+  const uint64_t longest = ((uint64_t)max_pages << shift) / PAGED_SPLIT_MIN + 1;  // splits of one block
+  const uint32_t grid = (uint32_t)std::min<uint64_t>({(uint64_t)target, blocks + max_parts, blocks * longest});
+  const uint32_t qreg = kv_type == SMITH_KV_F32 ? dims / 16 : dims / 32 * (kv_type == SMITH_KV_F16 ? 2 : 3);
+  const uint32_t lds = 4 * (4 * 16 * (dims + 4) + 4 * 16 * 2) + (tiles > 1 ? tiles * qreg * 64 * 16 : 0) + 4 * (2 * n_req + 1);
+  struct {
+    const float* q;
+    const int32_t *row_start, *lens, *tables;
+    const void *kpages, *vpages;
+    float *out, *parts;
+    uint32_t* counters;
+    uint64_t* err;
+    uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift, target;
+    float scale;
+  } a = {q, row_start, lens, tables, kpages, vpages, out, (float*)c->paged_ws, c->paged_cnt, c->paged_err_dev(),
+         ld_q, ld_out, max_rows, n_req, max_pages, n_kv_heads, G, head_dim, n_pages, shift, target, scale};
+  char name[64];
+  snprintf(name, sizeof name, "smith_paged_attention_%s_d%u_t%u", kv_name(kv_type), dims, tiles);
+  void* args[] = {&a};
+  return launch(c, name, dim3(grid), dim3(256), args, lds);
 }
 
 int smith_set_i32(void* ctx, int32_t* p, int32_t v) {
