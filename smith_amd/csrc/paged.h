@@ -6,9 +6,9 @@
 #define PAGED_MAX_REQ 4096u
 
 // attention: fewest keys that a split is made for, most splits of a block (their
-// weights are kept in LDS, 16 columns of them in the 17 KB of a merge buffer)
+// weights are kept in LDS, 16 columns of them)
 #define PAGED_SPLIT_MIN 128u
-#define PAGED_SPLIT_MAX 256u
+#define PAGED_SPLIT_MAX 128u
 
 #define PAGED_ROPE_ROW 1u   // SMITH_ROPE_ROW
 #define PAGED_ROPE_HEAD 2u  // SMITH_ROPE_HEAD

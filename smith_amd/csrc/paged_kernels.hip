@@ -15,6 +15,11 @@
 #include "paged.h"
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+// rows and tables of the caller need start on no more than 4 bytes; the
+// hardware's 16-byte accesses want no more either
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ f32x4 load4(const float* p) { return *(const f32x4_any*)p; }
+__device__ __forceinline__ void store4(float* p, f32x4 v) { *(f32x4_any*)p = v; }
 
 // One 64-bit word of host-mapped memory: (code, argument), the first one kept.
 __device__ __forceinline__ void paged_err(uint64_t* __restrict__ err, uint32_t code, uint32_t arg) {
@@ -175,20 +180,6 @@ extern "C" __global__ __launch_bounds__(PLAN_THREADS) void smith_paged_plan(
 // or half the head.  Bound by memory: a thread takes four neighbouring pairs
 // (two 16-byte loads of x, one each of cos and sin), or eight elements of v.
 // ---------------------------------------------------------------------------
-template <bool VEC>
-__device__ __forceinline__ f32x4 load4(const float* p) {
-  if (VEC) return *(const f32x4*)p;
-  return (f32x4){p[0], p[1], p[2], p[3]};
-}
-template <bool VEC>
-__device__ __forceinline__ void store4(float* p, f32x4 v) {
-  if (VEC) {
-    *(f32x4*)p = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) p[i] = v[i];
-  }
-}
 template <class KV>
 __device__ __forceinline__ void put4(typename KV::T* p, f32x4 v) {
   typedef typename KV::T T4 __attribute__((ext_vector_type(4)));
@@ -198,7 +189,7 @@ __device__ __forceinline__ void put4(typename KV::T* p, f32x4 v) {
   *(T4*)p = t;
 }
 
-template <class KV, bool VEC>
+template <class KV>
 __device__ __forceinline__ void append_body(const float* qkv, uint32_t ld, const int32_t* __restrict__ slots,
                                             const int32_t* __restrict__ positions, uint32_t nH, uint32_t nKV,
                                             uint32_t hd, uint32_t rope, const float* __restrict__ cosT,
@@ -240,17 +231,17 @@ __device__ __forceinline__ void append_body(const float* qkv, uint32_t ld, const
       t = i4 % half;
       e0 = i4 / half * hd + t;
     }
-    f32x4 x0 = load4<VEC>(x + e0), x1 = load4<VEC>(x + e0 + half);
+    f32x4 x0 = load4(x + e0), x1 = load4(x + e0 + half);
     if (rope) {
       const size_t a = (size_t)(uint32_t)pos * half + t;
-      const f32x4 c = load4<VEC>(cosT + a), s = load4<VEC>(sinT + a);
+      const f32x4 c = load4(cosT + a), s = load4(sinT + a);
       const f32x4 y0 = x0 * c - x1 * s;
       x1 = x0 * s + x1 * c;
       x0 = y0;
     }
     if (isq) {
-      store4<VEC>(q_out + (size_t)r * ld_q + e0, x0);
-      store4<VEC>(q_out + (size_t)r * ld_q + e0 + half, x1);
+      store4(q_out + (size_t)r * ld_q + e0, x0);
+      store4(q_out + (size_t)r * ld_q + e0 + half, x1);
     } else {
       put4<KV>(kpages + at(e0), x0);
       put4<KV>(kpages + at(e0 + half), x1);
@@ -258,26 +249,23 @@ __device__ __forceinline__ void append_body(const float* qkv, uint32_t ld, const
   } else if (item < nq + 2 * nk) {
     const uint32_t e = 8 * (item - nq - nk);
     const float* x = row + Wq + Wk + e;
-    put4<KV>(vpages + at(e), load4<VEC>(x));
-    put4<KV>(vpages + at(e) + 4, load4<VEC>(x + 4));
+    put4<KV>(vpages + at(e), load4(x));
+    put4<KV>(vpages + at(e) + 4, load4(x + 4));
   }
 }
 
-#define DEF_APPEND(NAME, KV, VEC)                                                                                   \
+#define DEF_APPEND(NAME, KV)                                                                                        \
   extern "C" __global__ __launch_bounds__(256) void NAME(                                                          \
       const float* qkv, uint32_t ld, const int32_t* __restrict__ slots, const int32_t* __restrict__ positions,      \
       uint32_t nH, uint32_t nKV, uint32_t hd, uint32_t rope, const float* __restrict__ cosT,                        \
       const float* __restrict__ sinT, uint32_t rope_len, KV::T* __restrict__ kpages, KV::T* __restrict__ vpages,    \
       uint32_t n_slots, uint32_t shift, float* q_out, uint32_t ld_q, uint64_t* __restrict__ err) {                  \
-    append_body<KV, VEC>(qkv, ld, slots, positions, nH, nKV, hd, rope, cosT, sinT, rope_len, kpages, vpages, n_slots, \
-                         shift, q_out, ld_q, err);                                                                  \
+    append_body<KV>(qkv, ld, slots, positions, nH, nKV, hd, rope, cosT, sinT, rope_len, kpages, vpages, n_slots,    \
+                    shift, q_out, ld_q, err);                                                                       \
   }
-DEF_APPEND(smith_paged_append_f32, KvF32, true)
-DEF_APPEND(smith_paged_append_f16, KvF16, true)
-DEF_APPEND(smith_paged_append_bf16, KvBf16, true)
-DEF_APPEND(smith_paged_append_f32_u, KvF32, false)
-DEF_APPEND(smith_paged_append_f16_u, KvF16, false)
-DEF_APPEND(smith_paged_append_bf16_u, KvBf16, false)
+DEF_APPEND(smith_paged_append_f32, KvF32)
+DEF_APPEND(smith_paged_append_f16, KvF16)
+DEF_APPEND(smith_paged_append_bf16, KvBf16)
 
 // ---------------------------------------------------------------------------
 // Attention over the pages: row i of request b's n rows is position p = len -
@@ -319,6 +307,26 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// maximum over the lanes l, l ^ 16, l ^ 32, l ^ 48 (a number wins over a NaN)
+__device__ __forceinline__ float max_xor16_32(float v) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+// sum over the lanes up to this one: within rows of 16, then across them
+__device__ __forceinline__ uint32_t scan64_lanes(uint32_t v) {
+#define SCAN_DPP(CTRL, ROWS) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false)
+  SCAN_DPP(0x111, 0xF);  // row_shr 1, 2, 4, 8
+  SCAN_DPP(0x112, 0xF);
+  SCAN_DPP(0x114, 0xF);
+  SCAN_DPP(0x118, 0xF);
+  SCAN_DPP(0x142, 0xA);  // row_bcast 15 into rows 1 and 3, 31 into 2 and 3
+  SCAN_DPP(0x143, 0xC);
+#undef SCAN_DPP
+  return v;
+}
 
 #define P_EXP 6.0f   // P = 2^(score - m + P_EXP)
 #define M_SLACK 8.0f // m follows a new maximum only when it is this far (log2) above
@@ -372,82 +380,84 @@ struct Tile16 {
   static constexpr int NJ = 2, KS = DPL / 2, TERMS = MM::TERMS, QREG = KS * TERMS;
   u32x4 K[NJ][KS];
   uint32_t V[8][DPL / 2];  // a key's dims of this lane
-  u32x4 D[DPL];            // a dim's keys
-  // Q: parts of the lane's column, dims s*32 + 8g .. +7
-  static __device__ __forceinline__ void load_q(const float* q, bool there, uint32_t g, uint32_t hd, float sign, int& e2,
-                                                u32x4 (&Q)[QREG]) {
-    float x[KS][8];
+  // the lane's column of q: dims s*32 + 8g .. +7 (past the head others, then 0)
+  static constexpr int QRAW = 2 * KS;
+  static __device__ __forceinline__ void load_q(const float* q, uint32_t g, uint32_t hd, f32x4 (&x)[QRAW]) {
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const uint32_t e = s * 32 + 8 * g;
+      const float* at = q + (e < hd ? e : hd - 8);
+      x[2 * s] = load4(at);
+      x[2 * s + 1] = load4(at + 4);
+    }
+  }
+  // ... in parts, times +-1 and a power of two that brings its largest element
+  // to [2^14, 2^15); what is not finite stays as it is
+  static __device__ __forceinline__ void split_q(const f32x4 (&x)[QRAW], bool there, uint32_t g, uint32_t hd, float sign,
+                                                 int& e2, u32x4 (&Q)[QREG]) {
+    float y[KS][8];
     float big = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        x[s][e] = there && s * 32 + 8 * g < hd ? q[s * 32 + 8 * g + e] * sign : 0.f;
-        big = fmaxf(big, fabsf(x[s][e]));
+        y[s][e] = there && s * 32 + 8 * g < hd ? x[2 * s + e / 4][e % 4] * sign : 0.f;
+        big = fmaxf(big, fabsf(y[s][e]));
       }
-    big = fmaxf(big, __shfl_xor(big, 16));
-    big = fmaxf(big, __shfl_xor(big, 32));
-    // largest element to [2^14, 2^15); what is not finite stays as it is
-    int ex;
-    (void)frexpf(big, &ex);
-    e2 = big > 0.f && big < __builtin_inff() ? 15 - ex : 0;
+    big = max_xor16_32(big);
+    e2 = big > 0.f && big < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(big) : 0;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[s][e] = ldexpf(x[s][e], e2);
+      for (int e = 0; e < 8; e++) y[s][e] = __builtin_amdgcn_ldexpf(y[s][e], e2);
       u32x4 t[TERMS];
-      MM::split(x[s], t);
+      MM::split(y[s], t);
 #pragma unroll
       for (int k = 0; k < TERMS; k++) Q[s * TERMS + k] = t[k];
     }
   }
-  __device__ __forceinline__ void load_k(int j, const T* key, uint32_t g, uint32_t hd) {
+  // of the j-th 16 keys, lane n's: `off` values behind `key`
+  __device__ __forceinline__ void load_k(int j, const T* key, uint32_t off, uint32_t g, uint32_t hd) {
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-      K[j][s] = (u32x4){0u, 0u, 0u, 0u};
-      if (s * 32 + 8 * g < hd) K[j][s] = *(const u32x4*)(key + s * 32 + 8 * g);
+      const uint32_t e = s * 32 + 8 * g;
+      K[j][s] = *(const u32x4*)(key + (off + (e < hd ? e : hd - 8)));  // past the head: against zeros of Q
     }
   }
   // key 4g + i of the j-th 16
-  __device__ __forceinline__ void load_v(int j, int i, const T* key, uint32_t n, uint32_t hd) {
+  __device__ __forceinline__ void load_v(int j, int i, const T* key, uint32_t off, uint32_t n, uint32_t hd) {
     uint32_t(&r)[DPL / 2] = V[4 * j + i];
+    const T* at = key + (off + (n * DPL < hd ? n * DPL : hd - DPL));  // past the head: dims that nobody writes out
+    if constexpr (DPL == 8) {
+      const u32x4 v = *(const u32x4*)at;
 #pragma unroll
-    for (int k = 0; k < DPL / 2; k++) r[k] = 0u;
-    if (n * DPL < hd) {
-      if constexpr (DPL == 8) {
-        const u32x4 v = *(const u32x4*)(key + 8 * n);
-#pragma unroll
-        for (int k = 0; k < 4; k++) r[k] = v[k];
-      } else {
-        const u32x2 v = *(const u32x2*)(key + 4 * n);
-        r[0] = v[0];
-        r[1] = v[1];
-      }
+      for (int k = 0; k < 4; k++) r[k] = v[k];
+    } else {
+      const u32x2 v = *(const u32x2*)at;
+      r[0] = v[0];
+      r[1] = v[1];
     }
   }
   __device__ __forceinline__ void zero_v(int j, int i) {
 #pragma unroll
     for (int k = 0; k < DPL / 2; k++) V[4 * j + i][k] = 0u;
   }
-  // V's rows of dims into rows of keys: word k of dim d is keys 2k, 2k+1
-  __device__ __forceinline__ void turn() {
+  // dim d of the lane's keys: word k holds keys 2k, 2k+1
+  __device__ __forceinline__ u32x4 dim(int d) const {
+    u32x4 a;
 #pragma unroll
-    for (int d = 0; d < DPL; d++)
-#pragma unroll
-      for (int k = 0; k < 4; k++)
-        D[d][k] = __builtin_amdgcn_perm(V[2 * k + 1][d / 2], V[2 * k][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
+    for (int k = 0; k < 4; k++)
+      a[k] = __builtin_amdgcn_perm(V[2 * k + 1][d / 2], V[2 * k][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
+    return a;
   }
-  __device__ __forceinline__ bool all_finite() const {
-    uint32_t bad = 0;
+  __device__ __forceinline__ bool finite_v(int j, int i) const {
+    bool ok = true;
 #pragma unroll
-    for (int d = 0; d < DPL; d++)
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const uint32_t x = D[d][k];
-        bad |= (uint32_t)((x & MM::EXPONENT) == MM::EXPONENT) |
-               (uint32_t)((x & (MM::EXPONENT << 16)) == (MM::EXPONENT << 16));
-      }
-    return !bad;
+    for (int d = 0; d < DPL / 2; d++) {
+      const uint32_t x = V[4 * j + i][d];
+      ok = ok && (x & MM::EXPONENT) != MM::EXPONENT && (x & (MM::EXPONENT << 16)) != (MM::EXPONENT << 16);
+    }
+    return ok;
   }
   template <class QF>
   __device__ __forceinline__ void scores(QF q, f32x4 (&S)[NJ]) const {
@@ -472,24 +482,10 @@ struct Tile16 {
     u32x4 t[TERMS];
     weights(S, t);
 #pragma unroll
-    for (int d = 0; d < DPL; d++)
-#pragma unroll
-      for (int k = 0; k < TERMS; k++) O[d] = MM::mfma(D[d], t[k], O[d]);
-  }
-  // only the values that seen(j, i) says, and only into the columns of `mine`
-  template <class SEEN>
-  __device__ __forceinline__ void add_pv_seen(const f32x4 (&S)[NJ], f32x4 (&O)[DPL], SEEN seen, bool mine) const {
-    u32x4 t[TERMS], mask;
-    weights(S, t);
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-      mask[k] = (seen(k / 2, 2 * (k % 2)) ? 0x0000FFFFu : 0u) | (seen(k / 2, 2 * (k % 2) + 1) ? 0xFFFF0000u : 0u);
-#pragma unroll
     for (int d = 0; d < DPL; d++) {
-      f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
+      const u32x4 v = dim(d);
 #pragma unroll
-      for (int k = 0; k < TERMS; k++) o = MM::mfma(D[d] & mask, t[k], o);
-      if (mine) O[d] += o;
+      for (int k = 0; k < TERMS; k++) O[d] = MM::mfma(v, t[k], O[d]);
     }
   }
 };
@@ -501,49 +497,50 @@ struct Tile32 {
   static constexpr int NJ = 1, KS = DPL, QREG = KS;
   f32x4 K[KS];  // dims s*16 + 4g .. +3
   float V[4][DPL];
-  static __device__ __forceinline__ void load_q(const float* q, bool there, uint32_t g, uint32_t hd, float sign, int& e2,
-                                                u32x4 (&Q)[QREG]) {
+  static constexpr int QRAW = KS;
+  static __device__ __forceinline__ void load_q(const float* q, uint32_t g, uint32_t hd, f32x4 (&x)[QRAW]) {
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const uint32_t e = s * 16 + 4 * g;
+      x[s] = load4(q + (e < hd ? e : hd - 4));
+    }
+  }
+  static __device__ __forceinline__ void split_q(const f32x4 (&x)[QRAW], bool there, uint32_t g, uint32_t hd, float sign,
+                                                 int& e2, u32x4 (&Q)[QREG]) {
     e2 = 0;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-      f32x4 x;
-#pragma unroll
-      for (int e = 0; e < 4; e++) x[e] = there && s * 16 + 4 * g < hd ? q[s * 16 + 4 * g + e] * sign : 0.f;
-      Q[s] = __builtin_bit_cast(u32x4, x);
+      f32x4 y = x[s] * sign;
+      if (!there || s * 16 + 4 * g >= hd) y = (f32x4){0.f, 0.f, 0.f, 0.f};
+      Q[s] = __builtin_bit_cast(u32x4, y);
     }
   }
-  __device__ __forceinline__ void load_k(int, const float* key, uint32_t g, uint32_t hd) {
+  __device__ __forceinline__ void load_k(int, const float* key, uint32_t off, uint32_t g, uint32_t hd) {
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-      K[s] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      if (s * 16 + 4 * g < hd) K[s] = *(const f32x4*)(key + s * 16 + 4 * g);
+      const uint32_t e = s * 16 + 4 * g;
+      K[s] = *(const f32x4*)(key + (off + (e < hd ? e : hd - 4)));
     }
   }
-  __device__ __forceinline__ void load_v(int, int i, const float* key, uint32_t n, uint32_t hd) {
+  __device__ __forceinline__ void load_v(int, int i, const float* key, uint32_t off, uint32_t n, uint32_t hd) {
+    const float* at = key + (off + (n * DPL < hd ? n * DPL : hd - DPL));
 #pragma unroll
-    for (int k = 0; k < DPL; k++) V[i][k] = 0.f;
-    if (n * DPL < hd) {
+    for (int k = 0; k < DPL; k += 4) {
+      const f32x4 v = *(const f32x4*)(at + k);
 #pragma unroll
-      for (int k = 0; k < DPL; k += 4) {
-        const f32x4 v = *(const f32x4*)(key + n * DPL + k);
-#pragma unroll
-        for (int e = 0; e < 4; e++) V[i][k + e] = v[e];
-      }
+      for (int e = 0; e < 4; e++) V[i][k + e] = v[e];
     }
   }
   __device__ __forceinline__ void zero_v(int, int i) {
 #pragma unroll
     for (int k = 0; k < DPL; k++) V[i][k] = 0.f;
   }
-  __device__ __forceinline__ bool all_finite() const {
-    uint32_t bad = 0;
+  __device__ __forceinline__ bool finite_v(int, int i) const {
+    bool ok = true;
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-#pragma unroll
-      for (int d = 0; d < DPL; d++) bad |= (uint32_t)((__float_as_uint(V[k][d]) & 0x7F800000u) == 0x7F800000u);
-    return !bad;
+    for (int d = 0; d < DPL; d++) ok = ok && (__float_as_uint(V[i][d]) & 0x7F800000u) != 0x7F800000u;
+    return ok;
   }
-  __device__ __forceinline__ void turn() {}
   template <class QF>
   __device__ __forceinline__ void scores(QF q, f32x4 (&S)[NJ]) const {
     // two independent chains, summed at the end
@@ -564,17 +561,6 @@ struct Tile32 {
 #pragma unroll
       for (int d = 0; d < DPL; d++) O[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[i][d], S[0][i], O[d], 0, 0, 0);
   }
-  template <class SEEN>
-  __device__ __forceinline__ void add_pv_seen(const f32x4 (&S)[NJ], f32x4 (&O)[DPL], SEEN seen, bool mine) const {
-#pragma unroll
-    for (int d = 0; d < DPL; d++) {
-      f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        o = __builtin_amdgcn_mfma_f32_16x16x4f32(seen(0, i) ? V[i][d] : 0.f, S[0][i], o, 0, 0, 0);
-      if (mine) O[d] += o;
-    }
-  }
 };
 
 struct AttArgs {
@@ -588,11 +574,15 @@ struct AttArgs {
   float* parts;        // a split's partial: O [columns][head dim], then (m, l) of each column
   uint32_t* counters;  // splits of a block that are done, by the index of its first partial; zero between calls
   uint64_t* err;
-  uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift, target;
+  uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift;
+  uint32_t rows_blk, heads_blk, groups;  // rows to a block of columns, heads of each, blocks to a row's heads
+  float per_target;                     // KV heads / items wanted
   float scale;
 };
 
-__device__ __forceinline__ uint32_t div_up(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
+// by divisors that are mostly 1
+__device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t b) { return b == 1 ? a : a / b; }
+__device__ __forceinline__ uint32_t div_up(uint32_t a, uint32_t b) { return b == 1 ? a : (a + b - 1) / b; }
 
 // a partial's words cross from one XCD's L2 to another's: written and read
 // through to the agent's coherence point
@@ -605,12 +595,19 @@ __device__ __forceinline__ float2 get2(const float* p) {
   return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-// Request b's first row, rows and length; no rows if they do not fit.
+// Request b's first row, rows and length; no rows if they do not fit, or if
+// row_start does not end in the rows there are.
 __device__ __forceinline__ void request(const AttArgs& a, uint32_t b, bool tell, uint32_t& r0, uint32_t& n, uint32_t& len) {
   int32_t s = (int32_t)b, e = s + 1;
   if (a.row_start) {
     s = a.row_start[b];
     e = a.row_start[b + 1];
+    const int32_t total = a.row_start[a.n_req];
+    if (total < 0 || (uint32_t)total > a.max_rows) {
+      if (tell && b == 0) paged_err(a.err, PAGED_ERR_ATT_ROWS, (uint32_t)total);
+      tell = false;
+      e = -1;
+    }
   }
   const int32_t l = a.lens[b];
   r0 = (uint32_t)s;
@@ -627,74 +624,61 @@ __device__ __forceinline__ void request(const AttArgs& a, uint32_t b, bool tell,
 
 #define MERGE_PAD 4  // floats between the columns of a wave's O in LDS
 
-template <class TILE, int DPL, int NT>
+template <class TILE, int DPL, int NT, bool SMALL>
 __device__ __forceinline__ void attention_body(const AttArgs& a) {
   typedef typename TILE::T T;
   constexpr int NJ = TILE::NJ, QREG = TILE::QREG;
   constexpr uint32_t TK = 16 * NJ, HDP = 16 * DPL, CB = 16 * NT;
   constexpr uint32_t OS = HDP + MERGE_PAD;
+  constexpr uint32_t QBYTES = NT * QREG * 64 * 16, OBYTES = 4 * 16 * OS * 4;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  float* s_o = (float*)lds;                 // [4 waves][16 columns][OS], or the splits' weights
-  float* s_ml = s_o + 4 * 16 * OS;          // [4 waves][16 columns][m, l]
-  u32x4* s_q = (u32x4*)(s_ml + 4 * 16 * 2);  // NT > 1: [NT][QREG][64 lanes]
-  uint32_t* s_item = (uint32_t*)(s_q + (NT > 1 ? NT * QREG * 64 : 0));  // [n_req + 1] first item of a request
-  uint32_t* s_part = s_item + a.n_req + 1;                              // [n_req] its first partial
-  __shared__ uint64_t s_sum[4];
+  u32x4* s_q = (u32x4*)lds;  // Q [NT][QREG][64 lanes], until the keys are through; then
+  float* s_o = (float*)lds;  // [4 waves][16 columns][OS], or the splits' weights
+  float* s_ml = (float*)(lds + (QBYTES > OBYTES ? QBYTES : OBYTES));  // [4 waves][16 columns][m, l]
+  uint32_t* s_item = (uint32_t*)(s_ml + 4 * 16 * 2);  // [n_req + 1] first item of a request
+  uint32_t* s_part = s_item + a.n_req + 1;            // its first partial
+  uint32_t* s_row = s_part + a.n_req + 1;             // its first row
+  uint32_t* s_len = s_row + a.n_req + 1;              // its length
+  __shared__ float s_sum[4];
   __shared__ uint32_t s_wave[4][2];
   __shared__ uint32_t s_last;
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t ln = lane & 15, lg = lane >> 4;
   const uint32_t P = 1u << a.shift, G = a.G, hd = a.hd;
-  const uint32_t gcols = G < CB ? G : CB, groups = div_up(G, CB), RB = CB / gcols;  // rows to a block
-  const bool first_wg = blockIdx.x == 0;
+  const uint32_t gcols = a.heads_blk, groups = a.groups, RB = a.rows_blk;
 
   // ---- the items of the call ----
-  if (a.row_start) {
-    const int32_t total = a.row_start[a.n_req];
-    if (total < 0 || (uint32_t)total > a.max_rows) {
-      if (first_wg && tid == 0) paged_err(a.err, PAGED_ERR_ATT_ROWS, (uint32_t)total);
-      return;
-    }
-  }
-  const uint32_t per = div_up(a.n_req, 256);
-  uint64_t work = 0;
+  const uint32_t per = (a.n_req + 255) / 256;
+  float work = 0.f;  // only a measure of how much there is: the cuts below hold for any
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
     if (b >= a.n_req) break;
     uint32_t r0, n, len;
-    request(a, b, first_wg, r0, n, len);
-    work += (uint64_t)(div_up(n, RB) * groups) * len;
+    request(a, b, blockIdx.x == 0, r0, n, len);
+    s_row[b] = r0;
+    s_len[b] = len;
+    s_item[b] = n;
+    work = __builtin_fmaf((float)(div_up(n, RB) * groups), (float)len, work);
   }
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) work += __shfl_xor(work, d);
+  work = sum64_lanes(work);
   if (lane == 0) s_sum[w] = work;
   __syncthreads();
-  work = (s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) * a.nKV;
-  const uint64_t c64 = (work + a.target - 1) / a.target;
-  const uint32_t C = c64 < PAGED_SPLIT_MIN ? PAGED_SPLIT_MIN : c64 > 0x40000000u ? 0x40000000u : (uint32_t)c64;
-  auto splits = [&](uint32_t len) {
-    const uint32_t s = (len + C / 2) / C;
+  work = ((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3])) * a.per_target;
+  const uint32_t C = (uint32_t)fminf(fmaxf(work, (float)PAGED_SPLIT_MIN), 1073741824.f);
+  const float inv_c = 1.0f / (float)C;
+  auto splits = [&](uint32_t len) {  // about len / C
+    const uint32_t s = (uint32_t)((float)len * inv_c + 0.5f);
     return s < 1 ? 1u : s > PAGED_SPLIT_MAX ? PAGED_SPLIT_MAX : s;
   };
   uint32_t items = 0, parts = 0;
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
     if (b >= a.n_req) break;
-    uint32_t r0, n, len;
-    request(a, b, false, r0, n, len);
-    const uint32_t ns = splits(len), it = div_up(n, RB) * groups * a.nKV * ns;
+    const uint32_t ns = splits(s_len[b]), it = div_up(s_item[b], RB) * groups * a.nKV * ns;
     items += it;
     parts += ns > 1 ? it : 0;
   }
-  uint32_t ii = items, ip = parts;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t x = __shfl_up(ii, d), y = __shfl_up(ip, d);
-    if (lane >= (uint32_t)d) {
-      ii += x;
-      ip += y;
-    }
-  }
+  uint32_t ii = scan64_lanes(items), ip = scan64_lanes(parts);
   if (lane == 63) {
     s_wave[w][0] = ii;
     s_wave[w][1] = ip;
@@ -711,36 +695,37 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
     }
     n_items += s_wave[k][0];
   }
+  if (blockIdx.x >= n_items) return;
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
     if (b >= a.n_req) break;
-    uint32_t r0, n, len;
-    request(a, b, false, r0, n, len);
-    const uint32_t ns = splits(len), it = div_up(n, RB) * groups * a.nKV * ns;
+    const uint32_t ns = splits(s_len[b]), n = s_item[b], it = div_up(n, RB) * groups * a.nKV * ns;
     s_item[b] = ii;
     s_part[b] = ip;
+    if (b + 1 == a.n_req) s_row[a.n_req] = s_row[b] + n;
     ii += it;
     ip += ns > 1 ? it : 0;
   }
-  if (tid == 0) s_item[a.n_req] = n_items;
   __syncthreads();
 
   for (uint32_t item = blockIdx.x; item < n_items; item += gridDim.x) {
+    // the last request that starts at or before the item (those without items start there too)
     uint32_t b = 0, top = a.n_req;
     while (top - b > 1) {
       const uint32_t mid = (b + top) >> 1;
       if (s_item[mid] <= item) b = mid;
       else top = mid;
     }
-    b = (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
-    uint32_t r0, n, len;
-    request(a, b, false, r0, n, len);
+    auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+    b = uniform(b);
+    const uint32_t r0 = uniform(s_row[b]), len = uniform(s_len[b]), local = item - uniform(s_item[b]);
+    const uint32_t n = a.row_start ? uniform(s_row[b + 1]) - r0 : 1u;
     const uint32_t ns = splits(len), nblk = div_up(n, RB) * groups;
-    const uint32_t local = item - s_item[b];
     // the KV head first (neighbouring blocks of a head meet in one XCD's L2 when
     // there are 8 of them), the blocks with the most keys before the others
-    const uint32_t kvh = local % a.nKV, rest = local / a.nKV, split = rest % ns, blk = nblk - 1 - rest / ns;
-    const uint32_t hg = blk % groups, row0 = blk / groups * RB;
+    const uint32_t rest = quotient(local, a.nKV), kvh = local - rest * a.nKV;
+    const uint32_t later = quotient(rest, ns), split = rest - later * ns, blk = nblk - 1 - later;
+    const uint32_t rowblk = quotient(blk, groups), hg = blk - rowblk * groups, row0 = rowblk * RB;
     const uint32_t rows = n - row0 < RB ? n - row0 : RB;
     const uint32_t gc = G - hg * CB < gcols ? G - hg * CB : gcols;  // heads of this block
     const uint32_t ncols = rows * gc;
@@ -752,101 +737,116 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
     const uint64_t at0 = (uint64_t)split * chunk;
     const uint32_t k0 = at0 < keys ? (uint32_t)at0 : keys, k1 = keys - k0 < chunk ? keys : k0 + chunk;
 
-    // ---- this lane's columns ----
-    u32x4 Q[QREG];
-    float c[NT];
-    uint32_t limit[NT];
-    const float sign = a.scale < 0.f ? -1.f : 1.f, mul = fabsf(a.scale) * 1.44269504088896340736f;
+    // ---- the block's columns ----
     auto column = [&](uint32_t col, uint32_t& row, uint32_t& head) {
-      row = col / gc;
-      head = kvh * G + hg * CB + col % gc;
+      row = quotient(col, gc);
+      head = kvh * G + hg * CB + col - row * gc;
     };
-    if (NT == 1) {
+    f32x4 q_raw[TILE::QRAW];
+    const uint32_t qcol = w * 16 + ln;  // tile w of the columns is wave w's to prepare
+    if (w < NT) {
       uint32_t row, head;
-      column(ln, row, head);
+      column(qcol < ncols ? qcol : 0, row, head);
+      TILE::load_q(a.q + (size_t)(r0 + row0 + row) * a.ld_q + head * hd, lg, hd, q_raw);
+    }
+
+    // ---- this wave's keys, a tile's loads in flight before it is needed ----
+    TILE tile;
+    const int32_t* table = a.tables + (size_t)b * a.max_pages;
+    const size_t head_len = (size_t)hd << a.shift;  // values of a page's KV head
+    uint32_t bad = 0;
+    auto page_of = [&](uint32_t t) {  // of key t < k1
+      const uint32_t p = (uint32_t)table[t >> a.shift];
+      bad |= (uint32_t)(p >= a.n_pages);
+      return p < a.n_pages ? p : 0u;
+    };
+    auto address = [&](uint32_t page, uint32_t t) {
+      return ((size_t)page * a.nKV + kvh) * head_len + (size_t)(t & (P - 1)) * hd;
+    };
+    // Keys from k1 on are loaded as others of their page, or as key k1 - 1.
+    // Pages of 16 keys and more: 16 keys at a multiple of 16 lie in one, whose
+    // address is the wave's; a lane holds the page of such 16 keys for the next
+    // AHEAD tiles of the wave (lane NJ x + j: tile x, its j-th 16).  Smaller pages:
+    // lane x holds key x's of the next tile.
+    constexpr uint32_t AHEAD = SMALL ? 1 : 64 / NJ;
+    uint32_t t0 = k0 + w * TK, pages = 0, tiles = 0;
+    auto load_pages = [&](uint32_t t) {
+      const uint32_t k = SMALL ? t + (lane & (TK - 1)) : t + lane / NJ * 4 * TK + lane % NJ * 16;
+      pages = page_of(k < k1 ? k : k1 - 1);
+    };
+    auto load_k = [&](uint32_t t) {
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        if constexpr (SMALL) {
+          const uint32_t x = 16 * j + ln, k = t + x < k1 ? t + x : k1 - 1;
+          tile.load_k(j, (const T*)a.kpages + address((uint32_t)__shfl((int)pages, (int)(k - t)), k), 0, lg, hd);
+        } else {
+          const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)(tiles * NJ + j));
+          tile.load_k(j, (const T*)a.kpages + address(p, t + 16 * j), ln * hd, lg, hd);
+        }
+      }
+    };
+    auto load_v = [&](uint32_t t) {
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        if constexpr (SMALL) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t x = 16 * j + 4 * lg + i, k = t + x < k1 ? t + x : k1 - 1;
+            tile.load_v(j, i, (const T*)a.vpages + address((uint32_t)__shfl((int)pages, (int)(k - t)), k), 0, ln, hd);
+          }
+        } else {
+          const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)(tiles * NJ + j));
+#pragma unroll
+          for (int i = 0; i < 4; i++) tile.load_v(j, i, (const T*)a.vpages + address(p, t + 16 * j), (4 * lg + i) * hd, ln, hd);
+        }
+      }
+    };
+    if (t0 < k1) {
+      load_pages(t0);
+      load_k(t0);
+      load_v(t0);
+    }
+
+    if (w < NT) {
       int e2;
-      TILE::load_q(a.q + (size_t)(r0 + row0 + row) * a.ld_q + head * hd, ln < ncols, lg, hd, sign, e2, Q);
-      c[0] = fmaxf(ldexpf(mul, -e2), 1.17549435e-38f);
-      limit[0] = least + row;
-    } else {
-      // tile w is this wave's to prepare
-      uint32_t row, head;
-      column(w * 16 + ln, row, head);
-      int e2;
-      TILE::load_q(a.q + (size_t)(r0 + row0 + row) * a.ld_q + head * hd, w * 16 + ln < ncols, lg, hd, sign, e2, Q);
+      u32x4 Q[QREG];
+      TILE::split_q(q_raw, qcol < ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2, Q);
 #pragma unroll
       for (int k = 0; k < QREG; k++) s_q[(w * QREG + k) * 64 + lane] = Q[k];
-      if (lg == 0) s_ml[w * 16 + ln] = fmaxf(ldexpf(mul, -e2), 1.17549435e-38f);
-      __syncthreads();
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        c[t] = s_ml[t * 16 + ln];
-        limit[t] = least + (t * 16 + ln) / gc;
-      }
+      // |scale| log2 e, without the power of two that q was multiplied by
+      if (lg == 0) s_ml[qcol] = fmaxf(__builtin_amdgcn_ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -e2), 1.17549435e-38f);
     }
+    __syncthreads();
     f32x4 O[NT][DPL];
-    float m[NT], l[NT];
+    float m[NT], l[NT], c[NT];
+    uint32_t limit[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
+      c[t] = s_ml[t * 16 + ln];
+      limit[t] = least + quotient(t * 16 + ln, gc);
       m[t] = -__builtin_inff();
       l[t] = 0.f;
 #pragma unroll
       for (int d = 0; d < DPL; d++) O[t][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
 
-    // ---- this wave's keys ----
-    const int32_t* table = a.tables + (size_t)b * a.max_pages;
-    const size_t head_len = (size_t)hd << a.shift;  // values of a page's KV head
-    auto page_of = [&](uint32_t t) {
-      uint32_t p = (uint32_t)table[t >> a.shift];
-      if (p >= a.n_pages) {
-        paged_err(a.err, PAGED_ERR_ATT_PAGE, b);
-        p = 0;
-      }
-      return p;
-    };
-    for (uint32_t t0 = k0 + w * TK; t0 < k1; t0 += 4 * TK) {
-      TILE tile;
-      if (a.shift >= 4) {
-        // 16 keys lie in one page: its address is the wave's
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-          const uint32_t tj = t0 + 16 * j < k1 ? t0 + 16 * j : t0;
-          const size_t at = ((size_t)page_of(tj) * a.nKV + kvh) * head_len + (size_t)(tj & (P - 1)) * hd;
-          const T *kp = (const T*)a.kpages + at, *vp = (const T*)a.vpages + at;
-          tile.load_k(j, kp + ln * hd, lg, hd);
-#pragma unroll
-          for (int i = 0; i < 4; i++) tile.load_v(j, i, vp + (4 * lg + i) * hd, ln, hd);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-          auto at = [&](uint32_t t) {
-            t = t < k1 ? t : k1 - 1;
-            return ((size_t)page_of(t) * a.nKV + kvh) * head_len + (size_t)(t & (P - 1)) * hd;
-          };
-          tile.load_k(j, (const T*)a.kpages + at(t0 + 16 * j + ln), lg, hd);
-#pragma unroll
-          for (int i = 0; i < 4; i++) tile.load_v(j, i, (const T*)a.vpages + at(t0 + 16 * j + 4 * lg + i), ln, hd);
-        }
-      }
-      const bool masked = t0 + TK > least || t0 + TK > k1;
-      bool apart = false;  // values that some columns must not touch, not even with a weight of 0
-      if (masked) {
-        // values behind the block's keys may be anything: their weight is 0, they must be finite
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (t0 + 16 * j + 4 * lg + i >= k1) tile.zero_v(j, i);
-      }
-      tile.turn();
-      if (masked && rows > 1) apart = __any(!tile.all_finite());
+    for (; t0 < k1; t0 += 4 * TK) {
+      const bool masked = t0 + TK > least || t0 + TK > k1, more = t0 + 4 * TK < k1;
+      uint32_t odd = 0;  // the lane's keys with a value that is not finite
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        if (t * 16 >= ncols) break;
+        if (t > 0 && t * 16 >= ncols) break;
         f32x4 S[NJ];
-        tile.scores([&](int k) { return NT > 1 ? s_q[(t * QREG + k) * 64 + lane] : Q[k]; }, S);
+        asm volatile("" ::: "memory");  // Q is read from LDS here, not kept in registers over the keys
+        tile.scores([&](int k) { return s_q[(t * QREG + k) * 64 + lane]; }, S);
+        if ((t + 1 == NT || (t + 1) * 16 >= ncols) && more) {
+          if (++tiles == AHEAD) {
+            tiles = 0;
+            load_pages(t0 + 4 * TK);
+          }
+          load_k(t0 + 4 * TK);
+        }
         if (masked) {
           const uint32_t end = limit[t] < k1 ? limit[t] : k1;
 #pragma unroll
@@ -860,8 +860,7 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
         for (int j = 0; j < NJ; j++)
 #pragma unroll
           for (int i = 0; i < 4; i++) x = fmaxf(x, S[j][i]);
-        x = fmaxf(x, __shfl_xor(x, 16));
-        x = fmaxf(x, __shfl_xor(x, 32)) * c[t];
+        x = max_xor16_32(x) * c[t];
         if (__any(x > m[t] + M_SLACK)) {
           const float mn = fmaxf(x, m[t]);
           const float f = mn == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[t] - mn);
@@ -878,17 +877,38 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
             S[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[j][i], c[t], shift));
             l[t] += S[j][i];
           }
-        if (!apart) {
-          tile.add_pv(S, O[t]);
-        } else {
-          // row by row, with the values that the row does not see at 0
-          const uint32_t last = t * 16 + 15 < ncols ? t * 16 + 15 : ncols - 1;
-          for (uint32_t row = t * 16 / gc; row <= last / gc; row++)
-            tile.add_pv_seen(S, O[t], [&](int j, int i) { return t0 + 16 * j + 4 * lg + i < least + row; },
-                             limit[t] == least + row);
+        if (masked) {
+          // a weight of 0 does not hide a value that is not finite: values behind
+          // the block's keys go to 0, and so do keys with such a value that only
+          // some rows see; those rows' sums take it up instead
+          if (t == 0) {
+            odd = 0;
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                bool hide = t0 + 16 * j + 4 * lg + i >= k1;
+                if (rows > 1) {
+                  const bool some = (__ballot(!hide && !tile.finite_v(j, i)) >> (16 * lg)) & 0xFFFFu;
+                  odd |= (uint32_t)some << (4 * j + i);
+                  hide |= some;
+                }
+                if (hide) tile.zero_v(j, i);
+              }
+          }
+          if (__any(odd)) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                if ((odd >> (4 * j + i) & 1) && t0 + 16 * j + 4 * lg + i < limit[t]) l[t] = __builtin_nanf("");
+          }
         }
+        tile.add_pv(S, O[t]);
       }
+      if (more) load_v(t0 + 4 * TK);
     }
+    if (bad) paged_err(a.err, PAGED_ERR_ATT_PAGE, b);
 
     // ---- join the waves, 16 columns at a time ----
     const uint32_t part = s_part[b] + local;  // of ns > 1; a split's are nKV apart
@@ -896,9 +916,9 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
     const uint32_t col = tid >> 4, d0 = (tid & 15) * DPL;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      if (t * 16 >= ncols) break;
+      if (t > 0 && t * 16 >= ncols) break;
       l[t] = add_xor32(add_xor16(l[t]));
-      __syncthreads();  // s_ml and s_o are free
+      __syncthreads();  // s_q, s_o and s_ml are free
       if (lg == 0) {
         s_ml[(w * 16 + ln) * 2] = m[t];
         s_ml[(w * 16 + ln) * 2 + 1] = l[t];
@@ -951,37 +971,51 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
         const float* all = a.parts + (size_t)first * CB * (hd + 2);
         if (tid == 0) __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         for (uint32_t c0 = 0; c0 < ncols; c0 += 16) {
-          // weights 2^(m - max) of the splits, 16 threads to a column
-          const uint32_t cc = c0 + (tid & 15), sp0 = tid >> 4;
+          // weights 2^(m - max) of the splits, 16 threads to a column; 0 behind the last
+          constexpr int PER = PAGED_SPLIT_MAX / 16;
+          const uint32_t cc = c0 + ln < ncols ? c0 + ln : 0, sp0 = tid >> 4;
+          const float* ml = all + CB * hd + cc * 2;
+          float2 v[PER];
           float mx = -__builtin_inff(), sum = 0.f;
-          if (cc < ncols)
-            for (uint32_t s = sp0; s < ns; s += 16) mx = fmaxf(mx, get2(all + s * stride + CB * hd + cc * 2).x);
-          mx = fmaxf(mx, __shfl_xor(mx, 16));
-          mx = fmaxf(mx, __shfl_xor(mx, 32));
+#pragma unroll
+          for (int k = 0; k < PER; k++) v[k] = get2(ml + (sp0 + 16 * k < ns ? sp0 + 16 * k : 0u) * stride);
+#pragma unroll
+          for (int k = 0; k < PER; k++) {
+            if (sp0 + 16 * k >= ns) v[k] = make_float2(-__builtin_inff(), 0.f);
+            mx = fmaxf(mx, v[k].x);
+          }
+          mx = max_xor16_32(mx);
           __syncthreads();
           if (lg == 0) s_ml[w * 16 + ln] = mx;
           __syncthreads();
           mx = fmaxf(fmaxf(s_ml[ln], s_ml[16 + ln]), fmaxf(s_ml[32 + ln], s_ml[48 + ln]));
-          if (cc < ncols)
-            for (uint32_t s = sp0; s < ns; s += 16) {
-              const float2 v = get2(all + s * stride + CB * hd + cc * 2);
-              const float f = v.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(v.x - mx);
-              s_o[s * 16 + ln] = f;
-              sum = __builtin_fmaf(f, v.y, sum);
-            }
+#pragma unroll
+          for (int k = 0; k < PER; k++) {
+            const float f = v[k].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(v[k].x - mx);
+            s_o[(sp0 + 16 * k) * 16 + ln] = f;
+            sum = __builtin_fmaf(f, v[k].y, sum);
+          }
           sum = add_xor32(add_xor16(sum));
-          __syncthreads();
           if (lg == 0) s_ml[64 + w * 16 + ln] = sum;
           __syncthreads();
+          // a thread's pair of dims over the splits, JOIN_BATCH loads in flight;
+          // behind the last split it again, with a weight of 0
+          constexpr uint32_t JOIN_BATCH = 16;
           const uint32_t nc = ncols - c0 < 16 ? ncols - c0 : 16;
           for (uint32_t e = 2 * tid; e < nc * hd; e += 512) {
             const uint32_t k = e / hd, d = e % hd;
+            const float* src = all + c0 * hd + e;
             float2 o = make_float2(0.f, 0.f);
-#pragma unroll 8
-            for (uint32_t s = 0; s < ns; s++) {
-              const float2 v = get2(all + s * stride + c0 * hd + e);
-              o.x = __builtin_fmaf(s_o[s * 16 + k], v.x, o.x);
-              o.y = __builtin_fmaf(s_o[s * 16 + k], v.y, o.y);
+            for (uint32_t s0 = 0; s0 < ns; s0 += JOIN_BATCH) {
+              float2 x[JOIN_BATCH];
+#pragma unroll
+              for (uint32_t s = 0; s < JOIN_BATCH; s++) x[s] = get2(src + (s0 + s < ns ? s0 + s : ns - 1) * stride);
+#pragma unroll
+              for (uint32_t s = 0; s < JOIN_BATCH; s++) {
+                const float f = s_o[(s0 + s) * 16 + k];
+                o.x = __builtin_fmaf(f, x[s].x, o.x);
+                o.y = __builtin_fmaf(f, x[s].y, o.y);
+              }
             }
             const float tot = s_ml[64 + k] + s_ml[80 + k] + s_ml[96 + k] + s_ml[112 + k];
             uint32_t row, head;
@@ -997,19 +1031,22 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
   }
 }
 
-#define DEF_ATTENTION(NAME, TILE, DPL, NT)                                                         \
-  extern "C" __global__ __launch_bounds__(256, 2) void NAME(AttArgs a) {                           \
-    attention_body<TILE, DPL, NT>(a);                                                              \
+#define DEF_ATTENTION(NAME, DPL, NT, SMALL, ...)                                       \
+  extern "C" __global__ __launch_bounds__(256, 2) void NAME(AttArgs a) { \
+    attention_body<__VA_ARGS__, DPL, NT, SMALL>(a);                                    \
   }
-#define COMMA ,
-// named by page type, head dims held (64 or 128) and tiles of 16 columns to a workgroup
-DEF_ATTENTION(smith_paged_attention_f32_d64_t1, Tile32<4>, 4, 1)
-DEF_ATTENTION(smith_paged_attention_f32_d128_t1, Tile32<8>, 8, 1)
-DEF_ATTENTION(smith_paged_attention_f16_d64_t1, Tile16<MmF16 COMMA 4>, 4, 1)
-DEF_ATTENTION(smith_paged_attention_f16_d128_t1, Tile16<MmF16 COMMA 8>, 8, 1)
-DEF_ATTENTION(smith_paged_attention_f16_d64_t4, Tile16<MmF16 COMMA 4>, 4, 4)
-DEF_ATTENTION(smith_paged_attention_f16_d128_t4, Tile16<MmF16 COMMA 8>, 8, 4)
-DEF_ATTENTION(smith_paged_attention_bf16_d64_t1, Tile16<MmBf16 COMMA 4>, 4, 1)
-DEF_ATTENTION(smith_paged_attention_bf16_d128_t1, Tile16<MmBf16 COMMA 8>, 8, 1)
-DEF_ATTENTION(smith_paged_attention_bf16_d64_t4, Tile16<MmBf16 COMMA 4>, 4, 4)
-DEF_ATTENTION(smith_paged_attention_bf16_d128_t4, Tile16<MmBf16 COMMA 8>, 8, 4)
+// named by page type, head dims held (64 or 128) and tiles of 16 columns to a
+// workgroup; _s for pages of less than 16 keys
+#define DEF_ATTENTIONS(TYPE, D, DPL, ...)                                           \
+  DEF_ATTENTION(smith_paged_attention_##TYPE##_d##D##_t1, DPL, 1, false, __VA_ARGS__) \
+  DEF_ATTENTION(smith_paged_attention_##TYPE##_d##D##_t1_s, DPL, 1, true, __VA_ARGS__)
+DEF_ATTENTIONS(f32, 64, 4, Tile32<4>)
+DEF_ATTENTIONS(f32, 128, 8, Tile32<8>)
+DEF_ATTENTIONS(f16, 64, 4, Tile16<MmF16, 4>)
+DEF_ATTENTIONS(f16, 128, 8, Tile16<MmF16, 8>)
+DEF_ATTENTIONS(bf16, 64, 4, Tile16<MmBf16, 4>)
+DEF_ATTENTIONS(bf16, 128, 8, Tile16<MmBf16, 8>)
+DEF_ATTENTION(smith_paged_attention_f16_d64_t4, 4, 4, false, Tile16<MmF16, 4>)
+DEF_ATTENTION(smith_paged_attention_f16_d128_t4, 8, 4, false, Tile16<MmF16, 8>)
+DEF_ATTENTION(smith_paged_attention_bf16_d64_t4, 4, 4, false, Tile16<MmBf16, 4>)
+DEF_ATTENTION(smith_paged_attention_bf16_d128_t4, 8, 4, false, Tile16<MmBf16, 8>)

@@ -2394,11 +2394,8 @@ int smith_paged_append(void* ctx, uint32_t kv_type, const float* qkv, uint32_t l
   if (set_device(c)) return -1;
   uint32_t n_slots = n_pages << shift;
   uint64_t* perr = c->paged_err_dev();
-  // 16-byte accesses where every row and table starts on 16 bytes
-  const bool vec = (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)rope_cos | (uintptr_t)rope_sin) % 16) == 0 &&
-                   ld % 4 == 0 && ld_q % 4 == 0;
   char name[48];
-  snprintf(name, sizeof name, "smith_paged_append_%s%s", kv_name(kv_type), vec ? "" : "_u");
+  snprintf(name, sizeof name, "smith_paged_append_%s", kv_name(kv_type));
   const uint32_t items = (uint32_t)((Wq + 2 * Wk) / 8);
   // rows along the grid's second axis, which ends at 65535
   for (uint32_t r0 = 0; r0 < rows; r0 += 65535) {
@@ -2443,21 +2440,24 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   // tiles of 16 columns (row, head) to a workgroup: one where requests bring a
   // row or so each (the keys are read once, columns hardly matter), four where
   // they fill more than two; the f32 matrix cores are the bound at one already
+  // (and pages of less than 16 keys, looked up key by key, have no other kernel)
   const uint32_t G = n_heads / n_kv_heads;
-  const uint32_t tiles = row_start && kv_type != SMITH_KV_F32 && (uint64_t)max_rows * G > 32ull * n_req ? 4 : 1;
+  const bool small = shift < 4;
+  const uint32_t tiles =
+      row_start && kv_type != SMITH_KV_F32 && !small && (uint64_t)max_rows * G > 32ull * n_req ? 4 : 1;
   const uint32_t CB = 16 * tiles, dims = head_dim <= 64 ? 64 : 128;
   const uint32_t target = tiles == 1 ? 1024 : 512;
-  // splits have at least 1.5 C keys between two of them, so there are fewer
-  // than 4/3 W / C of those that leave a partial
-  const uint32_t max_parts = target + target / 3 + 1;
+  // a block that is cut has 1.5 C keys or more and so at most 4/3 of its keys / C
+  // splits: 4/3 W / C <= 4/3 target of them in all (and some for what f32 rounds)
+  const uint32_t max_parts = target + target / 3 + 16;
   if (ensure(c, &c->paged_ws, &c->paged_ws_bytes, (size_t)max_parts * CB * (head_dim + 2) * sizeof(float))) return -1;
   if (ensure_paged_counters(c)) return -1;
-  const uint64_t RB = CB / std::min(G, CB), groups = (G + CB - 1) / CB;
-  const uint64_t blocks = groups * n_kv_heads * (row_start ? n_req + max_rows / RB : n_req);
+  const uint32_t heads_blk = std::min(G, CB), RB = CB / heads_blk, groups = (G + CB - 1) / CB;
+  const uint64_t blocks = (uint64_t)groups * n_kv_heads * (row_start ? (uint64_t)n_req + max_rows / RB : n_req);
   const uint64_t longest = ((uint64_t)max_pages << shift) / PAGED_SPLIT_MIN + 1;  // splits of one block
   const uint32_t grid = (uint32_t)std::min<uint64_t>({(uint64_t)target, blocks + max_parts, blocks * longest});
   const uint32_t qreg = kv_type == SMITH_KV_F32 ? dims / 16 : dims / 32 * (kv_type == SMITH_KV_F16 ? 2 : 3);
-  const uint32_t lds = 4 * (4 * 16 * (dims + 4) + 4 * 16 * 2) + (tiles > 1 ? tiles * qreg * 64 * 16 : 0) + 4 * (2 * n_req + 1);
+  const uint32_t lds = std::max<uint32_t>(4 * 16 * (dims + 4) * 4, tiles * qreg * 64 * 16) + 4 * 16 * 2 * 4 + 16 * (n_req + 1);
   struct {
     const float* q;
     const int32_t *row_start, *lens, *tables;
@@ -2465,12 +2465,13 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
     float *out, *parts;
     uint32_t* counters;
     uint64_t* err;
-    uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift, target;
-    float scale;
+    uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift, rows_blk, heads_blk, groups;
+    float per_target, scale;
   } a = {q, row_start, lens, tables, kpages, vpages, out, (float*)c->paged_ws, c->paged_cnt, c->paged_err_dev(),
-         ld_q, ld_out, max_rows, n_req, max_pages, n_kv_heads, G, head_dim, n_pages, shift, target, scale};
+         ld_q, ld_out, max_rows, n_req, max_pages, n_kv_heads, G, head_dim, n_pages, shift, RB, heads_blk, groups,
+         (float)n_kv_heads / (float)target, scale};
   char name[64];
-  snprintf(name, sizeof name, "smith_paged_attention_%s_d%u_t%u", kv_name(kv_type), dims, tiles);
+  snprintf(name, sizeof name, "smith_paged_attention_%s_d%u_t%u%s", kv_name(kv_type), dims, tiles, small ? "_s" : "");
   void* args[] = {&a};
   return launch(c, name, dim3(grid), dim3(256), args, lds);
 }

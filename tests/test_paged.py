@@ -14,9 +14,9 @@ def test_code_object_has_kernels():
     out = subprocess.run(["/opt/rocm/llvm/bin/llvm-readelf", "--syms", device.PAGED_CODE_OBJECT_PATH],
                          capture_output=True, text=True, check=True).stdout
     need = ["smith_paged_plan"]
-    need += ["smith_paged_append_%s%s" % (t, u) for t in ("f32", "f16", "bf16") for u in ("", "_u")]
-    need += ["smith_paged_attention_%s_d%d_t%d" % (t, d, n) for t in ("f32", "f16", "bf16") for d in (64, 128)
-             for n in (1, 4) if t != "f32" or n == 1]
+    need += ["smith_paged_append_%s" % t for t in ("f32", "f16", "bf16")]
+    need += ["smith_paged_attention_%s_d%d_%s" % (t, d, n) for t in ("f32", "f16", "bf16") for d in (64, 128)
+             for n in ("t1", "t1_s", "t4") if t != "f32" or n != "t4"]
     for k in need:
         assert re.search(r"\b%s\.kd\b" % k, out), k
 
