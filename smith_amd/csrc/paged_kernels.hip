@@ -622,59 +622,48 @@ __device__ __forceinline__ void request(const AttArgs& a, uint32_t b, bool tell,
   }
 }
 
-#define MERGE_PAD 4  // floats between the columns of a wave's O in LDS
+// The items of a call, by the prefix sums that each workgroup forms in LDS.
+struct Items {
+  uint32_t *item, *part, *row, *len;  // [n_req + 1] of a request: its first item and partial, its first row, its length
+  uint32_t total;
+  float inv_c;
 
-template <class TILE, int DPL, int NT, bool SMALL>
-__device__ __forceinline__ void attention_body(const AttArgs& a) {
-  typedef typename TILE::T T;
-  constexpr int NJ = TILE::NJ, QREG = TILE::QREG;
-  constexpr uint32_t TK = 16 * NJ, HDP = 16 * DPL, CB = 16 * NT;
-  constexpr uint32_t OS = HDP + MERGE_PAD;
-  constexpr uint32_t QBYTES = NT * QREG * 64 * 16, OBYTES = 4 * 16 * OS * 4;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  u32x4* s_q = (u32x4*)lds;  // Q [NT][QREG][64 lanes], until the keys are through; then
-  float* s_o = (float*)lds;  // [4 waves][16 columns][OS], or the splits' weights
-  float* s_ml = (float*)(lds + (QBYTES > OBYTES ? QBYTES : OBYTES));  // [4 waves][16 columns][m, l]
-  uint32_t* s_item = (uint32_t*)(s_ml + 4 * 16 * 2);  // [n_req + 1] first item of a request
-  uint32_t* s_part = s_item + a.n_req + 1;            // its first partial
-  uint32_t* s_row = s_part + a.n_req + 1;             // its first row
-  uint32_t* s_len = s_row + a.n_req + 1;              // its length
+  __device__ __forceinline__ uint32_t splits(uint32_t keys) const {  // about keys / C
+    const uint32_t s = (uint32_t)((float)keys * inv_c + 0.5f);
+    return s < 1 ? 1u : s > PAGED_SPLIT_MAX ? PAGED_SPLIT_MAX : s;
+  }
+};
+
+__device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Items& t) {
+  t.item = lds;
+  t.part = t.item + a.n_req + 1;
+  t.row = t.part + a.n_req + 1;
+  t.len = t.row + a.n_req + 1;
   __shared__ float s_sum[4];
   __shared__ uint32_t s_wave[4][2];
-  __shared__ uint32_t s_last;
-  const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
-  const uint32_t ln = lane & 15, lg = lane >> 4;
-  const uint32_t P = 1u << a.shift, G = a.G, hd = a.hd;
-  const uint32_t gcols = a.heads_blk, groups = a.groups, RB = a.rows_blk;
-
-  // ---- the items of the call ----
+  const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6, RB = a.rows_blk, groups = a.groups;
   const uint32_t per = (a.n_req + 255) / 256;
-  float work = 0.f;  // only a measure of how much there is: the cuts below hold for any
+  float work = 0.f;  // only a measure of how much there is: the cuts hold for any
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
     if (b >= a.n_req) break;
     uint32_t r0, n, len;
     request(a, b, blockIdx.x == 0, r0, n, len);
-    s_row[b] = r0;
-    s_len[b] = len;
-    s_item[b] = n;
+    t.row[b] = r0;
+    t.len[b] = len;
+    t.item[b] = n;
     work = __builtin_fmaf((float)(div_up(n, RB) * groups), (float)len, work);
   }
   work = sum64_lanes(work);
   if (lane == 0) s_sum[w] = work;
   __syncthreads();
   work = ((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3])) * a.per_target;
-  const uint32_t C = (uint32_t)fminf(fmaxf(work, (float)PAGED_SPLIT_MIN), 1073741824.f);
-  const float inv_c = 1.0f / (float)C;
-  auto splits = [&](uint32_t len) {  // about len / C
-    const uint32_t s = (uint32_t)((float)len * inv_c + 0.5f);
-    return s < 1 ? 1u : s > PAGED_SPLIT_MAX ? PAGED_SPLIT_MAX : s;
-  };
+  t.inv_c = 1.0f / fmaxf(work, (float)PAGED_SPLIT_MIN);
   uint32_t items = 0, parts = 0;
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
     if (b >= a.n_req) break;
-    const uint32_t ns = splits(s_len[b]), it = div_up(s_item[b], RB) * groups * a.nKV * ns;
+    const uint32_t ns = t.splits(t.len[b]), it = div_up(t.item[b], RB) * groups * a.nKV * ns;
     items += it;
     parts += ns > 1 ? it : 0;
   }
@@ -684,7 +673,7 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
     s_wave[w][1] = ip;
   }
   __syncthreads();
-  uint32_t n_items = 0;
+  t.total = 0;
   ii -= items;
   ip -= parts;
 #pragma unroll
@@ -693,66 +682,209 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
       ii += s_wave[k][0];
       ip += s_wave[k][1];
     }
-    n_items += s_wave[k][0];
+    t.total += s_wave[k][0];
   }
-  if (blockIdx.x >= n_items) return;
+  if (blockIdx.x >= t.total) return;
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
     if (b >= a.n_req) break;
-    const uint32_t ns = splits(s_len[b]), n = s_item[b], it = div_up(n, RB) * groups * a.nKV * ns;
-    s_item[b] = ii;
-    s_part[b] = ip;
-    if (b + 1 == a.n_req) s_row[a.n_req] = s_row[b] + n;
+    const uint32_t ns = t.splits(t.len[b]), n = t.item[b], it = div_up(n, RB) * groups * a.nKV * ns;
+    t.item[b] = ii;
+    t.part[b] = ip;
+    if (b + 1 == a.n_req) t.row[a.n_req] = t.row[b] + n;
     ii += it;
     ip += ns > 1 ? it : 0;
   }
   __syncthreads();
+}
 
-  for (uint32_t item = blockIdx.x; item < n_items; item += gridDim.x) {
+// One item, the same in all lanes: columns (row, head) of a request, numbered
+// row by row, and the keys k0 .. k1 - 1 of those that they see.
+struct Item {
+  uint32_t b, r0, n, len, kvh, split, ns, row0, rows, head0, heads, ncols;
+  uint32_t keys, least;  // keys that the block's last and first row see
+  uint32_t k0, k1;
+  uint32_t part;  // of ns > 1: its partial; a block's next split has the one nKV further on
+
+  __device__ __forceinline__ Item(const AttArgs& a, const Items& t, uint32_t item, uint32_t CB, uint32_t unit) {
     // the last request that starts at or before the item (those without items start there too)
-    uint32_t b = 0, top = a.n_req;
-    while (top - b > 1) {
-      const uint32_t mid = (b + top) >> 1;
-      if (s_item[mid] <= item) b = mid;
+    uint32_t lo = 0, top = a.n_req;
+    while (top - lo > 1) {
+      const uint32_t mid = (lo + top) >> 1;
+      if (t.item[mid] <= item) lo = mid;
       else top = mid;
     }
     auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
-    b = uniform(b);
-    const uint32_t r0 = uniform(s_row[b]), len = uniform(s_len[b]), local = item - uniform(s_item[b]);
-    const uint32_t n = a.row_start ? uniform(s_row[b + 1]) - r0 : 1u;
-    const uint32_t ns = splits(len), nblk = div_up(n, RB) * groups;
+    b = uniform(lo);
+    r0 = uniform(t.row[b]);
+    len = uniform(t.len[b]);
+    const uint32_t local = item - uniform(t.item[b]);
+    part = uniform(t.part[b]) + local;
+    n = a.row_start ? uniform(t.row[b + 1]) - r0 : 1u;
+    ns = t.splits(len);
     // the KV head first (neighbouring blocks of a head meet in one XCD's L2 when
     // there are 8 of them), the blocks with the most keys before the others
-    const uint32_t rest = quotient(local, a.nKV), kvh = local - rest * a.nKV;
-    const uint32_t later = quotient(rest, ns), split = rest - later * ns, blk = nblk - 1 - later;
-    const uint32_t rowblk = quotient(blk, groups), hg = blk - rowblk * groups, row0 = rowblk * RB;
-    const uint32_t rows = n - row0 < RB ? n - row0 : RB;
-    const uint32_t gc = G - hg * CB < gcols ? G - hg * CB : gcols;  // heads of this block
-    const uint32_t ncols = rows * gc;
-    // keys: row i of the request sees base + i + 1 of them
-    const uint32_t base = len - n;  // a lone row without keys: -1
-    const uint32_t keys = base + row0 + rows;
-    const uint32_t least = base + row0 + 1;  // what the block's first row sees
-    const uint32_t chunk = ns > 1 ? div_up(div_up(keys, ns), TK) * TK : keys;
-    const uint64_t at0 = (uint64_t)split * chunk;
-    const uint32_t k0 = at0 < keys ? (uint32_t)at0 : keys, k1 = keys - k0 < chunk ? keys : k0 + chunk;
+    const uint32_t rest = quotient(local, a.nKV), later = quotient(rest, ns);
+    kvh = local - rest * a.nKV;
+    split = rest - later * ns;
+    const uint32_t blk = div_up(n, a.rows_blk) * a.groups - 1 - later, rowblk = quotient(blk, a.groups);
+    head0 = (blk - rowblk * a.groups) * CB;
+    heads = a.G - head0 < a.heads_blk ? a.G - head0 : a.heads_blk;
+    head0 += kvh * a.G;
+    row0 = rowblk * a.rows_blk;
+    rows = n - row0 < a.rows_blk ? n - row0 : a.rows_blk;
+    ncols = rows * heads;
+    // row i of the request sees len - n + i + 1 keys (a lone row without keys none)
+    keys = len - n + row0 + rows;
+    least = len - n + row0 + 1;
+    const uint32_t chunk = ns > 1 ? (div_up(keys, ns) + unit - 1) / unit * unit : keys;
+    const uint64_t at = (uint64_t)split * chunk;
+    k0 = at < keys ? (uint32_t)at : keys;
+    k1 = keys - k0 < chunk ? keys : k0 + chunk;
+  }
+  __device__ __forceinline__ uint32_t row_of(uint32_t col) const { return quotient(col, heads); }
+  // element 0 of a column in q or out
+  __device__ __forceinline__ size_t at(uint32_t col, uint32_t ld, uint32_t hd) const {
+    const uint32_t row = row_of(col);
+    return (size_t)(r0 + row0 + row) * ld + (head0 + col - row * heads) * hd;
+  }
+};
 
-    // ---- the block's columns ----
-    auto column = [&](uint32_t col, uint32_t& row, uint32_t& head) {
-      row = quotient(col, gc);
-      head = kvh * G + hg * CB + col - row * gc;
-    };
-    f32x4 q_raw[TILE::QRAW];
-    const uint32_t qcol = w * 16 + ln;  // tile w of the columns is wave w's to prepare
-    if (w < NT) {
-      uint32_t row, head;
-      column(qcol < ncols ? qcol : 0, row, head);
-      TILE::load_q(a.q + (size_t)(r0 + row0 + row) * a.ld_q + head * hd, lg, hd, q_raw);
+// A split is through: its partial [CB][hd] and (m, l) [CB] are written (by all
+// of the workgroup); the last split of the block joins them.  s: LDS of
+// PAGED_SPLIT_MAX * 16 + 128 floats that nobody uses any more.
+__device__ __forceinline__ void join_splits(const AttArgs& a, const Item& I, uint32_t CB, float* s) {
+  __shared__ uint32_t s_last;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6, ln = lane & 15, lg = lane >> 4;
+  const uint32_t hd = a.hd, ns = I.ns, ncols = I.ncols, first = I.part - I.split * a.nKV;
+  float *s_o = s, *s_ml = s + PAGED_SPLIT_MAX * 16;
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (tid == 0)
+    s_last = __hip_atomic_fetch_add(a.counters + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ns - 1;
+  __syncthreads();
+  if (!s_last) return;
+  const float* all = a.parts + (size_t)first * CB * (hd + 2);
+  const size_t stride = (size_t)a.nKV * CB * (hd + 2);
+  if (tid == 0) __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (uint32_t c0 = 0; c0 < ncols; c0 += 16) {
+    // weights 2^(m - max) of the splits, 16 threads to a column; 0 behind the last
+    constexpr int PER = PAGED_SPLIT_MAX / 16;
+    const uint32_t cc = c0 + ln < ncols ? c0 + ln : 0, sp0 = tid >> 4;
+    const float* ml = all + CB * hd + cc * 2;
+    float2 v[PER];
+    float mx = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < PER; k++) v[k] = get2(ml + (sp0 + 16 * k < ns ? sp0 + 16 * k : 0u) * stride);
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      if (sp0 + 16 * k >= ns) v[k] = make_float2(-__builtin_inff(), 0.f);
+      mx = fmaxf(mx, v[k].x);
     }
+    mx = max_xor16_32(mx);
+    __syncthreads();
+    if (lg == 0) s_ml[w * 16 + ln] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(s_ml[ln], s_ml[16 + ln]), fmaxf(s_ml[32 + ln], s_ml[48 + ln]));
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const float f = v[k].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(v[k].x - mx);
+      s_o[(sp0 + 16 * k) * 16 + ln] = f;
+      sum = __builtin_fmaf(f, v[k].y, sum);
+    }
+    sum = add_xor32(add_xor16(sum));
+    if (lg == 0) s_ml[64 + w * 16 + ln] = sum;
+    __syncthreads();
+    // a thread's pair of dims over the splits, JOIN_BATCH loads in flight;
+    // behind the last split it again, with a weight of 0
+    constexpr uint32_t JOIN_BATCH = 16;
+    const uint32_t nc = ncols - c0 < 16 ? ncols - c0 : 16;
+    for (uint32_t e = 2 * tid; e < nc * hd; e += 512) {
+      const uint32_t k = e / hd, d = e - k * hd;
+      const float* src = all + c0 * hd + e;
+      float2 o = make_float2(0.f, 0.f);
+      for (uint32_t s0 = 0; s0 < ns; s0 += JOIN_BATCH) {
+        float2 x[JOIN_BATCH];
+#pragma unroll
+        for (uint32_t j = 0; j < JOIN_BATCH; j++) x[j] = get2(src + (s0 + j < ns ? s0 + j : ns - 1) * stride);
+#pragma unroll
+        for (uint32_t j = 0; j < JOIN_BATCH; j++) {
+          const float f = s_o[(s0 + j) * 16 + k];
+          o.x = __builtin_fmaf(f, x[j].x, o.x);
+          o.y = __builtin_fmaf(f, x[j].y, o.y);
+        }
+      }
+      const float tot = s_ml[64 + k] + s_ml[80 + k] + s_ml[96 + k] + s_ml[112 + k];
+      float* y = a.out + I.at(c0 + k, a.ld_out, hd) + d;
+      y[0] = o.x / tot;
+      y[1] = o.y / tot;
+    }
+  }
+}
+
+#define MERGE_PAD 4  // floats between the columns of a wave's O in LDS
+
+// |scale| log2 e without the power of two that q was multiplied by, never 0
+__device__ __forceinline__ float score_factor(float scale, int e2) {
+  return fmaxf(__builtin_amdgcn_ldexpf(fabsf(scale) * 1.44269504088896340736f, -e2), 1.17549435e-38f);
+}
+
+// Scores of one column (times c: in powers of two) into weights 2^(score - m +
+// P_EXP), with the column's running maximum m, sum l (this lane's share) and O.
+template <int NJ, int DPL>
+__device__ __forceinline__ void weigh(f32x4 (&S)[NJ], float c, float& m, float& l, f32x4 (&O)[DPL]) {
+  float x = -__builtin_inff();
+#pragma unroll
+  for (int j = 0; j < NJ; j++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) x = fmaxf(x, S[j][i]);
+  x = max_xor16_32(x) * c;
+  if (__any(x > m + M_SLACK)) {
+    const float mn = fmaxf(x, m);
+    const float f = mn == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= f;
+#pragma unroll
+    for (int d = 0; d < DPL; d++) O[d] *= f;
+  }
+  const float shift = m == -__builtin_inff() ? 0.f : P_EXP - m;
+#pragma unroll
+  for (int j = 0; j < NJ; j++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      S[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[j][i], c, shift));
+      l += S[j][i];
+    }
+}
+
+// One tile of 16 columns to a workgroup, its keys in registers.
+template <class TILE, int DPL, bool SMALL>
+__device__ __forceinline__ void attention_body(const AttArgs& a) {
+  typedef typename TILE::T T;
+  constexpr int NJ = TILE::NJ, QREG = TILE::QREG;
+  constexpr uint32_t TK = 16 * NJ, HDP = 16 * DPL, CB = 16;
+  constexpr uint32_t OS = HDP + MERGE_PAD;
+  constexpr uint32_t OFLOATS = 4 * 16 * OS;
+  static_assert(QREG * 64 * 4 <= OFLOATS && PAGED_SPLIT_MAX * 16 + 128 <= OFLOATS, "Q, and the weights of a join, fit where O does");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  u32x4* s_q = (u32x4*)lds;  // Q [QREG][64 lanes], until the keys are through; then
+  float* s_o = (float*)lds;  // [4 waves][16 columns][OS]
+  float* s_ml = s_o + OFLOATS;  // [4 waves][16 columns][m, l]
+  const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  const uint32_t ln = lane & 15, lg = lane >> 4;
+  const uint32_t P = 1u << a.shift, hd = a.hd;
+  Items items;
+  find_items(a, (uint32_t*)(s_ml + 4 * 16 * 2), items);
+
+  for (uint32_t item = blockIdx.x; item < items.total; item += gridDim.x) {
+    const Item I(a, items, item, CB, TK);
+    const uint32_t k0 = I.k0, k1 = I.k1, kvh = I.kvh;
+    f32x4 q_raw[TILE::QRAW];
+    if (w == 0) TILE::load_q(a.q + I.at(ln < I.ncols ? ln : 0, a.ld_q, hd), lg, hd, q_raw);
 
     // ---- this wave's keys, a tile's loads in flight before it is needed ----
     TILE tile;
-    const int32_t* table = a.tables + (size_t)b * a.max_pages;
+    const int32_t* table = a.tables + (size_t)I.b * a.max_pages;
     const size_t head_len = (size_t)hd << a.shift;  // values of a page's KV head
     uint32_t bad = 0;
     auto page_of = [&](uint32_t t) {  // of key t < k1
@@ -808,245 +940,438 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
       load_v(t0);
     }
 
-    if (w < NT) {
+    if (w == 0) {
       int e2;
       u32x4 Q[QREG];
-      TILE::split_q(q_raw, qcol < ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2, Q);
+      TILE::split_q(q_raw, ln < I.ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2, Q);
 #pragma unroll
-      for (int k = 0; k < QREG; k++) s_q[(w * QREG + k) * 64 + lane] = Q[k];
-      // |scale| log2 e, without the power of two that q was multiplied by
-      if (lg == 0) s_ml[qcol] = fmaxf(__builtin_amdgcn_ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -e2), 1.17549435e-38f);
+      for (int k = 0; k < QREG; k++) s_q[k * 64 + lane] = Q[k];
+      if (lg == 0) s_ml[ln] = score_factor(a.scale, e2);
     }
     __syncthreads();
-    f32x4 O[NT][DPL];
-    float m[NT], l[NT], c[NT];
-    uint32_t limit[NT];
+    const float c = s_ml[ln];
+    const uint32_t limit = I.least + I.row_of(ln);
+    f32x4 O[DPL];
+    float m = -__builtin_inff(), l = 0.f;
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-      c[t] = s_ml[t * 16 + ln];
-      limit[t] = least + quotient(t * 16 + ln, gc);
+    for (int d = 0; d < DPL; d++) O[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    for (; t0 < k1; t0 += 4 * TK) {
+      const bool masked = t0 + TK > I.least || t0 + TK > k1, more = t0 + 4 * TK < k1;
+      f32x4 S[NJ];
+      asm volatile("" ::: "memory");  // Q is read from LDS here, not kept in registers over the keys
+      tile.scores([&](int k) { return s_q[k * 64 + lane]; }, S);
+      if (more) {
+        if (++tiles == AHEAD) {
+          tiles = 0;
+          load_pages(t0 + 4 * TK);
+        }
+        load_k(t0 + 4 * TK);
+      }
+      if (masked) {
+        const uint32_t end = limit < k1 ? limit : k1;
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (t0 + 16 * j + 4 * lg + i >= end) S[j][i] = -__builtin_inff();
+      }
+      weigh<NJ, DPL>(S, c, m, l, O);
+      if (masked) {
+        // a weight of 0 does not hide a value that is not finite: values behind
+        // the block's keys go to 0, and so do keys with such a value that only
+        // some rows see; those rows' sums take it up instead
+        uint32_t odd = 0;
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            bool hide = t0 + 16 * j + 4 * lg + i >= k1;
+            if (I.rows > 1) {
+              const bool some = (__ballot(!hide && !tile.finite_v(j, i)) >> (16 * lg)) & 0xFFFFu;
+              odd |= (uint32_t)some << (4 * j + i);
+              hide |= some;
+            }
+            if (hide) tile.zero_v(j, i);
+          }
+        if (__any(odd)) {
+#pragma unroll
+          for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              if ((odd >> (4 * j + i) & 1) && t0 + 16 * j + 4 * lg + i < limit) l = __builtin_nanf("");
+        }
+      }
+      tile.add_pv(S, O);
+      if (more) load_v(t0 + 4 * TK);
+    }
+    if (bad) paged_err(a.err, PAGED_ERR_ATT_PAGE, I.b);
+
+    // ---- join the waves ----
+    l = add_xor32(add_xor16(l));
+    __syncthreads();  // s_q and s_ml are free
+    if (lg == 0) {
+      s_ml[(w * 16 + ln) * 2] = m;
+      s_ml[(w * 16 + ln) * 2 + 1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int d = 0; d < DPL; d += 4)
+        *(f32x4*)&s_o[(w * 16 + ln) * OS + (4 * lg + i) * DPL + d] = (f32x4){O[d][i], O[d + 1][i], O[d + 2][i], O[d + 3][i]};
+    __syncthreads();
+    const uint32_t col = tid >> 4, d0 = (tid & 15) * DPL;
+    float mx = s_ml[col * 2];
+#pragma unroll
+    for (int k = 1; k < 4; k++) mx = fmaxf(mx, s_ml[(k * 16 + col) * 2]);
+    float sum = 0.f, o[DPL];
+#pragma unroll
+    for (int d = 0; d < DPL; d++) o[d] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const float mk = s_ml[(k * 16 + col) * 2];
+      const float f = mk == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mk - mx);
+      sum = __builtin_fmaf(f, s_ml[(k * 16 + col) * 2 + 1], sum);
+#pragma unroll
+      for (int d = 0; d < DPL; d++) o[d] = __builtin_fmaf(f, s_o[(k * 16 + col) * OS + d0 + d], o[d]);
+    }
+    float* mine = a.parts + (size_t)I.part * CB * (hd + 2);
+    if (col < I.ncols && d0 < hd) {
+      if (I.ns == 1) {
+        float* y = a.out + I.at(col, a.ld_out, hd) + d0;
+#pragma unroll
+        for (int d = 0; d < DPL; d += 4) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[e] = I.keys ? o[d + e] / sum : 0.f;
+          store4(y + d, v);
+        }
+      } else {
+#pragma unroll
+        for (int d = 0; d < DPL; d += 2) put2(mine + col * hd + d0 + d, o[d], o[d + 1]);
+        if (d0 == 0) put2(mine + CB * hd + col * 2, mx, sum);
+      }
+    }
+    if (I.ns > 1) join_splits(a, I, CB, s_o);
+    __syncthreads();  // LDS is free for the next item
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many columns: each of the four waves has CT tiles of 16 columns of its own, Q
+// and O^T in registers, and all share the keys, KT at a time through LDS (two
+// stages, filled by DMA while the other is multiplied; one barrier a stage).
+// A stage's rows are [K row][V row] regions of KT rows in 16-byte chunks, chunk
+// c of row r at c ^ swizzle(r), so that the 16 rows that an operand read takes
+// lie in different banks; the DMA writes lane after lane, so each lane picks
+// its source chunk accordingly.  K operands are read as they lie; f16 and bf16
+// values through the transposing LDS read, lane (4k + c) of 16 supplying dims
+// 4c .. 4c+3 of the k-th of four keys and receiving one dim of all four.
+// ---------------------------------------------------------------------------
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// 16 bytes per lane from base + off to LDS byte address lds + 16 * lane.  In asm
+// so that the compiler does not see an LDS write, for which it would wait at the
+// next LDS read; there is no destination register, and stage_done() waits.  One
+// wait state between the write of M0 and its use; the compiler warns that M0 is
+// reserved, and must keep nothing there across this.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2"
+      :
+      : "s"(lds), "v"(off), "s"(base)
+      : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ void stage_done() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// CHUNKS 16-byte chunks to a row: the rows whose chunks share a bank, 16 / CHUNKS
+// of them in 256 bytes, get different keys
+template <uint32_t CHUNKS>
+__device__ __forceinline__ uint32_t swizzle(uint32_t r) {
+  return CHUNKS >= 16 ? r & 15 : (r / (16 / CHUNKS)) & (CHUNKS - 1);
+}
+
+template <class MM_, int DPL>
+struct Rows16 {
+  typedef MM_ MM;
+  typedef Tile16<MM, DPL> TILE;
+  typedef typename MM::T T;
+  static constexpr int CT = 2, KT = 64, NJ = KT / 16, TERMS = MM::TERMS;
+  static constexpr uint32_t CHUNKS = 2 * DPL, ROWB = 32 * DPL;  // of 16 * DPL dims
+  // scores of the CT tiles' columns against the stage's keys
+  static __device__ __forceinline__ void scores(const uint8_t* k, uint32_t ln, uint32_t lg,
+                                                const u32x4 (&Q)[CT][TILE::QREG], f32x4 (&S)[CT][NJ]) {
+#pragma unroll
+    for (int c = 0; c < CT; c++)
+#pragma unroll
+      for (int j = 0; j < NJ; j++) S[c][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+      for (int s = 0; s < TILE::KS; s++) {
+        const uint32_t r = 16 * j + ln;
+        const u32x4 x = *(const u32x4*)(k + r * ROWB + ((4 * s + lg) ^ swizzle<CHUNKS>(r)) * 16);
+#pragma unroll
+        for (int t = 0; t < TERMS; t++)
+#pragma unroll
+          for (int c = 0; c < CT; c++) S[c][j] = MM::mfma(x, Q[c][s * TERMS + t], S[c][j]);
+      }
+  }
+  static __device__ __forceinline__ void add_pv(const uint8_t* v, uint32_t ln, uint32_t lg, const f32x4 (&S)[CT][NJ],
+                                                f32x4 (&O)[CT][DPL]) {
+#pragma unroll
+    for (int h = 0; h < NJ / 2; h++) {
+      u32x4 p[CT][TERMS];
+#pragma unroll
+      for (int c = 0; c < CT; c++) {
+        const f32x4 two[2] = {S[c][2 * h], S[c][2 * h + 1]};
+        TILE::weights(two, p[c]);
+      }
+#pragma unroll
+      for (int d = 0; d < DPL; d++) {
+        u32x2 x[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const uint32_t r = 16 * (2 * h + j) + 4 * lg + ln / 4, cc = ln & 3;
+          const uint8_t* at = v + r * ROWB + (((2 * d + cc / 2) ^ swizzle<CHUNKS>(r)) * 16) + (cc & 1) * 8;
+          x[j] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
+        }
+        const u32x4 y = (u32x4){x[0][0], x[0][1], x[1][0], x[1][1]};
+#pragma unroll
+        for (int t = 0; t < TERMS; t++)
+#pragma unroll
+          for (int c = 0; c < CT; c++) O[c][d] = MM::mfma(y, p[c][t], O[c][d]);
+      }
+    }
+  }
+  static __device__ __forceinline__ bool finite(u32x4 x) {
+    bool ok = true;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      ok = ok && (x[k] & MM::EXPONENT) != MM::EXPONENT && (x[k] & (MM::EXPONENT << 16)) != (MM::EXPONENT << 16);
+    return ok;
+  }
+};
+
+template <int DPL>
+struct Rows32 {
+  typedef Tile32<DPL> TILE;
+  typedef float T;
+  static constexpr int CT = 1, KT = 32, NJ = KT / 16;
+  static constexpr uint32_t CHUNKS = 4 * DPL, ROWB = 64 * DPL;
+  static __device__ __forceinline__ void scores(const uint8_t* k, uint32_t ln, uint32_t lg,
+                                                const u32x4 (&Q)[CT][TILE::QREG], f32x4 (&S)[CT][NJ]) {
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      f32x4 a = (f32x4){0.f, 0.f, 0.f, 0.f}, b = a;
+      const uint32_t r = 16 * j + ln;
+#pragma unroll
+      for (int s = 0; s < DPL; s++) {
+        const f32x4 x = *(const f32x4*)(k + r * ROWB + ((4 * s + lg) ^ swizzle<CHUNKS>(r)) * 16);
+        const f32x4 q = __builtin_bit_cast(f32x4, Q[0][s]);
+        a = __builtin_amdgcn_mfma_f32_16x16x4f32(x[0], q[0], a, 0, 0, 0);
+        b = __builtin_amdgcn_mfma_f32_16x16x4f32(x[1], q[1], b, 0, 0, 0);
+        a = __builtin_amdgcn_mfma_f32_16x16x4f32(x[2], q[2], a, 0, 0, 0);
+        b = __builtin_amdgcn_mfma_f32_16x16x4f32(x[3], q[3], b, 0, 0, 0);
+      }
+      S[0][j] = a + b;
+    }
+  }
+  static __device__ __forceinline__ void add_pv(const uint8_t* v, uint32_t ln, uint32_t lg, const f32x4 (&S)[CT][NJ],
+                                                f32x4 (&O)[CT][DPL]) {
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int d = 0; d < DPL; d++) {
+          const uint32_t r = 16 * j + 4 * lg + i;
+          const float x = *(const float*)(v + r * ROWB + (((4 * d + ln / 4) ^ swizzle<CHUNKS>(r)) * 16) + (ln & 3) * 4);
+          O[0][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, S[0][j][i], O[0][d], 0, 0, 0);
+        }
+  }
+  static __device__ __forceinline__ bool finite(u32x4 x) {
+    bool ok = true;
+#pragma unroll
+    for (int k = 0; k < 4; k++) ok = ok && (x[k] & 0x7F800000u) != 0x7F800000u;
+    return ok;
+  }
+};
+
+template <class ROWS, int DPL>
+__device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
+  typedef typename ROWS::TILE TILE;
+  typedef typename ROWS::T T;
+  constexpr int CT = ROWS::CT, KT = ROWS::KT, NJ = ROWS::NJ, QREG = TILE::QREG;
+  constexpr uint32_t CB = 64 * CT, ROWB = ROWS::ROWB, CHUNKS = ROWS::CHUNKS, REGION = KT * ROWB;
+  static_assert((PAGED_SPLIT_MAX * 16 + 128) * 4 <= 4 * REGION, "the weights of a join fit in the stages");
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];  // [2 stages][K, V][KT rows]
+  uint32_t* s_odd = (uint32_t*)(lds + 4 * REGION);                // [2 stages][2] a bit to a key
+  const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  const uint32_t ln = lane & 15, lg = lane >> 4;
+  const uint32_t P = 1u << a.shift, hd = a.hd;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  Items items;
+  find_items(a, s_odd + 4, items);
+
+  for (uint32_t item = blockIdx.x; item < items.total; item += gridDim.x) {
+    const Item I(a, items, item, CB, KT);
+    const uint32_t k0 = I.k0, k1 = I.k1;
+    // ---- this wave's share of a stage: KT / 4 rows of K and of V, all of one page ----
+    constexpr uint32_t SHARE = KT / 4, RPI = 1024 / ROWB, INSTR = SHARE / RPI;  // rows to an instruction
+    const int32_t* table = a.tables + (size_t)I.b * a.max_pages;
+    const size_t head_len = (size_t)hd << a.shift;
+    uint32_t bad = 0, pages = 0, ahead = 64;  // lane x: page of this wave's rows x stages on
+    auto fetch = [&](uint32_t t, uint32_t stage) {
+      if (ahead == 64) {
+        const uint32_t k = t + lane * KT + w * SHARE;
+        const uint32_t p = (uint32_t)table[(k < k1 ? k : k1 - 1) >> a.shift];
+        bad |= (uint32_t)(p >= a.n_pages);
+        pages = p < a.n_pages ? p : 0u;
+        ahead = 0;
+      }
+      const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)ahead++);
+      const uint32_t first = t + w * SHARE;  // rows from k1 on: others of the page
+      const size_t at = ((size_t)p * a.nKV + I.kvh) * head_len + (size_t)(first & (P - 1)) * hd;
+      const uint32_t to = lds0 + stage * 2 * REGION + w * SHARE * ROWB;
+#pragma unroll
+      for (uint32_t i = 0; i < INSTR; i++) {
+        const uint32_t r = i * RPI + lane / CHUNKS;  // row of the share
+        uint32_t c = (lane % CHUNKS) ^ swizzle<CHUNKS>(w * SHARE + r);
+        const uint32_t last = hd * sizeof(T) / 16 - 1;  // past the head: against zeros of Q, into dims that nobody reads
+        c = c < last ? c : last;
+        const uint32_t off = r * hd * sizeof(T) + c * 16;
+        dma16((const T*)a.kpages + at, off, to + i * 1024);
+        dma16((const T*)a.vpages + at, off, to + REGION + i * 1024);
+      }
+    };
+    __syncthreads();  // the stages and s_odd are free
+    if (k0 < k1) fetch(k0, 0);
+
+    // ---- this wave's columns ----
+    u32x4 Q[CT][QREG];
+    f32x4 O[CT][DPL];
+    float m[CT], l[CT], c[CT];
+    uint32_t limit[CT];
+#pragma unroll
+    for (int t = 0; t < CT; t++) {
+      const uint32_t col = (w * CT + t) * 16 + ln;
+      f32x4 raw[TILE::QRAW];
+      TILE::load_q(a.q + I.at(col < I.ncols ? col : 0, a.ld_q, hd), lg, hd, raw);
+      int e2;
+      TILE::split_q(raw, col < I.ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2, Q[t]);
+      c[t] = score_factor(a.scale, e2);
+      limit[t] = I.least + I.row_of(col);
       m[t] = -__builtin_inff();
       l[t] = 0.f;
 #pragma unroll
       for (int d = 0; d < DPL; d++) O[t][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
+    const bool some = w * CT * 16 < I.ncols;  // this wave has columns
 
-    for (; t0 < k1; t0 += 4 * TK) {
-      const bool masked = t0 + TK > least || t0 + TK > k1, more = t0 + 4 * TK < k1;
-      uint32_t odd = 0;  // the lane's keys with a value that is not finite
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        if (t > 0 && t * 16 >= ncols) break;
-        f32x4 S[NJ];
-        asm volatile("" ::: "memory");  // Q is read from LDS here, not kept in registers over the keys
-        tile.scores([&](int k) { return s_q[(t * QREG + k) * 64 + lane]; }, S);
-        if ((t + 1 == NT || (t + 1) * 16 >= ncols) && more) {
-          if (++tiles == AHEAD) {
-            tiles = 0;
-            load_pages(t0 + 4 * TK);
+    uint32_t stage = 0;
+    for (uint32_t t0 = k0; t0 < k1; t0 += KT, stage ^= 1) {
+      uint8_t* k = lds + stage * 2 * REGION;
+      uint8_t* v = k + REGION;
+      const bool masked = t0 + KT > I.least || t0 + KT > k1;
+      uint32_t* odd = s_odd + 2 * stage;
+      if (masked && tid < 2) odd[tid] = 0;
+      stage_done();  // this stage is there, and the other one read by all
+      if (t0 + KT < k1) fetch(t0 + KT, stage ^ 1);
+      if (masked) {
+        // a weight of 0 does not hide a value that is not finite: values behind
+        // the block's keys go to 0, and so do chunks with such a value that only
+        // some rows may see; the sums of those rows take it up instead
+        for (uint32_t x = tid; x < KT * CHUNKS; x += 256) {
+          const uint32_t r = x / CHUNKS;
+          u32x4* at = (u32x4*)(v + x * 16);
+          const bool hide = t0 + r >= k1;
+          if (hide || !ROWS::finite(*at)) {
+            *at = (u32x4){0u, 0u, 0u, 0u};
+            if (!hide) atomicOr(&odd[r >> 5], 1u << (r & 31));
           }
-          load_k(t0 + 4 * TK);
         }
+        __syncthreads();
+      }
+      if (!some) continue;
+      f32x4 S[CT][NJ];
+      ROWS::scores(k, ln, lg, Q, S);
+#pragma unroll
+      for (int t = 0; t < CT; t++) {
         if (masked) {
           const uint32_t end = limit[t] < k1 ? limit[t] : k1;
 #pragma unroll
           for (int j = 0; j < NJ; j++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              if (t0 + 16 * j + 4 * lg + i >= end) S[j][i] = -__builtin_inff();
-        }
-        float x = -__builtin_inff();
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) x = fmaxf(x, S[j][i]);
-        x = max_xor16_32(x) * c[t];
-        if (__any(x > m[t] + M_SLACK)) {
-          const float mn = fmaxf(x, m[t]);
-          const float f = mn == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[t] - mn);
-          m[t] = mn;
-          l[t] *= f;
-#pragma unroll
-          for (int d = 0; d < DPL; d++) O[t][d] *= f;
-        }
-        const float shift = m[t] == -__builtin_inff() ? 0.f : P_EXP - m[t];
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            S[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[j][i], c[t], shift));
-            l[t] += S[j][i];
-          }
-        if (masked) {
-          // a weight of 0 does not hide a value that is not finite: values behind
-          // the block's keys go to 0, and so do keys with such a value that only
-          // some rows see; those rows' sums take it up instead
-          if (t == 0) {
-            odd = 0;
-#pragma unroll
-            for (int j = 0; j < NJ; j++)
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                bool hide = t0 + 16 * j + 4 * lg + i >= k1;
-                if (rows > 1) {
-                  const bool some = (__ballot(!hide && !tile.finite_v(j, i)) >> (16 * lg)) & 0xFFFFu;
-                  odd |= (uint32_t)some << (4 * j + i);
-                  hide |= some;
-                }
-                if (hide) tile.zero_v(j, i);
-              }
-          }
-          if (__any(odd)) {
-#pragma unroll
-            for (int j = 0; j < NJ; j++)
-#pragma unroll
-              for (int i = 0; i < 4; i++)
-                if ((odd >> (4 * j + i) & 1) && t0 + 16 * j + 4 * lg + i < limit[t]) l[t] = __builtin_nanf("");
-          }
-        }
-        tile.add_pv(S, O[t]);
-      }
-      if (more) load_v(t0 + 4 * TK);
-    }
-    if (bad) paged_err(a.err, PAGED_ERR_ATT_PAGE, b);
-
-    // ---- join the waves, 16 columns at a time ----
-    const uint32_t part = s_part[b] + local;  // of ns > 1; a split's are nKV apart
-    float* mine = a.parts + (size_t)part * CB * (hd + 2);
-    const uint32_t col = tid >> 4, d0 = (tid & 15) * DPL;
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-      if (t > 0 && t * 16 >= ncols) break;
-      l[t] = add_xor32(add_xor16(l[t]));
-      __syncthreads();  // s_q, s_o and s_ml are free
-      if (lg == 0) {
-        s_ml[(w * 16 + ln) * 2] = m[t];
-        s_ml[(w * 16 + ln) * 2 + 1] = l[t];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int d = 0; d < DPL; d += 4)
-          *(f32x4*)&s_o[(w * 16 + ln) * OS + (4 * lg + i) * DPL + d] =
-              (f32x4){O[t][d][i], O[t][d + 1][i], O[t][d + 2][i], O[t][d + 3][i]};
-      __syncthreads();
-      float mx = s_ml[col * 2];
-#pragma unroll
-      for (int k = 1; k < 4; k++) mx = fmaxf(mx, s_ml[(k * 16 + col) * 2]);
-      float sum = 0.f, o[DPL];
-#pragma unroll
-      for (int d = 0; d < DPL; d++) o[d] = 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const float mk = s_ml[(k * 16 + col) * 2];
-        const float f = mk == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mk - mx);
-        sum = __builtin_fmaf(f, s_ml[(k * 16 + col) * 2 + 1], sum);
-#pragma unroll
-        for (int d = 0; d < DPL; d++) o[d] = __builtin_fmaf(f, s_o[(k * 16 + col) * OS + d0 + d], o[d]);
-      }
-      const uint32_t at = t * 16 + col;
-      if (at < ncols && d0 < hd) {
-        if (ns == 1) {
-          uint32_t row, head;
-          column(at, row, head);
-          float* y = a.out + (size_t)(r0 + row0 + row) * a.ld_out + head * hd + d0;
-#pragma unroll
-          for (int d = 0; d < DPL; d++) y[d] = keys ? o[d] / sum : 0.f;
-        } else {
-#pragma unroll
-          for (int d = 0; d < DPL; d += 2) put2(mine + at * hd + d0 + d, o[d], o[d + 1]);
-          if (d0 == 0) put2(mine + CB * hd + at * 2, mx, sum);
-        }
-      }
-    }
-    if (ns > 1) {
-      const size_t stride = (size_t)a.nKV * CB * (hd + 2);
-      const uint32_t first = part - split * a.nKV;
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
-      if (tid == 0)
-        s_last = __hip_atomic_fetch_add(a.counters + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ns - 1;
-      __syncthreads();
-      if (s_last) {
-        const float* all = a.parts + (size_t)first * CB * (hd + 2);
-        if (tid == 0) __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        for (uint32_t c0 = 0; c0 < ncols; c0 += 16) {
-          // weights 2^(m - max) of the splits, 16 threads to a column; 0 behind the last
-          constexpr int PER = PAGED_SPLIT_MAX / 16;
-          const uint32_t cc = c0 + ln < ncols ? c0 + ln : 0, sp0 = tid >> 4;
-          const float* ml = all + CB * hd + cc * 2;
-          float2 v[PER];
-          float mx = -__builtin_inff(), sum = 0.f;
-#pragma unroll
-          for (int k = 0; k < PER; k++) v[k] = get2(ml + (sp0 + 16 * k < ns ? sp0 + 16 * k : 0u) * stride);
-#pragma unroll
-          for (int k = 0; k < PER; k++) {
-            if (sp0 + 16 * k >= ns) v[k] = make_float2(-__builtin_inff(), 0.f);
-            mx = fmaxf(mx, v[k].x);
-          }
-          mx = max_xor16_32(mx);
-          __syncthreads();
-          if (lg == 0) s_ml[w * 16 + ln] = mx;
-          __syncthreads();
-          mx = fmaxf(fmaxf(s_ml[ln], s_ml[16 + ln]), fmaxf(s_ml[32 + ln], s_ml[48 + ln]));
-#pragma unroll
-          for (int k = 0; k < PER; k++) {
-            const float f = v[k].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(v[k].x - mx);
-            s_o[(sp0 + 16 * k) * 16 + ln] = f;
-            sum = __builtin_fmaf(f, v[k].y, sum);
-          }
-          sum = add_xor32(add_xor16(sum));
-          if (lg == 0) s_ml[64 + w * 16 + ln] = sum;
-          __syncthreads();
-          // a thread's pair of dims over the splits, JOIN_BATCH loads in flight;
-          // behind the last split it again, with a weight of 0
-          constexpr uint32_t JOIN_BATCH = 16;
-          const uint32_t nc = ncols - c0 < 16 ? ncols - c0 : 16;
-          for (uint32_t e = 2 * tid; e < nc * hd; e += 512) {
-            const uint32_t k = e / hd, d = e % hd;
-            const float* src = all + c0 * hd + e;
-            float2 o = make_float2(0.f, 0.f);
-            for (uint32_t s0 = 0; s0 < ns; s0 += JOIN_BATCH) {
-              float2 x[JOIN_BATCH];
-#pragma unroll
-              for (uint32_t s = 0; s < JOIN_BATCH; s++) x[s] = get2(src + (s0 + s < ns ? s0 + s : ns - 1) * stride);
-#pragma unroll
-              for (uint32_t s = 0; s < JOIN_BATCH; s++) {
-                const float f = s_o[(s0 + s) * 16 + k];
-                o.x = __builtin_fmaf(f, x[s].x, o.x);
-                o.y = __builtin_fmaf(f, x[s].y, o.y);
-              }
+            for (int i = 0; i < 4; i++) {
+              const uint32_t r = 16 * j + 4 * lg + i;
+              if (t0 + r >= end) S[t][j][i] = -__builtin_inff();
+              else if (odd[r >> 5] >> (r & 31) & 1) l[t] = __builtin_nanf("");
             }
-            const float tot = s_ml[64 + k] + s_ml[80 + k] + s_ml[96 + k] + s_ml[112 + k];
-            uint32_t row, head;
-            column(c0 + k, row, head);
-            float* y = a.out + (size_t)(r0 + row0 + row) * a.ld_out + head * hd + d;
-            y[0] = o.x / tot;
-            y[1] = o.y / tot;
-          }
         }
+        weigh<NJ, DPL>(S[t], c[t], m[t], l[t], O[t]);
+      }
+      ROWS::add_pv(v, ln, lg, S, O);
+    }
+    if (bad) paged_err(a.err, PAGED_ERR_ATT_PAGE, I.b);
+
+    // ---- out, or a partial ----
+    float* mine = a.parts + (size_t)I.part * CB * (hd + 2);
+#pragma unroll
+    for (int t = 0; t < CT; t++) {
+      const uint32_t col = (w * CT + t) * 16 + ln;
+      l[t] = add_xor32(add_xor16(l[t]));
+      if (col >= I.ncols) continue;
+      if (I.ns == 1) {
+        const float inv = I.keys ? 1.0f / l[t] : 0.f;
+        float* y = a.out + I.at(col, a.ld_out, hd) + 4 * lg;
+#pragma unroll
+        for (int d = 0; d < DPL; d++)
+          if (16 * d + 4 * lg < hd) store4(y + 16 * d, O[t][d] * inv);
+      } else {
+#pragma unroll
+        for (int d = 0; d < DPL; d++)
+          if (16 * d + 4 * lg < hd) {
+            put2(mine + col * hd + 16 * d + 4 * lg, O[t][d][0], O[t][d][1]);
+            put2(mine + col * hd + 16 * d + 4 * lg + 2, O[t][d][2], O[t][d][3]);
+          }
+        if (lg == 0) put2(mine + CB * hd + col * 2, m[t], l[t]);
       }
     }
-    __syncthreads();  // LDS is free for the next item
+    if (I.ns > 1) join_splits(a, I, CB, (float*)lds);
   }
 }
 
-#define DEF_ATTENTION(NAME, DPL, NT, SMALL, ...)                                       \
+#define DEF_ATTENTION(NAME, BODY, ...)                             \
   extern "C" __global__ __launch_bounds__(256, 2) void NAME(AttArgs a) { \
-    attention_body<__VA_ARGS__, DPL, NT, SMALL>(a);                                    \
+    BODY<__VA_ARGS__>(a);                                          \
   }
-// named by page type, head dims held (64 or 128) and tiles of 16 columns to a
-// workgroup; _s for pages of less than 16 keys
-#define DEF_ATTENTIONS(TYPE, D, DPL, ...)                                           \
-  DEF_ATTENTION(smith_paged_attention_##TYPE##_d##D##_t1, DPL, 1, false, __VA_ARGS__) \
-  DEF_ATTENTION(smith_paged_attention_##TYPE##_d##D##_t1_s, DPL, 1, true, __VA_ARGS__)
-DEF_ATTENTIONS(f32, 64, 4, Tile32<4>)
-DEF_ATTENTIONS(f32, 128, 8, Tile32<8>)
-DEF_ATTENTIONS(f16, 64, 4, Tile16<MmF16, 4>)
-DEF_ATTENTIONS(f16, 128, 8, Tile16<MmF16, 8>)
-DEF_ATTENTIONS(bf16, 64, 4, Tile16<MmBf16, 4>)
-DEF_ATTENTIONS(bf16, 128, 8, Tile16<MmBf16, 8>)
-DEF_ATTENTION(smith_paged_attention_f16_d64_t4, 4, 4, false, Tile16<MmF16, 4>)
-DEF_ATTENTION(smith_paged_attention_f16_d128_t4, 8, 4, false, Tile16<MmF16, 8>)
-DEF_ATTENTION(smith_paged_attention_bf16_d64_t4, 4, 4, false, Tile16<MmBf16, 4>)
-DEF_ATTENTION(smith_paged_attention_bf16_d128_t4, 8, 4, false, Tile16<MmBf16, 8>)
+// named by page type and head dims held (64 or 128); _s for pages of less than
+// 16 keys
+#define DEF_ATTENTIONS(TYPE, D, DPL, TILE, ROWS)                                                 \
+  DEF_ATTENTION(smith_paged_attention_##TYPE##_d##D, attention_body, TILE, DPL, false)           \
+  DEF_ATTENTION(smith_paged_attention_##TYPE##_d##D##_s, attention_body, TILE, DPL, true)        \
+  DEF_ATTENTION(smith_paged_attention_rows_##TYPE##_d##D, attention_rows_body, ROWS, DPL)
+typedef Tile16<MmF16, 4> TileF16d64;
+typedef Tile16<MmF16, 8> TileF16d128;
+typedef Tile16<MmBf16, 4> TileBf16d64;
+typedef Tile16<MmBf16, 8> TileBf16d128;
+typedef Rows16<MmF16, 4> RowsF16d64;
+typedef Rows16<MmF16, 8> RowsF16d128;
+typedef Rows16<MmBf16, 4> RowsBf16d64;
+typedef Rows16<MmBf16, 8> RowsBf16d128;
+DEF_ATTENTIONS(f32, 64, 4, Tile32<4>, Rows32<4>)
+DEF_ATTENTIONS(f32, 128, 8, Tile32<8>, Rows32<8>)
+DEF_ATTENTIONS(f16, 64, 4, TileF16d64, RowsF16d64)
+DEF_ATTENTIONS(f16, 128, 8, TileF16d128, RowsF16d128)
+DEF_ATTENTIONS(bf16, 64, 4, TileBf16d64, RowsBf16d64)
+DEF_ATTENTIONS(bf16, 128, 8, TileBf16d128, RowsBf16d128)

@@ -2437,16 +2437,16 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
     return fail(c, "%s: out overlaps q", fn);
   if (set_device(c)) return -1;
   if (scale == 0.f) scale = 1.0f / sqrtf((float)head_dim);
-  // tiles of 16 columns (row, head) to a workgroup: one where requests bring a
-  // row or so each (the keys are read once, columns hardly matter), four where
-  // they fill more than two; the f32 matrix cores are the bound at one already
-  // (and pages of less than 16 keys, looked up key by key, have no other kernel)
+  // Where a request brings a row or so its columns (row, head) are few and its
+  // keys the work: 16 columns to a workgroup, keys in registers.  Where the
+  // columns fill most of two such tiles a workgroup shares the keys among four
+  // waves' columns.  Pages of less than 16 keys, looked up key by key, have the
+  // first kernel only.
   const uint32_t G = n_heads / n_kv_heads;
   const bool small = shift < 4;
-  const uint32_t tiles =
-      row_start && kv_type != SMITH_KV_F32 && !small && (uint64_t)max_rows * G > 32ull * n_req ? 4 : 1;
-  const uint32_t CB = 16 * tiles, dims = head_dim <= 64 ? 64 : 128;
-  const uint32_t target = tiles == 1 ? 1024 : 512;
+  const bool many = row_start && !small && (uint64_t)max_rows * G > 24ull * n_req;
+  const uint32_t CB = !many ? 16 : kv_type == SMITH_KV_F32 ? 64 : 128, dims = head_dim <= 64 ? 64 : 128;
+  const uint32_t target = 512;  // two workgroups to a CU
   // a block that is cut has 1.5 C keys or more and so at most 4/3 of its keys / C
   // splits: 4/3 W / C <= 4/3 target of them in all (and some for what f32 rounds)
   const uint32_t max_parts = target + target / 3 + 16;
@@ -2456,8 +2456,9 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   const uint64_t blocks = (uint64_t)groups * n_kv_heads * (row_start ? (uint64_t)n_req + max_rows / RB : n_req);
   const uint64_t longest = ((uint64_t)max_pages << shift) / PAGED_SPLIT_MIN + 1;  // splits of one block
   const uint32_t grid = (uint32_t)std::min<uint64_t>({(uint64_t)target, blocks + max_parts, blocks * longest});
-  const uint32_t qreg = kv_type == SMITH_KV_F32 ? dims / 16 : dims / 32 * (kv_type == SMITH_KV_F16 ? 2 : 3);
-  const uint32_t lds = std::max<uint32_t>(4 * 16 * (dims + 4) * 4, tiles * qreg * 64 * 16) + 4 * 16 * 2 * 4 + 16 * (n_req + 1);
+  // of attention_body: O and (m, l) of four waves; of attention_rows_body: two
+  // stages of K and V rows (64 of f16 / bf16 or 32 of f32: 256 bytes a head dim) and their marks
+  const uint32_t lds = (many ? 256 * 2 * dims + 16 : 4 * 16 * (dims + 4) * 4 + 4 * 16 * 2 * 4) + 16 * (n_req + 1);
   struct {
     const float* q;
     const int32_t *row_start, *lens, *tables;
@@ -2471,7 +2472,7 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
          ld_q, ld_out, max_rows, n_req, max_pages, n_kv_heads, G, head_dim, n_pages, shift, RB, heads_blk, groups,
          (float)n_kv_heads / (float)target, scale};
   char name[64];
-  snprintf(name, sizeof name, "smith_paged_attention_%s_d%u_t%u%s", kv_name(kv_type), dims, tiles, small ? "_s" : "");
+  snprintf(name, sizeof name, "smith_paged_attention_%s%s_d%u%s", many ? "rows_" : "", kv_name(kv_type), dims, small ? "_s" : "");
   void* args[] = {&a};
   return launch(c, name, dim3(grid), dim3(256), args, lds);
 }
