@@ -307,6 +307,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // maximum over the lanes l, l ^ 16, l ^ 32, l ^ 48 (a number wins over a NaN)
 __device__ __forceinline__ float max_xor16_32(float v) {
@@ -337,14 +340,13 @@ struct MmF16 {
   static constexpr int TERMS = 2;
   static constexpr uint32_t EXPONENT = 0x7C00u;
   static __device__ __forceinline__ void split(const float (&x)[8], u32x4 (&t)[TERMS]) {
-    f16x8 hi, lo;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      hi[e] = (_Float16)x[e];
-      lo[e] = (_Float16)(x[e] - (float)hi[e]);
+    for (int k = 0; k < 4; k++) {
+      const f16x2 hi = __builtin_convertvector((f32x2){x[2 * k], x[2 * k + 1]}, f16x2);
+      const f32x2 r = (f32x2){__builtin_fmaf((float)hi[0], -1.f, x[2 * k]), __builtin_fmaf((float)hi[1], -1.f, x[2 * k + 1])};
+      t[0][k] = __builtin_bit_cast(uint32_t, hi);
+      t[1][k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, f16x2));
     }
-    t[0] = __builtin_bit_cast(u32x4, hi);
-    t[1] = __builtin_bit_cast(u32x4, lo);
   }
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -355,17 +357,16 @@ struct MmBf16 {
   static constexpr int TERMS = 3;
   static constexpr uint32_t EXPONENT = 0x7F80u;
   static __device__ __forceinline__ void split(const float (&x)[8], u32x4 (&t)[TERMS]) {
-    bf16x8 a, b, c;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      a[e] = (__bf16)x[e];
-      const float r = x[e] - (float)a[e];
-      b[e] = (__bf16)r;
-      c[e] = (__bf16)(r - (float)b[e]);
+    for (int k = 0; k < 4; k++) {
+      f32x2 r = (f32x2){x[2 * k], x[2 * k + 1]};
+#pragma unroll
+      for (int p = 0; p < TERMS; p++) {
+        t[p][k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+        r[0] -= __uint_as_float(t[p][k] << 16);
+        r[1] -= __uint_as_float(t[p][k] & 0xFFFF0000u);
+      }
     }
-    t[0] = __builtin_bit_cast(u32x4, a);
-    t[1] = __builtin_bit_cast(u32x4, b);
-    t[2] = __builtin_bit_cast(u32x4, c);
   }
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
@@ -969,12 +970,13 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
         load_k(t0 + 4 * TK);
       }
       if (masked) {
-        const uint32_t end = limit < k1 ? limit : k1;
+        // the lane's first hidden key behind t0 + 4 lg
+        const int end = (int)((limit < k1 ? limit : k1) - t0 - 4 * lg);
 #pragma unroll
         for (int j = 0; j < NJ; j++)
 #pragma unroll
           for (int i = 0; i < 4; i++)
-            if (t0 + 16 * j + 4 * lg + i >= end) S[j][i] = -__builtin_inff();
+            if (16 * j + i >= end) S[j][i] = -__builtin_inff();
       }
       weigh<NJ, DPL>(S, c, m, l, O);
       if (masked) {
@@ -1114,17 +1116,25 @@ struct Rows16 {
     for (int c = 0; c < CT; c++)
 #pragma unroll
       for (int j = 0; j < NJ; j++) S[c][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < NJ; j++)
+    u32x4 x[2][TILE::KS];
+    auto load = [&](int j) {
 #pragma unroll
       for (int s = 0; s < TILE::KS; s++) {
         const uint32_t r = 16 * j + ln;
-        const u32x4 x = *(const u32x4*)(k + r * ROWB + ((4 * s + lg) ^ swizzle<CHUNKS>(r)) * 16);
+        x[j & 1][s] = *(const u32x4*)(k + r * ROWB + ((4 * s + lg) ^ swizzle<CHUNKS>(r)) * 16);
+      }
+    };
+    load(0);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      if (j + 1 < NJ) load(j + 1);
+#pragma unroll
+      for (int s = 0; s < TILE::KS; s++)
 #pragma unroll
         for (int t = 0; t < TERMS; t++)
 #pragma unroll
-          for (int c = 0; c < CT; c++) S[c][j] = MM::mfma(x, Q[c][s * TERMS + t], S[c][j]);
-      }
+          for (int c = 0; c < CT; c++) S[c][j] = MM::mfma(x[j & 1][s], Q[c][s * TERMS + t], S[c][j]);
+    }
   }
   static __device__ __forceinline__ void add_pv(const uint8_t* v, uint32_t ln, uint32_t lg, const f32x4 (&S)[CT][NJ],
                                                 f32x4 (&O)[CT][DPL]) {
@@ -1231,7 +1241,7 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
     const int32_t* table = a.tables + (size_t)I.b * a.max_pages;
     const size_t head_len = (size_t)hd << a.shift;
     uint32_t bad = 0, pages = 0, ahead = 64;  // lane x: page of this wave's rows x stages on
-    auto fetch = [&](uint32_t t, uint32_t stage) {
+    auto fetch = [&](uint32_t t, uint32_t stage, uint32_t lane) {
       if (ahead == 64) {
         const uint32_t k = t + lane * KT + w * SHARE;
         const uint32_t p = (uint32_t)table[(k < k1 ? k : k1 - 1) >> a.shift];
@@ -1254,10 +1264,15 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
         dma16((const T*)a.vpages + at, off, to + REGION + i * 1024);
       }
     };
+    // ---- this wave's columns, their loads ahead of the keys' ----
+    f32x4 raw[CT][TILE::QRAW];
+#pragma unroll
+    for (int t = 0; t < CT; t++) {
+      const uint32_t col = (w * CT + t) * 16 + ln;
+      TILE::load_q(a.q + I.at(col < I.ncols ? col : 0, a.ld_q, hd), lg, hd, raw[t]);
+    }
     __syncthreads();  // the stages and s_odd are free
-    if (k0 < k1) fetch(k0, 0);
-
-    // ---- this wave's columns ----
+    if (k0 < k1) fetch(k0, 0, lane);
     u32x4 Q[CT][QREG];
     f32x4 O[CT][DPL];
     float m[CT], l[CT], c[CT];
@@ -1265,10 +1280,8 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
 #pragma unroll
     for (int t = 0; t < CT; t++) {
       const uint32_t col = (w * CT + t) * 16 + ln;
-      f32x4 raw[TILE::QRAW];
-      TILE::load_q(a.q + I.at(col < I.ncols ? col : 0, a.ld_q, hd), lg, hd, raw);
       int e2;
-      TILE::split_q(raw, col < I.ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2, Q[t]);
+      TILE::split_q(raw[t], col < I.ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2, Q[t]);
       c[t] = score_factor(a.scale, e2);
       limit[t] = I.least + I.row_of(col);
       m[t] = -__builtin_inff();
@@ -1286,7 +1299,13 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
       uint32_t* odd = s_odd + 2 * stage;
       if (masked && tid < 2) odd[tid] = 0;
       stage_done();  // this stage is there, and the other one read by all
-      if (t0 + KT < k1) fetch(t0 + KT, stage ^ 1);
+      // with two tiles of columns the lanes' places are worked out anew for every
+      // stage: kept over the loop they cost registers that Q, S and O need (spills,
+      // which wait for the DMA)
+      uint32_t here = lane;
+      if (CT > 1) asm volatile("" : "+v"(here));
+      const uint32_t hn = here & 15, hg = here >> 4;
+      if (t0 + KT < k1) fetch(t0 + KT, stage ^ 1, here);
       if (masked) {
         // a weight of 0 does not hide a value that is not finite: values behind
         // the block's keys go to 0, and so do chunks with such a value that only
@@ -1304,23 +1323,29 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
       }
       if (!some) continue;
       f32x4 S[CT][NJ];
-      ROWS::scores(k, ln, lg, Q, S);
+      ROWS::scores(k, hn, hg, Q, S);
 #pragma unroll
       for (int t = 0; t < CT; t++) {
         if (masked) {
-          const uint32_t end = limit[t] < k1 ? limit[t] : k1;
+          // the lane's first hidden key behind t0 + 4 lg
+          const int end = (int)((limit[t] < k1 ? limit[t] : k1) - t0 - 4 * hg);
+          const uint64_t marks = ((uint64_t)(KT > 32 ? odd[1] : 0u) << 32 | odd[0]) >> (4 * hg);
 #pragma unroll
           for (int j = 0; j < NJ; j++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const uint32_t r = 16 * j + 4 * lg + i;
-              if (t0 + r >= end) S[t][j][i] = -__builtin_inff();
-              else if (odd[r >> 5] >> (r & 31) & 1) l[t] = __builtin_nanf("");
-            }
+            for (int i = 0; i < 4; i++)
+              if (16 * j + i >= end) S[t][j][i] = -__builtin_inff();
+          if (__any(marks != 0)) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                if (16 * j + i < end && (marks >> (16 * j + i) & 1)) l[t] = __builtin_nanf("");
+          }
         }
         weigh<NJ, DPL>(S[t], c[t], m[t], l[t], O[t]);
       }
-      ROWS::add_pv(v, ln, lg, S, O);
+      ROWS::add_pv(v, hn, hg, S, O);
     }
     if (bad) paged_err(a.err, PAGED_ERR_ATT_PAGE, I.b);
 
