@@ -296,9 +296,10 @@ DEF_APPEND(smith_paged_append_bf16, KvBf16)
 //
 // Work is cut on the device, where the lengths are: an item is (request, block
 // of columns, KV head, split of the block's keys).  With W = sum over blocks of
-// their request's length, a request of more than 1.5 C keys, C = max(SPLIT_MIN,
-// W / target), has its keys cut into about len / C splits, so that target items
-// or so of about C keys each fill the chip whatever the lengths are.  Every
+// their request's length, a request of more than 5/4 C keys, C = max(SPLIT_MIN,
+// W / target), has its keys cut into splits of at most that many, so that target
+// items or so fill the chip whatever the lengths are; requests of nearly one length
+// (their longest within 5/4 of the mean) get one item to a workgroup and no more.  Every
 // workgroup forms the prefix sums of the items by itself.  The last of a block's
 // splits to finish (agent-scope counter) joins their partials in split order:
 // the same sums whichever finishes last.
@@ -574,6 +575,7 @@ struct AttArgs {
   float* out;
   float* parts;        // a split's partial: O [columns][head dim], then (m, l) of each column
   uint32_t* counters;  // splits of a block that are done, by the index of its first partial; zero between calls
+  uint32_t* queue;     // items taken beyond each workgroup's first; zero between calls
   uint64_t* err;
   uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift;
   uint32_t rows_blk, heads_blk, groups;  // rows to a block of columns, heads of each, blocks to a row's heads
@@ -623,25 +625,31 @@ __device__ __forceinline__ void request(const AttArgs& a, uint32_t b, bool tell,
   }
 }
 
-// The items of a call, by the prefix sums that each workgroup forms in LDS.
+// The items of a call, by the prefix sums that each workgroup forms in LDS:
+// those of the long requests (half of C keys and more) come before the others,
+// so that what is taken last is short.
 struct Items {
-  uint32_t *item, *part, *row, *len;  // [n_req + 1] of a request: its first item and partial, its first row, its length
-  uint32_t total;
+  // [n_req + 1] of a request: its first item of its class (in the other class's
+  // array the next request's), its first partial, its first row, its length
+  uint32_t *longs, *shorts, *part, *row, *len;
+  uint32_t total, total_long;
   float inv_c;
 
-  __device__ __forceinline__ uint32_t splits(uint32_t keys) const {  // about keys / C
-    const uint32_t s = (uint32_t)((float)keys * inv_c + 0.5f);
+  __device__ __forceinline__ uint32_t splits(uint32_t keys) const {  // of at most about 5/4 C keys
+    const uint32_t s = (uint32_t)((float)keys * inv_c * 0.8f + 0.999f);
     return s < 1 ? 1u : s > PAGED_SPLIT_MAX ? PAGED_SPLIT_MAX : s;
   }
+  __device__ __forceinline__ bool is_long(uint32_t keys) const { return (float)keys * inv_c >= 0.5f; }
 };
 
 __device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Items& t) {
-  t.item = lds;
-  t.part = t.item + a.n_req + 1;
+  t.longs = lds;
+  t.shorts = t.longs + a.n_req + 1;
+  t.part = t.shorts + a.n_req + 1;
   t.row = t.part + a.n_req + 1;
   t.len = t.row + a.n_req + 1;
   __shared__ float s_sum[4];
-  __shared__ uint32_t s_wave[4][2];
+  __shared__ uint32_t s_wave[4][3];
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6, RB = a.rows_blk, groups = a.groups;
   const uint32_t per = (a.n_req + 255) / 256;
   float work = 0.f;  // only a measure of how much there is: the cuts hold for any
@@ -652,7 +660,7 @@ __device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Item
     request(a, b, blockIdx.x == 0, r0, n, len);
     t.row[b] = r0;
     t.len[b] = len;
-    t.item[b] = n;
+    t.longs[b] = n;
     work = __builtin_fmaf((float)(div_up(n, RB) * groups), (float)len, work);
   }
   work = sum64_lanes(work);
@@ -660,40 +668,47 @@ __device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Item
   __syncthreads();
   work = ((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3])) * a.per_target;
   t.inv_c = 1.0f / fmaxf(work, (float)PAGED_SPLIT_MIN);
-  uint32_t items = 0, parts = 0;
+  uint32_t longs = 0, shorts = 0, parts = 0;
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
     if (b >= a.n_req) break;
-    const uint32_t ns = t.splits(t.len[b]), it = div_up(t.item[b], RB) * groups * a.nKV * ns;
-    items += it;
+    const uint32_t ns = t.splits(t.len[b]), it = div_up(t.longs[b], RB) * groups * a.nKV * ns;
+    (t.is_long(t.len[b]) ? longs : shorts) += it;
     parts += ns > 1 ? it : 0;
   }
-  uint32_t ii = scan64_lanes(items), ip = scan64_lanes(parts);
+  uint32_t il = scan64_lanes(longs), is = scan64_lanes(shorts), ip = scan64_lanes(parts);
   if (lane == 63) {
-    s_wave[w][0] = ii;
-    s_wave[w][1] = ip;
+    s_wave[w][0] = il;
+    s_wave[w][1] = is;
+    s_wave[w][2] = ip;
   }
   __syncthreads();
-  t.total = 0;
-  ii -= items;
+  t.total = t.total_long = 0;
+  il -= longs;
+  is -= shorts;
   ip -= parts;
 #pragma unroll
   for (uint32_t k = 0; k < 4; k++) {
     if (k < w) {
-      ii += s_wave[k][0];
-      ip += s_wave[k][1];
+      il += s_wave[k][0];
+      is += s_wave[k][1];
+      ip += s_wave[k][2];
     }
-    t.total += s_wave[k][0];
+    t.total_long += s_wave[k][0];
+    t.total += s_wave[k][1];
   }
+  t.total += t.total_long;
   if (blockIdx.x >= t.total) return;
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
     if (b >= a.n_req) break;
-    const uint32_t ns = t.splits(t.len[b]), n = t.item[b], it = div_up(n, RB) * groups * a.nKV * ns;
-    t.item[b] = ii;
+    const uint32_t ns = t.splits(t.len[b]), n = t.longs[b], it = div_up(n, RB) * groups * a.nKV * ns;
+    const bool lg = t.is_long(t.len[b]);
+    t.longs[b] = il;
+    t.shorts[b] = is;
     t.part[b] = ip;
     if (b + 1 == a.n_req) t.row[a.n_req] = t.row[b] + n;
-    ii += it;
+    (lg ? il : is) += it;
     ip += ns > 1 ? it : 0;
   }
   __syncthreads();
@@ -708,18 +723,21 @@ struct Item {
   uint32_t part;  // of ns > 1: its partial; a block's next split has the one nKV further on
 
   __device__ __forceinline__ Item(const AttArgs& a, const Items& t, uint32_t item, uint32_t CB, uint32_t unit) {
-    // the last request that starts at or before the item (those without items start there too)
+    // the last request that starts at or before the item (those without items of
+    // its class start there too)
+    const uint32_t* from = item < t.total_long ? t.longs : t.shorts;
+    if (item >= t.total_long) item -= t.total_long;
     uint32_t lo = 0, top = a.n_req;
     while (top - lo > 1) {
       const uint32_t mid = (lo + top) >> 1;
-      if (t.item[mid] <= item) lo = mid;
+      if (from[mid] <= item) lo = mid;
       else top = mid;
     }
     auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
     b = uniform(lo);
     r0 = uniform(t.row[b]);
     len = uniform(t.len[b]);
-    const uint32_t local = item - uniform(t.item[b]);
+    const uint32_t local = item - uniform(from[b]);
     part = uniform(t.part[b]) + local;
     n = a.row_start ? uniform(t.row[b + 1]) - r0 : 1u;
     ns = t.splits(len);
@@ -748,6 +766,32 @@ struct Item {
   __device__ __forceinline__ size_t at(uint32_t col, uint32_t ld, uint32_t hd) const {
     const uint32_t row = row_of(col);
     return (size_t)(r0 + row0 + row) * ld + (head0 + col - row * heads) * hd;
+  }
+};
+
+// The workgroup's next item: its own number first, then whichever is next, so
+// that workgroups with short items take more of them.  take() when an item's keys
+// are through (thread 0's atomic is under way while the waves are joined; ahead of
+// the keys every load would wait for it), next() by all at its end.  As many are taken as there are items; the last one taken clears the
+// queue for the next call.
+struct Turn {
+  uint32_t item = blockIdx.x, taken = 0;
+  bool more;
+  __device__ __forceinline__ void take(const AttArgs& a, uint32_t total) {
+    more = total > gridDim.x;
+    if (more && threadIdx.x == 0) taken = __hip_atomic_fetch_add(a.queue, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __device__ __forceinline__ void next(const AttArgs& a, uint32_t total) {
+    __shared__ uint32_t s_next;
+    item = total;
+    if (!more) return;
+    if (threadIdx.x == 0) {
+      s_next = taken + gridDim.x;
+      if (taken == total - 1) __hip_atomic_store(a.queue, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    item = (uint32_t)__builtin_amdgcn_readfirstlane((int)s_next);
+    __syncthreads();  // everybody's copy is taken (and LDS free for the next item)
   }
 };
 
@@ -877,8 +921,8 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
   Items items;
   find_items(a, (uint32_t*)(s_ml + 4 * 16 * 2), items);
 
-  for (uint32_t item = blockIdx.x; item < items.total; item += gridDim.x) {
-    const Item I(a, items, item, CB, TK);
+  for (Turn turn; turn.item < items.total; turn.next(a, items.total)) {
+    const Item I(a, items, turn.item, CB, TK);
     const uint32_t k0 = I.k0, k1 = I.k1, kvh = I.kvh;
     f32x4 q_raw[TILE::QRAW];
     if (w == 0) TILE::load_q(a.q + I.at(ln < I.ncols ? ln : 0, a.ld_q, hd), lg, hd, q_raw);
@@ -1008,6 +1052,7 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
       if (more) load_v(t0 + 4 * TK);
     }
     if (bad) paged_err(a.err, PAGED_ERR_ATT_PAGE, I.b);
+    turn.take(a, items.total);
 
     // ---- join the waves ----
     l = add_xor32(add_xor16(l));
@@ -1055,7 +1100,6 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
       }
     }
     if (I.ns > 1) join_splits(a, I, CB, s_o);
-    __syncthreads();  // LDS is free for the next item
   }
 }
 
@@ -1233,8 +1277,8 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
   Items items;
   find_items(a, s_odd + 4, items);
 
-  for (uint32_t item = blockIdx.x; item < items.total; item += gridDim.x) {
-    const Item I(a, items, item, CB, KT);
+  for (Turn turn; turn.item < items.total; turn.next(a, items.total)) {
+    const Item I(a, items, turn.item, CB, KT);
     const uint32_t k0 = I.k0, k1 = I.k1;
     // ---- this wave's share of a stage: KT / 4 rows of K and of V, all of one page ----
     constexpr uint32_t SHARE = KT / 4, RPI = 1024 / ROWB, INSTR = SHARE / RPI;  // rows to an instruction
@@ -1348,6 +1392,7 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
       ROWS::add_pv(v, hn, hg, S, O);
     }
     if (bad) paged_err(a.err, PAGED_ERR_ATT_PAGE, I.b);
+    turn.take(a, items.total);
 
     // ---- out, or a partial ----
     float* mine = a.parts + (size_t)I.part * CB * (hd + 2);

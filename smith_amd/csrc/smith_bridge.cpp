@@ -332,16 +332,17 @@ int ensure_amx(Ctx* c) {
   return 0;
 }
 
-// One counter to a partial of smith_paged_attention, whatever the call.
+// One counter to a partial of smith_paged_attention, whatever the call, and the
+// queue of its items.
 constexpr uint32_t PAGED_COUNTERS = 4096;
 
 int ensure_paged_counters(Ctx* c) {
   if (c->paged_cnt) return 0;
   if (c->capturing)
     return fail(c, "smith_paged_attention: counters needed while capturing a graph; run the op once first");
-  HIPCHK(c, hipMalloc((void**)&c->paged_cnt, PAGED_COUNTERS * sizeof(uint32_t)));
-  c->allocated += PAGED_COUNTERS * sizeof(uint32_t);
-  return zero_now(c, c->paged_cnt, PAGED_COUNTERS * sizeof(uint32_t));
+  HIPCHK(c, hipMalloc((void**)&c->paged_cnt, (PAGED_COUNTERS + 1) * sizeof(uint32_t)));
+  c->allocated += (PAGED_COUNTERS + 1) * sizeof(uint32_t);
+  return zero_now(c, c->paged_cnt, (PAGED_COUNTERS + 1) * sizeof(uint32_t));
 }
 
 // Kernel argument of smith_lmhead_q4_0_nb (same layout as the device struct).
@@ -2447,9 +2448,9 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   const bool many = row_start && !small && (uint64_t)max_rows * G > 24ull * n_req;
   const uint32_t CB = !many ? 16 : kv_type == SMITH_KV_F32 ? 64 : 128, dims = head_dim <= 64 ? 64 : 128;
   const uint32_t target = 512;  // two workgroups to a CU
-  // a block that is cut has 1.5 C keys or more and so at most 4/3 of its keys / C
-  // splits: 4/3 W / C <= 4/3 target of them in all (and some for what f32 rounds)
-  const uint32_t max_parts = target + target / 3 + 16;
+  // a block that is cut has more than C keys and so less than twice its keys / C
+  // splits: 2 W / C <= 2 target of them in all (and some for what f32 rounds)
+  const uint32_t max_parts = 2 * target + 16;
   if (ensure(c, &c->paged_ws, &c->paged_ws_bytes, (size_t)max_parts * CB * (head_dim + 2) * sizeof(float))) return -1;
   if (ensure_paged_counters(c)) return -1;
   const uint32_t heads_blk = std::min(G, CB), RB = CB / heads_blk, groups = (G + CB - 1) / CB;
@@ -2458,17 +2459,18 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   const uint32_t grid = (uint32_t)std::min<uint64_t>({(uint64_t)target, blocks + max_parts, blocks * longest});
   // of attention_body: O and (m, l) of four waves; of attention_rows_body: two
   // stages of K and V rows (64 of f16 / bf16 or 32 of f32: 256 bytes a head dim) and their marks
-  const uint32_t lds = (many ? 256 * 2 * dims + 16 : 4 * 16 * (dims + 4) * 4 + 4 * 16 * 2 * 4) + 16 * (n_req + 1);
+  const uint32_t lds = (many ? 256 * 2 * dims + 16 : 4 * 16 * (dims + 4) * 4 + 4 * 16 * 2 * 4) + 20 * (n_req + 1);
   struct {
     const float* q;
     const int32_t *row_start, *lens, *tables;
     const void *kpages, *vpages;
     float *out, *parts;
-    uint32_t* counters;
+    uint32_t *counters, *queue;
     uint64_t* err;
     uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift, rows_blk, heads_blk, groups;
     float per_target, scale;
-  } a = {q, row_start, lens, tables, kpages, vpages, out, (float*)c->paged_ws, c->paged_cnt, c->paged_err_dev(),
+  } a = {q, row_start, lens, tables, kpages, vpages, out, (float*)c->paged_ws, c->paged_cnt, c->paged_cnt + PAGED_COUNTERS,
+         c->paged_err_dev(),
          ld_q, ld_out, max_rows, n_req, max_pages, n_kv_heads, G, head_dim, n_pages, shift, RB, heads_blk, groups,
          (float)n_kv_heads / (float)target, scale};
   char name[64];
