@@ -795,74 +795,170 @@ struct Turn {
   }
 };
 
-// A split is through: its partial [CB][hd] and (m, l) [CB] are written (by all
-// of the workgroup); the last split of the block joins them.  s: LDS of
-// PAGED_SPLIT_MAX * 16 + 128 floats that nobody uses any more.
-__device__ __forceinline__ void join_splits(const AttArgs& a, const Item& I, uint32_t CB, float* s) {
+// A split is through: its partial [CB][hd] and (m, l) [CB] are written by all of
+// the workgroup.  True in the last split of the block, which joins them.
+__device__ __forceinline__ bool last_split(const AttArgs& a, const Item& I) {
   __shared__ uint32_t s_last;
+  uint32_t* done = a.counters + (I.part - I.split * a.nKV);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s_last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == I.ns - 1;
+    if (s_last) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return s_last;
+}
+
+// A block of at most 16 columns.  s: LDS of PAGED_SPLIT_MAX * 16 + 128 floats that
+// nobody uses any more.
+__device__ __forceinline__ void join_16(const AttArgs& a, const Item& I, float* s) {
+  constexpr uint32_t CB = 16;
+  if (!last_split(a, I)) return;
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6, ln = lane & 15, lg = lane >> 4;
   const uint32_t hd = a.hd, ns = I.ns, ncols = I.ncols, first = I.part - I.split * a.nKV;
   float *s_o = s, *s_ml = s + PAGED_SPLIT_MAX * 16;
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (tid == 0)
-    s_last = __hip_atomic_fetch_add(a.counters + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ns - 1;
-  __syncthreads();
-  if (!s_last) return;
   const float* all = a.parts + (size_t)first * CB * (hd + 2);
   const size_t stride = (size_t)a.nKV * CB * (hd + 2);
-  if (tid == 0) __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  for (uint32_t c0 = 0; c0 < ncols; c0 += 16) {
-    // weights 2^(m - max) of the splits, 16 threads to a column; 0 behind the last
-    constexpr int PER = PAGED_SPLIT_MAX / 16;
-    const uint32_t cc = c0 + ln < ncols ? c0 + ln : 0, sp0 = tid >> 4;
-    const float* ml = all + CB * hd + cc * 2;
-    float2 v[PER];
-    float mx = -__builtin_inff(), sum = 0.f;
+  // weights 2^(m - max) of the splits, 16 threads to a column; 0 behind the last
+  constexpr int PER = PAGED_SPLIT_MAX / 16;
+  const uint32_t cc = ln < ncols ? ln : 0, sp0 = tid >> 4;
+  const float* ml = all + CB * hd + cc * 2;
+  float2 v[PER];
+  float mx = -__builtin_inff(), sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < PER; k++) v[k] = get2(ml + (sp0 + 16 * k < ns ? sp0 + 16 * k : 0u) * stride);
+  for (int k = 0; k < PER; k++) v[k] = get2(ml + (sp0 + 16 * k < ns ? sp0 + 16 * k : 0u) * stride);
 #pragma unroll
-    for (int k = 0; k < PER; k++) {
-      if (sp0 + 16 * k >= ns) v[k] = make_float2(-__builtin_inff(), 0.f);
-      mx = fmaxf(mx, v[k].x);
-    }
-    mx = max_xor16_32(mx);
-    __syncthreads();
-    if (lg == 0) s_ml[w * 16 + ln] = mx;
-    __syncthreads();
-    mx = fmaxf(fmaxf(s_ml[ln], s_ml[16 + ln]), fmaxf(s_ml[32 + ln], s_ml[48 + ln]));
+  for (int k = 0; k < PER; k++) {
+    if (sp0 + 16 * k >= ns) v[k] = make_float2(-__builtin_inff(), 0.f);
+    mx = fmaxf(mx, v[k].x);
+  }
+  mx = max_xor16_32(mx);
+  if (lg == 0) s_ml[w * 16 + ln] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(s_ml[ln], s_ml[16 + ln]), fmaxf(s_ml[32 + ln], s_ml[48 + ln]));
 #pragma unroll
-    for (int k = 0; k < PER; k++) {
-      const float f = v[k].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(v[k].x - mx);
-      s_o[(sp0 + 16 * k) * 16 + ln] = f;
-      sum = __builtin_fmaf(f, v[k].y, sum);
-    }
-    sum = add_xor32(add_xor16(sum));
-    if (lg == 0) s_ml[64 + w * 16 + ln] = sum;
-    __syncthreads();
-    // a thread's pair of dims over the splits, JOIN_BATCH loads in flight;
-    // behind the last split it again, with a weight of 0
-    constexpr uint32_t JOIN_BATCH = 16;
-    const uint32_t nc = ncols - c0 < 16 ? ncols - c0 : 16;
-    for (uint32_t e = 2 * tid; e < nc * hd; e += 512) {
-      const uint32_t k = e / hd, d = e - k * hd;
-      const float* src = all + c0 * hd + e;
-      float2 o = make_float2(0.f, 0.f);
-      for (uint32_t s0 = 0; s0 < ns; s0 += JOIN_BATCH) {
-        float2 x[JOIN_BATCH];
+  for (int k = 0; k < PER; k++) {
+    const float f = v[k].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(v[k].x - mx);
+    s_o[(sp0 + 16 * k) * 16 + ln] = f;
+    sum = __builtin_fmaf(f, v[k].y, sum);
+  }
+  sum = add_xor32(add_xor16(sum));
+  if (lg == 0) s_ml[64 + w * 16 + ln] = sum;
+  __syncthreads();
+  // a thread's pair of dims over the splits, JOIN_BATCH loads in flight;
+  // behind the last split it again, with a weight of 0
+  constexpr uint32_t JOIN_BATCH = 16;
+  for (uint32_t e = 2 * tid; e < ncols * hd; e += 512) {
+    const uint32_t k = e / hd, d = e - k * hd;
+    const float* src = all + e;
+    float2 o = make_float2(0.f, 0.f);
+    for (uint32_t s0 = 0; s0 < ns; s0 += JOIN_BATCH) {
+      float2 x[JOIN_BATCH];
 #pragma unroll
-        for (uint32_t j = 0; j < JOIN_BATCH; j++) x[j] = get2(src + (s0 + j < ns ? s0 + j : ns - 1) * stride);
+      for (uint32_t j = 0; j < JOIN_BATCH; j++) x[j] = get2(src + (s0 + j < ns ? s0 + j : ns - 1) * stride);
 #pragma unroll
-        for (uint32_t j = 0; j < JOIN_BATCH; j++) {
-          const float f = s_o[(s0 + j) * 16 + k];
-          o.x = __builtin_fmaf(f, x[j].x, o.x);
-          o.y = __builtin_fmaf(f, x[j].y, o.y);
-        }
+      for (uint32_t j = 0; j < JOIN_BATCH; j++) {
+        const float f = s_o[(s0 + j) * 16 + k];
+        o.x = __builtin_fmaf(f, x[j].x, o.x);
+        o.y = __builtin_fmaf(f, x[j].y, o.y);
       }
-      const float tot = s_ml[64 + k] + s_ml[80 + k] + s_ml[96 + k] + s_ml[112 + k];
-      float* y = a.out + I.at(c0 + k, a.ld_out, hd) + d;
+    }
+    const float tot = s_ml[64 + k] + s_ml[80 + k] + s_ml[96 + k] + s_ml[112 + k];
+    float* y = a.out + I.at(k, a.ld_out, hd) + d;
+    y[0] = o.x / tot;
+    y[1] = o.y / tot;
+  }
+}
+
+// Blocks of more columns.  s: LDS of `room` floats, JOIN_ROOM at least, that
+// nobody uses any more.
+#define JOIN_ROOM (PAGED_SPLIT_MAX * 16 * 2 + 256)
+__device__ __forceinline__ void join_many(const AttArgs& a, const Item& I, uint32_t CB, float* s, uint32_t room) {
+  if (!last_split(a, I)) return;
+  const uint32_t tid = threadIdx.x, hd = a.hd, ns = I.ns, ncols = I.ncols, first = I.part - I.split * a.nKV;
+  const float* all = a.parts + (size_t)first * CB * (hd + 2);
+  const size_t stride = (size_t)a.nKV * CB * (hd + 2);
+  // as many columns at once as (m, l) of their splits fit: 16, 32, .. 128
+  uint32_t lw = 4;
+  while (lw < 7 && (1u << lw) < ncols && (ns << (lw + 2)) + 256 <= room) lw++;
+  const uint32_t width = 1u << lw, group = tid >> lw, groups = 256u >> lw;
+  float *s_m = s + 256, *s_l = s_m + (ns << lw);  // [ns][width]; s: a number of each thread's
+  for (uint32_t c0 = 0; c0 < ncols; c0 += width) {
+    // weights 2^(m - max) of the splits: groups of threads, each some splits of all columns
+    const uint32_t c = tid & (width - 1);
+    const float* ml = all + CB * hd + (c0 + c < ncols ? c0 + c : 0) * 2;
+    float mx = -__builtin_inff(), sum = 0.f;
+    if (c0) __syncthreads();  // the columns before are through
+#pragma unroll 8
+    for (uint32_t k = group; k < ns; k += groups) {
+      const float2 v = get2(ml + k * stride);
+      s_m[(k << lw) + c] = v.x;
+      s_l[(k << lw) + c] = v.y;
+      mx = fmaxf(mx, v.x);
+    }
+    s[tid] = mx;
+    __syncthreads();
+    for (uint32_t k = 0; k < groups; k++) mx = fmaxf(mx, s[(k << lw) + c]);
+    for (uint32_t k = group; k < ns; k += groups) {
+      const float m = s_m[(k << lw) + c], f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+      s_m[(k << lw) + c] = f;
+      sum = __builtin_fmaf(f, s_l[(k << lw) + c], sum);
+    }
+    __syncthreads();
+    s[tid] = sum;
+    __syncthreads();
+    const uint32_t nc = ncols - c0 < width ? ncols - c0 : width;
+    auto put = [&](uint32_t e, float2 o) {
+      const uint32_t k = e / hd;
+      float tot = 0.f;
+      for (uint32_t g = 0; g < groups; g++) tot += s[(g << lw) + k];
+      float* y = a.out + I.at(c0 + k, a.ld_out, hd) + (e - k * hd);
       y[0] = o.x / tot;
       y[1] = o.y / tot;
+    };
+    // pairs of dims, 16 loads in flight: of the splits where there are many, of
+    // the thread's next pairs where there are few; what is behind the last split
+    // or pair is loaded as that and weighs 0 or is not written
+    const uint32_t pairs = nc * hd / 2;
+    if (ns <= 4) {
+      for (uint32_t e0 = tid; e0 < pairs; e0 += 8 * 256) {
+        float2 o[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) o[j] = make_float2(0.f, 0.f);
+#pragma unroll 2
+        for (uint32_t k = 0; k < ns; k++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const uint32_t e = e0 + 256 * j < pairs ? e0 + 256 * j : pairs - 1;
+            const float2 x = get2(all + k * stride + c0 * hd + 2 * e);
+            const float f = s_m[(k << lw) + 2 * e / hd];
+            o[j].x = __builtin_fmaf(f, x.x, o[j].x);
+            o[j].y = __builtin_fmaf(f, x.y, o[j].y);
+          }
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (e0 + 256 * j < pairs) put(2 * (e0 + 256 * j), o[j]);
+      }
+    } else {
+      constexpr uint32_t BATCH = 16;
+      for (uint32_t e = tid; e < pairs; e += 256) {
+        const float* src = all + c0 * hd + 2 * e;
+        const uint32_t k = 2 * e / hd;
+        float2 o = make_float2(0.f, 0.f);
+        for (uint32_t s0 = 0; s0 < ns; s0 += BATCH) {
+          float2 x[BATCH];
+#pragma unroll
+          for (uint32_t j = 0; j < BATCH; j++) x[j] = get2(src + (s0 + j < ns ? s0 + j : ns - 1) * stride);
+#pragma unroll
+          for (uint32_t j = 0; j < BATCH; j++) {
+            const float f = s0 + j < ns ? s_m[((s0 + j) << lw) + k] : 0.f;
+            o.x = __builtin_fmaf(f, x[j].x, o.x);
+            o.y = __builtin_fmaf(f, x[j].y, o.y);
+          }
+        }
+        put(2 * e, o);
+      }
     }
   }
 }
@@ -1099,7 +1195,7 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
         if (d0 == 0) put2(mine + CB * hd + col * 2, mx, sum);
       }
     }
-    if (I.ns > 1) join_splits(a, I, CB, s_o);
+    if (I.ns > 1) join_16(a, I, s_o);
   }
 }
 
@@ -1267,7 +1363,7 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
   typedef typename ROWS::T T;
   constexpr int CT = ROWS::CT, KT = ROWS::KT, NJ = ROWS::NJ, QREG = TILE::QREG;
   constexpr uint32_t CB = 64 * CT, ROWB = ROWS::ROWB, CHUNKS = ROWS::CHUNKS, REGION = KT * ROWB;
-  static_assert((PAGED_SPLIT_MAX * 16 + 128) * 4 <= 4 * REGION, "the weights of a join fit in the stages");
+  static_assert(JOIN_ROOM * 4 <= 4 * REGION, "the weights of a join fit in the stages");
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];  // [2 stages][K, V][KT rows]
   uint32_t* s_odd = (uint32_t*)(lds + 4 * REGION);                // [2 stages][2] a bit to a key
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
@@ -1417,7 +1513,7 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
         if (lg == 0) put2(mine + CB * hd + col * 2, m[t], l[t]);
       }
     }
-    if (I.ns > 1) join_splits(a, I, CB, (float*)lds);
+    if (I.ns > 1) join_many(a, I, CB, (float*)lds, REGION);
   }
 }
 
