@@ -28,6 +28,7 @@ import os
 import numpy as np
 
 from . import device
+from .paged import ROPE_ROW
 
 # SMITH_DECODE_GRAPH=0 runs every decode step eagerly (kernel-level profilers
 # that cannot trace graph replays); results are identical.
@@ -233,9 +234,11 @@ class _Engine:
     def lm_head_rows(self, model, r0, M, out_ptr):
         """lm_head of rows x[r0:r0+M] into [M, vocab] at out_ptr: one launch over
         the rows for a Q4_0 or Q6_K head, else row by row."""
+        self._lm_head_rows_at(model, self.x.ptr + r0 * self.cfg["dim"] * 4, M, out_ptr)
+
+    def _lm_head_rows_at(self, model, x, M, out_ptr):
         cfg, ctx = self.cfg, device.ops_ctx()
         head, g, eps = model["lmHead"], model["lnFGamma"].ptr, model["normEps"]
-        x = self.x.ptr + r0 * cfg["dim"] * 4
         if head["kind"] == "q4_0_nb":
             rc = device.lib.smith_lmhead_q4_0_rows(ctx, x, M, g, eps, head["nib"].ptr, head["d"].ptr, out_ptr,
                                                    cfg["dim"], cfg["vocabSize"])
@@ -248,6 +251,48 @@ class _Engine:
             for r in range(M):
                 self.lm_head(model, x + r * cfg["dim"] * 4, out_ptr + r * cfg["vocabSize"] * 4)
 
+    def _row_logits(self):
+        if self.row_logits is None:
+            from .gguf_loader import DeviceArray
+            step, vocab = _chunk_rows(self.cfg), self.cfg["vocabSize"]
+            self.row_logits = DeviceArray((min(step, max(64, ROW_LOGITS_BYTES // (vocab * 4) // 64 * 64)), vocab))
+        return self.row_logits
+
+    def paged_step(self, model, tokens, cache):
+        """Rows of several requests (tokens[b]: request b's) through every layer on
+        a PagedCache; the logits of each request's last row, in order."""
+        cfg, ctx, eps = self.cfg, device.ops_ctx(), model["normEps"]
+        dim, vocab, H, hd, ld = cfg["dim"], cfg["vocabSize"], cfg["numHeads"], cfg["headDim"], self.qkv_ld
+        added = [len(t) for t in tokens]
+        M = sum(added)
+        if M > _chunk_rows(cfg):
+            raise ValueError("paged step: %d rows (at most %d)" % (M, _chunk_rows(cfg)))
+        plan = cache.plan(added)
+        self.embed(model, [t for req in tokens for t in req])
+        x, x2, qkv, attn, h = self.x.ptr, self.x2.ptr, self.qkv.ptr, self.attn.ptr, self.h.ptr
+        rope = model["rope"]
+        for li, blk in enumerate(model["blocks"]):
+            blk["qkv"](x, qkv, M, gamma=blk["ln1Gamma"].ptr, eps=eps)
+            cache.append(li, plan, qkv, ld, M, H, ROPE_ROW, rope["cos"].ptr, rope["sin"].ptr, rope["cos"].shape[0])
+            cache.attention(li, plan, qkv, ld, M, H, attn)
+            blk["outProj"](attn, x2, M, resid=x, epilogue=1)
+            blk["gateUp"](x2, h, M, gamma=blk["ln2Gamma"].ptr, eps=eps, epilogue=2)
+            blk["ffnDown"](h, x, M, resid=x2, epilogue=1)
+        # the last rows side by side (where every request has one row they are)
+        last = [r - 1 for r, n in zip(np.cumsum(added), added) if n]
+        rows = x
+        if len(last) < M:
+            rows = x2
+            for i, r in enumerate(last):
+                device.check(device.lib.smith_copy_d2d(ctx, x2, i * dim * 4, x, int(r) * dim * 4, dim * 4), "last rows")
+        logits = np.empty((len(last), vocab), np.float32)
+        out = self._row_logits()
+        for b0 in range(0, len(last), out.shape[0]):
+            b1 = min(len(last), b0 + out.shape[0])
+            self._lm_head_rows_at(model, rows + b0 * dim * 4, b1 - b0, out.ptr)
+            device.download_into(logits[b0:b1], out.ptr)
+        return logits
+
     def prefill(self, model, tokens, caches, all_logits=False):
         """Prompt rows in chunks of <= 256 (attention keeps a chunk's keys in
         LDS); returns the logits of every row if asked, else of the last."""
@@ -257,10 +302,7 @@ class _Engine:
         step, dim, vocab = _chunk_rows(self.cfg), self.cfg["dim"], self.cfg["vocabSize"]
         logits = np.empty((n, vocab), np.float32) if all_logits else None
         if all_logits:
-            if self.row_logits is None:
-                from .gguf_loader import DeviceArray
-                self.row_logits = DeviceArray((min(step, max(64, ROW_LOGITS_BYTES // (vocab * 4) // 64 * 64)), vocab))
-            block = self.row_logits.shape[0]
+            block = self._row_logits().shape[0]
         for r0 in range(0, n, step):
             r1 = min(n, r0 + step)
             self.embed(model, tokens[r0:r1])
@@ -313,6 +355,22 @@ def forwardLlamaCachedDecode(model, tokenId, position, caches):
     for c in caches:
         c["len"] = position + 1
     return {"logits": e.logits.numpy()[None, :].copy()}
+
+
+def forwardPagedStep(model, tokens, cache):
+    """One step of several requests on a PagedCache (paged.py): tokens[b] are the
+    new tokens of request b, any number of them -- a prompt, a chunk of one, the
+    last token that was generated, none -- up to 256 in all.  Returns {'logits':
+    [n, vocab] (host), 'requests': the n requests that had tokens}: the logits
+    behind each one's last token."""
+    e = _engine(model)
+    tokens = [list(t) for t in tokens]
+    if len(tokens) != cache.requests:
+        raise ValueError("paged step: tokens of %d requests for a cache of %d" % (len(tokens), cache.requests))
+    for n, t in zip(cache.lens, tokens):
+        if t:
+            _check_rope_range(e.cfg, int(n) + len(t) - 1)
+    return {"logits": e.paged_step(model, tokens, cache), "requests": [b for b, t in enumerate(tokens) if t]}
 
 
 # --- host sampling (generate.js:11-70), used when temperature > 0 or a

@@ -21,8 +21,9 @@ import numpy as np
 
 from . import device
 from . import gguf as G
-from .gguf_cache import (createGGUFCache, forwardLlamaCachedDecode, forwardLlamaCachedPrefill, generateGGUF,
-                         resetCache)
+from .gguf_cache import (createGGUFCache, forwardLlamaCachedDecode, forwardLlamaCachedPrefill, forwardPagedStep,
+                         generateGGUF, resetCache)
+from .paged import createPagedCache
 
 LLAMA_MAP = {
     "token_embd.weight": "embedding.tokenWeight",
@@ -472,7 +473,7 @@ def loadGGUF(path):
         return GGUFModel(model=model, config=config, metadata=parsed["metadata"], loaded=loaded, skipped=skipped,
                          forward=unsupported, createCache=lambda: createGGUFCache(model["config"]),
                          forwardPrefill=unsupported, forwardDecode=unsupported, generate=unsupported,
-                         resetCache=resetCache)
+                         createPagedCache=unsupported, forwardPagedStep=unsupported, resetCache=resetCache)
     model = createGGUFModel(config)
     res = loadWeights(parsed, model)
     return GGUFModel(
@@ -483,5 +484,8 @@ def loadGGUF(path):
         forwardDecode=lambda tokenId, position, caches: forwardLlamaCachedDecode(model, tokenId, position, caches),
         generate=lambda promptIds, genConfig=None, callbacks=None: generateGGUF(model, promptIds, genConfig or {},
                                                                                callbacks or {}),
+        createPagedCache=lambda requests, pages, pageSize=16, dtype="f16": createPagedCache(
+            model["config"], requests, pages, pageSize, dtype),
+        forwardPagedStep=lambda tokens, cache: forwardPagedStep(model, tokens, cache),
         resetCache=resetCache,
     )

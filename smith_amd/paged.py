@@ -96,3 +96,103 @@ def pagedAttention(q, lens, tables, kPages, vPages, rowStart=None, scale=0.0, ou
         rowStart.buffer if rowStart is not None else None, lens.buffer, tables.buffer, n, tables.shape[1], width // hd,
         nKV, hd, scale, kPages.buffer, vPages.buffer, nPages, P, out.buffer, width), "pagedAttention")
     return out
+
+
+class PagedCache:
+    """The paged cache of a model's requests: per layer the pools k and v, and on
+    the device the block tables [requests, maxPages], lengths and free list, which
+    the host mirrors in `lens` and `freeCount`.  A request is its number, 0 ..
+    requests - 1; it takes pages as it grows and gives them back with release()."""
+
+    def __init__(self, config, requests, pages, pageSize=16, dtype="f16"):
+        if dtype not in KV_TYPES:
+            raise ValueError("createPagedCache: pages of %s (f32, f16 or bf16)" % dtype)
+        if not 1 <= requests <= MAX_REQUESTS:
+            raise ValueError("createPagedCache: %d requests (1 .. %d)" % (requests, MAX_REQUESTS))
+        if pageSize < 1 or pageSize & (pageSize - 1):
+            raise ValueError("createPagedCache: page size %d is no power of two" % pageSize)
+        if pages < 1 or pages * pageSize >= 1 << 31:
+            raise ValueError("createPagedCache: %d pages of %d keys" % (pages, pageSize))
+        self.requests, self.pages, self.pageSize, self.dtype = requests, pages, pageSize, dtype
+        self.maxPages = -(-config["maxSeqLen"] // pageSize)
+        shape = [pages, config["numKVHeads"], pageSize, config["headDim"]]
+        self.layers = [{"k": T.create(shape, dtype), "v": T.create(shape, dtype)} for _ in range(config["numLayers"])]
+        self.lens = np.zeros(requests, np.int32)
+        self.freeCount = pages
+        self._tables = T.zeros([requests, self.maxPages], "i32")
+        self._free = T.tensor(np.arange(pages - 1, -1, -1), dtype="i32")  # page 0 goes first
+        # what a step reads and what it writes, in turn
+        self._lens = [T.zeros([requests], "i32"), T.zeros([requests], "i32")]
+        self._count = [T.tensor([pages], dtype="i32"), T.tensor([pages], dtype="i32")]
+        self._turn = 0
+        self._added = T.zeros([requests], "i32")
+        self._row_start = T.zeros([requests + 1], "i32")
+        self._rows = None
+
+    def plan(self, added):
+        """The step in which request b brings added[b] rows: {rowStart, lens, slots,
+        positions, tables}.  Nothing happens (ValueError) if it does not fit."""
+        added = np.asarray(added, np.int32)
+        rows = int(added.sum())
+        lens = self.lens + added
+        if added.shape != (self.requests,) or (added < 0).any() or not rows:
+            raise ValueError("paged step: the rows of %d requests, one at least" % self.requests)
+        if (lens > self.maxPages * self.pageSize).any():
+            raise ValueError("paged step: request %d grows past %d keys" % (int(lens.argmax()), self.maxPages * self.pageSize))
+        new = int((-(-lens // self.pageSize) - -(-self.lens // self.pageSize)).sum())
+        if new > self.freeCount:
+            raise ValueError("paged step: %d new pages, %d are free" % (new, self.freeCount))
+        if self._rows is None or self._rows["slots"].shape[0] < rows:
+            # rows behind a step's last stay at slot -1: one pair of buffers serves all sizes up to theirs
+            room = max(256, rows)
+            for t in (self._rows or {}).values():
+                t.release()
+            self._rows = {"slots": T.create([room], "i32"), "positions": T.create([room], "i32")}
+        self._added.set_data(added)
+        a, b = self._turn, 1 - self._turn
+        slots, positions = self._rows["slots"], self._rows["positions"]
+        device.check(device.lib.smith_paged_plan(
+            device.ops_ctx(), self._lens[a].buffer, self._added.buffer, self.requests, self._free.buffer,
+            self._count[a].buffer, self.pages, self.pageSize, self.maxPages, slots.shape[0], self._tables.buffer,
+            self._row_start.buffer, self._lens[b].buffer, slots.buffer, positions.buffer, self._count[b].buffer),
+            "paged step")
+        self._turn, self.lens, self.freeCount = b, lens, self.freeCount - new
+        return {"rowStart": self._row_start, "lens": self._lens[b], "slots": slots, "positions": positions,
+                "tables": self._tables}
+
+    def append(self, layer, plan, qkv, ld, rows, numHeads, rope, cos, sin, ropeLen):
+        """A layer's rows [q | k | v] (device pointer, row stride ld floats) into its
+        pages; q is rotated in place."""
+        k, v = self.layers[layer]["k"], self.layers[layer]["v"]
+        device.check(device.lib.smith_paged_append(
+            device.ops_ctx(), KV_TYPES[self.dtype], qkv, ld, rows, plan["slots"].buffer, plan["positions"].buffer,
+            numHeads, k.shape[1], k.shape[3], rope, cos, sin, ropeLen, k.buffer, v.buffer, self.pages, self.pageSize,
+            qkv, ld), "paged append")
+
+    def attention(self, layer, plan, q, ld, rows, numHeads, out):
+        """A layer's attention of the step's rows into out [rows, numHeads * headDim]."""
+        k, v = self.layers[layer]["k"], self.layers[layer]["v"]
+        device.check(device.lib.smith_paged_attention(
+            device.ops_ctx(), KV_TYPES[self.dtype], q, ld, rows, plan["rowStart"].buffer, plan["lens"].buffer,
+            plan["tables"].buffer, self.requests, self.maxPages, numHeads, k.shape[1], k.shape[3], 0.0, k.buffer,
+            v.buffer, self.pages, self.pageSize, out, numHeads * k.shape[3]), "paged attention")
+
+    def release(self, request):
+        """The request's pages back to the free list; its number is free for another."""
+        n = -(-int(self.lens[request]) // self.pageSize)
+        if not n:
+            return
+        a = self._turn
+        free = self._free.data
+        free[self.freeCount:self.freeCount + n] = self._tables.data[request, :n]
+        self._free.set_data(free)
+        self.freeCount += n
+        self.lens[request] = 0
+        self._count[a].set_data(np.array([self.freeCount], np.int32))
+        self._lens[a].set_data(self.lens)
+
+
+def createPagedCache(config, requests, pages, pageSize=16, dtype="f16"):
+    """A PagedCache for a model of this config (GGUFModel.config's fields of
+    createGGUFCache): pools of `pages` pages of pageSize keys per layer."""
+    return PagedCache(config, requests, pages, pageSize, dtype)
