@@ -583,9 +583,16 @@ struct AttArgs {
   float scale;
 };
 
-// by divisors that are mostly 1
-__device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t b) { return b == 1 ? a : a / b; }
-__device__ __forceinline__ uint32_t div_up(uint32_t a, uint32_t b) { return b == 1 ? a : (a + b - 1) / b; }
+// a / b: below 2^20 by a reciprocal, (a + 1/2) / b being 1 / 2b away from the next
+// whole number and off by less than a / b 2^-22
+__device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t b) {
+  if (a < 1u << 20) return (uint32_t)(((float)a + 0.5f) * __builtin_amdgcn_rcpf((float)b));
+  return a / b;
+}
+__device__ __forceinline__ uint32_t div_up(uint32_t a, uint32_t b) { return quotient(a + b - 1, b); }
+// of values that are the same in all lanes, in scalar registers
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+__device__ __forceinline__ uint32_t quotient_u(uint32_t a, uint32_t b) { return uniform(quotient(a, b)); }
 
 // a partial's words cross from one XCD's L2 to another's: written and read
 // through to the agent's coherence point
@@ -733,20 +740,19 @@ struct Item {
       if (from[mid] <= item) lo = mid;
       else top = mid;
     }
-    auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
     b = uniform(lo);
     r0 = uniform(t.row[b]);
     len = uniform(t.len[b]);
     const uint32_t local = item - uniform(from[b]);
     part = uniform(t.part[b]) + local;
     n = a.row_start ? uniform(t.row[b + 1]) - r0 : 1u;
-    ns = t.splits(len);
+    ns = uniform(t.splits(len));
     // the KV head first (neighbouring blocks of a head meet in one XCD's L2 when
     // there are 8 of them), the blocks with the most keys before the others
-    const uint32_t rest = quotient(local, a.nKV), later = quotient(rest, ns);
+    const uint32_t rest = quotient_u(local, a.nKV), later = quotient_u(rest, ns);
     kvh = local - rest * a.nKV;
     split = rest - later * ns;
-    const uint32_t blk = div_up(n, a.rows_blk) * a.groups - 1 - later, rowblk = quotient(blk, a.groups);
+    const uint32_t blk = quotient_u(n + a.rows_blk - 1, a.rows_blk) * a.groups - 1 - later, rowblk = quotient_u(blk, a.groups);
     head0 = (blk - rowblk * a.groups) * CB;
     heads = a.G - head0 < a.heads_blk ? a.G - head0 : a.heads_blk;
     head0 += kvh * a.G;
@@ -756,7 +762,7 @@ struct Item {
     // row i of the request sees len - n + i + 1 keys (a lone row without keys none)
     keys = len - n + row0 + rows;
     least = len - n + row0 + 1;
-    const uint32_t chunk = ns > 1 ? (div_up(keys, ns) + unit - 1) / unit * unit : keys;
+    const uint32_t chunk = ns > 1 ? (quotient_u(keys + ns - 1, ns) + unit - 1) / unit * unit : keys;
     const uint64_t at = (uint64_t)split * chunk;
     k0 = at < keys ? (uint32_t)at : keys;
     k1 = keys - k0 < chunk ? keys : k0 + chunk;
