@@ -394,28 +394,29 @@ struct Tile16 {
     }
   }
   // ... in parts, times +-1 and a power of two that brings its largest element
-  // to [2^14, 2^15); what is not finite stays as it is
+  // to [2^14, 2^15); what is not finite stays as it is.  Register k of the steps
+  // that do(s) says goes to put(k, parts).
+  template <class DO, class PUT>
   static __device__ __forceinline__ void split_q(const f32x4 (&x)[QRAW], bool there, uint32_t g, uint32_t hd, float sign,
-                                                 int& e2, u32x4 (&Q)[QREG]) {
-    float y[KS][8];
+                                                 int& e2, DO todo, PUT put) {
     float big = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        y[s][e] = there && s * 32 + 8 * g < hd ? x[2 * s + e / 4][e % 4] * sign : 0.f;
-        big = fmaxf(big, fabsf(y[s][e]));
-      }
+      for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[2 * s + e / 4][e % 4]));  // a repeated element is one of the row's
     big = max_xor16_32(big);
-    e2 = big > 0.f && big < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(big) : 0;
+    e2 = there && big > 0.f && big < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(big) : 0;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
+      if (!todo(s)) continue;
+      float y[8];
+      const bool in = there && s * 32 + 8 * g < hd;
 #pragma unroll
-      for (int e = 0; e < 8; e++) y[s][e] = __builtin_amdgcn_ldexpf(y[s][e], e2);
+      for (int e = 0; e < 8; e++) y[e] = in ? __builtin_amdgcn_ldexpf(x[2 * s + e / 4][e % 4] * sign, e2) : 0.f;
       u32x4 t[TERMS];
-      MM::split(y[s], t);
+      MM::split(y, t);
 #pragma unroll
-      for (int k = 0; k < TERMS; k++) Q[s * TERMS + k] = t[k];
+      for (int k = 0; k < TERMS; k++) put(s * TERMS + k, t[k]);
     }
   }
   // of the j-th 16 keys, lane n's: `off` values behind `key`
@@ -507,14 +508,16 @@ struct Tile32 {
       x[s] = load4(q + (e < hd ? e : hd - 4));
     }
   }
+  template <class DO, class PUT>
   static __device__ __forceinline__ void split_q(const f32x4 (&x)[QRAW], bool there, uint32_t g, uint32_t hd, float sign,
-                                                 int& e2, u32x4 (&Q)[QREG]) {
+                                                 int& e2, DO todo, PUT put) {
     e2 = 0;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
+      if (!todo(s)) continue;
       f32x4 y = x[s] * sign;
       if (!there || s * 16 + 4 * g >= hd) y = (f32x4){0.f, 0.f, 0.f, 0.f};
-      Q[s] = __builtin_bit_cast(u32x4, y);
+      put(s, __builtin_bit_cast(u32x4, y));
     }
   }
   __device__ __forceinline__ void load_k(int, const float* key, uint32_t off, uint32_t g, uint32_t hd) {
@@ -655,9 +658,31 @@ __device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Item
   t.part = t.shorts + a.n_req + 1;
   t.row = t.part + a.n_req + 1;
   t.len = t.row + a.n_req + 1;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6, RB = a.rows_blk, groups = a.groups;
+  auto set_work = [&](float work) { t.inv_c = 1.0f / fmaxf(work * a.per_target, (float)PAGED_SPLIT_MIN); };
+  if (a.n_req <= 64) {
+    // every wave for itself, request to lane: no barriers (they all write the same)
+    uint32_t r0 = 0, n = 0, len = 0;
+    if (lane < a.n_req) request(a, lane, blockIdx.x == 0, r0, n, len);
+    const uint32_t blocks = div_up(n, RB) * groups;
+    set_work(sum64_lanes((float)blocks * (float)len));
+    const uint32_t ns = t.splits(len), it = blocks * a.nKV * ns;
+    const bool lg = t.is_long(len);
+    const uint32_t il = scan64_lanes(lg ? it : 0u), is = scan64_lanes(lg ? 0u : it), ip = scan64_lanes(ns > 1 ? it : 0u);
+    t.total_long = (uint32_t)__builtin_amdgcn_readlane((int)il, 63);
+    t.total = t.total_long + (uint32_t)__builtin_amdgcn_readlane((int)is, 63);
+    if (lane < a.n_req) {
+      t.longs[lane] = il - (lg ? it : 0u);
+      t.shorts[lane] = is - (lg ? 0u : it);
+      t.part[lane] = ip - (ns > 1 ? it : 0u);
+      t.row[lane] = r0;
+      t.len[lane] = len;
+      if (lane + 1 == a.n_req) t.row[a.n_req] = r0 + n;
+    }
+    return;
+  }
   __shared__ float s_sum[4];
   __shared__ uint32_t s_wave[4][3];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6, RB = a.rows_blk, groups = a.groups;
   const uint32_t per = (a.n_req + 255) / 256;
   float work = 0.f;  // only a measure of how much there is: the cuts hold for any
   for (uint32_t k = 0; k < per; k++) {
@@ -673,8 +698,7 @@ __device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Item
   work = sum64_lanes(work);
   if (lane == 0) s_sum[w] = work;
   __syncthreads();
-  work = ((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3])) * a.per_target;
-  t.inv_c = 1.0f / fmaxf(work, (float)PAGED_SPLIT_MIN);
+  set_work((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]));
   uint32_t longs = 0, shorts = 0, parts = 0;
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
@@ -734,13 +758,14 @@ struct Item {
     // its class start there too)
     const uint32_t* from = item < t.total_long ? t.longs : t.shorts;
     if (item >= t.total_long) item -= t.total_long;
-    uint32_t lo = 0, top = a.n_req;
-    while (top - lo > 1) {
-      const uint32_t mid = (lo + top) >> 1;
-      if (from[mid] <= item) lo = mid;
-      else top = mid;
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = 0;
+    if (a.n_req > 64) {  // which 64 of them, then which one
+      const uint32_t k = lane * 64;
+      lo = 64 * (uint32_t)__popcll(__ballot(k < a.n_req && from[k < a.n_req ? k : 0] <= item)) - 64;
     }
-    b = uniform(lo);
+    const uint32_t k = lo + lane;
+    b = uniform(lo + (uint32_t)__popcll(__ballot(k < a.n_req && from[k < a.n_req ? k : 0] <= item)) - 1);
     r0 = uniform(t.row[b]);
     len = uniform(t.len[b]);
     const uint32_t local = item - uniform(from[b]);
@@ -1027,7 +1052,7 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
     const Item I(a, items, turn.item, CB, TK);
     const uint32_t k0 = I.k0, k1 = I.k1, kvh = I.kvh;
     f32x4 q_raw[TILE::QRAW];
-    if (w == 0) TILE::load_q(a.q + I.at(ln < I.ncols ? ln : 0, a.ld_q, hd), lg, hd, q_raw);
+    TILE::load_q(a.q + I.at(ln < I.ncols ? ln : 0, a.ld_q, hd), lg, hd, q_raw);
 
     // ---- this wave's keys, a tile's loads in flight before it is needed ----
     TILE tile;
@@ -1087,16 +1112,15 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
       load_v(t0);
     }
 
-    if (w == 0) {
+    float c;
+    {
+      // each wave splits the steps of its own number
       int e2;
-      u32x4 Q[QREG];
-      TILE::split_q(q_raw, ln < I.ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2, Q);
-#pragma unroll
-      for (int k = 0; k < QREG; k++) s_q[k * 64 + lane] = Q[k];
-      if (lg == 0) s_ml[ln] = score_factor(a.scale, e2);
+      TILE::split_q(q_raw, ln < I.ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2,
+                    [&](int s) { return (s & 3) == (int)w; }, [&](int k, u32x4 x) { s_q[k * 64 + lane] = x; });
+      c = score_factor(a.scale, e2);
     }
     __syncthreads();
-    const float c = s_ml[ln];
     const uint32_t limit = I.least + I.row_of(ln);
     f32x4 O[DPL];
     float m = -__builtin_inff(), l = 0.f;
@@ -1187,14 +1211,10 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
     float* mine = a.parts + (size_t)I.part * CB * (hd + 2);
     if (col < I.ncols && d0 < hd) {
       if (I.ns == 1) {
+        const float inv = I.keys ? 1.0f / sum : 0.f;
         float* y = a.out + I.at(col, a.ld_out, hd) + d0;
 #pragma unroll
-        for (int d = 0; d < DPL; d += 4) {
-          f32x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; e++) v[e] = I.keys ? o[d + e] / sum : 0.f;
-          store4(y + d, v);
-        }
+        for (int d = 0; d < DPL; d += 4) store4(y + d, (f32x4){o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv});
       } else {
 #pragma unroll
         for (int d = 0; d < DPL; d += 2) put2(mine + col * hd + d0 + d, o[d], o[d + 1]);
@@ -1427,7 +1447,8 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
     for (int t = 0; t < CT; t++) {
       const uint32_t col = (w * CT + t) * 16 + ln;
       int e2;
-      TILE::split_q(raw[t], col < I.ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2, Q[t]);
+      TILE::split_q(raw[t], col < I.ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2, [](int) { return true; },
+                    [&](int k, u32x4 x) { Q[t][k] = x; });
       c[t] = score_factor(a.scale, e2);
       limit[t] = I.least + I.row_of(col);
       m[t] = -__builtin_inff();
