@@ -5,9 +5,7 @@
 // the kernels keep prefix sums over the requests of a step in LDS
 #define PAGED_MAX_REQ 4096u
 
-// attention: fewest keys that a split is made for, most splits of a block (their
-// weights are kept in LDS, 16 columns of them)
-#define PAGED_SPLIT_MIN 128u
+// attention: most splits of a block (their weights are kept in LDS, 16 columns of them)
 #define PAGED_SPLIT_MAX 128u
 
 #define PAGED_ROPE_ROW 1u   // SMITH_ROPE_ROW

@@ -18,6 +18,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // rows and tables of the caller need start on no more than 4 bytes; the
 // hardware's 16-byte accesses want no more either
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x4_8 __attribute__((ext_vector_type(4), aligned(8)));
+__device__ __forceinline__ f32x4 load8(const float* p) { return *(const f32x4_8*)p; }
 __device__ __forceinline__ f32x4 load4(const float* p) { return *(const f32x4_any*)p; }
 __device__ __forceinline__ void store4(float* p, f32x4 v) { *(f32x4_any*)p = v; }
 
@@ -583,6 +585,7 @@ struct AttArgs {
   uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift;
   uint32_t rows_blk, heads_blk, groups;  // rows to a block of columns, heads of each, blocks to a row's heads
   float per_target;                     // KV heads / items wanted
+  float split_min;                      // least C
   float scale;
 };
 
@@ -659,7 +662,7 @@ __device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Item
   t.row = t.part + a.n_req + 1;
   t.len = t.row + a.n_req + 1;
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6, RB = a.rows_blk, groups = a.groups;
-  auto set_work = [&](float work) { t.inv_c = 1.0f / fmaxf(work * a.per_target, (float)PAGED_SPLIT_MIN); };
+  auto set_work = [&](float work) { t.inv_c = 1.0f / fmaxf(work * a.per_target, a.split_min); };
   if (a.n_req <= 64) {
     // every wave for itself, request to lane: no barriers (they all write the same)
     uint32_t r0 = 0, n = 0, len = 0;
@@ -907,6 +910,8 @@ __device__ __forceinline__ void join_16(const AttArgs& a, const Item& I, float* 
 #define JOIN_ROOM (PAGED_SPLIT_MAX * 16 * 2 + 256)
 __device__ __forceinline__ void join_many(const AttArgs& a, const Item& I, uint32_t CB, float* s, uint32_t room) {
   if (!last_split(a, I)) return;
+  // O is read with ordinary loads, 16 bytes each: nothing of it may be left in the caches
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   const uint32_t tid = threadIdx.x, hd = a.hd, ns = I.ns, ncols = I.ncols, first = I.part - I.split * a.nKV;
   const float* all = a.parts + (size_t)first * CB * (hd + 2);
   const size_t stride = (size_t)a.nKV * CB * (hd + 2);
@@ -940,55 +945,46 @@ __device__ __forceinline__ void join_many(const AttArgs& a, const Item& I, uint3
     s[tid] = sum;
     __syncthreads();
     const uint32_t nc = ncols - c0 < width ? ncols - c0 : width;
-    auto put = [&](uint32_t e, float2 o) {
-      const uint32_t k = e / hd;
+    auto put = [&](uint32_t e, f32x4 o) {
+      const uint32_t k = quotient(e, hd);
       float tot = 0.f;
       for (uint32_t g = 0; g < groups; g++) tot += s[(g << lw) + k];
-      float* y = a.out + I.at(c0 + k, a.ld_out, hd) + (e - k * hd);
-      y[0] = o.x / tot;
-      y[1] = o.y / tot;
+      store4(a.out + I.at(c0 + k, a.ld_out, hd) + (e - k * hd), o * (1.0f / tot));
     };
-    // pairs of dims, 16 loads in flight: of the splits where there are many, of
-    // the thread's next pairs where there are few; what is behind the last split
-    // or pair is loaded as that and weighs 0 or is not written
-    const uint32_t pairs = nc * hd / 2;
+    // four dims at a time, 8 loads in flight: of the splits where there are
+    // many, of the thread's next dims where there are few; what is behind the last
+    // split or dim is loaded as that and weighs 0 or is not written
+    const uint32_t quads = nc * hd / 4;
+    const float* src = all + c0 * hd;
     if (ns <= 4) {
-      for (uint32_t e0 = tid; e0 < pairs; e0 += 8 * 256) {
-        float2 o[8];
+      for (uint32_t e0 = tid; e0 < quads; e0 += 8 * 256) {
+        f32x4 o[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) o[j] = make_float2(0.f, 0.f);
+        for (int j = 0; j < 8; j++) o[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
         for (uint32_t k = 0; k < ns; k++)
 #pragma unroll
           for (int j = 0; j < 8; j++) {
-            const uint32_t e = e0 + 256 * j < pairs ? e0 + 256 * j : pairs - 1;
-            const float2 x = get2(all + k * stride + c0 * hd + 2 * e);
-            const float f = s_m[(k << lw) + 2 * e / hd];
-            o[j].x = __builtin_fmaf(f, x.x, o[j].x);
-            o[j].y = __builtin_fmaf(f, x.y, o[j].y);
+            const uint32_t e = 4 * (e0 + 256 * j < quads ? e0 + 256 * j : quads - 1);
+            o[j] += load8(src + k * stride + e) * s_m[(k << lw) + quotient(e, hd)];
           }
 #pragma unroll
         for (int j = 0; j < 8; j++)
-          if (e0 + 256 * j < pairs) put(2 * (e0 + 256 * j), o[j]);
+          if (e0 + 256 * j < quads) put(4 * (e0 + 256 * j), o[j]);
       }
     } else {
-      constexpr uint32_t BATCH = 16;
-      for (uint32_t e = tid; e < pairs; e += 256) {
-        const float* src = all + c0 * hd + 2 * e;
-        const uint32_t k = 2 * e / hd;
-        float2 o = make_float2(0.f, 0.f);
+      constexpr uint32_t BATCH = 8;
+      for (uint32_t e = 4 * tid; e < 4 * quads; e += 4 * 256) {
+        const uint32_t k = quotient(e, hd);
+        f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
         for (uint32_t s0 = 0; s0 < ns; s0 += BATCH) {
-          float2 x[BATCH];
+          f32x4 x[BATCH];
 #pragma unroll
-          for (uint32_t j = 0; j < BATCH; j++) x[j] = get2(src + (s0 + j < ns ? s0 + j : ns - 1) * stride);
+          for (uint32_t j = 0; j < BATCH; j++) x[j] = load8(src + (s0 + j < ns ? s0 + j : ns - 1) * stride + e);
 #pragma unroll
-          for (uint32_t j = 0; j < BATCH; j++) {
-            const float f = s0 + j < ns ? s_m[((s0 + j) << lw) + k] : 0.f;
-            o.x = __builtin_fmaf(f, x[j].x, o.x);
-            o.y = __builtin_fmaf(f, x[j].y, o.y);
-          }
+          for (uint32_t j = 0; j < BATCH; j++) o += x[j] * (s0 + j < ns ? s_m[((s0 + j) << lw) + k] : 0.f);
         }
-        put(2 * e, o);
+        put(e, o);
       }
     }
   }

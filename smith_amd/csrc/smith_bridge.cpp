@@ -2448,14 +2448,20 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   const bool many = row_start && !small && (uint64_t)max_rows * G > 24ull * n_req;
   const uint32_t CB = !many ? 16 : kv_type == SMITH_KV_F32 ? 64 : 128, dims = head_dim <= 64 ? 64 : 128;
   const uint32_t target = 512;  // two workgroups to a CU
-  // a block that is cut has more than C keys and so less than twice its keys / C
+  // Keys to a split at least.  A split of many columns leaves 64 KB and the join
+  // reads them again: 64 f16 rows behind 8000 keys, 32 heads, 65 us with 512, 78 with
+  // 384, 85 with 256 (300 rows of a prompt 23 us with 512, uncut, 46 with 128).  f32
+  // keys are eight times the work: 20 requests, half of them with chunks of up to 77
+  // rows, 68 us with 256, 92 with 512.
+  const float split_min = !many ? 128.f : kv_type == SMITH_KV_F32 ? 256.f : 512.f;
+  // a block that is cut has more than 5/4 C keys and so less than twice its keys / C
   // splits: 2 W / C <= 2 target of them in all (and some for what f32 rounds)
   const uint32_t max_parts = 2 * target + 16;
   if (ensure(c, &c->paged_ws, &c->paged_ws_bytes, (size_t)max_parts * CB * (head_dim + 2) * sizeof(float))) return -1;
   if (ensure_paged_counters(c)) return -1;
   const uint32_t heads_blk = std::min(G, CB), RB = CB / heads_blk, groups = (G + CB - 1) / CB;
   const uint64_t blocks = (uint64_t)groups * n_kv_heads * (row_start ? (uint64_t)n_req + max_rows / RB : n_req);
-  const uint64_t longest = ((uint64_t)max_pages << shift) / PAGED_SPLIT_MIN + 1;  // splits of one block
+  const uint64_t longest = ((uint64_t)max_pages << shift) / (uint32_t)split_min + 1;  // splits of one block
   const uint32_t grid = (uint32_t)std::min<uint64_t>({(uint64_t)target, blocks + max_parts, blocks * longest});
   // of attention_body: O and (m, l) of four waves; of attention_rows_body: two
   // stages of K and V rows (64 of f16 / bf16 or 32 of f32: 256 bytes a head dim) and their marks
@@ -2468,11 +2474,11 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
     uint32_t *counters, *queue;
     uint64_t* err;
     uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift, rows_blk, heads_blk, groups;
-    float per_target, scale;
+    float per_target, split_min, scale;
   } a = {q, row_start, lens, tables, kpages, vpages, out, (float*)c->paged_ws, c->paged_cnt, c->paged_cnt + PAGED_COUNTERS,
          c->paged_err_dev(),
          ld_q, ld_out, max_rows, n_req, max_pages, n_kv_heads, G, head_dim, n_pages, shift, RB, heads_blk, groups,
-         (float)n_kv_heads / (float)target, scale};
+         (float)n_kv_heads / (float)target, split_min, scale};
   char name[64];
   snprintf(name, sizeof name, "smith_paged_attention_%s%s_d%u%s", many ? "rows_" : "", kv_name(kv_type), dims, small ? "_s" : "");
   void* args[] = {&a};

@@ -346,6 +346,10 @@ def test_attention_one_long_request(dtype, n):
     (32, 8, 128, 32, [75, 200], [33, 3]),
     (20, 1, 96, 16, [40, 41], [13, 41]),                           # more heads to a KV head than a tile has columns
     (2, 2, 8, 1, [30, 2, 9], [30, 1, 4]),
+    (8, 1, 8, 16, [1500, 9], [1500, 2]),                           # more blocks than a wave has lanes
+    (8, 2, 16, 32, [4000, 60, 700], [100, 60, 1]),                 # a chunk far behind its cache, cut, beside short ones
+    (4, 4, 8, 16, [3000], [129]),
+    (6, 2, 24, 16, [900, 900, 900], [900, 450, 31]),
     (16, 4, 64, 64, [700], [9])])
 def test_attention_ragged_rows(dtype, H, nKV, D, P, lens, added):
     case = attention_case(H + sum(lens), dtype, H, nKV, D, P, lens, added)
