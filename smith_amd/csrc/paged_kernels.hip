@@ -854,6 +854,16 @@ __device__ __forceinline__ void join_16(const AttArgs& a, const Item& I, float* 
   float *s_o = s, *s_ml = s + PAGED_SPLIT_MAX * 16;
   const float* all = a.parts + (size_t)first * CB * (hd + 2);
   const size_t stride = (size_t)a.nKV * CB * (hd + 2);
+  // a thread's pair of dims over the splits, JOIN_BATCH loads in flight; behind
+  // the last split it again, with a weight of 0.  The first loads and those of (m,
+  // l) go out together.
+  constexpr uint32_t JOIN_BATCH = 16;
+  float2 x[JOIN_BATCH];
+  auto load = [&](uint32_t e, uint32_t s0) {
+    const float* src = all + (e < ncols * hd ? e : 0);
+#pragma unroll
+    for (uint32_t j = 0; j < JOIN_BATCH; j++) x[j] = get2(src + (s0 + j < ns ? s0 + j : ns - 1) * stride);
+  };
   // weights 2^(m - max) of the splits, 16 threads to a column; 0 behind the last
   constexpr int PER = PAGED_SPLIT_MAX / 16;
   const uint32_t cc = ln < ncols ? ln : 0, sp0 = tid >> 4;
@@ -862,6 +872,7 @@ __device__ __forceinline__ void join_16(const AttArgs& a, const Item& I, float* 
   float mx = -__builtin_inff(), sum = 0.f;
 #pragma unroll
   for (int k = 0; k < PER; k++) v[k] = get2(ml + (sp0 + 16 * k < ns ? sp0 + 16 * k : 0u) * stride);
+  load(2 * tid, 0);
 #pragma unroll
   for (int k = 0; k < PER; k++) {
     if (sp0 + 16 * k >= ns) v[k] = make_float2(-__builtin_inff(), 0.f);
@@ -880,28 +891,25 @@ __device__ __forceinline__ void join_16(const AttArgs& a, const Item& I, float* 
   sum = add_xor32(add_xor16(sum));
   if (lg == 0) s_ml[64 + w * 16 + ln] = sum;
   __syncthreads();
-  // a thread's pair of dims over the splits, JOIN_BATCH loads in flight;
-  // behind the last split it again, with a weight of 0
-  constexpr uint32_t JOIN_BATCH = 16;
   for (uint32_t e = 2 * tid; e < ncols * hd; e += 512) {
-    const uint32_t k = e / hd, d = e - k * hd;
-    const float* src = all + e;
+    const uint32_t k = quotient(e, hd), d = e - k * hd;
     float2 o = make_float2(0.f, 0.f);
-    for (uint32_t s0 = 0; s0 < ns; s0 += JOIN_BATCH) {
-      float2 x[JOIN_BATCH];
-#pragma unroll
-      for (uint32_t j = 0; j < JOIN_BATCH; j++) x[j] = get2(src + (s0 + j < ns ? s0 + j : ns - 1) * stride);
+    if (e >= 512) load(e, 0);
+    for (uint32_t s0 = 0;;) {
 #pragma unroll
       for (uint32_t j = 0; j < JOIN_BATCH; j++) {
         const float f = s_o[(s0 + j) * 16 + k];
         o.x = __builtin_fmaf(f, x[j].x, o.x);
         o.y = __builtin_fmaf(f, x[j].y, o.y);
       }
+      s0 += JOIN_BATCH;
+      if (s0 >= ns) break;
+      load(e, s0);
     }
-    const float tot = s_ml[64 + k] + s_ml[80 + k] + s_ml[96 + k] + s_ml[112 + k];
+    const float inv = 1.0f / (s_ml[64 + k] + s_ml[80 + k] + s_ml[96 + k] + s_ml[112 + k]);
     float* y = a.out + I.at(k, a.ld_out, hd) + d;
-    y[0] = o.x / tot;
-    y[1] = o.y / tot;
+    y[0] = o.x * inv;
+    y[1] = o.y * inv;
   }
 }
 
