@@ -1406,33 +1406,38 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
   for (Turn turn; turn.item < items.total; turn.next(a, items.total)) {
     const Item I(a, items, turn.item, CB, KT);
     const uint32_t k0 = I.k0, k1 = I.k1;
-    // ---- this wave's share of a stage: KT / 4 rows of K and of V, all of one page ----
-    constexpr uint32_t SHARE = KT / 4, RPI = 1024 / ROWB, INSTR = SHARE / RPI;  // rows to an instruction
+    // ---- this wave's share of a stage: KT / 4 rows of K and of V, 8 or 16, a page to 8 ----
+    constexpr uint32_t SHARE = KT / 4, RPI = 1024 / ROWB, PARTS = SHARE / 8, INSTR = 8 / RPI;  // rows, instructions to 8 rows
+    constexpr uint32_t AHEAD = 64 / PARTS;
     const int32_t* table = a.tables + (size_t)I.b * a.max_pages;
     const size_t head_len = (size_t)hd << a.shift;
-    uint32_t bad = 0, pages = 0, ahead = 64;  // lane x: page of this wave's rows x stages on
+    uint32_t bad = 0, pages = 0, ahead = AHEAD;  // lane PARTS x + h: page of this wave's h-th 8 rows x stages on
     auto fetch = [&](uint32_t t, uint32_t stage, uint32_t lane) {
-      if (ahead == 64) {
-        const uint32_t k = t + lane * KT + w * SHARE;
+      if (ahead == AHEAD) {
+        const uint32_t k = t + lane / PARTS * KT + w * SHARE + lane % PARTS * 8;
         const uint32_t p = (uint32_t)table[(k < k1 ? k : k1 - 1) >> a.shift];
         bad |= (uint32_t)(p >= a.n_pages);
         pages = p < a.n_pages ? p : 0u;
         ahead = 0;
       }
-      const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)ahead++);
-      const uint32_t first = t + w * SHARE;  // rows from k1 on: others of the page
-      const size_t at = ((size_t)p * a.nKV + I.kvh) * head_len + (size_t)(first & (P - 1)) * hd;
       const uint32_t to = lds0 + stage * 2 * REGION + w * SHARE * ROWB;
 #pragma unroll
-      for (uint32_t i = 0; i < INSTR; i++) {
-        const uint32_t r = i * RPI + lane / CHUNKS;  // row of the share
-        uint32_t c = (lane % CHUNKS) ^ swizzle<CHUNKS>(w * SHARE + r);
-        const uint32_t last = hd * sizeof(T) / 16 - 1;  // past the head: against zeros of Q, into dims that nobody reads
-        c = c < last ? c : last;
-        const uint32_t off = r * hd * sizeof(T) + c * 16;
-        dma16((const T*)a.kpages + at, off, to + i * 1024);
-        dma16((const T*)a.vpages + at, off, to + REGION + i * 1024);
+      for (uint32_t h = 0; h < PARTS; h++) {
+        const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)(ahead * PARTS + h));
+        const uint32_t first = t + w * SHARE + 8 * h;  // rows from k1 on: others of the page
+        const size_t at = ((size_t)p * a.nKV + I.kvh) * head_len + (size_t)(first & (P - 1)) * hd;
+#pragma unroll
+        for (uint32_t i = 0; i < INSTR; i++) {
+          const uint32_t r = i * RPI + lane / CHUNKS;  // row of the 8
+          uint32_t c = (lane % CHUNKS) ^ swizzle<CHUNKS>(w * SHARE + 8 * h + r);
+          const uint32_t last = hd * sizeof(T) / 16 - 1;  // past the head: against zeros of Q, into dims that nobody reads
+          c = c < last ? c : last;
+          const uint32_t off = r * hd * sizeof(T) + c * 16, piece = to + (h * INSTR + i) * 1024;
+          dma16((const T*)a.kpages + at, off, piece);
+          dma16((const T*)a.vpages + at, off, piece + REGION);
+        }
       }
+      ahead++;
     };
     // ---- this wave's columns, their loads ahead of the keys' ----
     f32x4 raw[CT][TILE::QRAW];

@@ -2441,11 +2441,11 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   // Where a request brings a row or so its columns (row, head) are few and its
   // keys the work: 16 columns to a workgroup, keys in registers.  Where the
   // columns fill most of two such tiles a workgroup shares the keys among four
-  // waves' columns.  Pages of less than 16 keys, looked up key by key, have the
-  // first kernel only.
+  // waves' columns; it loads 8 keys at once, of one page.  The first kernel takes
+  // 16 keys as one address, or looks them up one by one where pages are smaller.
   const uint32_t G = n_heads / n_kv_heads;
-  const bool small = shift < 4;
-  const bool many = row_start && !small && (uint64_t)max_rows * G > 24ull * n_req;
+  const bool many = row_start && shift >= 3 && (uint64_t)max_rows * G > 24ull * n_req;
+  const bool small = !many && shift < 4;
   const uint32_t CB = !many ? 16 : kv_type == SMITH_KV_F32 ? 64 : 128, dims = head_dim <= 64 ? 64 : 128;
   const uint32_t target = 512;  // two workgroups to a CU
   // Keys to a split at least.  A split of many columns leaves 64 KB and the join

@@ -350,6 +350,9 @@ def test_attention_one_long_request(dtype, n):
     (8, 2, 16, 32, [4000, 60, 700], [100, 60, 1]),                 # a chunk far behind its cache, cut, beside short ones
     (4, 4, 8, 16, [3000], [129]),
     (6, 2, 24, 16, [900, 900, 900], [900, 450, 31]),
+    (4, 1, 128, 8, [300, 41], [250, 41]),                          # pages of half a wave's share of a stage
+    (2, 2, 64, 8, [70, 200], [70, 111]),
+    (4, 1, 32, 4, [130, 9], [130, 9]),
     (16, 4, 64, 64, [700], [9])])
 def test_attention_ragged_rows(dtype, H, nKV, D, P, lens, added):
     case = attention_case(H + sum(lens), dtype, H, nKV, D, P, lens, added)
