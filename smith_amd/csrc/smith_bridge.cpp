@@ -2441,10 +2441,18 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   // Where a request brings a row or so its columns (row, head) are few and its
   // keys the work: 16 columns to a workgroup, keys in registers.  Where the
   // columns fill most of two such tiles a workgroup shares the keys among four
-  // waves' columns; it loads 8 keys at once, of one page.  The first kernel takes
-  // 16 keys as one address, or looks them up one by one where pages are smaller.
+  // waves' columns -- if there are enough of them for the waves of the card, which
+  // its 64 or 128 columns to a workgroup otherwise leave idle.  Microseconds, the
+  // first kernel's and the second's (32 heads on 8, f16 | bf16 | f32): a prompt of
+  // 300 rows (9600 columns) 18.5, 23.0 | 18.1, 27.2 | 22, 38; of 1000 rows 67, 51 |
+  // 68, 61 | 112, 132; of 2000 rows 195, 108 | 198, 133 | 389, 325; behind 8000 keys
+  // 64 rows (2048 columns) 53, 64 | 52, 75 | 109, 120, 256 rows (8192) 159, 105 |
+  // 155, 127 | 361, 319; 16 prompts of up to 200 rows 85, 41 | 88, 55 | 109, 79.
+  // The second loads 8 keys at once, of one page.  The first takes 16 keys as one
+  // address, or looks them up one by one where pages are smaller.
   const uint32_t G = n_heads / n_kv_heads;
-  const bool many = row_start && shift >= 3 && (uint64_t)max_rows * G > 24ull * n_req;
+  const bool many = row_start && shift >= 3 && (uint64_t)max_rows * G > 24ull * n_req &&
+                    (uint64_t)max_rows * n_heads >= 8192;
   const bool small = !many && shift < 4;
   const uint32_t CB = !many ? 16 : kv_type == SMITH_KV_F32 ? 64 : 128, dims = head_dim <= 64 ? 64 : 128;
   const uint32_t target = 512;  // two workgroups to a CU

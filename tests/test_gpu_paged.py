@@ -308,12 +308,24 @@ def check_attention(got, q, row_start, lens, tables, k, v, dtype, scale=None):
         assert np.linalg.norm(off) <= 1e-5 * norm, np.linalg.norm(off) / norm
 
 
-def run_attention(q, row_start, lens, tables, k, v, ragged, scale=0.0):
-    out = R.upload(np.full((len(q), q.shape[1] * q.shape[2]), 5, np.float32))
-    S.pagedAttention(R.upload(q.reshape(len(q), -1)), i32(lens), i32(tables), R.upload(k), R.upload(v),
+def room_for_many(H, nKV, n_req):
+    """max_rows with which the kernel of many rows answers: at least 8192 columns
+    (row, head) and more than 24 of a KV head to a request."""
+    return max(8192 // H, 24 * n_req * nKV // H) + 1
+
+
+def run_attention(q, row_start, lens, tables, k, v, ragged, scale=0.0, room=0):
+    """`room` rows in q and out, those behind the last sequence NaN in q; in out they stay."""
+    rows, W = len(q), q.shape[1] * q.shape[2]
+    room = max(room, rows)
+    hq = np.full((room, W), np.nan, np.float32)
+    hq[:rows] = q.reshape(rows, -1)
+    out = R.upload(np.full((room, W), 5, np.float32))
+    S.pagedAttention(R.upload(hq), i32(lens), i32(tables), R.upload(k), R.upload(v),
                      i32(row_start) if ragged else None, scale, out)
     device.sync()
-    return out.data
+    assert (out.data[rows:] == 5).all()
+    return out.data[:rows]
 
 
 LENGTHS = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200, 255, 256, 257, 511, 513, 1000]
@@ -353,10 +365,12 @@ def test_attention_one_long_request(dtype, n):
     (4, 1, 128, 8, [300, 41], [250, 41]),                          # pages of half a wave's share of a stage
     (2, 2, 64, 8, [70, 200], [70, 111]),
     (4, 1, 32, 4, [130, 9], [130, 9]),
+    (40, 1, 64, 16, [520, 7], [9, 7]),
     (16, 4, 64, 64, [700], [9])])
 def test_attention_ragged_rows(dtype, H, nKV, D, P, lens, added):
     case = attention_case(H + sum(lens), dtype, H, nKV, D, P, lens, added)
     check_attention(run_attention(*case, ragged=True), *case, dtype)
+    check_attention(run_attention(*case, ragged=True, room=room_for_many(H, nKV, len(lens))), *case, dtype)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
@@ -366,6 +380,63 @@ def test_attention_many_requests(dtype):
     added = np.minimum(rs.randint(0, 4, 1100), lens)
     case = attention_case(8, dtype, 4, 2, 16, 8, lens, added)
     check_attention(run_attention(*case, ragged=True), *case, dtype)
+    check_attention(run_attention(*case, ragged=True, room=room_for_many(4, 2, 1100)), *case, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_most_requests(dtype, D):
+    """4096 requests, the most that are taken: the largest request table in LDS."""
+    rs = np.random.RandomState(14)
+    lens = rs.randint(0, 20, 4096)
+    added = np.minimum(rs.randint(0, 3, 4096), lens)
+    lens[4095], added[4095] = 700, 2
+    case = attention_case(9, dtype, 2, 2, D, 16, lens, added)
+    check_attention(run_attention(*case, ragged=True), *case, dtype)
+    check_attention(run_attention(*case, ragged=True, room=room_for_many(2, 2, 4096)), *case, dtype)
+    one = attention_case(10, dtype, 2, 2, D, 16, lens, [1] * 4096)
+    check_attention(run_attention(*one, ragged=False), *one, dtype)
+
+
+def replays(launch, out, case, dtype):
+    """A captured call more than once, other work between: the same values each time."""
+    ctx = device.ops_ctx()
+    launch()
+    device.sync()
+    first = out.data.copy()
+    device.check(device.lib.smith_graph_begin(ctx), "begin")
+    launch()
+    g = device.lib.smith_graph_end(ctx)
+    assert g, last_error()
+    try:
+        for _ in range(4):
+            out.set_data(np.full(first.shape, 5, np.float32))
+            device.check(device.lib.smith_graph_launch(ctx, g))
+            device.sync()
+            assert np.array_equal(out.data, first)
+            other = attention_case(3, dtype, 8, 2, 32, 16, [400, 30], [1, 20])
+            check_attention(run_attention(*other, ragged=True), *other, dtype)
+    finally:
+        device.lib.smith_graph_destroy(g)
+    check_attention(first[:len(case[0])], *case, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("ragged,lens,added", [
+    (False, [900, 3, 40, 0, 2500] * 60, [1] * 300),        # 300 x 2 KV heads and more splits than workgroups
+    (True, [700, 60, 1] * 50, [9, 60, 1] * 50),
+    (True, [5000, 900, 33], [2000, 900, 33])])
+def test_attention_more_items_than_workgroups_replayed(dtype, ragged, lens, added):
+    """Workgroups that fetch further items off the queue, in a graph: what they
+    count with is as it was when they end, and a joined sum has one order."""
+    H, nKV = 8, 2
+    case = q, row_start, lens, tables, k, v = attention_case(31, dtype, H, nKV, 16, 16, lens, added)
+    rows = room_for_many(H, nKV, len(lens)) if ragged else len(q)
+    hq = np.zeros((max(rows, len(q)), H * 16), np.float32)
+    hq[:len(q)] = q.reshape(len(q), -1)
+    tq, tl, tt, tk, tv, tr = R.upload(hq), i32(lens), i32(tables), R.upload(k), R.upload(v), i32(row_start)
+    out = R.upload(np.full(hq.shape, 5, np.float32))
+    replays(lambda: S.pagedAttention(tq, tl, tt, tk, tv, tr if ragged else None, 0.0, out), out, case, dtype)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
@@ -377,9 +448,9 @@ def test_attention_request_without_keys_gives_zeros(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("ragged,room", [(False, 0), (True, 0), (True, room_for_many(6, 2, 4))])
 @pytest.mark.parametrize("junk", [np.nan, np.inf, -np.inf])
-def test_attention_ignores_what_a_row_does_not_see(dtype, ragged, junk):
+def test_attention_ignores_what_a_row_does_not_see(dtype, ragged, room, junk):
     """Slots behind a request's keys, pages of nobody and, for the rows before
     it, a later row's own key and value hold what is not finite."""
     lens, added = [5, 40, 64, 100], ([2, 20, 64, 1] if ragged else [1] * 4)
@@ -401,7 +472,7 @@ def test_attention_ignores_what_a_row_does_not_see(dtype, ragged, junk):
             for pool in (k, v):
                 pool[tables[b, t // P], :, t % P, 3] = bad
             poisoned.append(row_start[b + 1] - 1)
-        got = run_attention(q, row_start, lens, tables, k, v, True).reshape(q.shape)
+        got = run_attention(q, row_start, lens, tables, k, v, True, room=room).reshape(q.shape)
         assert not np.isfinite(got[poisoned][..., 3]).any()
         for pool in (k, v):
             pool[~np.isfinite(R.value(pool, dtype))] = clean
@@ -417,15 +488,17 @@ def test_attention_ignores_what_a_row_does_not_see(dtype, ragged, junk):
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("size", [1e-30, 1e-6, 1e4, 1e20])
-def test_attention_queries_of_any_size(dtype, size):
+@pytest.mark.parametrize("room", [0, room_for_many(4, 2, 2)])
+def test_attention_queries_of_any_size(dtype, size, room):
     """Queries far from 1 against a scale that brings the scores back."""
     q, row_start, lens, tables, k, v = attention_case(11, dtype, 4, 2, 64, 16, [300, 20], [3, 1])
-    check_attention(run_attention(q * np.float32(size), row_start, lens, tables, k, v, True, 0.125 / size),
+    check_attention(run_attention(q * np.float32(size), row_start, lens, tables, k, v, True, 0.125 / size, room),
                     q * np.float32(size), row_start, lens, tables, k, v, dtype, 0.125 / size)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-def test_attention_far_scores(dtype):
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attention_far_scores(dtype, ragged):
     """One key far above the others, one far below, equal ones: weights of one, of
     nothing, and all alike."""
     q, row_start, lens, tables, k, v = attention_case(12, dtype, 2, 1, 16, 8, [100, 100, 64], [1, 1, 1])
@@ -433,17 +506,18 @@ def test_attention_far_scores(dtype):
     q[2] = 0.0
     page = tables[0, 70 // 8]
     k[page, 0, 70 % 8] = R.stored(np.full(16, 3.0), dtype)
-    got = run_attention(q, row_start, lens, tables, k, v, False)
+    got = run_attention(q, row_start, lens, tables, k, v, ragged, room=room_for_many(2, 1, 3) if ragged else 0)
     check_attention(got, q, row_start, lens, tables, k, v, dtype)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-def test_attention_strides_and_rows_behind_the_last(dtype):
+@pytest.mark.parametrize("spare", [9, room_for_many(6, 3, 3)])
+def test_attention_strides_and_rows_behind_the_last(dtype, spare):
     """Row strides beyond the row, bases that are not 16-byte aligned, room for
     more rows than there are: everything else in out stays."""
     H, nKV, D, P = 6, 3, 56, 16
     q, row_start, lens, tables, k, v = attention_case(7, dtype, H, nKV, D, P, [20, 33, 50], [4, 1, 30])
-    rows, W, room = len(q), H * D, len(q) + 9
+    rows, W, room = len(q), H * D, len(q) + spare
     ld_q, ld_o = W + 3, W + 5
     hq = np.random.RandomState(1).standard_normal(1 + room * ld_q).astype(np.float32)
     ho = np.random.RandomState(2).standard_normal(3 + room * ld_o).astype(np.float32)
@@ -468,12 +542,14 @@ def test_attention_strides_and_rows_behind_the_last(dtype):
     ("rows", "row_start ends at 3"), ("rows_low", "row_start ends at -1"), ("short", "request 1: its length"),
     ("long", "request 1: its length"), ("negative", "request 1: its length"), ("page", "request 1: a page outside"),
     ("page_low", "request 1: a page outside")])
-def test_attention_leaves_out_what_does_not_fit(dtype, bad, message):
+@pytest.mark.parametrize("room", [2, room_for_many(4, 2, 2)])
+def test_attention_leaves_out_what_does_not_fit(dtype, bad, message, room):
     q, row_start, lens, tables, k, v = attention_case(5, dtype, 4, 2, 32, 16, [40, 30], [1, 1])
     want, _, _ = R.attention(q.astype(np.float64), row_start, lens, tables, R.value(k, dtype), R.value(v, dtype))
     rs, ln, tb = row_start.copy(), lens.copy(), tables.copy()
     if bad == "rows":
-        rs[2] = 3
+        rs[2] = room + 1
+        message = message.replace("3", str(room + 1))
     elif bad == "rows_low":
         rs[2] = -1
     elif bad == "short":
@@ -484,11 +560,14 @@ def test_attention_leaves_out_what_does_not_fit(dtype, bad, message):
         ln[1] = -3
     else:
         tb[1, 1] = -1 if bad == "page_low" else k.shape[0]
-    out = R.upload(np.full((2, 128), 5, np.float32))
-    S.pagedAttention(R.upload(q.reshape(2, -1)), i32(ln), i32(tb), R.upload(k), R.upload(v), i32(rs), 0.0, out)
+    out = R.upload(np.full((room, 128), 5, np.float32))
+    hq = np.zeros((room, 128), np.float32)
+    hq[:2] = q.reshape(2, -1)
+    S.pagedAttention(R.upload(hq), i32(ln), i32(tb), R.upload(k), R.upload(v), i32(rs), 0.0, out)
     assert message in sync_error()
     device.sync()
     got = out.data
+    assert (got[2:] == 5).all()
     if bad.startswith("rows"):
         assert (got == 5).all()
     else:
@@ -497,16 +576,18 @@ def test_attention_leaves_out_what_does_not_fit(dtype, bad, message):
             assert (got[1] == 5).all()
 
 
-def test_attention_row_start_out_of_order_stays_inside():
+@pytest.mark.parametrize("room", [4, room_for_many(4, 2, 3)])
+def test_attention_row_start_out_of_order_stays_inside(room):
     """Starts that go back and forth between 0 and the total: no request has
     rows outside the buffers, and the calls after it are right."""
     case = attention_case(6, "f16", 4, 2, 32, 16, [40, 30, 20], [2, 1, 1])
     q, row_start, lens, tables, k, v = case
     run = (q, np.array([3, 1, 9, 4], np.int32), lens, tables, k, v)
-    out = R.upload(np.zeros((4, 128), np.float32))
-    S.pagedAttention(R.upload(q.reshape(4, -1)), i32(lens), i32(tables), R.upload(k), R.upload(v), i32(run[1]), 0.0, out)
+    out, hq = R.upload(np.zeros((room, 128), np.float32)), np.zeros((room, 128), np.float32)
+    hq[:4] = q.reshape(4, -1)
+    S.pagedAttention(R.upload(hq), i32(lens), i32(tables), R.upload(k), R.upload(v), i32(run[1]), 0.0, out)
     assert "smith_paged_attention: request" in sync_error()
-    check_attention(run_attention(*case, ragged=True), *case, "f16")
+    check_attention(run_attention(*case, ragged=True, room=room), *case, "f16")
 
 
 # --------------------------------------------------------------------------
@@ -639,12 +720,13 @@ class Server:
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-def test_steps_of_several_requests(dtype):
+@pytest.mark.parametrize("max_rows", [96, room_for_many(8, 2, 6)])
+def test_steps_of_several_requests(dtype, max_rows):
     """Prompts, then chunks and single rows, one request sitting out now and
     then; nothing waits between a step's three calls.  A key that rounds the
     other way in 64 bits is off by a step of its type (f16 2^-10) in one of
     32 dims of one key: 2e-3 of the norm holds many of them, not a wrong key."""
-    sv = Server(5, 6, dtype)
+    sv = Server(5, 6, dtype, max_rows=max_rows)
     for step, added in enumerate(([20, 1, 33, 0, 17, 5], [1, 1, 1, 40, 0, 1], [1, 50, 1, 1, 16, 0], [1] * 6, [0, 0, 1, 1, 1, 1])):
         x = sv.rows(added)
         plan, _, out = sv.launch(R.upload(x), i32(added))
@@ -656,10 +738,11 @@ def test_steps_of_several_requests(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
-def test_captured_decode_steps(dtype):
+@pytest.mark.parametrize("max_rows", [96, room_for_many(8, 2, 5)])
+def test_captured_decode_steps(dtype, max_rows):
     """A captured step of one row each, fed by its own lengths, replayed with
     other work between the replays: each replay equals the eager step."""
-    a, b = Server(7, 5, dtype), Server(7, 5, dtype)
+    a, b = Server(7, 5, dtype, max_rows=max_rows), Server(7, 5, dtype, max_rows=max_rows)
     ctx = device.ops_ctx()
     first = [30, 3, 16, 1, 40]
     x = a.rows(first)
