@@ -377,6 +377,18 @@ struct MmBf16 {
   }
 };
 
+// The first of the DPL dims that lane n of 16 holds of a key: none past the head.
+// Where DPL does not divide the head the last two lanes share some dims, whose
+// sums are the same and go to the same place.
+template <int DPL>
+__device__ __forceinline__ uint32_t first_dim(uint32_t n, uint32_t hd) {
+  return n * DPL < hd - DPL ? n * DPL : hd - DPL;
+}
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+
 // One wave's tile of 32 keys of f16 or bf16: K and V operands in registers.
 template <class MM, int DPL>
 struct Tile16 {
@@ -432,16 +444,9 @@ struct Tile16 {
   // key 4g + i of the j-th 16
   __device__ __forceinline__ void load_v(int j, int i, const T* key, uint32_t off, uint32_t n, uint32_t hd) {
     uint32_t(&r)[DPL / 2] = V[4 * j + i];
-    const T* at = key + (off + (n * DPL < hd ? n * DPL : hd - DPL));  // past the head: dims that nobody writes out
-    if constexpr (DPL == 8) {
-      const u32x4 v = *(const u32x4*)at;
+    const Words<DPL / 2> v = *(const Words<DPL / 2>*)(key + (off + first_dim<DPL>(n, hd)));
 #pragma unroll
-      for (int k = 0; k < 4; k++) r[k] = v[k];
-    } else {
-      const u32x2 v = *(const u32x2*)at;
-      r[0] = v[0];
-      r[1] = v[1];
-    }
+    for (int k = 0; k < DPL / 2; k++) r[k] = v.w[k];
   }
   __device__ __forceinline__ void zero_v(int j, int i) {
 #pragma unroll
@@ -530,13 +535,9 @@ struct Tile32 {
     }
   }
   __device__ __forceinline__ void load_v(int, int i, const float* key, uint32_t off, uint32_t n, uint32_t hd) {
-    const float* at = key + (off + (n * DPL < hd ? n * DPL : hd - DPL));
+    const Words<DPL> v = *(const Words<DPL>*)(key + (off + first_dim<DPL>(n, hd)));
 #pragma unroll
-    for (int k = 0; k < DPL; k += 4) {
-      const f32x4 v = *(const f32x4*)(at + k);
-#pragma unroll
-      for (int e = 0; e < 4; e++) V[i][k + e] = v[e];
-    }
+    for (int k = 0; k < DPL; k++) V[i][k] = __uint_as_float(v.w[k]);
   }
   __device__ __forceinline__ void zero_v(int, int i) {
 #pragma unroll
@@ -1194,10 +1195,9 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-      for (int d = 0; d < DPL; d += 4)
-        *(f32x4*)&s_o[(w * 16 + ln) * OS + (4 * lg + i) * DPL + d] = (f32x4){O[d][i], O[d + 1][i], O[d + 2][i], O[d + 3][i]};
+      for (int d = 0; d < DPL; d++) s_o[(w * 16 + ln) * OS + (4 * lg + i) * DPL + d] = O[d][i];
     __syncthreads();
-    const uint32_t col = tid >> 4, d0 = (tid & 15) * DPL;
+    const uint32_t col = tid >> 4, at = (tid & 15) * DPL;
     float mx = s_ml[col * 2];
 #pragma unroll
     for (int k = 1; k < 4; k++) mx = fmaxf(mx, s_ml[(k * 16 + col) * 2]);
@@ -1210,15 +1210,18 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
       const float f = mk == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mk - mx);
       sum = __builtin_fmaf(f, s_ml[(k * 16 + col) * 2 + 1], sum);
 #pragma unroll
-      for (int d = 0; d < DPL; d++) o[d] = __builtin_fmaf(f, s_o[(k * 16 + col) * OS + d0 + d], o[d]);
+      for (int d = 0; d < DPL; d++) o[d] = __builtin_fmaf(f, s_o[(k * 16 + col) * OS + at + d], o[d]);
     }
     float* mine = a.parts + (size_t)I.part * CB * (hd + 2);
-    if (col < I.ncols && d0 < hd) {
+    if (col < I.ncols && at < hd) {
+      const uint32_t d0 = first_dim<DPL>(tid & 15, hd);
       if (I.ns == 1) {
         const float inv = I.keys ? 1.0f / sum : 0.f;
         float* y = a.out + I.at(col, a.ld_out, hd) + d0;
+        Words<DPL> x;
 #pragma unroll
-        for (int d = 0; d < DPL; d += 4) store4(y + d, (f32x4){o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv});
+        for (int d = 0; d < DPL; d++) x.w[d] = __float_as_uint(o[d] * inv);
+        *(Words<DPL>*)y = x;
       } else {
 #pragma unroll
         for (int d = 0; d < DPL; d += 2) put2(mine + col * hd + d0 + d, o[d], o[d + 1]);
@@ -1272,13 +1275,17 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t r) {
   return CHUNKS >= 16 ? r & 15 : (r / (16 / CHUNKS)) & (CHUNKS - 1);
 }
 
+// 16s of dims that a stage's row has room for
+template <int DPL>
+constexpr uint32_t LINE = DPL <= 4 ? 4 : 8;
+
 template <class MM_, int DPL>
 struct Rows16 {
   typedef MM_ MM;
   typedef Tile16<MM, DPL> TILE;
   typedef typename MM::T T;
   static constexpr int CT = 2, KT = 64, NJ = KT / 16, TERMS = MM::TERMS;
-  static constexpr uint32_t CHUNKS = 2 * DPL, ROWB = 32 * DPL;  // of 16 * DPL dims
+  static constexpr uint32_t CHUNKS = 2 * LINE<DPL>, ROWB = 32 * LINE<DPL>;
   // scores of the CT tiles' columns against the stage's keys
   static __device__ __forceinline__ void scores(const uint8_t* k, uint32_t ln, uint32_t lg,
                                                 const u32x4 (&Q)[CT][TILE::QREG], f32x4 (&S)[CT][NJ]) {
@@ -1347,7 +1354,7 @@ struct Rows32 {
   typedef Tile32<DPL> TILE;
   typedef float T;
   static constexpr int CT = 1, KT = 32, NJ = KT / 16;
-  static constexpr uint32_t CHUNKS = 4 * DPL, ROWB = 64 * DPL;
+  static constexpr uint32_t CHUNKS = 4 * LINE<DPL>, ROWB = 64 * LINE<DPL>;
   static __device__ __forceinline__ void scores(const uint8_t* k, uint32_t ln, uint32_t lg,
                                                 const u32x4 (&Q)[CT][TILE::QREG], f32x4 (&S)[CT][NJ]) {
 #pragma unroll
@@ -1557,23 +1564,33 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
   extern "C" __global__ __launch_bounds__(256, 2) void NAME(AttArgs a) { \
     BODY<__VA_ARGS__>(a);                                          \
   }
-// named by page type and head dims held (64 or 128); _s for pages of less than
-// 16 keys
+// Named by page type and head dims held (64, 96 or 128); _s for pages of less than
+// 16 keys.  Heads of 80 and 96 (10 and 12 heads) held as 96 dims against 128: 100
+// requests of 4000 keys, f32, 382 against 425 us, f16 190 and 191; 20 mixed
+// requests of up to 1500, f32, 29 and 32; prompts of 1300 rows 194 and 221 (f32), 70
+// and 76 (f16), 78 and 98 (bf16).
 #define DEF_ATTENTIONS(TYPE, D, DPL, TILE, ROWS)                                                 \
   DEF_ATTENTION(smith_paged_attention_##TYPE##_d##D, attention_body, TILE, DPL, false)           \
   DEF_ATTENTION(smith_paged_attention_##TYPE##_d##D##_s, attention_body, TILE, DPL, true)        \
   DEF_ATTENTION(smith_paged_attention_rows_##TYPE##_d##D, attention_rows_body, ROWS, DPL)
 typedef Tile16<MmF16, 4> TileF16d64;
+typedef Tile16<MmF16, 6> TileF16d96;
 typedef Tile16<MmF16, 8> TileF16d128;
 typedef Tile16<MmBf16, 4> TileBf16d64;
+typedef Tile16<MmBf16, 6> TileBf16d96;
 typedef Tile16<MmBf16, 8> TileBf16d128;
 typedef Rows16<MmF16, 4> RowsF16d64;
+typedef Rows16<MmF16, 6> RowsF16d96;
 typedef Rows16<MmF16, 8> RowsF16d128;
 typedef Rows16<MmBf16, 4> RowsBf16d64;
+typedef Rows16<MmBf16, 6> RowsBf16d96;
 typedef Rows16<MmBf16, 8> RowsBf16d128;
 DEF_ATTENTIONS(f32, 64, 4, Tile32<4>, Rows32<4>)
+DEF_ATTENTIONS(f32, 96, 6, Tile32<6>, Rows32<6>)
 DEF_ATTENTIONS(f32, 128, 8, Tile32<8>, Rows32<8>)
 DEF_ATTENTIONS(f16, 64, 4, TileF16d64, RowsF16d64)
+DEF_ATTENTIONS(f16, 96, 6, TileF16d96, RowsF16d96)
 DEF_ATTENTIONS(f16, 128, 8, TileF16d128, RowsF16d128)
 DEF_ATTENTIONS(bf16, 64, 4, TileBf16d64, RowsBf16d64)
+DEF_ATTENTIONS(bf16, 96, 6, TileBf16d96, RowsBf16d96)
 DEF_ATTENTIONS(bf16, 128, 8, TileBf16d128, RowsBf16d128)

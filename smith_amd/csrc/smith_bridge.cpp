@@ -2454,7 +2454,7 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   const bool many = row_start && shift >= 3 && (uint64_t)max_rows * G > 24ull * n_req &&
                     (uint64_t)max_rows * n_heads >= 8192;
   const bool small = !many && shift < 4;
-  const uint32_t CB = !many ? 16 : kv_type == SMITH_KV_F32 ? 64 : 128, dims = head_dim <= 64 ? 64 : 128;
+  const uint32_t CB = !many ? 16 : kv_type == SMITH_KV_F32 ? 64 : 128, dims = head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : 128;
   const uint32_t target = 512;  // two workgroups to a CU
   // Keys to a split at least.  A split of many columns leaves 64 KB and the join
   // reads them again: 64 f16 rows behind 8000 keys, 32 heads, 65 us with 512, 78 with
@@ -2473,7 +2473,7 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   const uint32_t grid = (uint32_t)std::min<uint64_t>({(uint64_t)target, blocks + max_parts, blocks * longest});
   // of attention_body: O and (m, l) of four waves; of attention_rows_body: two
   // stages of K and V rows (64 of f16 / bf16 or 32 of f32: 256 bytes a head dim) and their marks
-  const uint32_t lds = (many ? 256 * 2 * dims + 16 : 4 * 16 * (dims + 4) * 4 + 4 * 16 * 2 * 4) + 20 * (n_req + 1);
+  const uint32_t lds = (many ? 256 * 2 * (dims <= 64 ? 64 : 128) + 16 : 4 * 16 * (dims + 4) * 4 + 4 * 16 * 2 * 4) + 20 * (n_req + 1);
   struct {
     const float* q;
     const int32_t *row_start, *lens, *tables;

@@ -334,7 +334,7 @@ LENGTHS = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200, 255, 25
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("H,nKV,D,P", [
     (4, 4, 64, 16), (16, 4, 64, 16), (32, 8, 128, 16), (8, 1, 128, 64), (9, 3, 64, 8), (10, 2, 80, 32), (12, 4, 96, 16),
-    (3, 1, 8, 1), (2, 1, 16, 2), (40, 2, 40, 128), (17, 1, 120, 4)])
+    (3, 1, 8, 1), (2, 1, 16, 2), (40, 2, 40, 128), (17, 1, 120, 4), (6, 2, 88, 16), (4, 4, 80, 8), (7, 7, 72, 16)])
 def test_attention_one_row_each(dtype, H, nKV, D, P):
     lens = LENGTHS if H * D < 2000 else LENGTHS[::3] + [129]
     case = attention_case(H + D + P, dtype, H, nKV, D, P, lens, [1] * len(lens))
@@ -366,6 +366,9 @@ def test_attention_one_long_request(dtype, n):
     (2, 2, 64, 8, [70, 200], [70, 111]),
     (4, 1, 32, 4, [130, 9], [130, 9]),
     (40, 1, 64, 16, [520, 7], [9, 7]),
+    (4, 2, 80, 8, [90, 700, 5], [41, 30, 5]),
+    (6, 2, 88, 16, [64, 1000], [64, 20]),
+    (5, 5, 72, 32, [33, 65], [33, 1]),
     (16, 4, 64, 64, [700], [9])])
 def test_attention_ragged_rows(dtype, H, nKV, D, P, lens, added):
     case = attention_case(H + sum(lens), dtype, H, nKV, D, P, lens, added)

@@ -16,7 +16,7 @@ def test_code_object_has_kernels():
     need = ["smith_paged_plan"]
     need += ["smith_paged_append_%s" % t for t in ("f32", "f16", "bf16")]
     need += ["smith_paged_attention_%s_d%d%s" % (t, d, e) for t in ("f32", "f16", "bf16", "rows_f32", "rows_f16", "rows_bf16")
-             for d in (64, 128) for e in ("", "_s") if not (e and t.startswith("rows"))]
+             for d in (64, 96, 128) for e in ("", "_s") if not (e and t.startswith("rows"))]
     for k in need:
         assert re.search(r"\b%s\.kd\b" % k, out), k
 
