@@ -415,8 +415,9 @@ int smith_paged_plan(void* ctx, const int32_t* cached, const int32_t* added, uin
 /* Rows of [q | k | v] (row stride ld floats) into the cache: k after its rotary
  * position, and v, rounded to the nearest value of kv_type (ties to even), into
  * the row's slot of kpages and vpages; q after its rotary position into q_out
- * (row stride ld_q; qkv itself with ld_q = ld rotates in place, else the two do
- * not overlap; may be NULL without rotary positions, where it would be a copy).
+ * (row stride ld_q; qkv itself with ld_q = ld rotates in place; may be NULL
+ * without rotary positions, where it would be a copy).  The pools and q_out
+ * overlap neither each other nor, but for that, an input.
  * Rows of slot -1 are padding: nothing of them is read or written.  The other
  * slots of a call are distinct.  rope_len: entries of each table.  A slot outside
  * the pool, or a position outside the tables, fails its row. */
@@ -431,7 +432,7 @@ int smith_paged_append(void* ctx, uint32_t kv_type, const float* qkv, uint32_t l
  * b is request b's one new row (max_rows = n_req); with lens[b] = 0 it has no key
  * and its output is 0.  Head h reads KV head h / (n_heads / n_kv_heads); scale 0
  * is 1 / sqrt(head_dim).  q and out are f32 with row strides ld_q and ld_out and
- * room for max_rows rows; they do not overlap.  Rows of out behind the last row
+ * room for max_rows rows; out overlaps no input.  Rows of out behind the last row
  * stay as they are.  f32 accuracy for every kv_type.  Keys that a row does not
  * see may hold anything; among those that it sees an entry that is not finite
  * makes that row's head not finite.  head_dim <= 128 and % 8 == 0.  A row_start

@@ -198,8 +198,8 @@ __device__ __forceinline__ void append_body(const float* qkv, uint32_t ld, const
                                             const float* __restrict__ sinT, uint32_t rope_len,
                                             typename KV::T* __restrict__ kpages, typename KV::T* __restrict__ vpages,
                                             uint32_t n_slots, uint32_t shift, float* q_out, uint32_t ld_q,
-                                            uint64_t* __restrict__ err) {
-  const uint32_t r = blockIdx.y, item = blockIdx.x * 256 + threadIdx.x;
+                                            uint32_t row0, uint64_t* __restrict__ err) {
+  const uint32_t r = row0 + blockIdx.y, item = blockIdx.x * 256 + threadIdx.x;
   const int32_t slot = slots[r], pos = positions[r];
   if (slot == -1) return;  // padding
   const bool lead = item == 0;
@@ -261,9 +261,9 @@ __device__ __forceinline__ void append_body(const float* qkv, uint32_t ld, const
       const float* qkv, uint32_t ld, const int32_t* __restrict__ slots, const int32_t* __restrict__ positions,      \
       uint32_t nH, uint32_t nKV, uint32_t hd, uint32_t rope, const float* __restrict__ cosT,                        \
       const float* __restrict__ sinT, uint32_t rope_len, KV::T* __restrict__ kpages, KV::T* __restrict__ vpages,    \
-      uint32_t n_slots, uint32_t shift, float* q_out, uint32_t ld_q, uint64_t* __restrict__ err) {                  \
+      uint32_t n_slots, uint32_t shift, float* q_out, uint32_t ld_q, uint32_t row0, uint64_t* __restrict__ err) {   \
     append_body<KV>(qkv, ld, slots, positions, nH, nKV, hd, rope, cosT, sinT, rope_len, kpages, vpages, n_slots,    \
-                    shift, q_out, ld_q, err);                                                                       \
+                    shift, q_out, ld_q, row0, err);                                                                 \
   }
 DEF_APPEND(smith_paged_append_f32, KvF32)
 DEF_APPEND(smith_paged_append_f16, KvF16)

@@ -2311,8 +2311,16 @@ static int pool_shift(Ctx* c, const char* fn, uint32_t n_pages, uint32_t page_si
   return 0;
 }
 
-static bool overlap(const void* a, uint64_t an, const void* b, uint64_t bn) {
-  return (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+struct Range {  // n bytes from p on
+  const void* p;
+  uint64_t n;
+};
+static bool overlap(const Range& a, const Range& b) {
+  return a.n && b.n && (uintptr_t)a.p < (uintptr_t)b.p + b.n && (uintptr_t)b.p < (uintptr_t)a.p + a.n;
+}
+
+static uint64_t pool_bytes(uint32_t kv_type, uint32_t n_kv_heads, uint32_t head_dim, uint32_t n_pages, uint32_t page_size) {
+  return (uint64_t)n_pages * page_size * n_kv_heads * head_dim * (kv_type == SMITH_KV_F32 ? 4 : 2);
 }
 
 // what append and attention ask of a cache and its heads
@@ -2348,18 +2356,14 @@ int smith_paged_plan(void* ctx, const int32_t* cached, const int32_t* added, uin
     return fail(c, "%s: block tables of %u pages of %u keys (less than 2^31 keys)", fn, max_pages, page_size);
   {
     // every workgroup reads all the lengths: a step in place would change them under it
-    struct Range {
-      const void* p;
-      uint64_t n;
-    };
     const uint64_t nb = 4ull * n_req, rb = 4ull * max_rows;
     const Range in[] = {{cached, nb}, {added, nb}, {free_pages, 4}, {free_count, 4}};
     const Range io[] = {{tables, nb * max_pages}, {row_start, nb + 4}, {lens, nb}, {slots, rb}, {positions, rb}, {free_left, 4}};
     for (size_t i = 0; i < sizeof io / sizeof io[0]; i++) {
       for (const Range& r : in)
-        if (overlap(io[i].p, io[i].n, r.p, r.n)) return fail(c, "%s: an output overlaps an input", fn);
+        if (overlap(io[i], r)) return fail(c, "%s: an output overlaps an input", fn);
       for (size_t k = 0; k < i; k++)
-        if (overlap(io[i].p, io[i].n, io[k].p, io[k].n)) return fail(c, "%s: two outputs overlap", fn);
+        if (overlap(io[i], io[k])) return fail(c, "%s: two outputs overlap", fn);
     }
   }
   if (set_device(c)) return -1;
@@ -2390,8 +2394,20 @@ int smith_paged_append(void* ctx, uint32_t kv_type, const float* qkv, uint32_t l
   if (!rows) return 0;
   if (!qkv || !slots || !positions) return fail(c, "%s: null buffer", fn);
   if (q_out && !(q_out == qkv && ld_q == ld) &&
-      overlap(q_out, 4 * ((uint64_t)(rows - 1) * ld_q + Wq), qkv, 4 * ((uint64_t)(rows - 1) * ld + Wq + 2 * Wk)))
+      overlap({q_out, 4 * ((uint64_t)(rows - 1) * ld_q + Wq)}, {qkv, 4 * ((uint64_t)(rows - 1) * ld + Wq + 2 * Wk)}))
     return fail(c, "%s: q_out overlaps qkv and is not it", fn);
+  {
+    const uint64_t pool = pool_bytes(kv_type, n_kv_heads, head_dim, n_pages, page_size), rb = 4ull * rows;
+    const Range out[] = {{kpages, pool}, {vpages, pool}, {q_out, q_out ? 4 * ((uint64_t)(rows - 1) * ld_q + Wq) : 0}};
+    const Range in[] = {{qkv, 4 * ((uint64_t)(rows - 1) * ld + Wq + 2 * Wk)}, {slots, rb}, {positions, rb},
+                        {rope ? rope_cos : nullptr, 4ull * rope_len}, {rope ? rope_sin : nullptr, 4ull * rope_len}};
+    for (int i = 0; i < 3; i++) {
+      for (const Range& r : in)  // (q_out in place of qkv was looked at above)
+        if (r.p && !(i == 2 && r.p == qkv) && overlap(out[i], r)) return fail(c, "%s: an output overlaps an input", fn);
+      for (int k = 0; k < i; k++)
+        if (overlap(out[i], out[k])) return fail(c, "%s: two outputs overlap", fn);
+    }
+  }
   if (set_device(c)) return -1;
   uint32_t n_slots = n_pages << shift;
   uint64_t* perr = c->paged_err_dev();
@@ -2401,11 +2417,8 @@ int smith_paged_append(void* ctx, uint32_t kv_type, const float* qkv, uint32_t l
   // rows along the grid's second axis, which ends at 65535
   for (uint32_t r0 = 0; r0 < rows; r0 += 65535) {
     const uint32_t n = std::min<uint32_t>(65535, rows - r0);
-    const float* x = qkv + (size_t)r0 * ld;
-    const int32_t *sl = slots + r0, *po = positions + r0;
-    float* qo = q_out ? q_out + (size_t)r0 * ld_q : nullptr;
-    void* args[] = {&x, &ld, &sl, &po, &n_heads, &n_kv_heads, &head_dim, &rope, &rope_cos, &rope_sin,
-                    &rope_len, &kpages, &vpages, &n_slots, &shift, &qo, &ld_q, &perr};
+    void* args[] = {&qkv, &ld, &slots, &positions, &n_heads, &n_kv_heads, &head_dim, &rope, &rope_cos, &rope_sin,
+                    &rope_len, &kpages, &vpages, &n_slots, &shift, &q_out, &ld_q, &r0, &perr};
     if (launch(c, name, dim3((items + 255) / 256, n), dim3(256), args)) return -1;
   }
   return 0;
@@ -2434,8 +2447,15 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   if (!std::isfinite(scale)) return fail(c, "%s: scale %g", fn, (double)scale);
   if (!max_rows) return 0;
   if (!q || !lens || !tables || !out) return fail(c, "%s: null buffer", fn);
-  if (overlap(out, 4 * ((uint64_t)(max_rows - 1) * ld_out + Wq), q, 4 * ((uint64_t)(max_rows - 1) * ld_q + Wq)))
-    return fail(c, "%s: out overlaps q", fn);
+  {
+    const Range o = {out, 4 * ((uint64_t)(max_rows - 1) * ld_out + Wq)};
+    if (overlap(o, {q, 4 * ((uint64_t)(max_rows - 1) * ld_q + Wq)})) return fail(c, "%s: out overlaps q", fn);
+    const uint64_t pool = pool_bytes(kv_type, n_kv_heads, head_dim, n_pages, page_size);
+    const Range in[] = {{row_start, row_start ? 4ull * n_req + 4 : 0}, {lens, 4ull * n_req},
+                        {tables, 4ull * n_req * max_pages}, {kpages, pool}, {vpages, pool}};
+    for (const Range& r : in)
+      if (overlap(o, r)) return fail(c, "%s: out overlaps an input", fn);
+  }
   if (set_device(c)) return -1;
   if (scale == 0.f) scale = 1.0f / sqrtf((float)head_dim);
   // Where a request brings a row or so its columns (row, head) are few and its

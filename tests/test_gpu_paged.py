@@ -270,6 +270,24 @@ def test_append_leaves_out_rows_that_do_not_fit(bad, message, rope):
         assert np.all(np.abs(R.value(t.data, dtype) - w) <= tol)
 
 
+def test_append_of_more_rows_than_a_grid_axis():
+    """65600 rows take two launches; a slot outside the pool is reported by its row."""
+    rs = np.random.RandomState(8)
+    rows, P = 65600, 16
+    x = rs.standard_normal((rows, 24)).astype(np.float32)
+    slots = rs.permutation(rows).astype(np.int32)
+    pools = [R.upload(np.zeros((rows // P, 1, P, 8), np.float16)) for _ in range(2)]
+    tx, pos = R.upload(x), i32(np.zeros(rows))
+    q = S.pagedAppend(tx, i32(slots), pos, 1, *pools)
+    device.sync()
+    assert np.array_equal(q.data, x[:, :8])
+    for t, part in zip(pools, (x[:, 8:16], x[:, 16:])):
+        assert np.array_equal(t.data.reshape(rows, 8)[slots], part.astype(np.float16))
+    slots[65590] = rows
+    S.pagedAppend(tx, i32(slots), pos, 1, *pools)
+    assert "row 65590" in sync_error()
+
+
 # --------------------------------------------------------------------------
 # attention
 # --------------------------------------------------------------------------
@@ -606,6 +624,7 @@ def placed(args, *pointers):
 
 
 def base_attention(**over):
+    # pools of 8 pages x 2 heads x 16 keys x 16 dims of 2 bytes: 8192 bytes
     a = dict(kv=1, q=4096, ld_q=64, max_rows=2, row_start=None, lens=4096, tables=4096, n_req=2, max_pages=4, H=4, nKV=2,
              D=16, scale=0.0, k=4096, v=4096, n_pages=8, P=16, out=1 << 20, ld_out=64)
     a.update(over)
@@ -621,6 +640,9 @@ def base_attention(**over):
     ({"max_rows": 3}, "max_rows 3 for one row"), ({"ld_q": 63}, "row strides 63"), ({"ld_out": 60}, "and 60"),
     ({"k": None}, "page pools"), ({"v": 4104}, "16-byte aligned"), ({"q": None}, "null buffer"), ({"lens": None}, "null buffer"),
     ({"tables": None}, "null buffer"), ({"out": None}, "null buffer"), ({"out": 4096 + 256}, "out overlaps q"),
+    ({"lens": (1 << 20) + 8}, "out overlaps an input"), ({"tables": 1 << 20}, "out overlaps an input"),
+    ({"k": (1 << 20) - 8176}, "out overlaps an input"), ({"v": (1 << 20) + 256}, "out overlaps an input"),
+    ({"row_start": 1 << 20}, "out overlaps an input"),
     ({"scale": float("nan")}, "scale nan"), ({"scale": float("inf")}, "scale inf"),
     ({"row_start": 4096, "max_rows": 1 << 31}, "max_rows 2147483648")])
 def test_attention_refusals(over, message):
@@ -640,7 +662,11 @@ def base_append(**over):
     ({"rope": 3}, "unknown rotary indexing 3"), ({"cos": None}, "need both tables"), ({"q": None}, "need both tables and q_out"),
     ({"ld": 127}, "row strides 127"), ({"ld_q": 63}, "and 63"), ({"x": None}, "null buffer"), ({"slots": None}, "null buffer"),
     ({"pos": None}, "null buffer"), ({"rows": 1 << 31}, "rows"), ({"q": 4096 + 64}, "overlaps qkv"),
-    ({"q": 4096, "ld_q": 64}, "overlaps qkv"), ({"k": 4100}, "16-byte aligned"), ({"v": None}, "page pools")])
+    ({"q": 4096, "ld_q": 64}, "overlaps qkv"), ({"k": 4100}, "16-byte aligned"), ({"v": None}, "page pools"),
+    ({"k": 1 << 17, "v": (1 << 17) + 8176}, "two outputs overlap"), ({"v": 1 << 17}, "overlaps an input"),
+    ({"k": 1 << 17, "v": 1 << 18, "q": 1 << 18}, "two outputs overlap"),
+    ({"k": 1 << 17, "v": 1 << 18, "slots": 1 << 17}, "overlaps an input"),
+    ({"k": 1 << 17, "v": 1 << 18, "sin": (1 << 20) + 4}, "overlaps an input")])
 def test_append_refusals(over, message):
     assert base_append(**over) == -1
     assert "smith_paged_append: " in last_error() and message in last_error()
