@@ -267,8 +267,12 @@ class _Engine:
         M = sum(added)
         if M > _chunk_rows(cfg):
             raise ValueError("paged step: %d rows (at most %d)" % (M, _chunk_rows(cfg)))
+        flat = [t for req in tokens for t in req]
+        if flat and not 0 <= min(flat) <= max(flat) < vocab:
+            raise ValueError("paged step: a token outside the vocabulary of %d" % vocab)
+        cache.check_model(cfg)
         plan = cache.plan(added)
-        self.embed(model, [t for req in tokens for t in req])
+        self.embed(model, flat)
         x, x2, qkv, attn, h = self.x.ptr, self.x2.ptr, self.qkv.ptr, self.attn.ptr, self.h.ptr
         rope = model["rope"]
         for li, blk in enumerate(model["blocks"]):

@@ -38,8 +38,8 @@ def _pools(kPages, vPages, what):
 
 def pagedPlan(cached, added, freePages, freeCount, tables, nPages, pageSize, maxRows):
     """Block tables, slots and positions of a step (smith_paged_plan).  cached,
-    added: [n] i32; freePages [..] and freeCount [1] i32: the free list; tables
-    [n, maxPages] i32, new pages are entered.  Returns {rowStart [n + 1], lens
+    added: [n] i32; freePages [..] and freeCount [1] i32: the free list, its first
+    freeCount entries; tables [n, maxPages] i32, new pages are entered.  Returns {rowStart [n + 1], lens
     [n], slots [maxRows], positions [maxRows], freeLeft [1]}, all i32."""
     n = cached.shape[0]
     _want(cached, [n], "i32", "pagedPlan: cached")
@@ -113,6 +113,8 @@ class PagedCache:
             raise ValueError("createPagedCache: page size %d is no power of two" % pageSize)
         if pages < 1 or pages * pageSize >= 1 << 31:
             raise ValueError("createPagedCache: %d pages of %d keys" % (pages, pageSize))
+        if config["headDim"] % 8 or not 8 <= config["headDim"] <= 128:
+            raise ValueError("createPagedCache: heads of %d dims (8, 16 .. 128)" % config["headDim"])
         self.requests, self.pages, self.pageSize, self.dtype = requests, pages, pageSize, dtype
         self.maxPages = -(-config["maxSeqLen"] // pageSize)
         shape = [pages, config["numKVHeads"], pageSize, config["headDim"]]
@@ -129,10 +131,17 @@ class PagedCache:
         self._row_start = T.zeros([requests + 1], "i32")
         self._rows = None
 
+    def check_model(self, config):
+        """Raises ValueError unless the pools are those of a model of this config."""
+        k = self.layers[0]["k"].shape if self.layers else [0] * 4
+        if (len(self.layers), k[1], k[3]) != (config["numLayers"], config["numKVHeads"], config["headDim"]):
+            raise ValueError("paged step: a cache of %d layers of %d heads of %d, a model of %d of %d of %d" % (
+                len(self.layers), k[1], k[3], config["numLayers"], config["numKVHeads"], config["headDim"]))
+
     def plan(self, added):
         """The step in which request b brings added[b] rows: {rowStart, lens, slots,
         positions, tables}.  Nothing happens (ValueError) if it does not fit."""
-        added = np.asarray(added, np.int32)
+        added = np.asarray(added, np.int64)
         rows = int(added.sum())
         lens = self.lens + added
         if added.shape != (self.requests,) or (added < 0).any() or not rows:
@@ -156,7 +165,7 @@ class PagedCache:
             self._count[a].buffer, self.pages, self.pageSize, self.maxPages, slots.shape[0], self._tables.buffer,
             self._row_start.buffer, self._lens[b].buffer, slots.buffer, positions.buffer, self._count[b].buffer),
             "paged step")
-        self._turn, self.lens, self.freeCount = b, lens, self.freeCount - new
+        self._turn, self.lens, self.freeCount = b, lens.astype(np.int32), self.freeCount - new
         return {"rowStart": self._row_start, "lens": self._lens[b], "slots": slots, "positions": positions,
                 "tables": self._tables}
 
@@ -179,6 +188,8 @@ class PagedCache:
 
     def release(self, request):
         """The request's pages back to the free list; its number is free for another."""
+        if not 0 <= request < self.requests:
+            raise ValueError("paged cache: request %d of %d" % (request, self.requests))
         n = -(-int(self.lens[request]) // self.pageSize)
         if not n:
             return

@@ -10,8 +10,18 @@ import numpy as np
 
 from . import device, prng
 
-# bf16: the upper halves of f32 words
+# bf16: the upper halves of f32 words on the host; floats are rounded to them
 _DTYPES = {"f32": np.float32, "i32": np.int32, "u8": np.uint8, "f16": np.float16, "bf16": np.uint16}
+
+
+def _host(values, dtype):
+    """values as the host array of a tensor of dtype."""
+    a = np.asarray(values)
+    if dtype == "bf16" and a.dtype.kind == "f":  # to nearest, ties to even
+        u = np.ascontiguousarray(a, dtype=np.float32).view(np.uint32)
+        return np.where((u & 0x7FFFFFFF) > 0x7F800000, u >> 16 | 0x40,
+                        (u + (0x7FFF + (u >> 16 & 1))) >> 16).astype(np.uint16).reshape(a.shape)
+    return np.ascontiguousarray(a, dtype=_DTYPES[dtype])
 
 
 class Tensor:
@@ -40,7 +50,7 @@ class Tensor:
         return device.download(self.buffer, self.nbytes, _DTYPES[self.dtype]).reshape(self.shape)
 
     def set_data(self, arr):
-        a = np.ascontiguousarray(arr, dtype=_DTYPES[self.dtype])
+        a = _host(arr, self.dtype)
         if a.size != self.size:
             raise ValueError("set_data: %d elements for a tensor of %d" % (a.size, self.size))
         device.upload(self.buffer, a)
@@ -60,7 +70,7 @@ def create(shape, dtype="f32"):
 
 
 def tensor(data, shape=None, dtype="f32"):
-    a = np.asarray(data, dtype=_DTYPES[dtype])
+    a = _host(data, dtype)
     t = Tensor(list(a.shape) if shape is None else shape, dtype)
     return t.set_data(a)
 
@@ -70,7 +80,7 @@ def zeros(shape, dtype="f32"):
 
 
 def ones(shape, dtype="f32"):
-    return tensor(np.ones(shape, dtype=_DTYPES[dtype]), dtype=dtype)
+    return tensor(np.ones(shape), dtype=dtype)
 
 
 def randn(shape, seed=0, std=1.0, mean=0.0):

@@ -3,6 +3,7 @@ request: several requests in one step, of any lengths, on a shared pool."""
 import numpy as np
 import pytest
 
+from smith_amd import createPagedCache
 from smith_amd.gguf_loader import loadGGUF
 from llama_fixtures import write_tiny_llama
 
@@ -117,6 +118,17 @@ def test_refusals(model):
         model.forwardPagedStep([[1] * 200, [2] * 57], cache)
     with pytest.raises(ValueError, match="whole-row RoPE"):
         model.forwardPagedStep([[1] * 256, []], cache) and model.forwardPagedStep([[1], []], cache)
+    with pytest.raises(ValueError, match="outside the vocabulary"):
+        model.forwardPagedStep([[], [3, 320]], cache)
+    with pytest.raises(ValueError, match="outside the vocabulary"):
+        model.forwardPagedStep([[], [-1]], cache)
+    for b in (-1, 2):
+        with pytest.raises(ValueError, match="request %d of 2" % b):
+            cache.release(b)
+    other = createPagedCache(dict(model.model["config"], numLayers=1), 2, 10)
+    with pytest.raises(ValueError, match="a cache of 1 layers"):
+        model.forwardPagedStep([[1], [2]], other)
+    assert cache.lens.tolist() == [256, 0] and cache.freeCount == 184 and other.freeCount == 10
     with pytest.raises(ValueError, match="pages of q8"):
         model.createPagedCache(2, 10, 16, "q8")
     with pytest.raises(ValueError, match="power of two"):

@@ -21,6 +21,23 @@ def test_code_object_has_kernels():
         assert re.search(r"\b%s\.kd\b" % k, out), k
 
 
+def test_bf16_of_floats_rounds():
+    from smith_amd.tensor import _host
+    one = np.float32(1.0).view(np.uint32)
+    bits = np.array([one, one + 0x7FFF, one + 0x8000, one + 0x8001, one + 0x18000, 0x7F7FFFFF, 0x7F800000, 0x7F800001,
+                     0xFFFFFFFF, 0x80000001], np.uint32)
+    want = [0x3F80, 0x3F80, 0x3F80, 0x3F81, 0x3F82, 0x7F80, 0x7F80, 0x7FC0, 0xFFFF, 0x8000]
+    assert _host(bits.view(np.float32), "bf16").tolist() == want
+    assert _host(np.array([1.0, -2.5]), "bf16").tolist() == [0x3F80, 0xC020]
+    assert _host([0x3F80, 7], "bf16").tolist() == [0x3F80, 7]  # whole numbers are the bits
+
+
+@pytest.mark.parametrize("dim", [4, 12, 136])
+def test_cache_of_heads_that_no_kernel_takes(dim):
+    with pytest.raises(ValueError, match="heads of %d dims" % dim):
+        S.createPagedCache(dict(maxSeqLen=64, numKVHeads=2, headDim=dim, numLayers=1), 1, 4)
+
+
 class Fake:
     """A tensor's shape and type without memory."""
     buffer = None
