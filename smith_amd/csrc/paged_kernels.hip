@@ -590,12 +590,12 @@ struct AttArgs {
   float scale;
 };
 
-// a / b: below 2^20 by a reciprocal, (a + 1/2) / b being 1 / 2b away from the next
+// a / b of a < 2^20 by a reciprocal: (a + 1/2) / b is 1 / 2b away from the next
 // whole number and off by less than a / b 2^-22
-__device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t b) {
-  if (a < 1u << 20) return (uint32_t)(((float)a + 0.5f) * __builtin_amdgcn_rcpf((float)b));
-  return a / b;
+__device__ __forceinline__ uint32_t small_quotient(uint32_t a, uint32_t b) {
+  return (uint32_t)(((float)a + 0.5f) * __builtin_amdgcn_rcpf((float)b));
 }
+__device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t b) { return a < 1u << 20 ? small_quotient(a, b) : a / b; }
 __device__ __forceinline__ uint32_t div_up(uint32_t a, uint32_t b) { return quotient(a + b - 1, b); }
 // of values that are the same in all lanes, in scalar registers
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
@@ -778,7 +778,8 @@ struct Item {
     ns = uniform(t.splits(len));
     // the KV head first (neighbouring blocks of a head meet in one XCD's L2 when
     // there are 8 of them), the blocks with the most keys before the others
-    const uint32_t rest = quotient_u(local, a.nKV), later = quotient_u(rest, ns);
+    // (a request that is cut has no more items than there is room for partials)
+    const uint32_t rest = quotient_u(local, a.nKV), later = ns > 1 ? uniform(small_quotient(rest, ns)) : rest;
     kvh = local - rest * a.nKV;
     split = rest - later * ns;
     const uint32_t blk = quotient_u(n + a.rows_blk - 1, a.rows_blk) * a.groups - 1 - later, rowblk = quotient_u(blk, a.groups);
@@ -796,7 +797,7 @@ struct Item {
     k0 = at < keys ? (uint32_t)at : keys;
     k1 = keys - k0 < chunk ? keys : k0 + chunk;
   }
-  __device__ __forceinline__ uint32_t row_of(uint32_t col) const { return quotient(col, heads); }
+  __device__ __forceinline__ uint32_t row_of(uint32_t col) const { return small_quotient(col, heads); }
   // element 0 of a column in q or out
   __device__ __forceinline__ size_t at(uint32_t col, uint32_t ld, uint32_t hd) const {
     const uint32_t row = row_of(col);
@@ -844,6 +845,11 @@ __device__ __forceinline__ bool last_split(const AttArgs& a, const Item& I) {
   __syncthreads();
   return s_last;
 }
+
+template <uint32_t N_>
+struct Count {
+  static constexpr uint32_t N = N_;
+};
 
 // A block of at most 16 columns.  s: LDS of PAGED_SPLIT_MAX * 16 + 128 floats that
 // nobody uses any more.
@@ -893,7 +899,7 @@ __device__ __forceinline__ void join_16(const AttArgs& a, const Item& I, float* 
   if (lg == 0) s_ml[64 + w * 16 + ln] = sum;
   __syncthreads();
   for (uint32_t e = 2 * tid; e < ncols * hd; e += 512) {
-    const uint32_t k = quotient(e, hd), d = e - k * hd;
+    const uint32_t k = small_quotient(e, hd), d = e - k * hd;
     float2 o = make_float2(0.f, 0.f);
     if (e >= 512) load(e, 0);
     for (uint32_t s0 = 0;;) {
@@ -955,36 +961,46 @@ __device__ __forceinline__ void join_many(const AttArgs& a, const Item& I, uint3
     __syncthreads();
     const uint32_t nc = ncols - c0 < width ? ncols - c0 : width;
     auto put = [&](uint32_t e, f32x4 o) {
-      const uint32_t k = quotient(e, hd);
+      const uint32_t k = small_quotient(e, hd);
       float tot = 0.f;
       for (uint32_t g = 0; g < groups; g++) tot += s[(g << lw) + k];
       store4(a.out + I.at(c0 + k, a.ld_out, hd) + (e - k * hd), o * (1.0f / tot));
     };
-    // four dims at a time, 8 loads in flight: of the splits where there are
-    // many, of the thread's next dims where there are few; what is behind the last
-    // split or dim is loaded as that and weighs 0 or is not written
+    // four dims at a time, all loads of 8 such in flight where there are few splits,
+    // of 8 splits where there are many; what is behind the last split or dim is
+    // loaded as that and weighs 0 or is not written
     const uint32_t quads = nc * hd / 4;
     const float* src = all + c0 * hd;
-    if (ns <= 4) {
+    auto few = [&](auto splits) {
+      constexpr uint32_t NS = decltype(splits)::N;
       for (uint32_t e0 = tid; e0 < quads; e0 += 8 * 256) {
-        f32x4 o[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) o[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-        for (uint32_t k = 0; k < ns; k++)
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const uint32_t e = 4 * (e0 + 256 * j < quads ? e0 + 256 * j : quads - 1);
-            o[j] += load8(src + k * stride + e) * s_m[(k << lw) + quotient(e, hd)];
-          }
+        f32x4 x[8][NS];
 #pragma unroll
         for (int j = 0; j < 8; j++)
-          if (e0 + 256 * j < quads) put(4 * (e0 + 256 * j), o[j]);
+#pragma unroll
+          for (uint32_t k = 0; k < NS; k++) x[j][k] = load8(src + k * stride + 4 * (e0 + 256 * j < quads ? e0 + 256 * j : quads - 1));
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const uint32_t e = 4 * (e0 + 256 * j);
+          if (e >= 4 * quads) break;
+          const float* f = s_m + small_quotient(e, hd);
+          f32x4 o = x[j][0] * f[0];
+#pragma unroll
+          for (uint32_t k = 1; k < NS; k++) o += x[j][k] * f[k << lw];
+          put(e, o);
+        }
       }
+    };
+    if (ns == 2) {
+      few(Count<2>());
+    } else if (ns == 3) {
+      few(Count<3>());
+    } else if (ns == 4) {
+      few(Count<4>());
     } else {
       constexpr uint32_t BATCH = 8;
       for (uint32_t e = 4 * tid; e < 4 * quads; e += 4 * 256) {
-        const uint32_t k = quotient(e, hd);
+        const uint32_t k = small_quotient(e, hd);
         f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
         for (uint32_t s0 = 0; s0 < ns; s0 += BATCH) {
           f32x4 x[BATCH];
