@@ -29,6 +29,19 @@ __device__ __forceinline__ void paged_err(uint64_t* __restrict__ err, uint32_t c
     __hip_atomic_store(err, ((uint64_t)arg << 32) | code, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
+// sum over the lanes up to this one: within rows of 16, then across them
+__device__ __forceinline__ uint32_t scan64_lanes(uint32_t v) {
+#define SCAN_DPP(CTRL, ROWS) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false)
+  SCAN_DPP(0x111, 0xF);  // row_shr 1, 2, 4, 8
+  SCAN_DPP(0x112, 0xF);
+  SCAN_DPP(0x114, 0xF);
+  SCAN_DPP(0x118, 0xF);
+  SCAN_DPP(0x142, 0xA);  // row_bcast 15 into rows 1 and 3, 31 into 2 and 3
+  SCAN_DPP(0x143, 0xC);
+#undef SCAN_DPP
+  return v;
+}
+
 // A page's values in f32, and f32 rounded to nearest even into a page.
 struct KvF32 {
   typedef float T;
@@ -68,7 +81,7 @@ extern "C" __global__ __launch_bounds__(PLAN_THREADS) void smith_paged_plan(
     uint32_t max_pages, uint32_t max_rows, int32_t* __restrict__ tables, int32_t* __restrict__ row_start,
     int32_t* __restrict__ lens, int32_t* __restrict__ slots, int32_t* __restrict__ positions,
     int32_t* __restrict__ free_left, uint64_t* __restrict__ err) {
-  __shared__ uint32_t s_row[PAGED_MAX_REQ + 1], s_page[PAGED_MAX_REQ];
+  __shared__ uint32_t s_row[PAGED_MAX_REQ + 1], s_page[PAGED_MAX_REQ], s_had[PAGED_MAX_REQ];
   __shared__ uint64_t s_wr[PLAN_THREADS / 64], s_wp[PLAN_THREADS / 64];
   __shared__ uint32_t s_bad[PLAN_THREADS / 64];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -76,28 +89,39 @@ extern "C" __global__ __launch_bounds__(PLAN_THREADS) void smith_paged_plan(
   const uint64_t cap = (uint64_t)max_pages << shift;
   const uint32_t per = (n_req + PLAN_THREADS - 1) / PLAN_THREADS;
   const int64_t have = free_count[0];
-  // this thread's requests: rows and new pages (64-bit sums: nothing wraps)
+  // f(request, its keys, its rows) of this thread's requests, four loaded at once
+  auto each = [&](auto f) {
+    for (uint32_t k0 = 0; k0 < per; k0 += 4) {
+      int32_t c[4], a[4];
+#pragma unroll
+      for (uint32_t k = 0; k < 4; k++) {
+        const uint32_t b = tid * per + k0 + k, at = b < n_req ? b : n_req - 1;
+        c[k] = cached[at];
+        a[k] = added[at];
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < 4; k++) {
+        const uint32_t b = tid * per + k0 + k;
+        if (k0 + k < per && b < n_req) f(b, c[k], a[k]);
+      }
+    }
+  };
+  auto new_pages = [&](int32_t c, int32_t a) {
+    return (uint32_t)(((uint64_t)((int64_t)c + a + P - 1) >> shift) - ((uint64_t)((int64_t)c + P - 1) >> shift));
+  };
   uint64_t rows = 0, pages = 0;
   uint32_t bad = 0;  // 1 + the first request whose lengths do not fit
-  for (uint32_t k = 0; k < per; k++) {
-    const uint32_t b = tid * per + k;
-    if (b >= n_req) break;
-    const int64_t c = cached[b], a = added[b];
-    if ((c < 0 || a < 0 || (uint64_t)(c + a) > cap) && !bad) bad = b + 1;
-    if (bad) break;
-    rows += (uint64_t)a;
-    pages += ((uint64_t)(c + a + P - 1) >> shift) - ((uint64_t)(c + P - 1) >> shift);
-  }
-  // prefix sums over the workgroup
-  uint64_t ir = rows, ip = pages;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t r = __shfl_up(ir, d), p = __shfl_up(ip, d);
-    if (lane >= (uint32_t)d) {
-      ir += r;
-      ip += p;
-    }
-  }
+  each([&](uint32_t b, int32_t c, int32_t a) {
+    if ((c < 0 || a < 0 || (uint64_t)((int64_t)c + a) > cap) && !bad) bad = b + 1;
+    if (bad) return;
+    rows += (uint32_t)a;
+    pages += new_pages(c, a);
+  });
+  // sums over the wave up to this thread, of less than 2^35 each, in two halves of 24 bits
+  auto scan = [](uint64_t v) {
+    return ((uint64_t)scan64_lanes((uint32_t)(v >> 24)) << 24) + scan64_lanes((uint32_t)v & 0xFFFFFFu);
+  };
+  const uint64_t ir = scan(rows), ip = scan(pages);
   const uint64_t bads = __ballot(bad != 0);
   const uint32_t first_bad = bads ? (uint32_t)__shfl((int)bad, __ffsll((unsigned long long)bads) - 1) : 0u;
   if (lane == 63) {
@@ -124,23 +148,19 @@ extern "C" __global__ __launch_bounds__(PLAN_THREADS) void smith_paged_plan(
                         : have < 0 || have > (int64_t)n_pages || tp > (uint64_t)have ? PAGED_ERR_PLAN_PAGES
                                             : 0u;
   if (code && blockIdx.x == 0 && tid == 0) paged_err(err, code, bad_req ? bad_req - 1 : code == PAGED_ERR_PLAN_ROWS ? max_rows : (uint32_t)have);
-  br += ir - rows;
-  bp += ip - pages;
-  for (uint32_t k = 0; k < per; k++) {
-    const uint32_t b = tid * per + k;
-    if (b >= n_req) break;
-    const int64_t c = cached[b], a = code ? 0 : added[b];
-    if (!code) {
-      s_row[b] = (uint32_t)br;
-      s_page[b] = (uint32_t)bp;
-    }
+  uint32_t at_row = (uint32_t)(br + ir - rows), at_page = (uint32_t)(bp + ip - pages);
+  each([&](uint32_t b, int32_t c, int32_t a) {
+    if (code) a = 0;
+    s_row[b] = at_row;
+    s_page[b] = at_page;
+    s_had[b] = (uint32_t)c;
     if (blockIdx.x == 0) {
-      row_start[b] = code ? 0 : (int32_t)br;
-      lens[b] = (int32_t)(c + a);
+      row_start[b] = code ? 0 : (int32_t)at_row;
+      lens[b] = (int32_t)((uint32_t)c + (uint32_t)a);
     }
-    br += (uint64_t)a;
-    if (!code) bp += ((uint64_t)(c + a + P - 1) >> shift) - ((uint64_t)(c + P - 1) >> shift);
-  }
+    at_row += (uint32_t)a;
+    if (!code) at_page += new_pages(c, a);
+  });
   const uint32_t total = code ? 0u : (uint32_t)tr;
   if (tid == 0) {
     s_row[n_req] = total;
@@ -161,7 +181,7 @@ extern "C" __global__ __launch_bounds__(PLAN_THREADS) void smith_paged_plan(
       if (s_row[mid] <= r) lo = mid;
       else hi = mid;
     }
-    const uint32_t c = (uint32_t)cached[lo], p = c + (r - s_row[lo]);
+    const uint32_t c = s_had[lo], p = c + (r - s_row[lo]);
     const uint32_t j = p >> shift, old = (c + P - 1) >> shift;
     const int32_t page = j < old ? tables[(size_t)lo * max_pages + j]
                                  : free_pages[(uint32_t)have - 1 - (s_page[lo] + (j - old))];
@@ -321,19 +341,6 @@ __device__ __forceinline__ float max_xor16_32(float v) {
   const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
-// sum over the lanes up to this one: within rows of 16, then across them
-__device__ __forceinline__ uint32_t scan64_lanes(uint32_t v) {
-#define SCAN_DPP(CTRL, ROWS) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false)
-  SCAN_DPP(0x111, 0xF);  // row_shr 1, 2, 4, 8
-  SCAN_DPP(0x112, 0xF);
-  SCAN_DPP(0x114, 0xF);
-  SCAN_DPP(0x118, 0xF);
-  SCAN_DPP(0x142, 0xA);  // row_bcast 15 into rows 1 and 3, 31 into 2 and 3
-  SCAN_DPP(0x143, 0xC);
-#undef SCAN_DPP
-  return v;
-}
-
 #define P_EXP 6.0f   // P = 2^(score - m + P_EXP)
 #define M_SLACK 8.0f // m follows a new maximum only when it is this far (log2) above
 
