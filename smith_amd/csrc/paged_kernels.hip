@@ -69,9 +69,10 @@ struct KvBf16 {
 //
 // Latency is all of it (a few bytes a row): one launch, no exchange between
 // workgroups.  Each of them forms both prefix sums of all the requests by
-// itself (they are a few KB, in L2) and then serves its PLAN_ROWS rows: a
+// itself (they are a few KB, in L2) and then serves its PLAN_THREADS rows: a
 // row's request by bisection, its page from the table or, if it is a new one,
-// from the free list; the row that opens a page writes the table entry.
+// from the free list; the row that opens a page writes the table entry.  24
+// requests, 20 rows: 3.2 us; 700 requests, 9631 rows: 4.8 us.
 // ---------------------------------------------------------------------------
 #define PLAN_THREADS 256
 
@@ -200,7 +201,9 @@ extern "C" __global__ __launch_bounds__(PLAN_THREADS) void smith_paged_plan(
 // (x0 cos - x1 sin, x0 sin + x1 cos) with table entry pos * H + i; H is half
 // the row's width (q's and k's own: the whole-row indexing of smith_attention)
 // or half the head.  Bound by memory: a thread takes four neighbouring pairs
-// (two 16-byte loads of x, one each of cos and sin), or eight elements of v.
+// (two 16-byte loads of x, one each of cos and sin), or eight elements of v.  6001
+// rows of 32 + 2 x 8 heads of 128 into bf16 pages, 273 MB: 49 us, 5.5 TB/s (a
+// large copy: 4.8); 57 of them into f16 pages 3.0 us.
 // ---------------------------------------------------------------------------
 template <class KV>
 __device__ __forceinline__ void put4(typename KV::T* p, f32x4 v) {
@@ -296,13 +299,11 @@ DEF_APPEND(smith_paged_append_bf16, KvBf16)
 // A row without keys gives zeros.
 //
 // The (row, head) pairs that read one KV head are the columns of a product:
-// S^T = K Q^T and O^T = V^T P^T on the matrix cores, 16 columns to a tile and
-// NT tiles to a workgroup (its block).  Its four waves take the block's keys in
-// turn, TK at a time, straight from the pages into the operands' registers, and
-// keep their own running maximum m, sum l and O^T; at the end they are joined
-// through LDS.  In this form nothing moves between lanes: a lane's four (or
-// eight) scores of S^T are one column's, so they become the P operand where they
-// are, and m, l and the rescaling of O^T are the lane's own.
+// S^T = K Q^T and O^T = V^T P^T on the matrix cores, 16 columns to a tile, in one
+// pass over the keys with each column's running maximum m, sum l and O^T.  In this
+// form nothing moves between lanes: a lane's four (or eight) scores of S^T are one
+// column's, so they become the P operand where they are, and m, l and the
+// rescaling of O^T are the lane's own.
 //   MFMA 16x16: lane (n = lane % 16, g = lane / 16) holds row n of A and column n
 //   of B at the k's of group g, and rows 4g .. 4g+3 of column n of D.
 //   K: A rows are keys, lane n its key's dims.  V: lane n holds dims n*DPL ..
@@ -318,13 +319,18 @@ DEF_APPEND(smith_paged_append_bf16, KvBf16)
 //
 // Work is cut on the device, where the lengths are: an item is (request, block
 // of columns, KV head, split of the block's keys).  With W = sum over blocks of
-// their request's length, a request of more than 5/4 C keys, C = max(SPLIT_MIN,
+// their request's length, a request of more than 5/4 C keys, C = max(split_min,
 // W / target), has its keys cut into splits of at most that many, so that target
-// items or so fill the chip whatever the lengths are; requests of nearly one length
-// (their longest within 5/4 of the mean) get one item to a workgroup and no more.  Every
-// workgroup forms the prefix sums of the items by itself.  The last of a block's
-// splits to finish (agent-scope counter) joins their partials in split order:
-// the same sums whichever finishes last.
+// items or so, two to a CU, fill the chip whatever the lengths are; requests of
+// nearly one length (their longest within 5/4 of the mean) get one item to a
+// workgroup and no more.  Every workgroup forms the prefix sums of the items by
+// itself.  The last of a block's splits to finish (agent-scope counter) joins
+// their partials in split order: the same sums whichever finishes last.  An item
+// costs 5 us before its keys count (cycles at 2.4 GHz, one row of 32 heads of 128
+// f16: lengths and cuts 1800, the item 2300, Q and the first page 4700, the waves'
+// join 1800; of a split 900 to write it, 900 to count it, 4000 to join them),
+// which is why twice or three times the items lose: one request of 20000 keys
+// 22.8 us with 512 wanted, 30 with 768.
 // ---------------------------------------------------------------------------
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -815,8 +821,8 @@ struct Item {
 // The workgroup's next item: its own number first, then whichever is next, so
 // that workgroups with short items take more of them.  take() when an item's keys
 // are through (thread 0's atomic is under way while the waves are joined; ahead of
-// the keys every load would wait for it), next() by all at its end.  As many are taken as there are items; the last one taken clears the
-// queue for the next call.
+// the keys every load would wait for it), next() by all at its end.  As many are
+// taken as there are items; the last one taken clears the queue for the next call.
 struct Turn {
   uint32_t item = blockIdx.x, taken = 0;
   bool more;
@@ -1057,7 +1063,15 @@ __device__ __forceinline__ void weigh(f32x4 (&S)[NJ], float c, float& m, float& 
     }
 }
 
-// One tile of 16 columns to a workgroup, its keys in registers.
+// One tile of 16 columns to a workgroup.  Its four waves take the keys in turn, TK
+// at a time, straight from the pages into the operands' registers, the next
+// tile's while this one's are multiplied, and are joined through LDS at the end.
+// For one row a request: bound by memory.  32 heads on 8 of 128 dims: 120 requests
+// of 2800 to 4000 keys in bf16 (1.67 GB) 302 us, 5.5 TB/s; one of 131071 in f16 101
+// us, 5.3 TB/s (a large copy: 4.8); 32 of 1 to 6000 31.7 us, 4.0 TB/s.  One of 517
+// f32 keys, 16 heads of 64: 9.3 us, latency.  More waves to a CU (3 and 4
+// workgroups by launch bounds) spill into scratch, whose loads wait for the
+// keys': 64 requests of 4000 keys 178 us with 2, 193 with 3, 269 with 4.
 template <class TILE, int DPL, bool SMALL>
 __device__ __forceinline__ void attention_body(const AttArgs& a) {
   typedef typename TILE::T T;
@@ -1265,6 +1279,10 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
 // its source chunk accordingly.  K operands are read as they lie; f16 and bf16
 // values through the transposing LDS read, lane (4k + c) of 16 supplying dims
 // 4c .. 4c+3 of the k-th of four keys and receiving one dim of all four.
+// Bound by the matrix cores: 2000 rows behind 6000 keys, 32 heads on 8 of 128 dims,
+// 229 GFLOP: f16 497 us, 922 TFLOP/s of split products (a large library product:
+// 1054), bf16 592 us, 1160 (1116), f32 1.99 ms, 115 (152).  Shorter prompts wait for
+// their longest blocks: four of 430 to 611 rows 48 us in f16, 46 % of that rate.
 // ---------------------------------------------------------------------------
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
