@@ -1328,8 +1328,9 @@ struct Rows16 {
   static constexpr int CT = 2, KT = 64, NJ = KT / 16, TERMS = MM::TERMS;
   static constexpr uint32_t CHUNKS = 2 * LINE<DPL>, ROWB = 32 * LINE<DPL>;
   // scores of the CT tiles' columns against the stage's keys
+  template <class BETWEEN>
   static __device__ __forceinline__ void scores(const uint8_t* k, uint32_t ln, uint32_t lg,
-                                                const u32x4 (&Q)[CT][TILE::QREG], f32x4 (&S)[CT][NJ]) {
+                                                const u32x4 (&Q)[CT][TILE::QREG], f32x4 (&S)[CT][NJ], BETWEEN between) {
 #pragma unroll
     for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -1352,6 +1353,7 @@ struct Rows16 {
         for (int t = 0; t < TERMS; t++)
 #pragma unroll
           for (int c = 0; c < CT; c++) S[c][j] = MM::mfma(x[j & 1][s], Q[c][s * TERMS + t], S[c][j]);
+      between(j);
     }
   }
   static __device__ __forceinline__ void add_pv(const uint8_t* v, uint32_t ln, uint32_t lg, const f32x4 (&S)[CT][NJ],
@@ -1396,8 +1398,9 @@ struct Rows32 {
   typedef float T;
   static constexpr int CT = 1, KT = 32, NJ = KT / 16;
   static constexpr uint32_t CHUNKS = 4 * LINE<DPL>, ROWB = 64 * LINE<DPL>;
+  template <class BETWEEN>
   static __device__ __forceinline__ void scores(const uint8_t* k, uint32_t ln, uint32_t lg,
-                                                const u32x4 (&Q)[CT][TILE::QREG], f32x4 (&S)[CT][NJ]) {
+                                                const u32x4 (&Q)[CT][TILE::QREG], f32x4 (&S)[CT][NJ], BETWEEN between) {
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
       f32x4 a = (f32x4){0.f, 0.f, 0.f, 0.f}, b = a;
@@ -1412,6 +1415,7 @@ struct Rows32 {
         b = __builtin_amdgcn_mfma_f32_16x16x4f32(x[3], q[3], b, 0, 0, 0);
       }
       S[0][j] = a + b;
+      between(j);
     }
   }
   static __device__ __forceinline__ void add_pv(const uint8_t* v, uint32_t ln, uint32_t lg, const f32x4 (&S)[CT][NJ],
@@ -1460,7 +1464,10 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
     const int32_t* table = a.tables + (size_t)I.b * a.max_pages;
     const size_t head_len = (size_t)hd << a.shift;
     uint32_t bad = 0, pages = 0, ahead = AHEAD;  // lane PARTS x + h: page of this wave's h-th 8 rows x stages on
-    auto fetch = [&](uint32_t t, uint32_t stage, uint32_t lane) {
+    const size_t page_bytes = a.nKV * head_len * sizeof(T);
+    const uint8_t* const k_head = (const uint8_t*)a.kpages + I.kvh * head_len * sizeof(T);
+    const ptrdiff_t to_v = (const uint8_t*)a.vpages - (const uint8_t*)a.kpages;
+    auto look_up = [&](uint32_t t, uint32_t lane) {
       if (ahead == AHEAD) {
         const uint32_t k = t + lane / PARTS * KT + w * SHARE + lane % PARTS * 8;
         const uint32_t p = (uint32_t)table[(k < k1 ? k : k1 - 1) >> a.shift];
@@ -1468,24 +1475,20 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
         pages = p < a.n_pages ? p : 0u;
         ahead = 0;
       }
-      const uint32_t to = lds0 + stage * 2 * REGION + w * SHARE * ROWB;
-#pragma unroll
-      for (uint32_t h = 0; h < PARTS; h++) {
-        const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)(ahead * PARTS + h));
-        const uint32_t first = t + w * SHARE + 8 * h;  // rows from k1 on: others of the page
-        const size_t at = ((size_t)p * a.nKV + I.kvh) * head_len + (size_t)(first & (P - 1)) * hd;
-#pragma unroll
-        for (uint32_t i = 0; i < INSTR; i++) {
-          const uint32_t r = i * RPI + lane / CHUNKS;  // row of the 8
-          uint32_t c = (lane % CHUNKS) ^ swizzle<CHUNKS>(w * SHARE + 8 * h + r);
-          const uint32_t last = hd * sizeof(T) / 16 - 1;  // past the head: against zeros of Q, into dims that nobody reads
-          c = c < last ? c : last;
-          const uint32_t off = r * hd * sizeof(T) + c * 16, piece = to + (h * INSTR + i) * 1024;
-          dma16((const T*)a.kpages + at, off, piece);
-          dma16((const T*)a.vpages + at, off, piece + REGION);
-        }
-      }
-      ahead++;
+    };
+    // the piece-th of PIECES 16 bytes a lane, of K and of V, of the stage at key t
+    constexpr uint32_t PIECES = PARTS * INSTR;
+    auto fetch = [&](uint32_t t, uint32_t stage, uint32_t lane, uint32_t piece) {
+      const uint32_t h = piece / INSTR, r = piece % INSTR * RPI + lane / CHUNKS;  // row of the part's 8
+      const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)(ahead * PARTS + h));
+      const uint32_t first = t + w * SHARE + 8 * h;  // rows from k1 on: others of the page
+      const uint8_t* at = k_head + (p * page_bytes + (size_t)(first & (P - 1)) * (hd * sizeof(T)));
+      uint32_t c = (lane % CHUNKS) ^ swizzle<CHUNKS>(w * SHARE + 8 * h + r);
+      const uint32_t last = hd * sizeof(T) / 16 - 1;  // past the head: against zeros of Q, into dims that nobody reads
+      c = c < last ? c : last;
+      const uint32_t off = r * hd * sizeof(T) + c * 16, to = lds0 + stage * 2 * REGION + w * SHARE * ROWB + piece * 1024;
+      dma16(at, off, to);
+      dma16(at + to_v, off, to + REGION);
     };
     // ---- this wave's columns, their loads ahead of the keys' ----
     f32x4 raw[CT][TILE::QRAW];
@@ -1495,7 +1498,12 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
       TILE::load_q(a.q + I.at(col < I.ncols ? col : 0, a.ld_q, hd), lg, hd, raw[t]);
     }
     __syncthreads();  // the stages and s_odd are free
-    if (k0 < k1) fetch(k0, 0, lane);
+    if (k0 < k1) {
+      look_up(k0, lane);
+#pragma unroll
+      for (uint32_t x = 0; x < PIECES; x++) fetch(k0, 0, lane, x);
+      ahead++;
+    }
     u32x4 Q[CT][QREG];
     f32x4 O[CT][DPL];
     float m[CT], l[CT], c[CT];
@@ -1529,7 +1537,8 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
       uint32_t here = lane;
       if (CT > 1) asm volatile("" : "+v"(here));
       const uint32_t hn = here & 15, hg = here >> 4;
-      if (t0 + KT < k1) fetch(t0 + KT, stage ^ 1, here);
+      const bool more = t0 + KT < k1;
+      if (more) look_up(t0 + KT, here);
       if (masked) {
         // a weight of 0 does not hide a value that is not finite: values behind
         // the block's keys go to 0, and so do chunks with such a value that only
@@ -1545,9 +1554,23 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
         }
         __syncthreads();
       }
-      if (!some) continue;
+      // the next stage's loads go out between the products of this one's scores
+      auto piece = [&](uint32_t x) {
+        if (more) fetch(t0 + KT, stage ^ 1, here, x);
+      };
+      if (!some) {
+#pragma unroll
+        for (uint32_t x = 0; x < PIECES; x++) piece(x);
+        ahead++;
+        continue;
+      }
       f32x4 S[CT][NJ];
-      ROWS::scores(k, hn, hg, Q, S);
+      ROWS::scores(k, hn, hg, Q, S, [&](int j) {
+#pragma unroll
+        for (uint32_t x = 0; x < PIECES; x++)
+          if ((int)(x * NJ / PIECES) == j) piece(x);
+      });
+      ahead++;
 #pragma unroll
       for (int t = 0; t < CT; t++) {
         if (masked) {
