@@ -356,12 +356,17 @@ struct MmF16 {
   static constexpr int TERMS = 2;
   static constexpr uint32_t EXPONENT = 0x7C00u;
   static __device__ __forceinline__ void split(const float (&x)[8], u32x4 (&t)[TERMS]) {
+    float minus = -1.f;
+    asm("" : "+s"(minus));
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       const f16x2 hi = __builtin_convertvector((f32x2){x[2 * k], x[2 * k + 1]}, f16x2);
-      const f32x2 r = (f32x2){__builtin_fmaf((float)hi[0], -1.f, x[2 * k]), __builtin_fmaf((float)hi[1], -1.f, x[2 * k + 1])};
+      // the rest in one mixed-precision operation each (x - hi by a factor that the
+      // compiler does not see would be a conversion and a subtraction)
+      const f16x2 lo = (f16x2){(_Float16)__builtin_fmaf((float)hi[0], minus, x[2 * k]),
+                               (_Float16)__builtin_fmaf((float)hi[1], minus, x[2 * k + 1])};
       t[0][k] = __builtin_bit_cast(uint32_t, hi);
-      t[1][k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, f16x2));
+      t[1][k] = __builtin_bit_cast(uint32_t, lo);
     }
   }
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
