@@ -355,19 +355,16 @@ struct MmF16 {
   typedef _Float16 T;
   static constexpr int TERMS = 2;
   static constexpr uint32_t EXPONENT = 0x7C00u;
-  static __device__ __forceinline__ void split(const float (&x)[8], u32x4 (&t)[TERMS]) {
+  // word k of the parts, from values 2k and 2k + 1
+  static __device__ __forceinline__ void split2(float x, float y, u32x4 (&t)[TERMS], int k) {
+    // the rest in one mixed-precision operation each (without a factor that the
+    // compiler does not know it makes a conversion and a subtraction)
     float minus = -1.f;
     asm("" : "+s"(minus));
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const f16x2 hi = __builtin_convertvector((f32x2){x[2 * k], x[2 * k + 1]}, f16x2);
-      // the rest in one mixed-precision operation each (x - hi by a factor that the
-      // compiler does not see would be a conversion and a subtraction)
-      const f16x2 lo = (f16x2){(_Float16)__builtin_fmaf((float)hi[0], minus, x[2 * k]),
-                               (_Float16)__builtin_fmaf((float)hi[1], minus, x[2 * k + 1])};
-      t[0][k] = __builtin_bit_cast(uint32_t, hi);
-      t[1][k] = __builtin_bit_cast(uint32_t, lo);
-    }
+    const f16x2 hi = __builtin_convertvector((f32x2){x, y}, f16x2);
+    const f16x2 lo = (f16x2){(_Float16)__builtin_fmaf((float)hi[0], minus, x), (_Float16)__builtin_fmaf((float)hi[1], minus, y)};
+    t[0][k] = __builtin_bit_cast(uint32_t, hi);
+    t[1][k] = __builtin_bit_cast(uint32_t, lo);
   }
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -377,16 +374,13 @@ struct MmBf16 {
   typedef __bf16 T;
   static constexpr int TERMS = 3;
   static constexpr uint32_t EXPONENT = 0x7F80u;
-  static __device__ __forceinline__ void split(const float (&x)[8], u32x4 (&t)[TERMS]) {
+  static __device__ __forceinline__ void split2(float x, float y, u32x4 (&t)[TERMS], int k) {
+    f32x2 r = (f32x2){x, y};
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      f32x2 r = (f32x2){x[2 * k], x[2 * k + 1]};
-#pragma unroll
-      for (int p = 0; p < TERMS; p++) {
-        t[p][k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
-        r[0] -= __uint_as_float(t[p][k] << 16);
-        r[1] -= __uint_as_float(t[p][k] & 0xFFFF0000u);
-      }
+    for (int p = 0; p < TERMS; p++) {
+      t[p][k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+      r[0] -= __uint_as_float(t[p][k] << 16);
+      r[1] -= __uint_as_float(t[p][k] & 0xFFFF0000u);
     }
   }
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -446,7 +440,8 @@ struct Tile16 {
 #pragma unroll
       for (int e = 0; e < 8; e++) y[e] = in ? __builtin_amdgcn_ldexpf(x[2 * s + e / 4][e % 4] * sign, e2) : 0.f;
       u32x4 t[TERMS];
-      MM::split(y, t);
+#pragma unroll
+      for (int k = 0; k < 4; k++) MM::split2(y[2 * k], y[2 * k + 1], t, k);
 #pragma unroll
       for (int k = 0; k < TERMS; k++) put(s * TERMS + k, t[k]);
     }
@@ -500,15 +495,10 @@ struct Tile16 {
         for (int j = 0; j < NJ; j++) S[j] = MM::mfma(K[j][s], x, S[j]);
       }
   }
-  static __device__ __forceinline__ void weights(const f32x4 (&S)[NJ], u32x4 (&t)[TERMS]) {
-    float p[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) p[e] = S[e / 4][e % 4];
-    MM::split(p, t);
-  }
   __device__ __forceinline__ void add_pv(const f32x4 (&S)[NJ], f32x4 (&O)[DPL]) const {
     u32x4 t[TERMS];
-    weights(S, t);
+#pragma unroll
+    for (int k = 0; k < 4; k++) MM::split2(S[k / 2][k % 2 * 2], S[k / 2][k % 2 * 2 + 1], t, k);
 #pragma unroll
     for (int d = 0; d < DPL; d++) {
       const u32x4 v = dim(d);
@@ -1040,10 +1030,11 @@ __device__ __forceinline__ float score_factor(float scale, int e2) {
   return fmaxf(__builtin_amdgcn_ldexpf(fabsf(scale) * 1.44269504088896340736f, -e2), 1.17549435e-38f);
 }
 
-// Scores of one column (times c: in powers of two) into weights 2^(score - m +
-// P_EXP), with the column's running maximum m, sum l (this lane's share) and O.
+// Scores of one column (times c: in powers of two) become weights 2^(score - m +
+// P_EXP): follow() moves the column's running maximum m, with its sum l (this
+// lane's share) and O, and says what is added to a score; weight() is one of them.
 template <int NJ, int DPL>
-__device__ __forceinline__ void weigh(f32x4 (&S)[NJ], float c, float& m, float& l, f32x4 (&O)[DPL]) {
+__device__ __forceinline__ float follow(const f32x4 (&S)[NJ], float c, float& m, float& l, f32x4 (&O)[DPL]) {
   float x = -__builtin_inff();
 #pragma unroll
   for (int j = 0; j < NJ; j++)
@@ -1058,14 +1049,20 @@ __device__ __forceinline__ void weigh(f32x4 (&S)[NJ], float c, float& m, float& 
 #pragma unroll
     for (int d = 0; d < DPL; d++) O[d] *= f;
   }
-  const float shift = m == -__builtin_inff() ? 0.f : P_EXP - m;
+  return m == -__builtin_inff() ? 0.f : P_EXP - m;
+}
+__device__ __forceinline__ float weight(float s, float c, float shift, float& l) {
+  const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, shift));
+  l += p;
+  return p;
+}
+template <int NJ, int DPL>
+__device__ __forceinline__ void weigh(f32x4 (&S)[NJ], float c, float& m, float& l, f32x4 (&O)[DPL]) {
+  const float shift = follow<NJ, DPL>(S, c, m, l, O);
 #pragma unroll
   for (int j = 0; j < NJ; j++)
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      S[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[j][i], c, shift));
-      l += S[j][i];
-    }
+    for (int i = 0; i < 4; i++) S[j][i] = weight(S[j][i], c, shift, l);
 }
 
 // One tile of 16 columns to a workgroup.  Its four waves take the keys in turn, TK
@@ -1361,16 +1358,22 @@ struct Rows16 {
       between(j);
     }
   }
-  static __device__ __forceinline__ void add_pv(const uint8_t* v, uint32_t ln, uint32_t lg, const f32x4 (&S)[CT][NJ],
+  // O += V^T P^T, 32 keys at a time; the weights of the next 32 are worked out
+  // between the products of these
+  static __device__ __forceinline__ void add_pv(const uint8_t* v, uint32_t ln, uint32_t lg, f32x4 (&S)[CT][NJ],
+                                                const float (&c)[CT], const float (&shift)[CT], float (&l)[CT],
                                                 f32x4 (&O)[CT][DPL]) {
+    u32x4 p[2][CT][TERMS];
+    auto pair = [&](int h, int x) {  // of CT * 4 to 32 keys
+      const int t = x / 4, k = x % 4;
+      const f32x4 s = S[t][2 * h + k / 2];
+      const float a = weight(s[k % 2 * 2], c[t], shift[t], l[t]), b = weight(s[k % 2 * 2 + 1], c[t], shift[t], l[t]);
+      MM::split2(a, b, p[h & 1][t], k);
+    };
+#pragma unroll
+    for (int x = 0; x < CT * 4; x++) pair(0, x);
 #pragma unroll
     for (int h = 0; h < NJ / 2; h++) {
-      u32x4 p[CT][TERMS];
-#pragma unroll
-      for (int c = 0; c < CT; c++) {
-        const f32x4 two[2] = {S[c][2 * h], S[c][2 * h + 1]};
-        TILE::weights(two, p[c]);
-      }
 #pragma unroll
       for (int d = 0; d < DPL; d++) {
         u32x2 x[2];
@@ -1384,7 +1387,15 @@ struct Rows16 {
 #pragma unroll
         for (int t = 0; t < TERMS; t++)
 #pragma unroll
-          for (int c = 0; c < CT; c++) O[c][d] = MM::mfma(y, p[c][t], O[c][d]);
+          for (int c = 0; c < CT; c++) O[c][d] = MM::mfma(y, p[h & 1][c][t], O[c][d]);
+        if (h + 1 < NJ / 2) {
+#pragma unroll
+          for (int x = 0; x < CT * 4; x++)
+            if (x * DPL / (CT * 4) == d) pair(h + 1, x);
+        }
+        // three parts: kept in this order, which the compiler's own spills (a chunk
+        // of 2000 rows behind 6000 keys 573 us, 591 without; two parts 470 and 462)
+        if (TERMS > 2) __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -1423,8 +1434,13 @@ struct Rows32 {
       between(j);
     }
   }
-  static __device__ __forceinline__ void add_pv(const uint8_t* v, uint32_t ln, uint32_t lg, const f32x4 (&S)[CT][NJ],
+  static __device__ __forceinline__ void add_pv(const uint8_t* v, uint32_t ln, uint32_t lg, f32x4 (&S)[CT][NJ],
+                                                const float (&c)[CT], const float (&shift)[CT], float (&l)[CT],
                                                 f32x4 (&O)[CT][DPL]) {
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) S[0][j][i] = weight(S[0][j][i], c[0], shift[0], l[0]);
 #pragma unroll
     for (int j = 0; j < NJ; j++)
 #pragma unroll
@@ -1570,6 +1586,7 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
         continue;
       }
       f32x4 S[CT][NJ];
+      float shift[CT];
       ROWS::scores(k, hn, hg, Q, S, [&](int j) {
 #pragma unroll
         for (uint32_t x = 0; x < PIECES; x++)
@@ -1595,9 +1612,9 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
                 if (16 * j + i < end && (marks >> (16 * j + i) & 1)) l[t] = __builtin_nanf("");
           }
         }
-        weigh<NJ, DPL>(S[t], c[t], m[t], l[t], O[t]);
+        shift[t] = follow<NJ, DPL>(S[t], c[t], m[t], l[t], O[t]);
       }
-      ROWS::add_pv(v, hn, hg, S, O);
+      ROWS::add_pv(v, hn, hg, S, c, shift, l, O);
     }
     if (bad) paged_err(a.err, PAGED_ERR_ATT_PAGE, I.b);
     turn.take(a, items.total);
