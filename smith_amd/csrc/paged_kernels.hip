@@ -29,6 +29,15 @@ __device__ __forceinline__ void paged_err(uint64_t* __restrict__ err, uint32_t c
     __hip_atomic_store(err, ((uint64_t)arg << 32) | code, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
+template <class T>
+__device__ __forceinline__ T max64_lanes(T v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const T o = __shfl_xor(v, d);
+    v = o > v ? o : v;
+  }
+  return v;
+}
 // sum over the lanes up to this one: within rows of 16, then across them
 __device__ __forceinline__ uint32_t scan64_lanes(uint32_t v) {
 #define SCAN_DPP(CTRL, ROWS) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false)
@@ -647,45 +656,80 @@ __device__ __forceinline__ void request(const AttArgs& a, uint32_t b, bool tell,
   }
 }
 
-// The items of a call, by the prefix sums that each workgroup forms in LDS:
-// those of the long requests (half of C keys and more) come before the others,
-// so that what is taken last is short.
+// The items of a call, from what each workgroup works out in LDS.  Which comes when
+// matters where a workgroup gets two and where two share a CU (a grid of two to a
+// CU puts workgroups i and i + CUS on one).  Blocks of many columns (SORT) of up to
+// 64 requests, more than CUS of them and none cut: the longest first, and the
+// second CUS in reverse.  4 prompts of 1000 rows, 16 heads of 128, microseconds by
+// requests and so: f16 62, 56, bf16 81, 70, f32 194, 154; 8 of 16 heads of 64 on 4 KV
+// heads 56, 46 | 70, 53 | 155, 132.  (To look an item up costs a microsecond more:
+// one row a request loses 3 to 8 % by it, 20 mixed requests that are cut 5 % in f16.)
+// Else by the request, those of the long ones (half of C keys and more) before the
+// others.
+#define CUS 256u
+template <bool SORT>
 struct Items {
   // [n_req + 1] of a request: its first item of its class (in the other class's
-  // array the next request's), its first partial, its first row, its length
+  // array the next request's), or its first level and its blocks of rows; its
+  // first partial, its first row, its length
   uint32_t *longs, *shorts, *part, *row, *len;
+  struct Head {
+    uint32_t total_long;
+    uint32_t levels;  // 0: not sorted
+    float inv_c;
+    uint32_t pad;
+  }* head;  // of SORT, read where an item is looked up: registers for it cost the key loop spills
   uint32_t total, total_long;
   float inv_c;
 
-  __device__ __forceinline__ uint32_t splits(uint32_t keys) const {  // of at most about 5/4 C keys
+  static __device__ __forceinline__ uint32_t splits(uint32_t keys, float inv_c) {  // of at most about 5/4 C keys
     const uint32_t s = (uint32_t)((float)keys * inv_c * 0.8f + 0.999f);
     return s < 1 ? 1u : s > PAGED_SPLIT_MAX ? PAGED_SPLIT_MAX : s;
   }
-  __device__ __forceinline__ bool is_long(uint32_t keys) const { return (float)keys * inv_c >= 0.5f; }
+  static __device__ __forceinline__ bool is_long(uint32_t keys, float inv_c) { return (float)keys * inv_c >= 0.5f; }
 };
 
-__device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Items& t) {
-  t.longs = lds;
+template <bool SORT>
+__device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Items<SORT>& t) {
+  t.head = (typename Items<SORT>::Head*)lds;
+  t.longs = lds + sizeof(typename Items<SORT>::Head) / 4;
   t.shorts = t.longs + a.n_req + 1;
   t.part = t.shorts + a.n_req + 1;
   t.row = t.part + a.n_req + 1;
   t.len = t.row + a.n_req + 1;
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6, RB = a.rows_blk, groups = a.groups;
-  auto set_work = [&](float work) { t.inv_c = 1.0f / fmaxf(work * a.per_target, a.split_min); };
+  float inv_c = 0.f;
+  uint32_t levels = 0, total_long = 0;
+  auto set_work = [&](float work) { inv_c = 1.0f / fmaxf(work * a.per_target, a.split_min); };
+  auto put_head = [&] {
+    t.total_long = total_long;
+    t.inv_c = inv_c;
+    if (SORT) *t.head = typename Items<SORT>::Head{total_long, levels, inv_c, 0u};
+  };
   if (a.n_req <= 64) {
     // every wave for itself, request to lane: no barriers (they all write the same)
     uint32_t r0 = 0, n = 0, len = 0;
     if (lane < a.n_req) request(a, lane, blockIdx.x == 0, r0, n, len);
     const uint32_t blocks = div_up(n, RB) * groups;
     set_work(sum64_lanes((float)blocks * (float)len));
-    const uint32_t ns = t.splits(len), it = blocks * a.nKV * ns;
-    const bool lg = t.is_long(len);
+    const uint32_t ns = t.splits(len, inv_c), it = blocks * a.nKV * ns;
+    const bool lg = t.is_long(len, inv_c);
     const uint32_t il = scan64_lanes(lg ? it : 0u), is = scan64_lanes(lg ? 0u : it), ip = scan64_lanes(ns > 1 ? it : 0u);
-    t.total_long = (uint32_t)__builtin_amdgcn_readlane((int)il, 63);
-    t.total = t.total_long + (uint32_t)__builtin_amdgcn_readlane((int)is, 63);
+    total_long = (uint32_t)__builtin_amdgcn_readlane((int)il, 63);
+    t.total = total_long + (uint32_t)__builtin_amdgcn_readlane((int)is, 63);
+    uint32_t first = il - (lg ? it : 0u), second = is - (lg ? 0u : it);
+    if (SORT && t.total > CUS && !__builtin_amdgcn_readlane((int)ip, 63)) {
+      // the level of a request's last rows: by how many blocks' rows it is shorter
+      // than the longest
+      const uint32_t keys = blocks ? len : 0u;
+      first = (uint32_t)((float)(max64_lanes(keys) - keys) * __builtin_amdgcn_rcpf((float)RB));
+      second = div_up(n, RB);
+      levels = uniform(max64_lanes(blocks ? first + second : 0u));
+    }
+    put_head();
     if (lane < a.n_req) {
-      t.longs[lane] = il - (lg ? it : 0u);
-      t.shorts[lane] = is - (lg ? 0u : it);
+      t.longs[lane] = first;
+      t.shorts[lane] = second;
       t.part[lane] = ip - (ns > 1 ? it : 0u);
       t.row[lane] = r0;
       t.len[lane] = len;
@@ -715,8 +759,8 @@ __device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Item
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
     if (b >= a.n_req) break;
-    const uint32_t ns = t.splits(t.len[b]), it = div_up(t.longs[b], RB) * groups * a.nKV * ns;
-    (t.is_long(t.len[b]) ? longs : shorts) += it;
+    const uint32_t ns = t.splits(t.len[b], inv_c), it = div_up(t.longs[b], RB) * groups * a.nKV * ns;
+    (t.is_long(t.len[b], inv_c) ? longs : shorts) += it;
     parts += ns > 1 ? it : 0;
   }
   uint32_t il = scan64_lanes(longs), is = scan64_lanes(shorts), ip = scan64_lanes(parts);
@@ -726,7 +770,7 @@ __device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Item
     s_wave[w][2] = ip;
   }
   __syncthreads();
-  t.total = t.total_long = 0;
+  t.total = total_long = 0;
   il -= longs;
   is -= shorts;
   ip -= parts;
@@ -737,16 +781,17 @@ __device__ __forceinline__ void find_items(const AttArgs& a, uint32_t* lds, Item
       is += s_wave[k][1];
       ip += s_wave[k][2];
     }
-    t.total_long += s_wave[k][0];
+    total_long += s_wave[k][0];
     t.total += s_wave[k][1];
   }
-  t.total += t.total_long;
+  t.total += total_long;
+  put_head();
   if (blockIdx.x >= t.total) return;
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
     if (b >= a.n_req) break;
-    const uint32_t ns = t.splits(t.len[b]), n = t.longs[b], it = div_up(n, RB) * groups * a.nKV * ns;
-    const bool lg = t.is_long(t.len[b]);
+    const uint32_t ns = t.splits(t.len[b], inv_c), n = t.longs[b], it = div_up(n, RB) * groups * a.nKV * ns;
+    const bool lg = t.is_long(t.len[b], inv_c);
     t.longs[b] = il;
     t.shorts[b] = is;
     t.part[b] = ip;
@@ -765,32 +810,76 @@ struct Item {
   uint32_t k0, k1;
   uint32_t part;  // of ns > 1: its partial; a block's next split has the one nKV further on
 
-  __device__ __forceinline__ Item(const AttArgs& a, const Items& t, uint32_t item, uint32_t CB, uint32_t unit) {
-    // the last request that starts at or before the item (those without items of
-    // its class start there too)
-    const uint32_t* from = item < t.total_long ? t.longs : t.shorts;
-    if (item >= t.total_long) item -= t.total_long;
+  template <bool SORT>
+  __device__ __forceinline__ Item(const AttArgs& a, const Items<SORT>& t, uint32_t item, uint32_t CB, uint32_t unit) {
     const uint32_t lane = threadIdx.x & 63;
-    uint32_t lo = 0;
-    if (a.n_req > 64) {  // which 64 of them, then which one
-      const uint32_t k = lane * 64;
-      lo = 64 * (uint32_t)__popcll(__ballot(k < a.n_req && from[k < a.n_req ? k : 0] <= item)) - 64;
+    uint32_t blk, rowblk;
+    uint32_t levels = 0, total_long = t.total_long;
+    float inv_c = t.inv_c;
+    if (SORT) {
+      levels = uniform(t.head->levels);
+      total_long = uniform(t.head->total_long);
+      inv_c = __uint_as_float(uniform(__float_as_uint(t.head->inv_c)));
     }
-    const uint32_t k = lo + lane;
-    b = uniform(lo + (uint32_t)__popcll(__ballot(k < a.n_req && from[k < a.n_req ? k : 0] <= item)) - 1);
-    r0 = uniform(t.row[b]);
-    len = uniform(t.len[b]);
-    const uint32_t local = item - uniform(from[b]);
-    part = uniform(t.part[b]) + local;
-    n = a.row_start ? uniform(t.row[b + 1]) - r0 : 1u;
-    ns = uniform(t.splits(len));
-    // the KV head first (neighbouring blocks of a head meet in one XCD's L2 when
-    // there are 8 of them), the blocks with the most keys before the others
-    // (a request that is cut has no more items than there is room for partials)
-    const uint32_t rest = quotient_u(local, a.nKV), later = ns > 1 ? uniform(small_quotient(rest, ns)) : rest;
-    kvh = local - rest * a.nKV;
-    split = rest - later * ns;
-    const uint32_t blk = quotient_u(n + a.rows_blk - 1, a.rows_blk) * a.groups - 1 - later, rowblk = quotient_u(blk, a.groups);
+    if (SORT && levels) {
+      // The request's keys fall by a block's rows from one level to the next, the
+      // longest's last block being level 0: N(L) = sum over requests of the levels
+      // that they have before L is the number of blocks before level L.
+      const bool in = lane < a.n_req;
+      const uint32_t from = in ? t.longs[lane] : 0u, deep = in ? t.shorts[lane] : 0u;
+      const uint32_t rest = quotient_u(item, a.nKV);
+      kvh = item - rest * a.nKV;
+      uint32_t lo = 0, hi = levels, before = 0;  // N(lo) <= rest < N(hi)
+      while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1, at = mid > from ? mid - from : 0u;
+        const uint32_t N =
+            (uint32_t)__builtin_amdgcn_readlane((int)scan64_lanes((at < deep ? at : deep) * a.groups), 63);
+        if (N <= rest) {
+          lo = mid;
+          before = N;
+        } else {
+          hi = mid;
+        }
+      }
+      const uint32_t here = lo >= from && lo - from < deep ? a.groups : 0u, upto = scan64_lanes(here), d = rest - before;
+      b = (uint32_t)__popcll(__ballot(upto <= d));
+      const uint32_t group = d - (uint32_t)__builtin_amdgcn_readlane((int)(upto - here), (int)b);
+      r0 = uniform(t.row[b]);
+      len = uniform(t.len[b]);
+      n = a.row_start ? uniform(t.row[b + 1]) - r0 : 1u;
+      ns = 1;
+      split = 0;
+      part = 0;
+      rowblk = (uint32_t)__builtin_amdgcn_readlane((int)deep, (int)b) - 1 -
+               (lo - (uint32_t)__builtin_amdgcn_readlane((int)from, (int)b));
+      blk = rowblk * a.groups + group;
+    } else {
+      // the last request that starts at or before the item (those without items of
+      // its class start there too)
+      const uint32_t* from = item < total_long ? t.longs : t.shorts;
+      if (item >= total_long) item -= total_long;
+      uint32_t lo = 0;
+      if (a.n_req > 64) {  // which 64 of them, then which one
+        const uint32_t k = lane * 64;
+        lo = 64 * (uint32_t)__popcll(__ballot(k < a.n_req && from[k < a.n_req ? k : 0] <= item)) - 64;
+      }
+      const uint32_t k = lo + lane;
+      b = uniform(lo + (uint32_t)__popcll(__ballot(k < a.n_req && from[k < a.n_req ? k : 0] <= item)) - 1);
+      r0 = uniform(t.row[b]);
+      len = uniform(t.len[b]);
+      const uint32_t local = item - uniform(from[b]);
+      part = uniform(t.part[b]) + local;
+      n = a.row_start ? uniform(t.row[b + 1]) - r0 : 1u;
+      ns = uniform(t.splits(len, inv_c));
+      // the KV head first (neighbouring blocks of a head meet in one XCD's L2 when
+      // there are 8 of them), the blocks with the most keys before the others (a
+      // request that is cut has no more items than there is room for partials)
+      const uint32_t rest = quotient_u(local, a.nKV), later = ns > 1 ? uniform(small_quotient(rest, ns)) : rest;
+      kvh = local - rest * a.nKV;
+      split = rest - later * ns;
+      blk = quotient_u(n + a.rows_blk - 1, a.rows_blk) * a.groups - 1 - later;
+      rowblk = quotient_u(blk, a.groups);
+    }
     head0 = (blk - rowblk * a.groups) * CB;
     heads = a.G - head0 < a.heads_blk ? a.G - head0 : a.heads_blk;
     head0 += kvh * a.G;
@@ -821,6 +910,13 @@ struct Item {
 struct Turn {
   uint32_t item = blockIdx.x, taken = 0;
   bool more;
+  __device__ __forceinline__ Turn(uint32_t total, bool sort) {
+    if (!sort) return;
+    const uint32_t first = total < gridDim.x ? total : gridDim.x;
+    const uint32_t eights = first > CUS ? (first - CUS) / 8 : 0, j = item - CUS;
+    if (item >= CUS && j / 8 < eights) item = uniform(CUS + (eights - 1 - j / 8) * 8 + j % 8);
+    item = uniform(item);
+  }
   __device__ __forceinline__ void take(const AttArgs& a, uint32_t total) {
     more = total > gridDim.x;
     if (more && threadIdx.x == 0) taken = __hip_atomic_fetch_add(a.queue, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -1089,10 +1185,10 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t ln = lane & 15, lg = lane >> 4;
   const uint32_t P = 1u << a.shift, hd = a.hd;
-  Items items;
+  Items<false> items;
   find_items(a, (uint32_t*)(s_ml + 4 * 16 * 2), items);
 
-  for (Turn turn; turn.item < items.total; turn.next(a, items.total)) {
+  for (Turn turn(items.total, false); turn.item < items.total; turn.next(a, items.total)) {
     const Item I(a, items, turn.item, CB, TK);
     const uint32_t k0 = I.k0, k1 = I.k1, kvh = I.kvh;
     f32x4 q_raw[TILE::QRAW];
@@ -1473,10 +1569,10 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
   const uint32_t ln = lane & 15, lg = lane >> 4;
   const uint32_t P = 1u << a.shift, hd = a.hd;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  Items items;
+  Items<true> items;
   find_items(a, s_odd + 4, items);
 
-  for (Turn turn; turn.item < items.total; turn.next(a, items.total)) {
+  for (Turn turn(items.total, true); turn.item < items.total; turn.next(a, items.total)) {
     const Item I(a, items, turn.item, CB, KT);
     const uint32_t k0 = I.k0, k1 = I.k1;
     // ---- this wave's share of a stage: KT / 4 rows of K and of V, 8 or 16, a page to 8 ----

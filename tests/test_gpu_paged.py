@@ -387,6 +387,10 @@ def test_attention_one_long_request(dtype, n):
     (4, 2, 80, 8, [90, 700, 5], [41, 30, 5]),
     (6, 2, 88, 16, [64, 1000], [64, 20]),
     (5, 5, 72, 32, [33, 65], [33, 1]),
+    # more than 256 blocks, none cut: taken longest first
+    (16, 16, 8, 16, [1000, 3, 90, 260, 0, 777, 128, 129], [1000, 3, 90, 260, 0, 777, 128, 129]),
+    (16, 16, 8, 8, [900, 30, 600], [500, 30, 600]),
+    (130, 1, 8, 16, [300, 40], [260, 40]),                         # several blocks to a row's heads
     (16, 4, 64, 64, [700], [9])])
 def test_attention_ragged_rows(dtype, H, nKV, D, P, lens, added):
     case = attention_case(H + sum(lens), dtype, H, nKV, D, P, lens, added)
