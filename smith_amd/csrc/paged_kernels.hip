@@ -1378,9 +1378,11 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
 // values through the transposing LDS read, lane (4k + c) of 16 supplying dims
 // 4c .. 4c+3 of the k-th of four keys and receiving one dim of all four.
 // Bound by the matrix cores: 2000 rows behind 6000 keys, 32 heads on 8 of 128 dims,
-// 229 GFLOP: f16 497 us, 922 TFLOP/s of split products (a large library product:
-// 1054), bf16 592 us, 1160 (1116), f32 1.99 ms, 115 (152).  Shorter prompts wait for
-// their longest blocks: four of 430 to 611 rows 48 us in f16, 46 % of that rate.
+// 229 GFLOP: f16 450 us, 1020 TFLOP/s of split products (a large library product:
+// 1097), bf16 542 us, 1270 (1136), f32 1.99 ms, 115 (152).  A wave's stage is a chain
+// of 6000 cycles for 2048 of products (f16), so the next stage's loads and the next
+// weights go out between products, and shorter prompts wait for their longest
+// blocks: four of 430 to 611 rows 42.6 us in f16, half of that rate.
 // ---------------------------------------------------------------------------
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;

@@ -2464,10 +2464,11 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   // waves' columns -- if there are enough of them for the waves of the card, which
   // its 64 or 128 columns to a workgroup otherwise leave idle.  Microseconds, the
   // first kernel's and the second's (32 heads on 8, f16 | bf16 | f32): a prompt of
-  // 300 rows (9600 columns) 18.5, 23.0 | 18.1, 27.2 | 22, 38; of 1000 rows 67, 51 |
-  // 68, 61 | 112, 132; of 2000 rows 195, 108 | 198, 133 | 389, 325; behind 8000 keys
-  // 64 rows (2048 columns) 53, 64 | 52, 75 | 109, 120, 256 rows (8192) 159, 105 |
-  // 155, 127 | 361, 319; 16 prompts of up to 200 rows 85, 41 | 88, 55 | 109, 79.
+  // 100 rows (3200 columns) 9.3, 14.2 | 9.0, 17.4 | 10.9, 17.7; of 300 rows 18.7, 21.3
+  // | 18.3, 26.1 | 22, 37; of 1000 rows 67, 47 | 70, 57 | 114, 114; of 2000 rows 191,
+  // 97 | 200, 124 | 394, 316; behind 8000 keys 64 rows (2048 columns) 52, 60 | 52, 71 |
+  // 109, 116, 256 rows (8192) 157, 99 | 157, 121 | 365, 308; 16 prompts of up to 200
+  // rows 85, 37 | 88, 51 | 109, 68.
   // The second loads 8 keys at once, of one page.  The first takes 16 keys as one
   // address, or looks them up one by one where pages are smaller.
   const uint32_t G = n_heads / n_kv_heads;
@@ -2477,10 +2478,10 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   const uint32_t CB = !many ? 16 : kv_type == SMITH_KV_F32 ? 64 : 128, dims = head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : 128;
   const uint32_t target = 512;  // two workgroups to a CU
   // Keys to a split at least.  A split of many columns leaves 64 KB and the join
-  // reads them again: 64 f16 rows behind 8000 keys, 32 heads, 65 us with 512, 78 with
-  // 384, 85 with 256 (300 rows of a prompt 23 us with 512, uncut, 46 with 128).  f32
-  // keys are eight times the work: 20 requests, half of them with chunks of up to 77
-  // rows, 68 us with 256, 92 with 512.
+  // reads them again: 64 f16 rows behind 8000 keys, 32 heads, in that kernel 65 us
+  // with 512, 78 with 384, 85 with 256 (300 rows of a prompt 23 us with 512, uncut, 46
+  // with 128).  f32 keys are eight times the work: 20 requests, half of them with
+  // chunks of up to 77 rows, 68 us with 256, 92 with 512.
   const float split_min = !many ? 128.f : kv_type == SMITH_KV_F32 ? 256.f : 512.f;
   // a block that is cut has more than 5/4 C keys and so less than twice its keys / C
   // splits: 2 W / C <= 2 target of them in all (and some for what f32 rounds)
