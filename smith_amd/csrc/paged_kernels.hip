@@ -1435,25 +1435,31 @@ struct Rows16 {
     for (int c = 0; c < CT; c++)
 #pragma unroll
       for (int j = 0; j < NJ; j++) S[c][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    u32x4 x[2][TILE::KS];
-    auto load = [&](int j) {
+    // 32 keys and 32 dims a step, the next step's operands on their way: products of
+    // one sum are CT * 2 apart, which covers the first's latency
+    u32x4 x[2][2];
+    auto load = [&](int step) {
 #pragma unroll
-      for (int s = 0; s < TILE::KS; s++) {
-        const uint32_t r = 16 * j + ln;
-        x[j & 1][s] = *(const u32x4*)(k + r * ROWB + ((4 * s + lg) ^ swizzle<CHUNKS>(r)) * 16);
+      for (int j = 0; j < 2; j++) {
+        const uint32_t r = 16 * (step / TILE::KS * 2 + j) + ln;
+        x[step & 1][j] = *(const u32x4*)(k + r * ROWB + ((4 * (step % TILE::KS) + lg) ^ swizzle<CHUNKS>(r)) * 16);
       }
     };
+    constexpr int STEPS = NJ / 2 * TILE::KS;
     load(0);
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      if (j + 1 < NJ) load(j + 1);
+    for (int step = 0; step < STEPS; step++) {
+      if (step + 1 < STEPS) load(step + 1);
 #pragma unroll
-      for (int s = 0; s < TILE::KS; s++)
+      for (int t = 0; t < TERMS; t++)
 #pragma unroll
-        for (int t = 0; t < TERMS; t++)
+        for (int j = 0; j < 2; j++)
 #pragma unroll
-          for (int c = 0; c < CT; c++) S[c][j] = MM::mfma(x[j & 1][s], Q[c][s * TERMS + t], S[c][j]);
-      between(j);
+          for (int c = 0; c < CT; c++) {
+            f32x4& sum = S[c][step / TILE::KS * 2 + j];
+            sum = MM::mfma(x[step & 1][j], Q[c][step % TILE::KS * TERMS + t], sum);
+          }
+      between(step, STEPS);
     }
   }
   // O += V^T P^T, 32 keys at a time; the weights of the next 32 are worked out
@@ -1473,23 +1479,29 @@ struct Rows16 {
 #pragma unroll
     for (int h = 0; h < NJ / 2; h++) {
 #pragma unroll
-      for (int d = 0; d < DPL; d++) {
-        u32x2 x[2];
+      for (int d = 0; d < DPL; d += 2) {
+        u32x4 y[2];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const uint32_t r = 16 * (2 * h + j) + 4 * lg + ln / 4, cc = ln & 3;
-          const uint8_t* at = v + r * ROWB + (((2 * d + cc / 2) ^ swizzle<CHUNKS>(r)) * 16) + (cc & 1) * 8;
-          x[j] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
+        for (int e = 0; e < 2; e++) {
+          u32x2 x[2];
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const uint32_t r = 16 * (2 * h + j) + 4 * lg + ln / 4, cc = ln & 3;
+            const uint8_t* at = v + r * ROWB + (((2 * (d + e) + cc / 2) ^ swizzle<CHUNKS>(r)) * 16) + (cc & 1) * 8;
+            x[j] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
+          }
+          y[e] = (u32x4){x[0][0], x[0][1], x[1][0], x[1][1]};
         }
-        const u32x4 y = (u32x4){x[0][0], x[0][1], x[1][0], x[1][1]};
 #pragma unroll
         for (int t = 0; t < TERMS; t++)
 #pragma unroll
-          for (int c = 0; c < CT; c++) O[c][d] = MM::mfma(y, p[h & 1][c][t], O[c][d]);
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int c = 0; c < CT; c++) O[c][d + e] = MM::mfma(y[e], p[h & 1][c][t], O[c][d + e]);
         if (h + 1 < NJ / 2) {
 #pragma unroll
           for (int x = 0; x < CT * 4; x++)
-            if (x * DPL / (CT * 4) == d) pair(h + 1, x);
+            if (x * DPL / (CT * 4) / 2 * 2 == d) pair(h + 1, x);
         }
         // three parts: kept in this order, which the compiler's own spills (a chunk
         // of 2000 rows behind 6000 keys 573 us, 591 without; two parts 470 and 462)
@@ -1529,7 +1541,7 @@ struct Rows32 {
         b = __builtin_amdgcn_mfma_f32_16x16x4f32(x[3], q[3], b, 0, 0, 0);
       }
       S[0][j] = a + b;
-      between(j);
+      between(j, NJ);
     }
   }
   static __device__ __forceinline__ void add_pv(const uint8_t* v, uint32_t ln, uint32_t lg, f32x4 (&S)[CT][NJ],
@@ -1558,8 +1570,18 @@ struct Rows32 {
   }
 };
 
+// The kernel's arguments, read again: held over the key loops they take scalar
+// registers, and then lanes of vector registers, that the loops need (three-part
+// weights of 128 dims reload some in every stage, behind the DMA).
+__device__ __forceinline__ const AttArgs& again() {
+  typedef const AttArgs __attribute__((address_space(4))) Kernarg;
+  Kernarg* p = (Kernarg*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttArgs*)p;
+}
+
 template <class ROWS, int DPL>
-__device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
+__device__ __forceinline__ void attention_rows_body(const AttArgs& args) {
   typedef typename ROWS::TILE TILE;
   typedef typename ROWS::T T;
   constexpr int CT = ROWS::CT, KT = ROWS::KT, NJ = ROWS::NJ, QREG = TILE::QREG;
@@ -1569,12 +1591,13 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
   uint32_t* s_odd = (uint32_t*)(lds + 4 * REGION);                // [2 stages][2] a bit to a key
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t ln = lane & 15, lg = lane >> 4;
-  const uint32_t P = 1u << a.shift, hd = a.hd;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   Items<true> items;
-  find_items(a, s_odd + 4, items);
+  find_items(args, s_odd + 4, items);
 
-  for (Turn turn(items.total, true); turn.item < items.total; turn.next(a, items.total)) {
+  for (Turn turn(items.total, true); turn.item < items.total; turn.next(again(), items.total)) {
+    const AttArgs& a = again();
+    const uint32_t P = 1u << a.shift, hd = a.hd;
     const Item I(a, items, turn.item, CB, KT);
     const uint32_t k0 = I.k0, k1 = I.k1;
     // ---- this wave's share of a stage: KT / 4 rows of K and of V, 8 or 16, a page to 8 ----
@@ -1626,7 +1649,6 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
     u32x4 Q[CT][QREG];
     f32x4 O[CT][DPL];
     float m[CT], l[CT], c[CT];
-    uint32_t limit[CT];
 #pragma unroll
     for (int t = 0; t < CT; t++) {
       const uint32_t col = (w * CT + t) * 16 + ln;
@@ -1634,7 +1656,6 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
       TILE::split_q(raw[t], col < I.ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2, [](int) { return true; },
                     [&](int k, u32x4 x) { Q[t][k] = x; });
       c[t] = score_factor(a.scale, e2);
-      limit[t] = I.least + I.row_of(col);
       m[t] = -__builtin_inff();
       l[t] = 0.f;
 #pragma unroll
@@ -1685,17 +1706,18 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
       }
       f32x4 S[CT][NJ];
       float shift[CT];
-      ROWS::scores(k, hn, hg, Q, S, [&](int j) {
+      ROWS::scores(k, hn, hg, Q, S, [&](int step, int steps) {
 #pragma unroll
         for (uint32_t x = 0; x < PIECES; x++)
-          if ((int)(x * NJ / PIECES) == j) piece(x);
+          if ((int)(x * steps / PIECES) == step) piece(x);
       });
       ahead++;
 #pragma unroll
       for (int t = 0; t < CT; t++) {
         if (masked) {
           // the lane's first hidden key behind t0 + 4 lg
-          const int end = (int)((limit[t] < k1 ? limit[t] : k1) - t0 - 4 * hg);
+          const uint32_t limit = I.least + I.row_of((w * CT + t) * 16 + hn);
+          const int end = (int)((limit < k1 ? limit : k1) - t0 - 4 * hg);
           const uint64_t marks = ((uint64_t)(KT > 32 ? odd[1] : 0u) << 32 | odd[0]) >> (4 * hg);
 #pragma unroll
           for (int j = 0; j < NJ; j++)
@@ -1714,11 +1736,12 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
       }
       ROWS::add_pv(v, hn, hg, S, c, shift, l, O);
     }
-    if (bad) paged_err(a.err, PAGED_ERR_ATT_PAGE, I.b);
-    turn.take(a, items.total);
+    const AttArgs& z = again();
+    if (bad) paged_err(z.err, PAGED_ERR_ATT_PAGE, I.b);
+    turn.take(z, items.total);
 
     // ---- out, or a partial ----
-    float* mine = a.parts + (size_t)I.part * CB * (hd + 2);
+    float* mine = z.parts + (size_t)I.part * CB * (z.hd + 2);
 #pragma unroll
     for (int t = 0; t < CT; t++) {
       const uint32_t col = (w * CT + t) * 16 + ln;
@@ -1726,21 +1749,21 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& a) {
       if (col >= I.ncols) continue;
       if (I.ns == 1) {
         const float inv = I.keys ? 1.0f / l[t] : 0.f;
-        float* y = a.out + I.at(col, a.ld_out, hd) + 4 * lg;
+        float* y = z.out + I.at(col, z.ld_out, z.hd) + 4 * lg;
 #pragma unroll
         for (int d = 0; d < DPL; d++)
-          if (16 * d + 4 * lg < hd) store4(y + 16 * d, O[t][d] * inv);
+          if (16 * d + 4 * lg < z.hd) store4(y + 16 * d, O[t][d] * inv);
       } else {
 #pragma unroll
         for (int d = 0; d < DPL; d++)
-          if (16 * d + 4 * lg < hd) {
-            put2(mine + col * hd + 16 * d + 4 * lg, O[t][d][0], O[t][d][1]);
-            put2(mine + col * hd + 16 * d + 4 * lg + 2, O[t][d][2], O[t][d][3]);
+          if (16 * d + 4 * lg < z.hd) {
+            put2(mine + col * z.hd + 16 * d + 4 * lg, O[t][d][0], O[t][d][1]);
+            put2(mine + col * z.hd + 16 * d + 4 * lg + 2, O[t][d][2], O[t][d][3]);
           }
-        if (lg == 0) put2(mine + CB * hd + col * 2, m[t], l[t]);
+        if (lg == 0) put2(mine + CB * z.hd + col * 2, m[t], l[t]);
       }
     }
-    if (I.ns > 1) join_many(a, I, CB, (float*)lds, REGION);
+    if (I.ns > 1) join_many(z, I, CB, (float*)lds, REGION);
   }
 }
 
