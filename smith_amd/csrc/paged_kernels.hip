@@ -493,26 +493,30 @@ struct Tile16 {
   }
   template <class QF>
   __device__ __forceinline__ void scores(QF q, f32x4 (&S)[NJ]) const {
+    // products of one sum are four apart, which covers the first's latency
+    f32x4 sum[2][NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; j++) S[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NJ; j++) sum[0][j] = sum[1][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < KS; s++)
+    for (int i = 0; i < KS * TERMS; i++) {
+      const u32x4 x = q(i);
 #pragma unroll
-      for (int k = 0; k < TERMS; k++) {
-        const u32x4 x = q(s * TERMS + k);
+      for (int j = 0; j < NJ; j++) sum[i & 1][j] = MM::mfma(K[j][i / TERMS], x, sum[i & 1][j]);
+    }
 #pragma unroll
-        for (int j = 0; j < NJ; j++) S[j] = MM::mfma(K[j][s], x, S[j]);
-      }
+    for (int j = 0; j < NJ; j++) S[j] = sum[0][j] + sum[1][j];
   }
   __device__ __forceinline__ void add_pv(const f32x4 (&S)[NJ], f32x4 (&O)[DPL]) const {
     u32x4 t[TERMS];
 #pragma unroll
     for (int k = 0; k < 4; k++) MM::split2(S[k / 2][k % 2 * 2], S[k / 2][k % 2 * 2 + 1], t, k);
 #pragma unroll
-    for (int d = 0; d < DPL; d++) {
-      const u32x4 v = dim(d);
+    for (int d = 0; d < DPL; d += 2) {
+      const u32x4 v[2] = {dim(d), dim(d + 1)};
 #pragma unroll
-      for (int k = 0; k < TERMS; k++) O[d] = MM::mfma(v, t[k], O[d]);
+      for (int k = 0; k < TERMS; k++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) O[d + e] = MM::mfma(v[e], t[k], O[d + e]);
     }
   }
 };
@@ -1161,6 +1165,17 @@ __device__ __forceinline__ void weigh(f32x4 (&S)[NJ], float c, float& m, float& 
     for (int i = 0; i < 4; i++) S[j][i] = weight(S[j][i], c, shift, l);
 }
 
+// The kernel's arguments, read again: held over the key loops they take scalar
+// registers and then lanes of vector registers (16 columns of f16, 128 dims: 230
+// and 49 spilled scalars, so 202 and none; one row behind 1024 keys 10.3 and 9.7 us),
+// or reloads in every stage behind the DMA (three-part weights of 128 dims).
+__device__ __forceinline__ const AttArgs& again() {
+  typedef const AttArgs __attribute__((address_space(4))) Kernarg;
+  Kernarg* p = (Kernarg*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttArgs*)p;
+}
+
 // One tile of 16 columns to a workgroup.  Its four waves take the keys in turn, TK
 // at a time, straight from the pages into the operands' registers, the next
 // tile's while this one's are multiplied, and are joined through LDS at the end.
@@ -1171,7 +1186,7 @@ __device__ __forceinline__ void weigh(f32x4 (&S)[NJ], float c, float& m, float& 
 // workgroups by launch bounds) spill into scratch, whose loads wait for the
 // keys': 64 requests of 4000 keys 178 us with 2, 193 with 3, 269 with 4.
 template <class TILE, int DPL, bool SMALL>
-__device__ __forceinline__ void attention_body(const AttArgs& a) {
+__device__ __forceinline__ void attention_body(const AttArgs& args) {
   typedef typename TILE::T T;
   constexpr int NJ = TILE::NJ, QREG = TILE::QREG;
   constexpr uint32_t TK = 16 * NJ, HDP = 16 * DPL, CB = 16;
@@ -1184,11 +1199,12 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
   float* s_ml = s_o + OFLOATS;  // [4 waves][16 columns][m, l]
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t ln = lane & 15, lg = lane >> 4;
-  const uint32_t P = 1u << a.shift, hd = a.hd;
   Items<false> items;
-  find_items(a, (uint32_t*)(s_ml + 4 * 16 * 2), items);
+  find_items(args, (uint32_t*)(s_ml + 4 * 16 * 2), items);
 
-  for (Turn turn(items.total, false); turn.item < items.total; turn.next(a, items.total)) {
+  for (Turn turn(items.total, false); turn.item < items.total; turn.next(again(), items.total)) {
+    const AttArgs& a = again();
+    const uint32_t P = 1u << a.shift, hd = a.hd;
     const Item I(a, items, turn.item, CB, TK);
     const uint32_t k0 = I.k0, k1 = I.k1, kvh = I.kvh;
     f32x4 q_raw[TILE::QRAW];
@@ -1317,8 +1333,9 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
       tile.add_pv(S, O);
       if (more) load_v(t0 + 4 * TK);
     }
-    if (bad) paged_err(a.err, PAGED_ERR_ATT_PAGE, I.b);
-    turn.take(a, items.total);
+    const AttArgs& z = again();
+    if (bad) paged_err(z.err, PAGED_ERR_ATT_PAGE, I.b);
+    turn.take(z, items.total);
 
     // ---- join the waves ----
     l = add_xor32(add_xor16(l));
@@ -1347,23 +1364,23 @@ __device__ __forceinline__ void attention_body(const AttArgs& a) {
 #pragma unroll
       for (int d = 0; d < DPL; d++) o[d] = __builtin_fmaf(f, s_o[(k * 16 + col) * OS + at + d], o[d]);
     }
-    float* mine = a.parts + (size_t)I.part * CB * (hd + 2);
-    if (col < I.ncols && at < hd) {
-      const uint32_t d0 = first_dim<DPL>(tid & 15, hd);
+    float* mine = z.parts + (size_t)I.part * CB * (z.hd + 2);
+    if (col < I.ncols && at < z.hd) {
+      const uint32_t d0 = first_dim<DPL>(tid & 15, z.hd);
       if (I.ns == 1) {
         const float inv = I.keys ? 1.0f / sum : 0.f;
-        float* y = a.out + I.at(col, a.ld_out, hd) + d0;
+        float* y = z.out + I.at(col, z.ld_out, z.hd) + d0;
         Words<DPL> x;
 #pragma unroll
         for (int d = 0; d < DPL; d++) x.w[d] = __float_as_uint(o[d] * inv);
         *(Words<DPL>*)y = x;
       } else {
 #pragma unroll
-        for (int d = 0; d < DPL; d += 2) put2(mine + col * hd + d0 + d, o[d], o[d + 1]);
-        if (d0 == 0) put2(mine + CB * hd + col * 2, mx, sum);
+        for (int d = 0; d < DPL; d += 2) put2(mine + col * z.hd + d0 + d, o[d], o[d + 1]);
+        if (d0 == 0) put2(mine + CB * z.hd + col * 2, mx, sum);
       }
     }
-    if (I.ns > 1) join_16(a, I, s_o);
+    if (I.ns > 1) join_16(z, I, s_o);
   }
 }
 
@@ -1569,16 +1586,6 @@ struct Rows32 {
     return ok;
   }
 };
-
-// The kernel's arguments, read again: held over the key loops they take scalar
-// registers, and then lanes of vector registers, that the loops need (three-part
-// weights of 128 dims reload some in every stage, behind the DMA).
-__device__ __forceinline__ const AttArgs& again() {
-  typedef const AttArgs __attribute__((address_space(4))) Kernarg;
-  Kernarg* p = (Kernarg*)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(p));
-  return *(const AttArgs*)p;
-}
 
 template <class ROWS, int DPL>
 __device__ __forceinline__ void attention_rows_body(const AttArgs& args) {
