@@ -615,6 +615,94 @@ def test_attention_row_start_out_of_order_stays_inside(room):
     check_attention(run_attention(*case, ragged=True, room=room), *case, "f16")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("room", [0, room_for_many(4, 2, 2)])
+@pytest.mark.parametrize("junk", [np.nan, np.inf])
+def test_attention_of_a_query_that_is_not_finite(dtype, room, junk):
+    """It spoils its own row's head and nothing else."""
+    case = q, row_start, lens, tables, k, v = attention_case(19, dtype, 4, 2, 64, 16, [150, 40], [37, 3])
+    clean = run_attention(*case, ragged=True, room=room).reshape(q.shape)
+    q[5, 1, 7] = junk
+    got = run_attention(*case, ragged=True, room=room).reshape(q.shape)
+    assert not np.isfinite(got[5, 1]).any()
+    got[5, 1] = clean[5, 1]
+    assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_two_graphs_on_one_scratch(dtype):
+    """A captured step of prompts and one of single rows, replayed in turn."""
+    ctx, H, nKV, D = device.ops_ctx(), 8, 2, 32
+    steps = []
+    for lens, added, ragged in (([900, 300, 80], [900, 300, 80], True), ([3000, 700, 41], [1, 1, 1], False)):
+        case = q, row_start, ln, tables, k, v = attention_case(23, dtype, H, nKV, D, 16, lens, added)
+        rows = max(len(q), room_for_many(H, nKV, 3)) if ragged else len(q)
+        hq = np.zeros((rows, H * D), np.float32)
+        hq[:len(q)] = q.reshape(len(q), -1)
+        args = [R.upload(hq), i32(ln), i32(tables), R.upload(k), R.upload(v), i32(row_start) if ragged else None, 0.0,
+                S.create([rows, H * D])]
+        S.pagedAttention(*args)
+        device.sync()
+        steps.append([case, args, args[-1].data.copy(), None])
+        check_attention(steps[-1][2][:len(q)], *case, dtype)
+    try:
+        for st in steps:
+            device.check(device.lib.smith_graph_begin(ctx), "begin")
+            S.pagedAttention(*st[1])
+            st[3] = device.lib.smith_graph_end(ctx)
+            assert st[3], last_error()
+        for _ in range(4):
+            for case, args, want, g in steps:
+                args[-1].set_data(np.zeros(want.shape, np.float32))
+            for case, args, want, g in steps:
+                device.check(device.lib.smith_graph_launch(ctx, g))
+            for case, args, want, g in steps:
+                assert np.array_equal(args[-1].data[:len(case[0])], want[:len(case[0])])
+    finally:
+        for st in steps:
+            if st[3]:
+                device.lib.smith_graph_destroy(st[3])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_pages_beyond_32_bit_offsets(dtype):
+    """Pools of 5 GiB: rows appended into their last pages, and attention over
+    them by both kernels.  Only the pages of the requests are ever written."""
+    H, nKV, D, P = 8, 4, 64, 64
+    page = nKV * P * D
+    n_pages = (5 << 30) // (page * (4 if dtype == "f32" else 2))
+    lens, added = np.array([200, 65, 130], np.int32), np.array([200, 1, 70], np.int32)
+    case = attention_case(17, dtype, H, nKV, D, P, lens, added, spare=0)
+    q, row_start, _, tables, k, v = case
+    used = -(-lens // P)
+    for b in range(3):
+        tables[b, used[b]:] = -1
+    far = np.where(tables >= 0, n_pages - 1 - tables, tables)
+    pools = [S.create([n_pages, nKV, P, D], dtype) for _ in range(2)]
+    try:
+        size = page * k.itemsize
+        for t, host in zip(pools, (k, v)):
+            for i in range(len(host)):
+                device.upload(t.buffer + (n_pages - 1 - i) * size, np.ascontiguousarray(host[i]))
+        rs = np.random.RandomState(3)
+        # request 2's last row anew, through append
+        x = rs.standard_normal((1, (H + 2 * nKV) * D)).astype(np.float32)
+        slot = far[2, 129 // P].astype(np.int64) * P + 129 % P
+        assert slot * nKV * D * k.itemsize > 1 << 32
+        S.pagedAppend(R.upload(x), i32([slot]), i32([129]), H, *pools)
+        for host, part in ((k, x[0, H * D:(H + nKV) * D]), (v, x[0, (H + nKV) * D:])):
+            host[tables[2, 129 // P], :, 129 % P] = R.stored(part, dtype).reshape(nKV, D)
+        for room in (len(q), room_for_many(H, nKV, 3)):
+            hq = np.zeros((room, H * D), np.float32)
+            hq[:len(q)] = q.reshape(len(q), -1)
+            got = S.pagedAttention(R.upload(hq), i32(lens), i32(far), *pools, i32(row_start))
+            device.sync()
+            check_attention(got.data[:len(q)], q, row_start, lens, tables, k, v, dtype)
+    finally:
+        for t in pools:
+            t.release()
+
+
 # --------------------------------------------------------------------------
 # refusals (nothing is launched); addresses are places in one buffer of zeros
 # --------------------------------------------------------------------------
