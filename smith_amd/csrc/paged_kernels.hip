@@ -1181,8 +1181,8 @@ __device__ __forceinline__ const AttArgs& again() {
 // tile's while this one's are multiplied, and are joined through LDS at the end.
 // For one row a request: bound by memory.  32 heads on 8 of 128 dims: 120 requests
 // of 2800 to 4000 keys in bf16 (1.67 GB) 302 us, 5.5 TB/s; one of 131071 in f16 101
-// us, 5.3 TB/s (a large copy: 4.8); 32 of 1 to 6000 31.7 us, 4.0 TB/s.  One of 517
-// f32 keys, 16 heads of 64: 9.3 us, latency.  More waves to a CU (3 and 4
+// us, 5.3 TB/s (a large copy: 4.8); 32 of 1 to 6000 31.1 us, 4.1 TB/s.  One of 517
+// f32 keys, 16 heads of 64: 8.9 us, latency.  More waves to a CU (3 and 4
 // workgroups by launch bounds) spill into scratch, whose loads wait for the
 // keys': 64 requests of 4000 keys 178 us with 2, 193 with 3, 269 with 4.
 template <class TILE, int DPL, bool SMALL>
@@ -1396,10 +1396,10 @@ __device__ __forceinline__ void attention_body(const AttArgs& args) {
 // 4c .. 4c+3 of the k-th of four keys and receiving one dim of all four.
 // Bound by the matrix cores: 2000 rows behind 6000 keys, 32 heads on 8 of 128 dims,
 // 229 GFLOP: f16 450 us, 1020 TFLOP/s of split products (a large library product:
-// 1097), bf16 542 us, 1270 (1136), f32 1.99 ms, 115 (152).  A wave's stage is a chain
-// of 6000 cycles for 2048 of products (f16), so the next stage's loads and the next
-// weights go out between products, and shorter prompts wait for their longest
-// blocks: four of 430 to 611 rows 42.6 us in f16, half of that rate.
+// 1097), bf16 512 to 560 us, 1230 to 1340 (1136), f32 1.98 ms, 116 (152).  A wave's
+// stage is a chain of 6000 cycles for 2048 of products (f16), so the next stage's
+// loads and the next weights go out between products, and shorter prompts wait for
+// their longest blocks: four of 430 to 611 rows 42 us in f16, half of that rate.
 // ---------------------------------------------------------------------------
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
