@@ -202,6 +202,13 @@ class PagedCache:
         self._count[a].set_data(np.array([self.freeCount], np.int32))
         self._lens[a].set_data(self.lens)
 
+    def free(self):
+        """Gives the device memory back; the cache is not used after it."""
+        tensors = [t for layer in self.layers for t in layer.values()] + self._lens + self._count
+        for t in tensors + [self._tables, self._free, self._added, self._row_start] + list((self._rows or {}).values()):
+            t.release()
+        self.layers, self._rows = [], None
+
 
 def createPagedCache(config, requests, pages, pageSize=16, dtype="f16"):
     """A PagedCache for a model of this config (GGUFModel.config's fields of

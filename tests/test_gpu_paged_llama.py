@@ -3,7 +3,7 @@ request: several requests in one step, of any lengths, on a shared pool."""
 import numpy as np
 import pytest
 
-from smith_amd import createPagedCache
+from smith_amd import createPagedCache, device
 from smith_amd.gguf_loader import loadGGUF
 from llama_fixtures import write_tiny_llama
 
@@ -135,6 +135,22 @@ def test_refusals(model):
         model.createPagedCache(2, 10, 12)
     with pytest.raises(ValueError, match="0 requests"):
         model.createPagedCache(0, 10)
+
+
+def test_a_cache_gives_its_memory_back(model):
+    before = device.allocated_size()
+    cache = model.createPagedCache(2, 64, 16, "f16")
+    model.forwardPagedStep([[1, 2], [3]], cache)
+    grown = device.allocated_size()  # with what the model keeps for such steps
+    cache.free()
+    model_keeps = device.allocated_size() - before
+    again = model.createPagedCache(2, 64, 16, "f16")
+    model.forwardPagedStep([[1, 2], [3]], again)
+    assert device.allocated_size() - before - model_keeps == grown - before - model_keeps > 0
+    again.free()
+    assert device.allocated_size() - before == model_keeps
+    with pytest.raises(ValueError, match="a cache of 0 layers"):
+        model.forwardPagedStep([[1], [2]], cache)
 
 
 def test_many_rows_in_one_step(model):
