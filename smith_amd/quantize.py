@@ -29,8 +29,15 @@ class QuantizedWeight(dict):
             raise AttributeError(k)
 
 
-def _as_device_weight(weight):
+def _want_f32(t, what):
+    # the kernels read and write 4 bytes an element, whatever a tensor is of
+    if t.dtype != "f32":
+        raise ValueError("%s: f32 wanted, got %s" % (what, t.dtype))
+
+
+def _as_device_weight(weight, what):
     if isinstance(weight, T.Tensor):
+        _want_f32(weight, what)
         return weight, None
     w = np.ascontiguousarray(weight, dtype=np.float32)
     if w.ndim != 2:
@@ -40,7 +47,7 @@ def _as_device_weight(weight):
 
 
 def _quantize(weight, block_bytes, entry, what):
-    w, tmp = _as_device_weight(weight)
+    w, tmp = _as_device_weight(weight, what)
     K, N = w.shape
     groups = -(-K // GROUP_SIZE)
     total = groups * N * block_bytes
@@ -64,11 +71,12 @@ def quantizeQ8(weight):
 
 
 def _matmul(a, bq, entry, what):
+    _want_f32(a, what)
     M = a.shape[0]
     N, K, groups = bq["N"], bq["K"], bq["groups"]
     if a.shape[1] != K:
         raise ValueError("%s: inner dims don't match: %d vs %d" % (what, a.shape[1], K))
-    out = T.create([M, N], a.dtype)
+    out = T.create([M, N])
     device.check(entry(device.ops_ctx(), a.buffer, bq["buffer"], out.buffer, M, N, K, groups), what)
     return out
 
@@ -90,12 +98,13 @@ def matmul_reference_dispatch(kernel, a, bQuant):
     through the generic encoder API of the bridge."""
     import struct
     from .dispatch import run
+    what = "matmulQ4" if kernel == "matmul_q4" else "matmulQ8"
+    _want_f32(a, what)
     M = a.shape[0]
     N, K, groups = bQuant["N"], bQuant["K"], bQuant["groups"]
     if a.shape[1] != K:
-        raise ValueError("%s: inner dims don't match: %d vs %d"
-                         % ("matmulQ4" if kernel == "matmul_q4" else "matmulQ8", a.shape[1], K))
-    out = T.create([M, N], a.dtype)
+        raise ValueError("%s: inner dims don't match: %d vs %d" % (what, a.shape[1], K))
+    out = T.create([M, N])
     run(kernel, [{"buffer": a.buffer, "index": 0}, {"buffer": bQuant["buffer"], "index": 1},
                  {"buffer": out.buffer, "index": 2}],
         {"x": N, "y": M}, {"x": min(N, 16), "y": min(M, 16)},
