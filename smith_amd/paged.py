@@ -64,8 +64,8 @@ def pagedAppend(qkv, slots, positions, numHeads, kPages, vPages, rope=ROPE_NONE,
     _want(qkv, [rows, (numHeads + 2 * nKV) * hd], "f32", "pagedAppend: qkv")
     _want(slots, [rows], "i32", "pagedAppend: slots")
     _want(positions, [rows], "i32", "pagedAppend: positions")
-    if rope and (cos is None or sin is None or cos.size != sin.size):
-        raise ValueError("pagedAppend: rotary positions need tables cos and sin of one size")
+    if rope and (cos is None or sin is None or cos.size != sin.size or (cos.dtype, sin.dtype) != ("f32", "f32")):
+        raise ValueError("pagedAppend: rotary positions need tables cos and sin, f32 of one size")
     q = T.create([rows, numHeads * hd])
     device.check(device.lib.smith_paged_append(
         device.ops_ctx(), KV_TYPES[kPages.dtype], qkv.buffer, ld, rows, slots.buffer, positions.buffer, numHeads, nKV,

@@ -28,3 +28,11 @@ def test_f32_is_asked_for(no_device, what, dtype):
             getattr(S, what)(a, wq)
         else:
             getattr(S, what)(a)
+
+
+@pytest.mark.parametrize("cos,sin", [("f16", "f16"), ("f32", "bf16"), ("u8", "f32"), ("f32", "i32")])
+def test_rotary_tables_are_f32(no_device, cos, sin):
+    pool = S.Tensor([8, 2, 16, 32], "f16", buffer=1)
+    with pytest.raises(ValueError, match="cos and sin, f32 of one size"):
+        S.pagedAppend(S.Tensor([5, 256], buffer=1), S.Tensor([5], "i32", buffer=1), S.Tensor([5], "i32", buffer=1), 4, pool,
+                      pool, S.ROPE_HEAD, S.Tensor([800], cos, buffer=1), S.Tensor([800], sin, buffer=1))
