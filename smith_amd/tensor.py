@@ -21,7 +21,7 @@ def _host(values, dtype):
         u = np.ascontiguousarray(a, dtype=np.float32).view(np.uint32)
         return np.where((u & 0x7FFFFFFF) > 0x7F800000, u >> 16 | 0x40,
                         (u + (0x7FFF + (u >> 16 & 1))) >> 16).astype(np.uint16).reshape(a.shape)
-    return np.ascontiguousarray(a, dtype=_DTYPES[dtype])
+    return np.asarray(a, dtype=_DTYPES[dtype], order="C")  # a scalar stays one
 
 
 class Tensor:

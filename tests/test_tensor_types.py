@@ -1,5 +1,6 @@
 """Tensors of other types than f32 without a GPU: what takes f32 refuses them
 before it allocates or launches anything."""
+import numpy as np
 import pytest
 
 import smith_amd as S
@@ -36,3 +37,22 @@ def test_rotary_tables_are_f32(no_device, cos, sin):
     with pytest.raises(ValueError, match="cos and sin, f32 of one size"):
         S.pagedAppend(S.Tensor([5, 256], buffer=1), S.Tensor([5], "i32", buffer=1), S.Tensor([5], "i32", buffer=1), 4, pool,
                       pool, S.ROPE_HEAD, S.Tensor([800], cos, buffer=1), S.Tensor([800], sin, buffer=1))
+
+
+@pytest.fixture
+def host_memory(monkeypatch):
+    """Tensors in host memory: what is uploaded is kept and downloaded."""
+    held = {}
+    monkeypatch.setattr(device, "alloc", lambda nbytes, mode=0: held.setdefault(len(held) + 1, None) or len(held))
+    monkeypatch.setattr(device, "upload", lambda buf, a, offset=0: held.__setitem__(buf, a.tobytes()))
+    monkeypatch.setattr(device, "download", lambda buf, nbytes, dtype, offset=0: np.frombuffer(held[buf][:nbytes], dtype))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16", "i32", "u8"])
+def test_scalars_have_no_dimension(host_memory, dtype):
+    one = 0x3F80 if dtype == "bf16" else 1
+    for t, want in ((S.tensor(1.0, dtype=dtype), one), (S.zeros([], dtype), 0), (S.ones([], dtype), one),
+                    (S.tensor(1.0, dtype=dtype).set_data(0.0), 0)):
+        assert t.shape == [] and t.data.shape == () and S.toArray(t) == want
+    assert S.tensor([[2.0, 4.0]], dtype=dtype).shape == [1, 2]
+    assert S.toArray(S.tensor(np.arange(6.0).reshape(2, 3).T, dtype="f32")) == [[0, 3], [1, 4], [2, 5]]
