@@ -10,7 +10,8 @@ import numpy as np
 
 from . import device, prng
 
-# bf16: the upper halves of f32 words on the host; floats are rounded to them
+# bf16: the upper halves of f32 words on the host, a uint16 array; numbers of any
+# other type are rounded to them
 _DTYPES = {"f32": np.float32, "i32": np.int32, "u8": np.uint8, "f16": np.float16, "bf16": np.uint16}
 
 
@@ -22,6 +23,15 @@ def _host(values, dtype):
         return np.where((u & 0x7FFFFFFF) > 0x7F800000, u >> 16 | 0x40,
                         (u + (0x7FFF + (u >> 16 & 1))) >> 16).astype(np.uint16).reshape(a.shape)
     return np.asarray(a, dtype=_DTYPES[dtype], order="C")  # a scalar stays one
+
+
+def _values(values, dtype):
+    """The same of a user's values: whole numbers are numbers, and a bf16 tensor's
+    bits only as uint16, which is what .data gives."""
+    a = np.asarray(values)
+    if dtype == "bf16" and a.dtype != np.uint16:
+        a = a.astype(np.float32)
+    return _host(a, dtype)
 
 
 class Tensor:
@@ -50,7 +60,7 @@ class Tensor:
         return device.download(self.buffer, self.nbytes, _DTYPES[self.dtype]).reshape(self.shape)
 
     def set_data(self, arr):
-        a = _host(arr, self.dtype)
+        a = _values(arr, self.dtype)
         if a.size != self.size:
             raise ValueError("set_data: %d elements for a tensor of %d" % (a.size, self.size))
         device.upload(self.buffer, a)
@@ -70,7 +80,7 @@ def create(shape, dtype="f32"):
 
 
 def tensor(data, shape=None, dtype="f32"):
-    a = _host(data, dtype)
+    a = _values(data, dtype)
     t = Tensor(list(a.shape) if shape is None else shape, dtype)
     return t.set_data(a)
 

@@ -56,3 +56,18 @@ def test_scalars_have_no_dimension(host_memory, dtype):
         assert t.shape == [] and t.data.shape == () and S.toArray(t) == want
     assert S.tensor([[2.0, 4.0]], dtype=dtype).shape == [1, 2]
     assert S.toArray(S.tensor(np.arange(6.0).reshape(2, 3).T, dtype="f32")) == [[0, 3], [1, 4], [2, 5]]
+
+
+def test_whole_numbers_in_bf16(host_memory):
+    """Numbers are rounded whatever type they come in; an array of uint16, as
+    .data gives it, is a bf16 tensor's own bits."""
+    want = [0x3F80, 0xC000, 0x4380, 0x4380, 0x4382, 0]  # 1, -2, 256, 257 (a tie, to even), 259 (a tie), 0
+    numbers = [1, -2, 256, 257, 259, 0]
+    for values in (numbers, np.array(numbers, np.int32), np.array(numbers, np.float32), [float(x) for x in numbers]):
+        assert S.tensor(values, dtype="bf16").data.tolist() == want
+        assert S.create([6], "bf16").set_data(values).data.tolist() == want
+    assert S.tensor(np.array([True, False]), dtype="bf16").data.tolist() == [0x3F80, 0]
+    t = S.tensor(numbers, dtype="bf16")
+    assert t.data.dtype == np.uint16
+    assert S.tensor(t.data, dtype="bf16").data.tolist() == want
+    assert S.create([6], "bf16").set_data(t.data).data.tolist() == want
