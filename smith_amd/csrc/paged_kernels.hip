@@ -321,10 +321,14 @@ DEF_APPEND(smith_paged_append_bf16, KvBf16)
 //
 // f16 and bf16 pages are exact in the matrix cores' operands; q and P are split
 // into parts of the pages' type that add up to 22 (two f16) or 24 (three bf16)
-// bits, the products are exact and summed in f32.  q is brought to [2^14, 2^15)
-// by a power of two first and P to at most 2^14 (P_EXP + the slack of the lazy
-// maximum), so that the small parts stay clear of f16's subnormals.  f32 pages
-// go through the f32 matrix cores.
+// bits, the products are exact and summed in f32.  q is brought to [2^13.5, 2^15.5)
+// by a power of two first and P to at most 2^P_TOP, so that the small parts stay
+// clear of f16's subnormals.  f32 pages go through the f32 matrix cores.
+//
+// scale log2 e is a factor of q but for a power of two c, by which the sums are
+// multiplied.  So a score in powers of two is exact from its sum, its difference
+// from m is rounded once and is 0 for the largest, however far up the scores are: a
+// weight never leaves its range.
 //
 // Work is cut on the device, where the lengths are: an item is (request, block
 // of columns, KV head, split of the block's keys).  With W = sum over blocks of
@@ -356,8 +360,13 @@ __device__ __forceinline__ float max_xor16_32(float v) {
   const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
-#define P_EXP 6.0f   // P = 2^(score - m + P_EXP)
-#define M_SLACK 8.0f // m follows a new maximum only when it is this far (log2) above
+// Weights are P = 2^(score - m).  m is P_EXP under a column's maximum, and follows a
+// new one only when that would have a weight above 2^P_TOP.
+#define P_EXP 6.0f
+#define P_TOP 14.0f
+// Scores this far up are multiples of 2^-7: m is the maximum itself, which P_EXP
+// below it would be rounded to something else.
+#define FAR_SCORE 65536.0f
 
 // the parts of eight f32 values in the pages' type, and the product of parts
 struct MmF16 {
@@ -428,11 +437,11 @@ struct Tile16 {
       x[2 * s + 1] = load4(at + 4);
     }
   }
-  // ... in parts, times +-1 and a power of two that brings its largest element
-  // to [2^14, 2^15); what is not finite stays as it is.  Register k of the steps
-  // that do(s) says goes to put(k, parts).
+  // ... in parts, times `factor` (at least 0.36, less than 0.73, of either sign) and a
+  // power of two that brings its largest element to [2^15, 2^16) before; what is not
+  // finite stays as it is.  Register k of the steps that do(s) says goes to put(k, parts).
   template <class DO, class PUT>
-  static __device__ __forceinline__ void split_q(const f32x4 (&x)[QRAW], bool there, uint32_t g, uint32_t hd, float sign,
+  static __device__ __forceinline__ void split_q(const f32x4 (&x)[QRAW], bool there, uint32_t g, uint32_t hd, float factor,
                                                  int& e2, DO todo, PUT put) {
     float big = 0.f;
 #pragma unroll
@@ -440,14 +449,14 @@ struct Tile16 {
 #pragma unroll
       for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[2 * s + e / 4][e % 4]));  // a repeated element is one of the row's
     big = max_xor16_32(big);
-    e2 = there && big > 0.f && big < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(big) : 0;
+    e2 = there && big > 0.f && big < __builtin_inff() ? 16 - __builtin_amdgcn_frexp_expf(big) : 0;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
       if (!todo(s)) continue;
       float y[8];
       const bool in = there && s * 32 + 8 * g < hd;
 #pragma unroll
-      for (int e = 0; e < 8; e++) y[e] = in ? __builtin_amdgcn_ldexpf(x[2 * s + e / 4][e % 4] * sign, e2) : 0.f;
+      for (int e = 0; e < 8; e++) y[e] = in ? __builtin_amdgcn_ldexpf(x[2 * s + e / 4][e % 4], e2) * factor : 0.f;
       u32x4 t[TERMS];
 #pragma unroll
       for (int k = 0; k < 4; k++) MM::split2(y[2 * k], y[2 * k + 1], t, k);
@@ -537,13 +546,13 @@ struct Tile32 {
     }
   }
   template <class DO, class PUT>
-  static __device__ __forceinline__ void split_q(const f32x4 (&x)[QRAW], bool there, uint32_t g, uint32_t hd, float sign,
+  static __device__ __forceinline__ void split_q(const f32x4 (&x)[QRAW], bool there, uint32_t g, uint32_t hd, float factor,
                                                  int& e2, DO todo, PUT put) {
     e2 = 0;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
       if (!todo(s)) continue;
-      f32x4 y = x[s] * sign;
+      f32x4 y = x[s] * factor;
       if (!there || s * 16 + 4 * g >= hd) y = (f32x4){0.f, 0.f, 0.f, 0.f};
       put(s, __builtin_bit_cast(u32x4, y));
     }
@@ -608,7 +617,8 @@ struct AttArgs {
   uint32_t rows_blk, heads_blk, groups;  // rows to a block of columns, heads of each, blocks to a row's heads
   float per_target;                     // KV heads / items wanted
   float split_min;                      // least C
-  float scale;
+  float q_factor;                       // scale log2 e = q_factor 2^c_exp, 0.36 < |q_factor| < 0.73
+  int32_t c_exp;
 };
 
 // a / b of a < 2^20 by a reciprocal: (a + 1/2) / b is 1 / 2b away from the next
@@ -1125,14 +1135,15 @@ __device__ __forceinline__ void join_many(const AttArgs& a, const Item& I, uint3
 
 #define MERGE_PAD 4  // floats between the columns of a wave's O in LDS
 
-// |scale| log2 e without the power of two that q was multiplied by, never 0
-__device__ __forceinline__ float score_factor(float scale, int e2) {
-  return fmaxf(__builtin_amdgcn_ldexpf(fabsf(scale) * 1.44269504088896340736f, -e2), 1.17549435e-38f);
+// 2^e, never 0 or infinite
+__device__ __forceinline__ float score_factor(int e) {
+  e = e < -126 ? -126 : e > 127 ? 127 : e;
+  return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// Scores of one column (times c: in powers of two) become weights 2^(score - m +
-// P_EXP): follow() moves the column's running maximum m, with its sum l (this
-// lane's share) and O, and says what is added to a score; weight() is one of them.
+// Scores of one column (times c: in powers of two) become weights 2^(score - m):
+// follow() moves the column's m, with its sum l (this lane's share) and O, and says
+// what is added to a score; weight() is one of them.
 template <int NJ, int DPL>
 __device__ __forceinline__ float follow(const f32x4 (&S)[NJ], float c, float& m, float& l, f32x4 (&O)[DPL]) {
   float x = -__builtin_inff();
@@ -1141,15 +1152,15 @@ __device__ __forceinline__ float follow(const f32x4 (&S)[NJ], float c, float& m,
 #pragma unroll
     for (int i = 0; i < 4; i++) x = fmaxf(x, S[j][i]);
   x = max_xor16_32(x) * c;
-  if (__any(x > m + M_SLACK)) {
-    const float mn = fmaxf(x, m);
+  if (__any(x - m > P_TOP)) {
+    const float mn = fmaxf(x - (fabsf(x) > FAR_SCORE ? 0.f : P_EXP), m);
     const float f = mn == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
     m = mn;
     l *= f;
 #pragma unroll
     for (int d = 0; d < DPL; d++) O[d] *= f;
   }
-  return m == -__builtin_inff() ? 0.f : P_EXP - m;
+  return m == -__builtin_inff() ? 0.f : -m;
 }
 __device__ __forceinline__ float weight(float s, float c, float shift, float& l) {
   const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, shift));
@@ -1272,9 +1283,9 @@ __device__ __forceinline__ void attention_body(const AttArgs& args) {
     {
       // each wave splits the steps of its own number
       int e2;
-      TILE::split_q(q_raw, ln < I.ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2,
+      TILE::split_q(q_raw, ln < I.ncols, lg, hd, a.q_factor, e2,
                     [&](int s) { return (s & 3) == (int)w; }, [&](int k, u32x4 x) { s_q[k * 64 + lane] = x; });
-      c = score_factor(a.scale, e2);
+      c = score_factor(a.c_exp - e2);
     }
     __syncthreads();
     const uint32_t limit = I.least + I.row_of(ln);
@@ -1660,9 +1671,9 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& args) {
     for (int t = 0; t < CT; t++) {
       const uint32_t col = (w * CT + t) * 16 + ln;
       int e2;
-      TILE::split_q(raw[t], col < I.ncols, lg, hd, a.scale < 0.f ? -1.f : 1.f, e2, [](int) { return true; },
+      TILE::split_q(raw[t], col < I.ncols, lg, hd, a.q_factor, e2, [](int) { return true; },
                     [&](int k, u32x4 x) { Q[t][k] = x; });
-      c[t] = score_factor(a.scale, e2);
+      c[t] = score_factor(a.c_exp - e2);
       m[t] = -__builtin_inff();
       l[t] = 0.f;
 #pragma unroll

@@ -2495,6 +2495,9 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   // of attention_body: O and (m, l) of four waves; of attention_rows_body: two
   // stages of K and V rows (64 of f16 / bf16 or 32 of f32: 256 bytes a head dim) and their marks
   const uint32_t lds = (many ? 256 * 2 * (dims <= 64 ? 64 : 128) + 16 : 4 * 16 * (dims + 4) * 4 + 4 * 16 * 2 * 4) + 16 + 20 * (n_req + 1);
+  int c_exp;
+  const float q_factor = (float)(frexp((double)scale, &c_exp) * (0.5 * 1.4426950408889634));
+  c_exp++;
   struct {
     const float* q;
     const int32_t *row_start, *lens, *tables;
@@ -2503,11 +2506,12 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
     uint32_t *counters, *queue;
     uint64_t* err;
     uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift, rows_blk, heads_blk, groups;
-    float per_target, split_min, scale;
+    float per_target, split_min, q_factor;
+    int32_t c_exp;
   } a = {q, row_start, lens, tables, kpages, vpages, out, (float*)c->paged_ws, c->paged_cnt, c->paged_cnt + PAGED_COUNTERS,
          c->paged_err_dev(),
          ld_q, ld_out, max_rows, n_req, max_pages, n_kv_heads, G, head_dim, n_pages, shift, RB, heads_blk, groups,
-         (float)n_kv_heads / (float)target, split_min, scale};
+         (float)n_kv_heads / (float)target, split_min, q_factor, c_exp};
   char name[64];
   snprintf(name, sizeof name, "smith_paged_attention_%s%s_d%u%s", many ? "rows_" : "", kv_name(kv_type), dims, small ? "_s" : "");
   void* args[] = {&a};
