@@ -433,9 +433,10 @@ int smith_paged_append(void* ctx, uint32_t kv_type, const float* qkv, uint32_t l
  * and its output is 0.  Head h reads KV head h / (n_heads / n_kv_heads); scale 0
  * is 1 / sqrt(head_dim).  q and out are f32 with row strides ld_q and ld_out and
  * room for max_rows rows; out overlaps no input.  Rows of out behind the last row
- * stay as they are.  f32 accuracy for every kv_type.  Keys that a row does not
- * see may hold anything; among those that it sees an entry that is not finite
- * makes that row's head not finite.  head_dim <= 128 and % 8 == 0.  A row_start
+ * stay as they are.  f32 accuracy; with f16 pages an element of q and a weight are
+ * held to 2^-22 of themselves, and to no less than 2^-38 of the largest of their
+ * head's.  Keys that a row does not see may hold anything; among those that it
+ * sees an entry that is not finite makes that row's head not finite.  head_dim <= 128 and % 8 == 0.  A row_start
  * past max_rows fails the call; starts that do not ascend, and a len below the
  * request's rows or past max_pages pages, fail the request (nothing of it is
  * written); a page outside the pool leaves its

@@ -322,8 +322,8 @@ DEF_APPEND(smith_paged_append_bf16, KvBf16)
 // f16 and bf16 pages are exact in the matrix cores' operands; q and P are split
 // into parts of the pages' type that add up to 22 (two f16) or 24 (three bf16)
 // bits, the products are exact and summed in f32.  q is brought to [2^13.5, 2^15.5)
-// by a power of two first and P to at most 2^P_TOP, so that the small parts stay
-// clear of f16's subnormals.  f32 pages go through the f32 matrix cores.
+// by a power of two first and P far up in f16 too, since small parts round at f16's
+// least step: 2^-38 of the largest.  f32 pages go through the f32 matrix cores.
 //
 // scale log2 e is a factor of q but for a power of two c, by which the sums are
 // multiplied.  So a score in powers of two is exact from its sum, its difference
@@ -360,19 +360,23 @@ __device__ __forceinline__ float max_xor16_32(float v) {
   const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
-// Weights are P = 2^(score - m).  m is P_EXP under a column's maximum, and follows a
-// new one only when that would have a weight above 2^P_TOP.
-#define P_EXP 6.0f
-#define P_TOP 14.0f
-// Scores this far up are multiples of 2^-7: m is the maximum itself, which P_EXP
-// below it would be rounded to something else.
-#define FAR_SCORE 65536.0f
+// Weights are P = 2^(score - m).  m is P_EXP (of the page type) under a column's
+// maximum, and follows a new one only when that would have a weight above 2^P_TOP.
+// From here on f32 holds every second whole number and less: m is the maximum
+// itself, which P_EXP below it would be rounded to something else.
+#define FAR_SCORE 16777216.0f
 
 // the parts of eight f32 values in the pages' type, and the product of parts
 struct MmF16 {
   typedef _Float16 T;
   static constexpr int TERMS = 2;
   static constexpr uint32_t EXPONENT = 0x7C00u;
+  // The largest weight is 2^13 to 2^15.9 of f16's 2^16: its second part rounds at
+  // 2^-25, half of f16's least step, so beside 2^-22 of itself a weight loses up to
+  // 2^-38 of the largest.  (2^6 to 2^14 would lose 2^-31, and be 1 % faster for rows: m
+  // moves less often.  A prompt of 2000 rows, 32 heads on 8 of 128, 83.0 and 83.8 us;
+  // 600 rows 31.1 and 31.7.)
+  static constexpr float P_EXP = 13.0f, P_TOP = 15.9f;
   // word k of the parts, from values 2k and 2k + 1
   static __device__ __forceinline__ void split2(float x, float y, u32x4 (&t)[TERMS], int k) {
     // the rest in one mixed-precision operation each (without a factor that the
@@ -392,6 +396,7 @@ struct MmBf16 {
   typedef __bf16 T;
   static constexpr int TERMS = 3;
   static constexpr uint32_t EXPONENT = 0x7F80u;
+  static constexpr float P_EXP = 6.0f, P_TOP = 14.0f;
   static __device__ __forceinline__ void split2(float x, float y, u32x4 (&t)[TERMS], int k) {
     f32x2 r = (f32x2){x, y};
 #pragma unroll
@@ -424,6 +429,7 @@ template <class MM, int DPL>
 struct Tile16 {
   typedef typename MM::T T;
   static constexpr int NJ = 2, KS = DPL / 2, TERMS = MM::TERMS, QREG = KS * TERMS;
+  static constexpr float P_EXP = MM::P_EXP, P_TOP = MM::P_TOP;
   u32x4 K[NJ][KS];
   uint32_t V[8][DPL / 2];  // a key's dims of this lane
   // the lane's column of q: dims s*32 + 8g .. +7 (past the head others, then 0)
@@ -535,6 +541,7 @@ template <int DPL>
 struct Tile32 {
   typedef float T;
   static constexpr int NJ = 1, KS = DPL, QREG = KS;
+  static constexpr float P_EXP = 6.0f, P_TOP = 14.0f;
   f32x4 K[KS];  // dims s*16 + 4g .. +3
   float V[4][DPL];
   static constexpr int QRAW = KS;
@@ -1144,7 +1151,7 @@ __device__ __forceinline__ float score_factor(int e) {
 // Scores of one column (times c: in powers of two) become weights 2^(score - m):
 // follow() moves the column's m, with its sum l (this lane's share) and O, and says
 // what is added to a score; weight() is one of them.
-template <int NJ, int DPL>
+template <class TILE, int NJ, int DPL>
 __device__ __forceinline__ float follow(const f32x4 (&S)[NJ], float c, float& m, float& l, f32x4 (&O)[DPL]) {
   float x = -__builtin_inff();
 #pragma unroll
@@ -1152,8 +1159,8 @@ __device__ __forceinline__ float follow(const f32x4 (&S)[NJ], float c, float& m,
 #pragma unroll
     for (int i = 0; i < 4; i++) x = fmaxf(x, S[j][i]);
   x = max_xor16_32(x) * c;
-  if (__any(x - m > P_TOP)) {
-    const float mn = fmaxf(x - (fabsf(x) > FAR_SCORE ? 0.f : P_EXP), m);
+  if (__any(x - m > TILE::P_TOP)) {
+    const float mn = fmaxf(x - (fabsf(x) > FAR_SCORE ? 0.f : TILE::P_EXP), m);
     const float f = mn == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn);
     m = mn;
     l *= f;
@@ -1167,9 +1174,9 @@ __device__ __forceinline__ float weight(float s, float c, float shift, float& l)
   l += p;
   return p;
 }
-template <int NJ, int DPL>
+template <class TILE, int NJ, int DPL>
 __device__ __forceinline__ void weigh(f32x4 (&S)[NJ], float c, float& m, float& l, f32x4 (&O)[DPL]) {
-  const float shift = follow<NJ, DPL>(S, c, m, l, O);
+  const float shift = follow<TILE, NJ, DPL>(S, c, m, l, O);
 #pragma unroll
   for (int j = 0; j < NJ; j++)
 #pragma unroll
@@ -1315,7 +1322,7 @@ __device__ __forceinline__ void attention_body(const AttArgs& args) {
           for (int i = 0; i < 4; i++)
             if (16 * j + i >= end) S[j][i] = -__builtin_inff();
       }
-      weigh<NJ, DPL>(S, c, m, l, O);
+      weigh<TILE, NJ, DPL>(S, c, m, l, O);
       if (masked) {
         // a weight of 0 does not hide a value that is not finite: values behind
         // the block's keys go to 0, and so do keys with such a value that only
@@ -1750,7 +1757,7 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& args) {
                 if (16 * j + i < end && (marks >> (16 * j + i) & 1)) l[t] = __builtin_nanf("");
           }
         }
-        shift[t] = follow<NJ, DPL>(S[t], c[t], m[t], l[t], O[t]);
+        shift[t] = follow<TILE, NJ, DPL>(S[t], c[t], m[t], l[t], O[t]);
       }
       ROWS::add_pv(v, hn, hg, S, c, shift, l, O);
     }

@@ -8,6 +8,27 @@ from test_gpu_paged import attention_case, check_attention, room_for_many, run_a
 
 pytestmark = pytest.mark.gpu
 
+
+def weights(q, row_start, lens, tables, k, v, dtype, scale=None):
+    """(sum of the weights relative to the largest, sum of |v| of the keys that are
+    seen, sum of weight times |v|), [rows, heads(, dim)] in f64."""
+    H, D = q.shape[1:]
+    G = H // k.shape[1]
+    scale = D ** -0.5 if not scale else scale
+    kf, vf = R.value(k, dtype), R.value(v, dtype)
+    sw, sv, swv = np.zeros(q.shape[:2]), np.zeros(q.shape), np.zeros(q.shape)
+    for b, n in enumerate(lens):
+        r0, r1 = row_start[b], row_start[b + 1]
+        kk, vv = R.gathered(kf, tables[b], n), np.abs(R.gathered(vf, tables[b], n))
+        for r in range(r0, r1):
+            t = n - (r1 - r0) + (r - r0) + 1
+            for h in range(H):
+                s = scale * (kk[h // G, :t] @ q[r, h].astype(np.float64))
+                w = np.exp(s - s.max())
+                sw[r, h], sv[r, h], swv[r, h] = w.sum(), vv[h // G, :t].sum(0), w @ vv[h // G, :t]
+    return sw, sv, swv
+
+
 # (columns of one kernel or of the other, rows of a request or one, pages of less than 16 keys)
 FORMS = [(False, 0, 16), (True, 0, 16), (True, room_for_many(4, 2, 3), 16), (False, 0, 4), (True, room_for_many(4, 2, 3), 8)]
 
@@ -58,3 +79,36 @@ def test_scores_of_any_size(dtype, ragged, room, P, size):
                     best = vv[h // 2, :t][s >= s.max() - reach]
                     slack = 1e-5 * np.abs(best).max(0)
                     assert (got[r, h] >= best.min(0) - slack).all() and (got[r, h] <= best.max(0) + slack).all(), (b, r, h)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("above", [12.0, 24.4, 30.4, 36.0])
+@pytest.mark.parametrize("at", [0, 70])
+@pytest.mark.parametrize("ragged,room,P", FORMS)
+def test_small_weights_beside_a_dominating_key(dtype, above, at, ragged, room, P):
+    """A key `above` powers of two over the others whose value is 0: the output is
+    made of the small weights alone.  f32 and bf16 pages hold each to f32's
+    accuracy.  f16 pages hold a weight to 2^-22 of itself and 2^-38 of the
+    largest: P is 2^13 or more there, in two f16 parts whose second rounds at
+    2^-25, half of f16's least step."""
+    H, nKV, D = 4, 2, 64
+    added = [3, 1, 20] if ragged else [1, 1, 1]
+    q, row_start, lens, tables, k, v = attention_case(41, dtype, H, nKV, D, P, [150, 90, 300], added, q_std=0.1)
+    rs = np.random.RandomState(5)
+    u = np.where(rs.rand(D) < 0.5, -1.0, 1.0)
+    q += u.astype(np.float32)  # all queries point along u, more or less
+    far = above * np.log(2.0) / D ** 0.5 * u  # scale q.k is about above * ln 2
+    for b in range(3):
+        page = tables[b, at // P]
+        k[page, :, at % P] = R.stored(np.broadcast_to(far, (nKV, D)), dtype)
+        v[page, :, at % P] = R.stored(np.zeros((nKV, D)), dtype)
+    got = run_attention(q, row_start, lens, tables, k, v, ragged, room=room).reshape(q.shape).astype(np.float64)
+    want, mag, big = R.attention(q.astype(np.float64), row_start, lens, tables, R.value(k, dtype), R.value(v, dtype))
+    # the bound of check_attention, and the floor of f16's weights
+    rel = 2 * ((D + 8) * 2.0 ** -24 + 2.0 ** -21) * big + 2.0 ** -20 + int(max(lens)) * 2.0 ** -23
+    bound = mag * rel[..., None]
+    if dtype == "f16":
+        sw, sv, _ = weights(q, row_start, lens, tables, k, v, dtype)
+        bound += 2.0 ** -38 * sv / sw[..., None]
+    off = np.abs(got - want)
+    assert np.all(off <= bound), (off / bound).max()
