@@ -396,7 +396,7 @@ struct MmBf16 {
   typedef __bf16 T;
   static constexpr int TERMS = 3;
   static constexpr uint32_t EXPONENT = 0x7F80u;
-  static constexpr float P_EXP = 6.0f, P_TOP = 14.0f;
+  static constexpr float P_EXP = -8.0f, P_TOP = 0.0f;  // no weight above 1: sums overflow where they would of weights of 1
   static __device__ __forceinline__ void split2(float x, float y, u32x4 (&t)[TERMS], int k) {
     f32x2 r = (f32x2){x, y};
 #pragma unroll
@@ -541,7 +541,7 @@ template <int DPL>
 struct Tile32 {
   typedef float T;
   static constexpr int NJ = 1, KS = DPL, QREG = KS;
-  static constexpr float P_EXP = 6.0f, P_TOP = 14.0f;
+  static constexpr float P_EXP = -8.0f, P_TOP = 0.0f;  // no weight above 1: sums overflow where they would of weights of 1
   f32x4 K[KS];  // dims s*16 + 4g .. +3
   float V[4][DPL];
   static constexpr int QRAW = KS;

@@ -112,3 +112,33 @@ def test_small_weights_beside_a_dominating_key(dtype, above, at, ragged, room, P
         bound += 2.0 ** -38 * sv / sw[..., None]
     off = np.abs(got - want)
     assert np.all(off <= bound), (off / bound).max()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("ragged,room,P", FORMS)
+@pytest.mark.parametrize("split", [False, True])
+def test_values_up_to_the_end_of_f32(dtype, ragged, room, P, split):
+    """Values whose weighted sum, of weights up to 1, is just inside f32."""
+    H, nKV, D = 4, 2, 64
+    lens = [3000, 700, 41] if split else [100, 64, 41]
+    case = attention_case(42, dtype, H, nKV, D, P, lens, [3, 1, 2] if ragged else [1, 1, 1])
+    q, row_start, lens, tables, k, v = case
+    _, _, swv = weights(*case, dtype)
+    v = R.stored(R.value(v, dtype) * (2.0 ** 127 / swv.max()), dtype)
+    case = q, row_start, lens, tables, k, v
+    check_attention(run_attention(*case, ragged=ragged, room=room), *case, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("ragged,room,P", FORMS)
+def test_values_near_the_least_of_f32(dtype, ragged, room, P):
+    """Values of 1e-36, which weights of 2^-8 and less make subnormal: each of the
+    sum's roundings is half of f32's least number there, over weights of 2^-8."""
+    H, nKV, D = 4, 2, 64
+    q, row_start, lens, tables, k, v = attention_case(46, dtype, H, nKV, D, P, [300, 64, 41], [3, 1, 2] if ragged else [1, 1, 1])
+    v = R.stored(R.value(v, dtype) * 1e-36, dtype)
+    got = run_attention(q, row_start, lens, tables, k, v, ragged, room=room).reshape(q.shape)
+    want, mag, big = R.attention(q.astype(np.float64), row_start, lens, tables, R.value(k, dtype), R.value(v, dtype))
+    rel = 2 * ((D + 8) * 2.0 ** -24 + 2.0 ** -21) * big + 2.0 ** -20 + int(max(lens)) * 2.0 ** -23
+    # three parts of a weight at the most, and a join of four waves
+    assert np.all(np.abs(got.astype(np.float64) - want) <= mag * rel[..., None] + (3 * 300 + 4) * 2.0 ** -150 * 2.0 ** 8)
