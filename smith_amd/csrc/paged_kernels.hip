@@ -321,9 +321,9 @@ DEF_APPEND(smith_paged_append_bf16, KvBf16)
 //
 // f16 and bf16 pages are exact in the matrix cores' operands; q and P are split
 // into parts of the pages' type that add up to 22 (two f16) or 24 (three bf16)
-// bits, the products are exact and summed in f32.  q is brought to [2^13.5, 2^15.5)
-// by a power of two first and P far up in f16 too, since small parts round at f16's
-// least step: 2^-38 of the largest.  f32 pages go through the f32 matrix cores.
+// bits, the products are exact and summed in f32.  For f16, q and P are brought far
+// up by a power of two first, since small parts round at f16's least step: 2^-38 of
+// the largest.  f32 pages go through the f32 matrix cores.
 //
 // scale log2 e is a factor of q but for a power of two c, by which the sums are
 // multiplied.  So a score in powers of two is exact from its sum, its difference
@@ -377,6 +377,9 @@ struct MmF16 {
   // moves less often.  A prompt of 2000 rows, 32 heads on 8 of 128, 83.0 and 83.8 us;
   // 600 rows 31.1 and 31.7.)
   static constexpr float P_EXP = 13.0f, P_TOP = 15.9f;
+  // by what power of two q of elements up to 2^e is multiplied: to [2^15, 2^16), far up
+  // in f16 as well
+  static __device__ __forceinline__ int q_shift(int e) { return 16 - e; }
   // word k of the parts, from values 2k and 2k + 1
   static __device__ __forceinline__ void split2(float x, float y, u32x4 (&t)[TERMS], int k) {
     // the rest in one mixed-precision operation each (without a factor that the
@@ -396,6 +399,9 @@ struct MmBf16 {
   typedef __bf16 T;
   static constexpr int TERMS = 3;
   static constexpr uint32_t EXPONENT = 0x7F80u;
+  // only what is far from 1 is moved, to where its parts and its sums of products with
+  // keys of any size are inside f32 if they were
+  static __device__ __forceinline__ int q_shift(int e) { return (e < -64 ? -64 : e > 64 ? 64 : e) - e; }
   static constexpr float P_EXP = -8.0f, P_TOP = 0.0f;  // no weight above 1: sums overflow where they would of weights of 1
   static __device__ __forceinline__ void split2(float x, float y, u32x4 (&t)[TERMS], int k) {
     f32x2 r = (f32x2){x, y};
@@ -444,8 +450,8 @@ struct Tile16 {
     }
   }
   // ... in parts, times `factor` (at least 0.36, less than 0.73, of either sign) and a
-  // power of two that brings its largest element to [2^15, 2^16) before; what is not
-  // finite stays as it is.  Register k of the steps that do(s) says goes to put(k, parts).
+  // power of two (MM::q_shift); what is not finite stays as it is.  Register k of the
+  // steps that do(s) says goes to put(k, parts).
   template <class DO, class PUT>
   static __device__ __forceinline__ void split_q(const f32x4 (&x)[QRAW], bool there, uint32_t g, uint32_t hd, float factor,
                                                  int& e2, DO todo, PUT put) {
@@ -455,7 +461,7 @@ struct Tile16 {
 #pragma unroll
       for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[2 * s + e / 4][e % 4]));  // a repeated element is one of the row's
     big = max_xor16_32(big);
-    e2 = there && big > 0.f && big < __builtin_inff() ? 16 - __builtin_amdgcn_frexp_expf(big) : 0;
+    e2 = there && big > 0.f && big < __builtin_inff() ? MM::q_shift(__builtin_amdgcn_frexp_expf(big)) : 0;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
       if (!todo(s)) continue;

@@ -142,3 +142,22 @@ def test_values_near_the_least_of_f32(dtype, ragged, room, P):
     rel = 2 * ((D + 8) * 2.0 ** -24 + 2.0 ** -21) * big + 2.0 ** -20 + int(max(lens)) * 2.0 ** -23
     # three parts of a weight at the most, and a join of four waves
     assert np.all(np.abs(got.astype(np.float64) - want) <= mag * rel[..., None] + (3 * 300 + 4) * 2.0 ** -150 * 2.0 ** 8)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("ragged,room,P", FORMS)
+@pytest.mark.parametrize("how", ["queries", "scale"])
+def test_keys_up_to_1e35(dtype, ragged, room, P, how):
+    """Large keys against small queries, or against a small scale: every product
+    and sum is inside f32."""
+    H, nKV, D = 4, 2, 64
+    q, row_start, lens, tables, k, v = attention_case(43, dtype, H, nKV, D, P, [300, 64, 41], [3, 1, 2] if ragged else [1, 1, 1])
+    k = R.stored(R.value(k, dtype) * 1e35, dtype)
+    q = np.copysign(1 + np.abs(q), q)
+    scale = 0.125
+    if how == "queries":
+        q = (q * 1e-35).astype(np.float32)
+    else:
+        scale = 0.125e-35
+    case = q, row_start, lens, tables, k, v
+    check_attention(run_attention(*case, ragged=ragged, scale=scale, room=room), *case, dtype, np.float32(scale))
