@@ -435,12 +435,15 @@ int smith_paged_append(void* ctx, uint32_t kv_type, const float* qkv, uint32_t l
  * room for max_rows rows; out overlaps no input.  Rows of out behind the last row
  * stay as they are.  f32 accuracy; with f16 pages an element of q and a weight are
  * held to 2^-22 of themselves, and to no less than 2^-38 of the largest of their
- * head's.  Keys that a row does not see may hold anything; among those that it
- * sees an entry that is not finite makes that row's head not finite.  head_dim <= 128 and % 8 == 0.  A row_start
- * past max_rows fails the call; starts that do not ascend, and a len below the
- * request's rows or past max_pages pages, fail the request (nothing of it is
- * written); a page outside the pool leaves its
- * request's rows undefined. */
+ * head's.  A row's weighted sum of values, of weights up to 1, is formed before it
+ * is divided by the weights' and has to be inside f32.  Keys that a row does not
+ * see may hold anything.  Among those that it sees a NaN in a key makes the row's
+ * head NaN, an infinity in a key makes it NaN or, where its score is -inf, weighs
+ * nothing, and what is not finite in a value makes at least that dim of the head
+ * not finite.  head_dim <= 128 and % 8 == 0.  A row_start past max_rows fails the
+ * call; starts that do not ascend, and a len below the request's rows or past
+ * max_pages pages, fail the request (nothing of it is written); a page outside the
+ * pool leaves its request's rows undefined. */
 int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
                           const int32_t* row_start, const int32_t* lens, const int32_t* tables, uint32_t n_req,
                           uint32_t max_pages, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,

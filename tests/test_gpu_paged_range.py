@@ -161,3 +161,44 @@ def test_keys_up_to_1e35(dtype, ragged, room, P, how):
         scale = 0.125e-35
     case = q, row_start, lens, tables, k, v
     check_attention(run_attention(*case, ragged=ragged, scale=scale, room=room), *case, dtype, np.float32(scale))
+
+
+def junk_of(x, dtype):
+    return {"f32": np.float32(x), "f16": np.float16(x),
+            "bf16": np.uint16(np.float32(x).view(np.uint32) >> 16 | (0x40 if np.isnan(x) else 0))}[dtype]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("room", [0, room_for_many(4, 2, 2)])
+@pytest.mark.parametrize("D,dim", [(64, 5), (72, 71), (128, 0)])
+@pytest.mark.parametrize("where", ["key", "value"])
+def test_one_entry_that_is_not_finite(dtype, room, D, dim, where):
+    """Key 3 is seen by all rows, and lies in a tile that is; 150 too, in one beside
+    hidden keys; 205 by the last rows only.  What the rows that see it may give is
+    what the header says; the others, and other KV heads, are as without it."""
+    H, nKV, P = 4, 2, 16
+    q, row_start, lens, tables, k, v = attention_case(47, dtype, H, nKV, D, P, [210, 40], [60, 1])
+    clean = run_attention(q, row_start, lens, tables, k, v, True, room=room).reshape(q.shape)
+    near = lambda a, b: np.linalg.norm(a - b) <= 1e-5 * np.linalg.norm(b)
+    pool = k if where == "key" else v
+    for junk in (np.nan, np.inf, -np.inf):
+        for at in (3, 150, 205):
+            place = tables[0, at // P], 1, at % P, dim
+            kept, pool[place] = pool[place], junk_of(junk, dtype)
+            got = run_attention(q, row_start, lens, tables, k, v, True, room=room).reshape(q.shape)
+            sees = np.zeros(q.shape[:2], bool)
+            sees[:60, 2:] = (210 - 60 + np.arange(60) >= at)[:, None]
+            assert near(got[~sees], clean[~sees]), (junk, at)
+            if where == "value":
+                assert not np.isfinite(got[sees][:, dim]).any(), (junk, at)
+                for a, b in zip(np.delete(got[sees], dim, 1), np.delete(clean[sees], dim, 1)):
+                    assert np.isnan(a).all() or near(a, b), (junk, at)
+            elif np.isnan(junk):
+                assert np.isnan(got[sees]).all(), (junk, at)
+            else:
+                with np.errstate(invalid="ignore"):
+                    want, _, _ = R.attention(q.astype(np.float64), row_start, lens, tables, R.value(k, dtype),
+                                             R.value(v, dtype))
+                for a, w in zip(got[sees], want[sees]):  # a score of -inf weighs nothing
+                    assert not np.isfinite(a).any() or (np.isfinite(w).all() and near(a, w)), (junk, at)
+            pool[place] = kept
