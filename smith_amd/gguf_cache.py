@@ -260,9 +260,9 @@ class _Engine:
 
     def paged_step(self, model, tokens, cache):
         """Rows of several requests (tokens[b]: request b's) through every layer on
-        a PagedCache; the logits of each request's last row, in order."""
-        cfg, ctx, eps = self.cfg, device.ops_ctx(), model["normEps"]
-        dim, vocab, H, hd, ld = cfg["dim"], cfg["vocabSize"], cfg["numHeads"], cfg["headDim"], self.qkv_ld
+        a PagedCache; the logits of each request's last row, in order.  Whatever
+        raises, the cache is as it was."""
+        cfg, vocab = self.cfg, self.cfg["vocabSize"]
         added = [len(t) for t in tokens]
         M = sum(added)
         if M > _chunk_rows(cfg):
@@ -271,7 +271,16 @@ class _Engine:
         if flat and not 0 <= min(flat) <= max(flat) < vocab:
             raise ValueError("paged step: a token outside the vocabulary of %d" % vocab)
         cache.check_model(cfg)
-        plan = cache.plan(added)
+        out, before = self._row_logits(), cache.state()
+        try:
+            return self._paged_rows(model, flat, added, cache, cache.plan(added), out)
+        except BaseException:
+            cache.restore(before)  # no keys of this step: it can be tried again
+            raise
+
+    def _paged_rows(self, model, flat, added, cache, plan, out):
+        cfg, ctx, eps = self.cfg, device.ops_ctx(), model["normEps"]
+        dim, vocab, H, ld, M = cfg["dim"], cfg["vocabSize"], cfg["numHeads"], self.qkv_ld, len(flat)
         self.embed(model, flat)
         x, x2, qkv, attn, h = self.x.ptr, self.x2.ptr, self.qkv.ptr, self.attn.ptr, self.h.ptr
         rope = model["rope"]
@@ -290,7 +299,6 @@ class _Engine:
             for i, r in enumerate(last):
                 device.check(device.lib.smith_copy_d2d(ctx, x2, i * dim * 4, x, int(r) * dim * 4, dim * 4), "last rows")
         logits = np.empty((len(last), vocab), np.float32)
-        out = self._row_logits()
         for b0 in range(0, len(last), out.shape[0]):
             b1 = min(len(last), b0 + out.shape[0])
             self._lm_head_rows_at(model, rows + b0 * dim * 4, b1 - b0, out.ptr)

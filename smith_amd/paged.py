@@ -169,6 +169,15 @@ class PagedCache:
         return {"rowStart": self._row_start, "lens": self._lens[b], "slots": slots, "positions": positions,
                 "tables": self._tables}
 
+    def state(self):
+        """For restore()."""
+        return self._turn, self.lens, self.freeCount
+
+    def restore(self, state):
+        """Back to a state() from before the last plan(), if nothing was released
+        since: what that step read on the device is still there."""
+        self._turn, self.lens, self.freeCount = state
+
     def append(self, layer, plan, qkv, ld, rows, numHeads, rope, cos, sin, ropeLen):
         """A layer's rows [q | k | v] (device pointer, row stride ld floats) into its
         pages; q is rotated in place."""
