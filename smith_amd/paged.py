@@ -98,6 +98,11 @@ def pagedAttention(q, lens, tables, kPages, vPages, rowStart=None, scale=0.0, ou
     return out
 
 
+def _release(tensors):
+    for t in tensors:
+        t.release()
+
+
 class PagedCache:
     """The paged cache of a model's requests: per layer the pools k and v, and on
     the device the block tables [requests, maxPages], lengths and free list, which
@@ -153,10 +158,15 @@ class PagedCache:
             raise ValueError("paged step: %d new pages, %d are free" % (new, self.freeCount))
         if self._rows is None or self._rows["slots"].shape[0] < rows:
             # rows behind a step's last stay at slot -1: one pair of buffers serves all sizes up to theirs
-            room = max(256, rows)
-            for t in (self._rows or {}).values():
-                t.release()
-            self._rows = {"slots": T.create([room], "i32"), "positions": T.create([room], "i32")}
+            room, pair = max(256, rows), {}
+            try:
+                for name in ("slots", "positions"):
+                    pair[name] = T.create([room], "i32")
+            except BaseException:
+                _release(pair.values())
+                raise
+            _release((self._rows or {}).values())
+            self._rows = pair
         self._added.set_data(added)
         a, b = self._turn, 1 - self._turn
         slots, positions = self._rows["slots"], self._rows["positions"]
@@ -214,8 +224,7 @@ class PagedCache:
     def free(self):
         """Gives the device memory back; the cache is not used after it."""
         tensors = [t for layer in self.layers for t in layer.values()] + self._lens + self._count
-        for t in tensors + [self._tables, self._free, self._added, self._row_start] + list((self._rows or {}).values()):
-            t.release()
+        _release(tensors + [self._tables, self._free, self._added, self._row_start] + list((self._rows or {}).values()))
         self.layers, self._rows = [], None
 
 
