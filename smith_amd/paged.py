@@ -122,19 +122,29 @@ class PagedCache:
             raise ValueError("createPagedCache: heads of %d dims (8, 16 .. 128)" % config["headDim"])
         self.requests, self.pages, self.pageSize, self.dtype = requests, pages, pageSize, dtype
         self.maxPages = -(-config["maxSeqLen"] // pageSize)
-        shape = [pages, config["numKVHeads"], pageSize, config["headDim"]]
-        self.layers = [{"k": T.create(shape, dtype), "v": T.create(shape, dtype)} for _ in range(config["numLayers"])]
         self.lens = np.zeros(requests, np.int32)
         self.freeCount = pages
-        self._tables = T.zeros([requests, self.maxPages], "i32")
-        self._free = T.tensor(np.arange(pages - 1, -1, -1), dtype="i32")  # page 0 goes first
+        self.layers, self._rows, self._turn, self._tensors = [], None, 0, []
+        try:
+            self._allocate(config)
+        except BaseException:
+            self.free()
+            raise
+
+    def _allocate(self, config):
+        def hold(t):
+            self._tensors.append(t)
+            return t
+        n, shape = self.requests, [self.pages, config["numKVHeads"], self.pageSize, config["headDim"]]
+        for _ in range(config["numLayers"]):
+            self.layers.append({name: hold(T.create(shape, self.dtype)) for name in ("k", "v")})
+        self._tables = hold(T.zeros([n, self.maxPages], "i32"))
+        self._free = hold(T.tensor(np.arange(self.pages - 1, -1, -1), dtype="i32"))  # page 0 goes first
         # what a step reads and what it writes, in turn
-        self._lens = [T.zeros([requests], "i32"), T.zeros([requests], "i32")]
-        self._count = [T.tensor([pages], dtype="i32"), T.tensor([pages], dtype="i32")]
-        self._turn = 0
-        self._added = T.zeros([requests], "i32")
-        self._row_start = T.zeros([requests + 1], "i32")
-        self._rows = None
+        self._lens = [hold(T.zeros([n], "i32")) for _ in range(2)]
+        self._count = [hold(T.tensor([self.pages], dtype="i32")) for _ in range(2)]
+        self._added = hold(T.zeros([n], "i32"))
+        self._row_start = hold(T.zeros([n + 1], "i32"))
 
     def check_model(self, config):
         """Raises ValueError unless the pools are those of a model of this config."""
@@ -223,9 +233,8 @@ class PagedCache:
 
     def free(self):
         """Gives the device memory back; the cache is not used after it."""
-        tensors = [t for layer in self.layers for t in layer.values()] + self._lens + self._count
-        _release(tensors + [self._tables, self._free, self._added, self._row_start] + list((self._rows or {}).values()))
-        self.layers, self._rows = [], None
+        _release(self._tensors + list((self._rows or {}).values()))
+        self.layers, self._rows, self._tensors = [], None, []
 
 
 def createPagedCache(config, requests, pages, pageSize=16, dtype="f16"):

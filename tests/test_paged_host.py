@@ -81,3 +81,18 @@ def test_rows_that_there_is_no_memory_for(fake):
     assert plan["slots"].shape[0] >= 300 and plan["slots"].buffer and kept.buffer is None
     cache.free()
     assert not fake.memory
+
+
+def test_a_cache_that_there_is_no_memory_for(fake):
+    """Whichever allocation fails: what was had goes back."""
+    for room in range(100):
+        fake.room = room
+        try:
+            cache = S.createPagedCache(CONFIG, 3, 20, 16)
+        except RuntimeError:
+            assert not fake.memory, room
+        else:
+            break
+    assert room == 14  # three layers' pools, tables, free list, two lengths and two counts, added, row starts
+    cache.free()
+    assert not fake.memory
