@@ -153,9 +153,14 @@ class PagedCache:
             raise ValueError("paged step: a cache of %d layers of %d heads of %d, a model of %d of %d of %d" % (
                 len(self.layers), k[1], k[3], config["numLayers"], config["numKVHeads"], config["headDim"]))
 
+    def _there(self):
+        if not self._tensors:
+            raise ValueError("paged cache: it was freed")
+
     def plan(self, added):
         """The step in which request b brings added[b] rows: {rowStart, lens, slots,
         positions, tables}.  Nothing happens (ValueError) if it does not fit."""
+        self._there()
         added = np.asarray(added, np.int64)
         rows = int(added.sum())
         lens = self.lens + added
@@ -201,6 +206,7 @@ class PagedCache:
     def append(self, layer, plan, qkv, ld, rows, numHeads, rope, cos, sin, ropeLen):
         """A layer's rows [q | k | v] (device pointer, row stride ld floats) into its
         pages; q is rotated in place."""
+        self._there()
         k, v = self.layers[layer]["k"], self.layers[layer]["v"]
         device.check(device.lib.smith_paged_append(
             device.ops_ctx(), KV_TYPES[self.dtype], qkv, ld, rows, plan["slots"].buffer, plan["positions"].buffer,
@@ -209,6 +215,7 @@ class PagedCache:
 
     def attention(self, layer, plan, q, ld, rows, numHeads, out):
         """A layer's attention of the step's rows into out [rows, numHeads * headDim]."""
+        self._there()
         k, v = self.layers[layer]["k"], self.layers[layer]["v"]
         device.check(device.lib.smith_paged_attention(
             device.ops_ctx(), KV_TYPES[self.dtype], q, ld, rows, plan["rowStart"].buffer, plan["lens"].buffer,
@@ -217,6 +224,7 @@ class PagedCache:
 
     def release(self, request):
         """The request's pages back to the free list; its number is free for another."""
+        self._there()
         if not 0 <= request < self.requests:
             raise ValueError("paged cache: request %d of %d" % (request, self.requests))
         n = -(-int(self.lens[request]) // self.pageSize)

@@ -96,3 +96,16 @@ def test_a_cache_that_there_is_no_memory_for(fake):
     assert room == 14  # three layers' pools, tables, free list, two lengths and two counts, added, row starts
     cache.free()
     assert not fake.memory
+
+
+def test_a_cache_that_was_freed(fake):
+    """Nothing is done on memory that it no longer has."""
+    cache = S.createPagedCache(CONFIG, 2, 20, 16)
+    cache.plan([20, 3])
+    cache.free()
+    cache.free()
+    for call in (lambda: cache.plan([1, 0]), lambda: cache.release(0), lambda: cache.append(0, {}, 0, 0, 1, 2, 0, 0, 0, 0),
+                 lambda: cache.attention(0, {}, 0, 0, 1, 2, 0)):
+        with pytest.raises(ValueError, match="paged cache: it was freed"):
+            call()
+    assert not fake.memory
