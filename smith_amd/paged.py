@@ -230,14 +230,13 @@ class PagedCache:
         n = -(-int(self.lens[request]) // self.pageSize)
         if not n:
             return
-        a = self._turn
-        free = self._free.data
-        free[self.freeCount:self.freeCount + n] = self._tables.data[request, :n]
-        self._free.set_data(free)
+        ctx, a = device.ops_ctx(), self._turn
+        device.check(device.lib.smith_copy_d2d(ctx, self._free.buffer, 4 * self.freeCount, self._tables.buffer,
+                                               4 * request * self.maxPages, 4 * n), "paged cache")
+        device.check(device.lib.smith_set_i32(ctx, self._lens[a].buffer + 4 * request, 0), "paged cache")
+        device.check(device.lib.smith_set_i32(ctx, self._count[a].buffer, self.freeCount + n), "paged cache")
         self.freeCount += n
         self.lens[request] = 0
-        self._count[a].set_data(np.array([self.freeCount], np.int32))
-        self._lens[a].set_data(self.lens)
 
     def free(self):
         """Gives the device memory back; the cache is not used after it."""

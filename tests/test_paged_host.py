@@ -109,3 +109,29 @@ def test_a_cache_that_was_freed(fake):
         with pytest.raises(ValueError, match="paged cache: it was freed"):
             call()
     assert not fake.memory
+
+
+@pytest.mark.parametrize("requests,pages", [(2, 40), (3000, 40000)])
+def test_release_moves_one_requests_pages(fake, requests, pages):
+    """However large the cache is: nothing is copied to the host, and the request's
+    own pages on the device."""
+    cache = S.createPagedCache(dict(CONFIG, numLayers=0, maxSeqLen=320), requests, pages, 16)
+    added = np.zeros(requests, int)
+    added[:2] = 33, 50
+    cache.plan(added)
+    tables = np.full((requests, 20), -1)
+    tables[0, :3], tables[1, :4] = [7, 2, 30], [9, 0, 5, 31]  # as the step's kernel would
+    cache._tables.set_data(tables)
+    cache._lens[cache._turn].set_data(cache.lens)
+    fake.moved.clear()
+    cache.release(0)
+    cache.release(0)
+    assert sum(fake.moved) <= 64
+    assert cache.freeCount == pages - 4 and cache.lens[:2].tolist() == [0, 50]
+    assert cache._free.data[pages - 7:pages - 4].tolist() == [7, 2, 30]
+    assert cache._count[cache._turn].data.tolist() == [pages - 4]
+    assert cache._lens[cache._turn].data.tolist() == cache.lens.tolist()
+    cache.release(1)
+    assert cache._free.data[pages - 4:].tolist() == [9, 0, 5, 31] and cache.freeCount == pages
+    with pytest.raises(ValueError, match="request %d of" % requests):
+        cache.release(requests)
