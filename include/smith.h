@@ -405,9 +405,10 @@ int smith_randn(void* ctx, float* out, uint64_t n, uint64_t seed, uint64_t offse
  * Outputs overlap no input (tables is both): the next step's cached and
  * free_count are this one's lens and free_left in buffers of their own.  A
  * length that is negative or longer than max_pages pages, more than max_rows
- * rows or too few free pages fail the step: no page is taken, row_start is all 0,
- * every slot -1 and lens = cached.  A page outside the pool fails the rows in it
- * (slot -1). */
+ * rows, too few free pages or a *free_count of more than n_pages (or than
+ * free_pages holds, where it is a buffer of smith_alloc) fail the step: no page
+ * is taken, row_start is all 0, every slot -1 and lens = cached.  A page outside
+ * the pool fails the rows in it (slot -1). */
 int smith_paged_plan(void* ctx, const int32_t* cached, const int32_t* added, uint32_t n_req,
                      const int32_t* free_pages, const int32_t* free_count, uint32_t n_pages, uint32_t page_size,
                      uint32_t max_pages, uint32_t max_rows, int32_t* tables, int32_t* row_start, int32_t* lens,

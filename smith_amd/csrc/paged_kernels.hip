@@ -87,8 +87,8 @@ struct KvBf16 {
 
 extern "C" __global__ __launch_bounds__(PLAN_THREADS) void smith_paged_plan(
     const int32_t* __restrict__ cached, const int32_t* __restrict__ added, uint32_t n_req,
-    const int32_t* __restrict__ free_pages, const int32_t* __restrict__ free_count, uint32_t n_pages, uint32_t shift,
-    uint32_t max_pages, uint32_t max_rows, int32_t* __restrict__ tables, int32_t* __restrict__ row_start,
+    const int32_t* __restrict__ free_pages, const int32_t* __restrict__ free_count, uint32_t n_list, uint32_t n_pages,
+    uint32_t shift, uint32_t max_pages, uint32_t max_rows, int32_t* __restrict__ tables, int32_t* __restrict__ row_start,
     int32_t* __restrict__ lens, int32_t* __restrict__ slots, int32_t* __restrict__ positions,
     int32_t* __restrict__ free_left, uint64_t* __restrict__ err) {
   __shared__ uint32_t s_row[PAGED_MAX_REQ + 1], s_page[PAGED_MAX_REQ], s_had[PAGED_MAX_REQ];
@@ -155,7 +155,7 @@ extern "C" __global__ __launch_bounds__(PLAN_THREADS) void smith_paged_plan(
   // the same in every workgroup
   const uint32_t code = bad_req             ? PAGED_ERR_PLAN_LENGTH
                         : tr > max_rows     ? PAGED_ERR_PLAN_ROWS
-                        : have < 0 || have > (int64_t)n_pages || tp > (uint64_t)have ? PAGED_ERR_PLAN_PAGES
+                        : have < 0 || have > (int64_t)n_list || tp > (uint64_t)have ? PAGED_ERR_PLAN_PAGES
                                             : 0u;
   if (code && blockIdx.x == 0 && tid == 0) paged_err(err, code, bad_req ? bad_req - 1 : code == PAGED_ERR_PLAN_ROWS ? max_rows : (uint32_t)have);
   uint32_t at_row = (uint32_t)(br + ir - rows), at_page = (uint32_t)(bp + ip - pages);

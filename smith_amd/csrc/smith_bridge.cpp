@@ -278,7 +278,7 @@ int check_paged_err(Ctx* c) {
       "?",
       "smith_paged_plan: request %u: a length is negative or longer than its block table; the step has no rows",
       "smith_paged_plan: the requests bring more than max_rows = %u rows; the step has no rows",
-      "smith_paged_plan: the requests need more than the %u free pages; the step has no rows",
+      "smith_paged_plan: the requests need more than the %u free pages, or the list holds fewer; the step has no rows",
       "smith_paged_plan: request %u: a page outside the pool",
       "smith_paged_append: row %u: its slot lies outside the pool",
       "smith_paged_append: row %u: its position lies outside the rotary tables",
@@ -2368,7 +2368,10 @@ int smith_paged_plan(void* ctx, const int32_t* cached, const int32_t* added, uin
   }
   if (set_device(c)) return -1;
   uint64_t* perr = c->paged_err_dev();
-  void* args[] = {&cached, &added, &n_req, &free_pages, &free_count, &n_pages, &shift, &max_pages, &max_rows,
+  // entries there can be: of a buffer of smith_alloc no more than it holds
+  uint32_t n_list = n_pages;
+  if (const uint64_t bytes = smith_buffer_length((void*)free_pages)) n_list = (uint32_t)std::min<uint64_t>(n_pages, bytes / 4);
+  void* args[] = {&cached, &added, &n_req, &free_pages, &free_count, &n_list, &n_pages, &shift, &max_pages, &max_rows,
                   &tables, &row_start, &lens, &slots, &positions, &free_left, &perr};
   const uint32_t groups = std::max<uint32_t>(1, (max_rows + 255) / 256);  // PLAN_THREADS rows each
   return launch(c, "smith_paged_plan", dim3(groups), dim3(256), args);
