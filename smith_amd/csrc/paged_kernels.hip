@@ -1544,9 +1544,6 @@ struct Rows16 {
           for (int x = 0; x < CT * 4; x++)
             if (x * DPL / (CT * 4) / 2 * 2 == d) pair(h + 1, x);
         }
-        // three parts: kept in this order, which the compiler's own spills (a chunk
-        // of 2000 rows behind 6000 keys 573 us, 591 without; two parts 470 and 462)
-        if (TERMS > 2) __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
