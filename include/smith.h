@@ -444,7 +444,10 @@ int smith_paged_append(void* ctx, uint32_t kv_type, const float* qkv, uint32_t l
  * not finite.  head_dim <= 128 and % 8 == 0.  A row_start past max_rows fails the
  * call; starts that do not ascend, and a len below the request's rows or past
  * max_pages pages, fail the request (nothing of it is written); a page outside the
- * pool leaves its request's rows undefined. */
+ * pool leaves its request's rows undefined.
+ * Two kernels compute the same, the faster for many rows taken by max_rows,
+ * n_heads and n_req: keep max_rows near the rows that there are, and requests that
+ * sit out few. */
 int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
                           const int32_t* row_start, const int32_t* lens, const int32_t* tables, uint32_t n_req,
                           uint32_t max_pages, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,

@@ -1191,7 +1191,7 @@ __device__ __forceinline__ void weigh(f32x4 (&S)[NJ], float c, float& m, float& 
 
 // The kernel's arguments, read again: held over the key loops they take scalar
 // registers and then lanes of vector registers (16 columns of f16, 128 dims: 230
-// and 49 spilled scalars, so 202 and none; one row behind 1024 keys 10.3 and 9.7 us),
+// and 49 spilled scalars, so 203 and none; one row behind 1024 keys 10.3 and 9.7 us),
 // or reloads in every stage behind the DMA (three-part weights of 128 dims).
 __device__ __forceinline__ const AttArgs& again() {
   typedef const AttArgs __attribute__((address_space(4))) Kernarg;
@@ -1419,8 +1419,8 @@ __device__ __forceinline__ void attention_body(const AttArgs& args) {
 // values through the transposing LDS read, lane (4k + c) of 16 supplying dims
 // 4c .. 4c+3 of the k-th of four keys and receiving one dim of all four.
 // Bound by the matrix cores: 2000 rows behind 6000 keys, 32 heads on 8 of 128 dims,
-// 229 GFLOP: f16 450 us, 1020 TFLOP/s of split products (a large library product:
-// 1097), bf16 512 to 560 us, 1230 to 1340 (1136), f32 1.98 ms, 116 (152).  A wave's
+// 229 GFLOP: f16 395 to 450 us, 1020 to 1160 TFLOP/s of split products (a large library
+// product: 1097), bf16 510 to 560 us, 1230 to 1350 (1136), f32 1.98 ms, 116 (152).  A wave's
 // stage is a chain of 6000 cycles for 2048 of products (f16), so the next stage's
 // loads and the next weights go out between products, and shorter prompts wait for
 // their longest blocks: four of 430 to 611 rows 42 us in f16, half of that rate.
@@ -1800,10 +1800,10 @@ __device__ __forceinline__ void attention_rows_body(const AttArgs& args) {
     BODY<__VA_ARGS__>(a);                                          \
   }
 // Named by page type and head dims held (64, 96 or 128); _s for pages of less than
-// 16 keys.  Heads of 80 and 96 (10 and 12 heads) held as 96 dims against 128: 100
-// requests of 4000 keys, f32, 382 against 425 us, f16 190 and 191; 20 mixed
-// requests of up to 1500, f32, 29 and 32; prompts of 1300 rows 194 and 221 (f32), 70
-// and 76 (f16), 78 and 98 (bf16).
+// 16 keys.  Heads of 96 (12 on 4) held as 96 dims against 128: 100 requests of 4000 keys,
+// f32, 231 against 243 us, f16 115 and 116; 20 mixed requests of up to 1500, f32, 37 and
+// 42, f16 25 and 28; a prompt of 1300 rows 76 and 75 (f32), 35 and 37 (f16), 38 and 48
+// (bf16).
 #define DEF_ATTENTIONS(TYPE, D, DPL, TILE, ROWS)                                                 \
   DEF_ATTENTION(smith_paged_attention_##TYPE##_d##D, attention_body, TILE, DPL, false)           \
   DEF_ATTENTION(smith_paged_attention_##TYPE##_d##D##_s, attention_body, TILE, DPL, true)        \

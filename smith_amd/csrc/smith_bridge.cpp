@@ -2466,12 +2466,19 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   // columns fill most of two such tiles a workgroup shares the keys among four
   // waves' columns -- if there are enough of them for the waves of the card, which
   // its 64 or 128 columns to a workgroup otherwise leave idle.  Microseconds, the
-  // first kernel's and the second's (32 heads on 8, f16 | bf16 | f32): a prompt of
-  // 100 rows (3200 columns) 9.3, 14.2 | 9.0, 17.4 | 10.9, 17.7; of 300 rows 18.7, 21.3
-  // | 18.3, 26.1 | 22, 37; of 1000 rows 67, 47 | 70, 57 | 114, 114; of 2000 rows 191,
-  // 97 | 200, 124 | 394, 316; behind 8000 keys 64 rows (2048 columns) 52, 60 | 52, 71 |
-  // 109, 116, 256 rows (8192) 157, 99 | 157, 121 | 365, 308; 16 prompts of up to 200
-  // rows 85, 37 | 88, 51 | 109, 68.
+  // first kernel's and the second's (32 heads on 8 of 128, f16 | bf16 | f32): a prompt
+  // of 100 rows (3200 columns) 8.5, 13.5 | 8.8, 17.9 | 9.9, 16.8; of 200 (6400) 31.9,
+  // 16.4 | 32.1, 21.9 | 35.3, 25.7; of 300 (9600) 18.5, 20.8 | 18.8, 26.9 | 22.9, 35.1;
+  // of 400 23.6, 23.7 | 24.1, 31.5 | 32.6, 34.4; of 600 34.8, 31.6 | 36.1, 40.9 | 52.6,
+  // 53.6; of 1000 62, 44 | 65, 53 | 110, 101; of 2000 179, 86 | 178, 113 | 387, 302; 256
+  // rows (8192) behind 2000 keys 46.9, 42.3 | 48.5, 52.4 | 112, 97; behind 8000 keys 64
+  // rows 51, 57 | 53, 68 | 112, 115, 128 rows 87, 75 | 88, 87 | 207, 186, 256 rows 150,
+  // 94 | 154, 115 | 392, 312; 16 prompts of up to 200 rows 88, 40 | 91, 58 | 113, 71.
+  // 8192 columns are right for several prompts and behind long caches; one prompt of 200
+  // to 600 rows it gives the slower kernel, by up to 2x: what tells it from the others
+  // is the lengths, which are on the device.  For the same reason max_rows and n_req
+  // stand for the rows and the requests that bring some: 256 rows behind 7744 keys take
+  // 101 us alone and 150 in a cache of 64 places.
   // The second loads 8 keys at once, of one page.  The first takes 16 keys as one
   // address, or looks them up one by one where pages are smaller.
   const uint32_t G = n_heads / n_kv_heads;
@@ -2481,10 +2488,10 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   const uint32_t CB = !many ? 16 : kv_type == SMITH_KV_F32 ? 64 : 128, dims = head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : 128;
   const uint32_t target = 512;  // two workgroups to a CU
   // Keys to a split at least.  A split of many columns leaves 64 KB and the join
-  // reads them again: 64 f16 rows behind 8000 keys, 32 heads, in that kernel 65 us
-  // with 512, 78 with 384, 85 with 256 (300 rows of a prompt 23 us with 512, uncut, 46
-  // with 128).  f32 keys are eight times the work: 20 requests, half of them with
-  // chunks of up to 77 rows, 68 us with 256, 92 with 512.
+  // reads them again: 64 rows behind 8000 keys, 32 heads, in that kernel 58 us (f16) and
+  // 69 (bf16) with 512, 64 and 77 with 768, 74 and 84 with 384; 300 rows of a prompt 20.8
+  // uncut, 24.8 with 128.  f32 keys are eight times the work: 20 requests, half of them
+  // with chunks of up to 77 rows, 63 us with 256, 70 with 384, 80 with 512.
   const float split_min = !many ? 128.f : kv_type == SMITH_KV_F32 ? 256.f : 512.f;
   // a block that is cut has more than 5/4 C keys and so less than twice its keys / C
   // splits: 2 W / C <= 2 target of them in all (and some for what f32 rounds)
