@@ -362,8 +362,8 @@ __device__ __forceinline__ float max_xor16_32(float v) {
 }
 // Weights are P = 2^(score - m).  m is P_EXP (of the page type) under a column's
 // maximum, and follows a new one only when that would have a weight above 2^P_TOP.
-// From here on f32 holds every second whole number and less: m is the maximum
-// itself, which P_EXP below it would be rounded to something else.
+// Past FAR_SCORE f32 holds every second whole number and fewer: m is the maximum
+// itself there, P_EXP below which would be rounded to something else.
 #define FAR_SCORE 16777216.0f
 
 // the parts of eight f32 values in the pages' type, and the product of parts
