@@ -454,6 +454,46 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
                           const void* kpages, const void* vpages, uint32_t n_pages, uint32_t page_size, float* out,
                           uint32_t ld_out);
 
+/* ---- pages that requests share ----
+ * Several continuations of one prompt name its full pages together; a page that
+ * is partly filled belongs to one request, so that smith_paged_plan and
+ * smith_paged_append go on as ever.  A page is live if a request names it for a
+ * key: of tables[b] the first ceil(lens[b] / page_size) entries count.  With
+ * window > 0 those that neither hold one of the first `sinks` keys nor one of
+ * the last window - 1 (what a later row of smith_paged_attention_window sees) do
+ * not: they may hold anything, become -1 in new_tables, and their pages are free.
+ *
+ * smith_paged_fork: request b goes on from request parents[b] as it was before
+ * the call (itself; another; -1: it ends and has no keys).  new_lens [n_req] and
+ * new_tables [n_req][max_pages] are the requests after it.  Those with one parent
+ * share its full pages; a partly filled last page stays with the first of them,
+ * and the others, in order, take the lowest-numbered pages that nobody names and
+ * get its keys copied, in each of the n_pools pools (a layer's keys or values
+ * each: a host array of n_pools <= 4096 device pointers).  free_pages [n_pages]
+ * and free_count [1] become the free list, highest page first, for
+ * smith_paged_plan.  Entries behind a request's pages, and behind the list's end,
+ * stay as they are.  The outputs overlap no input, and a pool none of them.
+ *
+ * smith_paged_compact: of n live pages those numbered n and above move to the
+ * free ones below, lowest to lowest, in every pool: pages n and above are free
+ * then, and the list says so.  new_tables may be tables.
+ *
+ * n_kv_heads, head_dim, n_pages and page_size as smith_paged_append.  Both are
+ * enqueued, and can be captured once they have run with the same sizes.  A parent
+ * that is no request, a length that is negative or longer than max_pages pages, a
+ * page outside the pool, or too few free pages for the copies fail the call: the
+ * pools (and in-place tables) are as they were, free_count is 0 and the other
+ * outputs are undefined; the next synchronising call returns -1 with the finding
+ * in smith_last_error. */
+int smith_paged_fork(void* ctx, uint32_t kv_type, const int32_t* lens, const int32_t* tables, const int32_t* parents,
+                     uint32_t n_req, uint32_t max_pages, uint32_t window, uint32_t sinks, uint32_t n_kv_heads,
+                     uint32_t head_dim, void* const* pools, uint32_t n_pools, uint32_t n_pages, uint32_t page_size,
+                     int32_t* new_lens, int32_t* new_tables, int32_t* free_pages, int32_t* free_count);
+int smith_paged_compact(void* ctx, uint32_t kv_type, const int32_t* lens, const int32_t* tables, uint32_t n_req,
+                        uint32_t max_pages, uint32_t window, uint32_t sinks, uint32_t n_kv_heads, uint32_t head_dim,
+                        void* const* pools, uint32_t n_pools, uint32_t n_pages, uint32_t page_size, int32_t* new_tables,
+                        int32_t* free_pages, int32_t* free_count);
+
 /* ---- HIP graphs: capture the context stream, replay it ----
  * Ops enqueued between begin and end are recorded, not run; their scratch
  * must already be allocated (run the same ops once before capturing).

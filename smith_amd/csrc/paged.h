@@ -1,12 +1,40 @@
-// paged.h -- what the paged cache's kernels and the bridge share: limits and
-// the codes of what a kernel finds wrong in device memory.
+// paged.h -- what the paged cache's kernels and the bridge share: limits,
+// arguments and the codes of what a kernel finds wrong in device memory.
 #pragma once
+#include <stdint.h>
 
 // the kernels keep prefix sums over the requests of a step in LDS
 #define PAGED_MAX_REQ 4096u
 
 // attention: most splits of a block (their weights are kept in LDS, 16 columns of them)
 #define PAGED_SPLIT_MAX 128u
+
+// fork and compact: pools whose addresses go to a kernel at once, and in all
+#define PAGES_POOLS_LAUNCH 440u
+#define PAGES_MAX_POOLS 4096u
+#define PAGES_THREADS 256u
+
+// a request's table as the calls see it
+struct PagesTables {
+  const int32_t* lens;
+  const int32_t* tables;
+  const int32_t* parents;  // null: every request is its own
+  uint32_t n_req, max_pages, n_pages, shift, window, sinks;
+};
+// what the kernels of a call hand on: device memory of the context
+struct PagesWork {
+  uint32_t* map;     // [words] a bit to a page; zero between calls
+  uint32_t* state;   // [0] something was wrong (zero between calls), [1] the moves
+  uint32_t* counts;  // [words / 256] live pages of 256 words' pages; null: not counted
+  uint32_t* src;     // [moves] pages, from and to
+  uint32_t* dst;
+  uint32_t* keys;    // [moves] keys of each; null: whole pages
+  uint32_t* rank;    // [n_pages] compact: the move of a page
+  uint32_t words;
+};
+struct PagesPools {
+  uint8_t* p[PAGES_POOLS_LAUNCH];
+};
 
 #define PAGED_ROPE_ROW 1u   // SMITH_ROPE_ROW
 #define PAGED_ROPE_HEAD 2u  // SMITH_ROPE_HEAD
@@ -21,4 +49,8 @@ enum {
   PAGED_ERR_ATT_ROWS,         // row_start's total
   PAGED_ERR_ATT_LENGTH,       // the request
   PAGED_ERR_ATT_PAGE,         // the request
+  PAGED_ERR_FORK_PARENT,      // the request
+  PAGED_ERR_FORK_LENGTH,      // the request
+  PAGED_ERR_FORK_PAGE,        // the request
+  PAGED_ERR_FORK_FREE,        // the free pages
 };

@@ -13,6 +13,7 @@
 
 #include "lanes.h"
 #include "paged.h"
+#include "paged_dev.h"
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 // rows and tables of the caller need start on no more than 4 bytes; the
@@ -23,12 +24,6 @@ __device__ __forceinline__ f32x4 load8(const float* p) { return *(const f32x4_8*
 __device__ __forceinline__ f32x4 load4(const float* p) { return *(const f32x4_any*)p; }
 __device__ __forceinline__ void store4(float* p, f32x4 v) { *(f32x4_any*)p = v; }
 
-// One 64-bit word of host-mapped memory: (code, argument), the first one kept.
-__device__ __forceinline__ void paged_err(uint64_t* __restrict__ err, uint32_t code, uint32_t arg) {
-  if (__hip_atomic_load(err, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM) == 0u)
-    __hip_atomic_store(err, ((uint64_t)arg << 32) | code, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-}
-
 template <class T>
 __device__ __forceinline__ T max64_lanes(T v) {
 #pragma unroll
@@ -36,18 +31,6 @@ __device__ __forceinline__ T max64_lanes(T v) {
     const T o = __shfl_xor(v, d);
     v = o > v ? o : v;
   }
-  return v;
-}
-// sum over the lanes up to this one: within rows of 16, then across them
-__device__ __forceinline__ uint32_t scan64_lanes(uint32_t v) {
-#define SCAN_DPP(CTRL, ROWS) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false)
-  SCAN_DPP(0x111, 0xF);  // row_shr 1, 2, 4, 8
-  SCAN_DPP(0x112, 0xF);
-  SCAN_DPP(0x114, 0xF);
-  SCAN_DPP(0x118, 0xF);
-  SCAN_DPP(0x142, 0xA);  // row_bcast 15 into rows 1 and 3, 31 into 2 and 3
-  SCAN_DPP(0x143, 0xC);
-#undef SCAN_DPP
   return v;
 }
 

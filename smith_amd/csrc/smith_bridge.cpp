@@ -83,6 +83,10 @@ struct Ctx {
   void* paged_ws = nullptr;  // partials of smith_paged_attention
   size_t paged_ws_bytes = 0;
   uint32_t* paged_cnt = nullptr;  // and the splits of a block that are done
+  void* pages_map = nullptr;      // fork and compact: the state and the map of live pages (zero between calls)
+  size_t pages_map_bytes = 0;
+  void* pages_ws = nullptr;  // and the moves
+  size_t pages_ws_bytes = 0;
   bool capturing = false;
   // set while an entry point that must not allocate runs on the static
   // scratch (its name, for the error when a region is too small)
@@ -285,6 +289,10 @@ int check_paged_err(Ctx* c) {
       "smith_paged_attention: row_start ends at %d, outside 0 .. max_rows",
       "smith_paged_attention: request %u: its length does not hold its rows, or is longer than its block table, or row_start does not ascend",
       "smith_paged_attention: request %u: a page outside the pool",
+      "smith_paged_fork: request %u: its parent is no request of the call; nothing was copied",
+      "smith_paged_fork or smith_paged_compact: request %u: its length is negative or longer than its block table; nothing was copied",
+      "smith_paged_fork or smith_paged_compact: request %u: a page outside the pool; nothing was copied",
+      "smith_paged_fork: the copies need more than the %u pages that nobody names; nothing was copied",
   };
   return fail(c, what[code < sizeof what / sizeof what[0] ? code : 0], arg);
 }
@@ -1023,6 +1031,8 @@ void smith_destroy(void* ctx) {
   if (c->amx) (void)hipFree(c->amx);
   if (c->paged_ws) (void)hipFree(c->paged_ws);
   if (c->paged_cnt) (void)hipFree(c->paged_cnt);
+  if (c->pages_map) (void)hipFree(c->pages_map);
+  if (c->pages_ws) (void)hipFree(c->pages_ws);
   for (void* r : c->retired) (void)hipFree(r);
   for (auto& r : c->recs) {
     (void)hipEventDestroy(r.a);
@@ -2526,6 +2536,156 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
   snprintf(name, sizeof name, "smith_paged_attention_%s%s_d%u%s", many ? "rows_" : "", kv_name(kv_type), dims, small ? "_s" : "");
   void* args[] = {&a};
   return launch(c, name, dim3(grid), dim3(256), args, lds);
+}
+
+// The state and map of fork and compact: as ensure(), and zero.
+static int ensure_pages_map(Ctx* c, const char* fn, size_t need) {
+  if (need <= c->pages_map_bytes) return 0;
+  if (c->capturing) return fail(c, "%s: scratch needed while capturing a graph; run the op once first", fn);
+  if (ensure(c, &c->pages_map, &c->pages_map_bytes, need)) return -1;
+  if (zero_now(c, c->pages_map, c->pages_map_bytes) == 0) return 0;
+  c->pages_map_bytes = 0;  // not to be used (and retired by the next call)
+  return -1;
+}
+
+// Pools of more than so many times 8192 pages get a launch that counts them
+constexpr uint32_t PAGES_COUNT_BLOCKS = 32;
+
+// What fork and compact have in common: checks, scratch and the first launch.
+struct PagesCall {
+  PagesTables t;
+  PagesWork w;
+  uint32_t row16, blocks;  // 16-byte units of a key, workgroups of 256 words
+  uint64_t page16;         // 16-byte units of a page
+};
+
+static int pages_begin(Ctx* c, const char* fn, PagesCall* call, uint32_t kv_type, const int32_t* lens, const int32_t* tables,
+                       const int32_t* parents, uint32_t n_req, uint32_t max_pages, uint32_t window, uint32_t sinks,
+                       uint32_t n_kv_heads, uint32_t head_dim, void* const* pools, uint32_t n_pools, uint32_t n_pages,
+                       uint32_t page_size, int32_t* new_lens, int32_t* new_tables, int32_t* free_pages, int32_t* free_count) {
+  const bool fork = parents != nullptr;
+  uint32_t shift;
+  if (!kv_name(kv_type)) return fail(c, "%s: unknown page type %u", fn, kv_type);
+  if (!n_req || n_req > PAGED_MAX_REQ) return fail(c, "%s: %u requests (1 .. %u)", fn, n_req, PAGED_MAX_REQ);
+  if (!n_kv_heads || n_kv_heads > 65535) return fail(c, "%s: %u kv heads", fn, n_kv_heads);
+  if (!head_dim || head_dim > 128 || head_dim % 8)
+    return fail(c, "%s: head_dim %u unsupported (<= 128, %% 8)", fn, head_dim);
+  if (pool_shift(c, fn, n_pages, page_size, &shift)) return -1;
+  if (!max_pages || ((uint64_t)max_pages << shift) > 0x7FFFFFFFull)
+    return fail(c, "%s: block tables of %u pages of %u keys (at least one page, less than 2^31 keys)", fn, max_pages, page_size);
+  if (sinks && !window) return fail(c, "%s: %u sinks without a window", fn, sinks);
+  if (!lens || !tables || !new_tables || !free_pages || !free_count || (fork && !new_lens))
+    return fail(c, "%s: null buffer", fn);
+  if (n_pools > PAGES_MAX_POOLS || (n_pools && !pools)) return fail(c, "%s: %u pools (up to %u)", fn, n_pools, PAGES_MAX_POOLS);
+  const uint64_t listed = smith_buffer_length(free_pages);  // 0: not a buffer of smith_alloc
+  if (listed && listed / 4 < n_pages) return fail(c, "%s: free_pages has room for %llu of %u pages", fn, (unsigned long long)(listed / 4), n_pages);
+  const uint64_t pool = pool_bytes(kv_type, n_kv_heads, head_dim, n_pages, page_size), nb = 4ull * n_req, tb = nb * max_pages;
+  if (pool / n_pages > 0xFFFFFFFFull) return fail(c, "%s: pages of %llu bytes", fn, (unsigned long long)(pool / n_pages));
+  const Range in[] = {{lens, nb}, {tables, tb}, {parents, fork ? nb : 0}};
+  const Range out[] = {{new_tables, tb}, {free_pages, 4ull * n_pages}, {free_count, 4}, {new_lens, new_lens ? nb : 0}};
+  const bool in_place = !fork && new_tables == tables;
+  for (int i = 0; i < 4; i++) {
+    for (int k = 0; k < 3; k++)
+      if (!(i == 0 && k == 1 && in_place) && overlap(out[i], in[k])) return fail(c, "%s: an output overlaps an input", fn);
+    for (int k = 0; k < i; k++)
+      if (overlap(out[i], out[k])) return fail(c, "%s: two outputs overlap", fn);
+  }
+  const void* order[PAGES_MAX_POOLS];
+  for (uint32_t k = 0; k < n_pools; k++) {
+    if (!pools[k] || (uintptr_t)pools[k] % 16) return fail(c, "%s: the page pools must be 16-byte aligned device memory", fn);
+    for (const Range& r : in)
+      if (overlap({pools[k], pool}, r)) return fail(c, "%s: a pool overlaps an input", fn);
+    for (const Range& r : out)
+      if (overlap({pools[k], pool}, r)) return fail(c, "%s: a pool overlaps an output", fn);
+    order[k] = pools[k];
+  }
+  std::sort(order, order + n_pools);
+  for (uint32_t k = 1; k < n_pools; k++)
+    if (overlap({order[k - 1], pool}, {order[k], pool})) return fail(c, "%s: two pools overlap", fn);
+  if (set_device(c)) return -1;
+
+  const uint32_t words = (n_pages + 31) / 32, blocks = (words + PAGES_THREADS - 1) / PAGES_THREADS;
+  const size_t moves = fork ? n_req : n_pages / 2 + 1;
+  const size_t n[] = {blocks > PAGES_COUNT_BLOCKS ? blocks : 0, moves, moves, fork ? moves : 0, fork ? 0 : (size_t)n_pages};
+  size_t total = 0;
+  for (size_t k : n) total += k;
+  if (ensure_pages_map(c, fn, (16 + (size_t)words) * 4) || ensure(c, &c->pages_ws, &c->pages_ws_bytes, total * 4)) return -1;
+  uint32_t* at[5];
+  uint32_t* next = (uint32_t*)c->pages_ws;
+  for (int k = 0; k < 5; k++) {
+    at[k] = n[k] ? next : nullptr;
+    next += n[k];
+  }
+  call->t = {lens, tables, parents, n_req, max_pages, n_pages, shift, window, sinks};
+  call->w = {(uint32_t*)c->pages_map + 16, (uint32_t*)c->pages_map, at[0], at[1], at[2], at[3], at[4], words};
+  call->row16 = head_dim * (kv_type == SMITH_KV_F32 ? 4 : 2) / 16;
+  call->page16 = pool / n_pages / 16;
+  call->blocks = blocks;
+  // a request's entries over as many workgroups as fill the card, 256 entries each at least
+  const uint32_t split = std::max<uint32_t>(1, std::min<uint32_t>(2048 / n_req, (max_pages + PAGES_THREADS - 1) / PAGES_THREADS));
+  uint64_t* perr = c->paged_err_dev();
+  int32_t* to = fork ? new_tables : nullptr;
+  void* args[] = {&call->t, &call->w, &to, &perr};
+  if (launch(c, "smith_pages_mark", dim3(n_req, split), dim3(PAGES_THREADS), args)) return -1;
+  if (call->w.counts) {
+    void* cargs[] = {&call->w};
+    if (launch(c, "smith_pages_count", dim3(blocks), dim3(PAGES_THREADS), cargs)) return -1;
+  }
+  return 0;
+}
+
+// The moves in all pools; the last launch clears the map.
+static int pages_end(Ctx* c, PagesCall* call, uint64_t moves, uint32_t n_kv_heads, void* const* pools, uint32_t n_pools) {
+  const uint64_t chunks = (call->page16 + 4 * PAGES_THREADS - 1) / (4 * PAGES_THREADS);
+  uint32_t k0 = 0;
+  do {
+    PagesPools some = {};
+    uint32_t n = std::min(n_pools - k0, PAGES_POOLS_LAUNCH);
+    for (uint32_t k = 0; k < n; k++) some.p[k] = (uint8_t*)pools[k0 + k];
+    k0 += n;
+    uint32_t clear = k0 == n_pools;
+    const uint32_t grid = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(2048, moves * n * chunks));
+    void* args[] = {&some, &call->w, &n, &n_kv_heads, &call->row16, &call->t.shift, &clear};
+    if (launch(c, "smith_pages_move", dim3(grid), dim3(PAGES_THREADS), args)) return -1;
+  } while (k0 < n_pools);
+  return 0;
+}
+
+int smith_paged_fork(void* ctx, uint32_t kv_type, const int32_t* lens, const int32_t* tables, const int32_t* parents,
+                     uint32_t n_req, uint32_t max_pages, uint32_t window, uint32_t sinks, uint32_t n_kv_heads,
+                     uint32_t head_dim, void* const* pools, uint32_t n_pools, uint32_t n_pages, uint32_t page_size,
+                     int32_t* new_lens, int32_t* new_tables, int32_t* free_pages, int32_t* free_count) {
+  Ctx* c = (Ctx*)ctx;
+  if (!c) return -1;
+  static const char fn[] = "smith_paged_fork";
+  if (!parents) return fail(c, "%s: null buffer", fn);
+  PagesCall call;
+  if (pages_begin(c, fn, &call, kv_type, lens, tables, parents, n_req, max_pages, window, sinks, n_kv_heads, head_dim,
+                  pools, n_pools, n_pages, page_size, new_lens, new_tables, free_pages, free_count))
+    return -1;
+  uint64_t* perr = c->paged_err_dev();
+  void* args[] = {&call.t, &call.w, &new_lens, &new_tables, &free_pages, &free_count, &perr};
+  if (launch(c, "smith_pages_fork", dim3(call.blocks), dim3(PAGES_THREADS), args)) return -1;
+  return pages_end(c, &call, n_req, n_kv_heads, pools, n_pools);
+}
+
+int smith_paged_compact(void* ctx, uint32_t kv_type, const int32_t* lens, const int32_t* tables, uint32_t n_req,
+                        uint32_t max_pages, uint32_t window, uint32_t sinks, uint32_t n_kv_heads, uint32_t head_dim,
+                        void* const* pools, uint32_t n_pools, uint32_t n_pages, uint32_t page_size, int32_t* new_tables,
+                        int32_t* free_pages, int32_t* free_count) {
+  Ctx* c = (Ctx*)ctx;
+  if (!c) return -1;
+  static const char fn[] = "smith_paged_compact";
+  PagesCall call;
+  if (pages_begin(c, fn, &call, kv_type, lens, tables, nullptr, n_req, max_pages, window, sinks, n_kv_heads, head_dim,
+                  pools, n_pools, n_pages, page_size, nullptr, new_tables, free_pages, free_count))
+    return -1;
+  void* args[] = {&call.w, &n_pages, &free_pages, &free_count};
+  if (launch(c, "smith_pages_line", dim3(call.blocks), dim3(PAGES_THREADS), args)) return -1;
+  const uint32_t split = std::max<uint32_t>(1, std::min<uint32_t>(2048 / n_req, (max_pages + PAGES_THREADS - 1) / PAGES_THREADS));
+  void* rargs[] = {&call.t, &call.w, &free_count, &new_tables};
+  if (launch(c, "smith_pages_remap", dim3(n_req, split), dim3(PAGES_THREADS), rargs)) return -1;
+  return pages_end(c, &call, n_pages / 2, n_kv_heads, pools, n_pools);
 }
 
 int smith_set_i32(void* ctx, int32_t* p, int32_t v) {

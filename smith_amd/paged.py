@@ -10,10 +10,17 @@ fill.  A step of any mix of prompts, chunks and decode rows is
     pagedAppend     rotary positions, then k and v into their slots   (per layer)
     pagedAttention  the rows' attention over the pages                (per layer)
 
+and between steps
+
+    pagedFork       requests go on from others, whose full pages they share
+    pagedCompact    the live pages at the pools' low end
+
 on Tensors (one call into libsmith.so each, include/smith.h states what each
 reads and writes).  PagedCache keeps the pools, tables and lengths of a model's
 requests on the device; forwardPagedStep of a loaded GGUF model runs on it.
 """
+import ctypes
+
 import numpy as np
 
 from . import device
@@ -96,6 +103,54 @@ def pagedAttention(q, lens, tables, kPages, vPages, rowStart=None, scale=0.0, ou
         rowStart.buffer if rowStart is not None else None, lens.buffer, tables.buffer, n, tables.shape[1], width // hd,
         nKV, hd, scale, kPages.buffer, vPages.buffer, nPages, P, out.buffer, width), "pagedAttention")
     return out
+
+
+def _all_pools(pools, what):
+    """(shape, dtype, host array of the addresses) of pools that are alike."""
+    pools = list(pools)
+    if not pools or pools[0].dtype not in KV_TYPES or len(pools[0].shape) != 4:
+        raise ValueError("%s: pools are [pages, kvHeads, pageSize, headDim] of f32, f16 or bf16" % what)
+    for t in pools:
+        _want(t, pools[0].shape, pools[0].dtype, what + ": pools")
+    return pools[0].shape, pools[0].dtype, (ctypes.c_void_p * len(pools))(*[t.buffer for t in pools])
+
+
+def pagedFork(lens, tables, parents, pools, window=0, sinks=0, newTables=None):
+    """Request b goes on from request parents[b] (itself, another, -1: none) as it
+    was, sharing its full pages; a partly filled page stays with the first and is
+    copied for the others in all `pools` (smith_paged_fork).  lens, parents [n] and
+    tables [n, maxPages] i32.  Returns {lens [n], tables, freePages [pages],
+    freeCount [1]}, i32; newTables is the tensor that tables are written to."""
+    n = lens.shape[0]
+    _want(lens, [n], "i32", "pagedFork: lens")
+    _want(parents, [n], "i32", "pagedFork: parents")
+    _want(tables, [n, tables.shape[-1]], "i32", "pagedFork: tables")
+    shape, dtype, pointers = _all_pools(pools, "pagedFork")
+    if newTables is None:
+        newTables = T.create(tables.shape, "i32")
+    _want(newTables, tables.shape, "i32", "pagedFork: newTables")
+    new = {"lens": T.create([n], "i32"), "tables": newTables, "freePages": T.create([shape[0]], "i32"),
+           "freeCount": T.create([1], "i32")}
+    device.check(device.lib.smith_paged_fork(
+        device.ops_ctx(), KV_TYPES[dtype], lens.buffer, tables.buffer, parents.buffer, n, tables.shape[1], window, sinks,
+        shape[1], shape[3], pointers, len(pointers), shape[0], shape[2], new["lens"].buffer, newTables.buffer,
+        new["freePages"].buffer, new["freeCount"].buffer), "pagedFork")
+    return new
+
+
+def pagedCompact(lens, tables, pools, window=0, sinks=0):
+    """The live pages moved to the pools' low end, in all `pools`; `tables` name
+    them there (smith_paged_compact).  Returns {freePages [pages], freeCount [1]}."""
+    n = lens.shape[0]
+    _want(lens, [n], "i32", "pagedCompact: lens")
+    _want(tables, [n, tables.shape[-1]], "i32", "pagedCompact: tables")
+    shape, dtype, pointers = _all_pools(pools, "pagedCompact")
+    new = {"freePages": T.create([shape[0]], "i32"), "freeCount": T.create([1], "i32")}
+    device.check(device.lib.smith_paged_compact(
+        device.ops_ctx(), KV_TYPES[dtype], lens.buffer, tables.buffer, n, tables.shape[1], window, sinks, shape[1],
+        shape[3], pointers, len(pointers), shape[0], shape[2], tables.buffer, new["freePages"].buffer,
+        new["freeCount"].buffer), "pagedCompact")
+    return new
 
 
 def _release(tensors):
