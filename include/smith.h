@@ -494,6 +494,25 @@ int smith_paged_compact(void* ctx, uint32_t kv_type, const int32_t* lens, const 
                         void* const* pools, uint32_t n_pools, uint32_t n_pages, uint32_t page_size, int32_t* new_tables,
                         int32_t* free_pages, int32_t* free_count);
 
+/* ---- scores ----
+ * Of rows of logits x (row stride ld elements) the distribution p = e^x / sum e^x:
+ * logprobs [rows][given] are log p of the row's given tokens ([rows][given]; -1:
+ * no token, its number is 0), entropy [rows] is -sum p log p, and top_ids,
+ * top_logprobs [rows][top] are the top <= 64 alternatives, largest first, of equal
+ * ones the lower number first.  given and top may be 0 and their buffers, and
+ * entropy, NULL.  Sums in f32.  A logit of -inf has p = 0.  A row with a NaN, or
+ * whose maximum is not finite, has no distribution: its numbers are NaN (its
+ * top_ids those of its largest elements that are numbers, -1 behind them).
+ * Outputs overlap no input and each other.  Enqueued, and can be captured once it
+ * has run with the same sizes.  A token outside the vocabulary gets NaN, and the
+ * next synchronising call returns -1 with the first such row in smith_last_error. */
+#define SMITH_F32 SMITH_KV_F32
+#define SMITH_F16 SMITH_KV_F16
+#define SMITH_BF16 SMITH_KV_BF16
+int smith_logprobs(void* ctx, uint32_t type, const void* logits, uint32_t ld, uint32_t rows, uint32_t vocab,
+                   const int32_t* tokens, uint32_t given, uint32_t top, float* logprobs, float* entropy,
+                   int32_t* top_ids, float* top_logprobs);
+
 /* ---- HIP graphs: capture the context stream, replay it ----
  * Ops enqueued between begin and end are recorded, not run; their scratch
  * must already be allocated (run the same ops once before capturing).

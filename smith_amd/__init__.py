@@ -11,6 +11,7 @@ from .paged import (ROPE_HEAD, ROPE_NONE, ROPE_ROW, PagedCache, createPagedCache
                     pagedCompact, pagedFork, pagedPlan)
 from .quantize import (GROUP_BYTES, GROUP_SIZE, Q8_BLOCK_BYTES, Q8_BLOCK_SIZE, QuantizedWeight, matmulQ4,
                        matmulQ8, quantizeQ4, quantizeQ8)
+from .score import logProbs
 from .tensor import Tensor, create, ones, randn, tensor, to_array, zeros
 
 toArray = to_array
@@ -19,5 +20,6 @@ __all__ = [
     "quantizeQ4", "matmulQ4", "matmulQ8", "quantizeQ8", "QuantizedWeight",
     "GROUP_SIZE", "GROUP_BYTES", "Q8_BLOCK_SIZE", "Q8_BLOCK_BYTES",
     "pagedPlan", "pagedAppend", "pagedAttention", "pagedFork", "pagedCompact", "PagedCache", "createPagedCache", "ROPE_NONE", "ROPE_ROW", "ROPE_HEAD",
+    "logProbs",
     "Tensor", "create", "tensor", "zeros", "ones", "randn", "to_array", "toArray",
 ]

@@ -5,6 +5,7 @@
   smith_amd/lib/smith_gemm.hsaco      (the prefill MFMA GEMM, same flags)
   smith_amd/lib/smith_paged.hsaco     (the paged KV cache's kernels, same flags)
   smith_amd/lib/smith_pages.hsaco     (fork and compact of its pages, same flags)
+  smith_amd/lib/smith_score.hsaco     (log probabilities, same flags)
   smith_amd/lib/libsmith.so           hipcc -x hip: host code against libamdhip64 (+ static device scratch)
   smith_amd/lib/smith_bench.hsaco     bench-only floor kernels (bench_floor.hip)
   smith_amd/lib/libsmith_bench.so     bench-only host helper that times them (bench_floor_host.cpp)
@@ -24,6 +25,7 @@ HSACO_LLAMA = os.path.join(LIBDIR, "smith_llama.hsaco")
 HSACO_GEMM = os.path.join(LIBDIR, "smith_gemm.hsaco")
 HSACO_PAGED = os.path.join(LIBDIR, "smith_paged.hsaco")
 HSACO_PAGES = os.path.join(LIBDIR, "smith_pages.hsaco")
+HSACO_SCORE = os.path.join(LIBDIR, "smith_score.hsaco")
 LIBSMITH = os.path.join(LIBDIR, "libsmith.so")
 # bench-only: the floor kernels bench.py times beside the product's steps
 HSACO_BENCH = os.path.join(LIBDIR, "smith_bench.hsaco")
@@ -47,7 +49,7 @@ def _kernel_cmds():
              "-c", os.path.join(CSRC, src), "-o", dst]
             for src, dst in (("smith_kernels.hip", HSACO), ("llama_kernels.hip", HSACO_LLAMA),
                              ("gemm_kernels.hip", HSACO_GEMM), ("paged_kernels.hip", HSACO_PAGED),
-                             ("pages_kernels.hip", HSACO_PAGES),
+                             ("pages_kernels.hip", HSACO_PAGES), ("score_kernels.hip", HSACO_SCORE),
                              ("bench_floor.hip", HSACO_BENCH))]
 
 

@@ -1,4 +1,4 @@
-// paged.h -- what the paged cache's kernels and the bridge share: limits,
+// paged.h -- what the paged cache's and smith_logprobs' kernels and the bridge share: limits,
 // arguments and the codes of what a kernel finds wrong in device memory.
 #pragma once
 #include <stdint.h>
@@ -36,6 +36,25 @@ struct PagesPools {
   uint8_t* p[PAGES_POOLS_LAUNCH];
 };
 
+// log probabilities: threads of a workgroup, elements that a wave takes at once, most splits
+// of a row (a lane each where they are joined) and top alternatives (a lane each)
+#define SCORE_THREADS 256u
+#define SCORE_WAVE_CHUNK 1024u
+#define SCORE_MAX_SPLITS 64u
+#define SCORE_MAX_TOP 64u
+struct ScoreArgs {
+  const void* logits;
+  const int32_t* tokens;
+  float* logprobs;
+  float* entropy;
+  int32_t* top_ids;
+  float* top_logprobs;
+  uint64_t* parts;     // [rows][splits][2 + top]
+  uint32_t* counters;  // splits of a row that are done; zero between calls
+  uint64_t* err;
+  uint32_t ld, vocab, given, top, splits, per_split, row0;
+};
+
 #define PAGED_ROPE_ROW 1u   // SMITH_ROPE_ROW
 #define PAGED_ROPE_HEAD 2u  // SMITH_ROPE_HEAD
 
@@ -53,4 +72,5 @@ enum {
   PAGED_ERR_FORK_LENGTH,      // the request
   PAGED_ERR_FORK_PAGE,        // the request
   PAGED_ERR_FORK_FREE,        // the free pages
+  PAGED_ERR_SCORE_TOKEN,      // the row
 };

@@ -1,0 +1,300 @@
+// score_kernels.hip -- gfx950 kernels of smith_logprobs (smith_score.hsaco): log
+// probabilities of given tokens, entropy and top alternatives of rows of logits.
+//
+// Of a row x with m = max x, d = x - m, l = sum e^d and s = sum e^d d:
+//   log p(t) = d_t - log l,   entropy = -sum p log p = log l - s / l,
+// in one pass: a thread keeps (m, l, s) of what it has seen, and when m grows to M
+//   l' = e^(m - M) l,   s' = e^(m - M) (s + (m - M) l).
+//
+// The top k are found in the same pass.  An element is a 64-bit key: its value,
+// ordered as a whole number, above the complement of its place, so that keys are
+// all different and the larger one is the larger value or, of equal ones, the
+// lower place.  A wave keeps the 64 best of its elements sorted over its lanes;
+// an element goes in if it is above the k-th, which after a few thousand elements
+// is rare, so that the pass costs a comparison with the maximum of 16.  Lists are
+// joined by bitonic merges: the result does not depend on who comes first.
+//
+// Bound by memory: the logits are read once.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "lanes.h"
+#include "paged.h"
+#include "paged_dev.h"
+
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
+
+#define LOG2E 1.44269504088896341f
+#define THREADS SCORE_THREADS
+#define WAVES (SCORE_THREADS / 64)
+#define PER 16                    // elements of a thread to a chunk
+#define CHUNK SCORE_WAVE_CHUNK    // of a wave
+
+struct LogitsF32 {
+  typedef float T;
+  static constexpr uint32_t WIDTH = 4;  // elements to a 16-byte load
+  static __device__ __forceinline__ void load(const T* p, float* x) {
+    const f32x4_any v = *(const f32x4_any*)p;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = v[i];
+  }
+  static __device__ __forceinline__ float up(T v) { return v; }
+};
+template <class T_>
+struct Logits16 {
+  typedef T_ T;
+  static constexpr uint32_t WIDTH = 8;
+  static __device__ __forceinline__ void load(const T* p, float* x) {
+    const u32x4_2 v = *(const u32x4_2*)p;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      x[2 * i] = (float)__builtin_bit_cast(T, (uint16_t)v[i]);
+      x[2 * i + 1] = (float)__builtin_bit_cast(T, (uint16_t)(v[i] >> 16));
+    }
+  }
+  static __device__ __forceinline__ float up(T v) { return (float)v; }
+};
+
+// ---- keys ----
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t place) {
+  const uint32_t u = __float_as_uint(x + 0.0f);  // -0 is 0
+  return ((uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32) | ~place;
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+}
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t k, int d) {
+  return ((uint64_t)(uint32_t)__shfl_xor((int)(k >> 32), d) << 32) | (uint32_t)__shfl_xor((int)k, d);
+}
+__device__ __forceinline__ uint64_t readlane64(uint64_t k, uint32_t lane) {
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), (int)lane) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)k, (int)lane);
+}
+// the larger (or smaller) of a lane's key and its partner's
+__device__ __forceinline__ uint64_t exchange(uint64_t k, int d, bool larger) {
+  const uint64_t o = shfl_xor64(k, d);
+  return (o > k) == larger ? o : k;
+}
+// a bitonic sequence over the lanes, sorted: the largest in lane 0
+__device__ __forceinline__ uint64_t sort_bitonic(uint64_t k, uint32_t lane) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) k = exchange(k, d, !(lane & d));
+  return k;
+}
+__device__ __forceinline__ uint64_t sort64(uint64_t k, uint32_t lane) {
+#pragma unroll
+  for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+    for (int d = n >> 1; d; d >>= 1) k = exchange(k, d, !(lane & d) == !(lane & n));
+  return sort_bitonic(k, lane);
+}
+// the 64 largest of two sorted lists, sorted
+__device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b, uint32_t lane) {
+  const uint64_t o = ((uint64_t)(uint32_t)__shfl((int)(b >> 32), (int)(63 - lane)) << 32) |
+                     (uint32_t)__shfl((int)b, (int)(63 - lane));
+  return sort_bitonic(a > o ? a : o, lane);
+}
+// key c (the same in all lanes) into a sorted list
+__device__ __forceinline__ uint64_t insert(uint64_t list, uint64_t c, uint32_t lane) {
+  const uint32_t at = (uint32_t)__popcll(__ballot(list > c));
+  const uint64_t up = ((uint64_t)dpp_u32<0x138>((uint32_t)(list >> 32)) << 32) | dpp_u32<0x138>((uint32_t)list);  // lane - 1's
+  return lane < at ? list : lane == at ? c : up;
+}
+
+// ---- (m, l, s) ----
+struct Sums {
+  float m, l, s;
+};
+__device__ __forceinline__ Sums moved(Sums a, float M) {  // to a maximum that is no lower
+  const bool some = a.m != -__builtin_inff();
+  const float d = a.m - M, f = some ? __builtin_amdgcn_exp2f(d * LOG2E) : 0.f;
+  return {M, f * a.l, some ? f * (f == 0.f ? 0.f : __builtin_fmaf(d, a.l, a.s)) : 0.f};
+}
+__device__ __forceinline__ Sums over_lanes(Sums a) {
+  float M = a.m;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
+  a = moved(a, M);
+  return {M, sum64_lanes(a.l), sum64_lanes(a.s)};
+}
+
+// a partial's words cross from one XCD's L2 to another's
+__device__ __forceinline__ void put64(uint64_t* p, uint64_t v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t get64(uint64_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  return ((uint64_t)__float_as_uint(b) << 32) | __float_as_uint(a);
+}
+
+template <class L>
+__device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
+  typedef typename L::T T;
+  constexpr uint32_t LOADS = PER / L::WIDTH;
+  __shared__ uint64_t s_list[WAVES][64];
+  __shared__ Sums s_sums[WAVES];
+  __shared__ uint32_t s_last;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  const uint32_t row = a.row0 + blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const T* x = (const T*)a.logits + (size_t)row * a.ld;
+  // this split's chunks, to the waves in turn
+  const uint32_t begin = split * a.per_split, end = a.vocab - begin < a.per_split ? a.vocab : begin + a.per_split;
+
+  Sums sum = {-__builtin_inff(), 0.f, 0.f};
+  uint64_t list = 0, least = 0;  // sorted over the lanes; its k-th
+  float least_value = -__builtin_inff();
+  auto load = [&](uint32_t at, float (&v)[PER]) {
+    if (at + CHUNK <= end) {
+#pragma unroll
+      for (uint32_t k = 0; k < LOADS; k++) L::load(x + at + k * 64 * L::WIDTH + lane * L::WIDTH, v + k * L::WIDTH);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < PER; i++) {
+        const uint32_t e = at + i / L::WIDTH * 64 * L::WIDTH + lane * L::WIDTH + i % L::WIDTH;
+        v[i] = e < end ? L::up(x[e]) : -__builtin_inff();  // weighs nothing
+      }
+    }
+  };
+  // the chunk's elements above the list's k-th
+  auto pick = [&](uint32_t at, const float (&v)[PER]) {
+    uint64_t below = ~0ull;  // the lane's elements from this key on are through
+    for (;;) {
+      uint64_t best = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < PER; i++) {
+        const uint32_t e = at + i / L::WIDTH * 64 * L::WIDTH + lane * L::WIDTH + i % L::WIDTH;
+        const uint64_t k = key_of(v[i], e);
+        if (v[i] == v[i] && e < end && k < below && k > best) best = k;
+      }
+      if (best <= least) best = 0;
+      uint64_t there = __ballot(best != 0);
+      if (!there) break;
+      if (__popcll(there) > 12) {
+        list = merge64(list, sort64(best, lane), lane);
+        least = readlane64(list, a.top - 1);
+      } else {
+        do {
+          const uint32_t from = (uint32_t)__ffsll((unsigned long long)there) - 1;
+          there &= there - 1;
+          const uint64_t c = readlane64(best, from);
+          if (c > least) {
+            list = insert(list, c, lane);
+            least = readlane64(list, a.top - 1);
+          }
+        } while (there);
+      }
+      below = best ? best : 0;
+    }
+    least_value = least ? value_of(least) : -__builtin_inff();
+  };
+  float v[PER], next[PER];
+  uint32_t at = begin + w * CHUNK;
+  if (at < end) load(at, v);
+  for (; at < end; at += WAVES * CHUNK) {
+    const bool more = at + WAVES * CHUNK < end;
+    if (more) load(at + WAVES * CHUNK, next);
+    float mx = v[0];
+#pragma unroll
+    for (uint32_t i = 1; i < PER; i++) mx = fmaxf(mx, v[i]);
+    if (__any(mx > sum.m)) sum = moved(sum, fmaxf(mx, sum.m));
+    const float m = sum.m == -__builtin_inff() ? 0.f : sum.m;
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) {
+      const float d = v[i] - m, e = __builtin_amdgcn_exp2f(d * LOG2E);
+      sum.l += e;
+      sum.s = __builtin_fmaf(e, fmaxf(d, -1000.f), sum.s);  // 0 of -inf
+    }
+    if (a.top && __any(least ? mx > least_value : true)) pick(at, v);
+    if (more)
+#pragma unroll
+      for (uint32_t i = 0; i < PER; i++) v[i] = next[i];
+  }
+
+  // ---- the waves', then the splits' ----
+  sum = over_lanes(sum);
+  s_list[w][lane] = list;
+  if (lane == 0) s_sums[w] = sum;
+  __syncthreads();
+  auto join = [&](Sums b) {
+    const float M = fmaxf(sum.m, b.m);
+    const Sums p = moved(sum, M), q = moved(b, M);
+    sum = {M, p.l + q.l, p.s + q.s};
+  };
+  if (w == 0) {
+    for (uint32_t k = 1; k < WAVES; k++) {
+      if (a.top) list = merge64(list, s_list[k][lane], lane);
+      join(s_sums[k]);
+    }
+  }
+  if (a.splits > 1) {
+    // per split: (m, l), (s, -), the keys
+    const size_t stride = a.top + 2;
+    uint64_t* all = a.parts + (size_t)(row - a.row0) * a.splits * stride;
+    if (w == 0) {
+      uint64_t* mine = all + split * stride;
+      if (lane < a.top) put64(mine + 2 + lane, list);
+      if (lane == 0) {
+        put64(mine, two(sum.m, sum.l));
+        put64(mine + 1, two(sum.s, 0.f));
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) {
+      uint32_t* done = a.counters + (row - a.row0);
+      s_last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.splits - 1;
+      if (s_last) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!s_last) return;
+    list = 0;
+    if (a.top) {
+      for (uint32_t k = w; k < a.splits; k += WAVES)
+        list = merge64(list, lane < a.top ? get64(all + k * stride + 2 + lane) : 0ull, lane);
+      s_list[w][lane] = list;
+    }
+    sum = {-__builtin_inff(), 0.f, 0.f};
+    if (lane < a.splits) {  // at most 64
+      const uint64_t ml = get64(all + lane * stride), s = get64(all + lane * stride + 1);
+      sum = {__uint_as_float((uint32_t)ml), __uint_as_float((uint32_t)(ml >> 32)), __uint_as_float((uint32_t)s)};
+    }
+    sum = over_lanes(sum);
+    __syncthreads();
+    if (w == 0 && a.top)
+      for (uint32_t k = 1; k < WAVES; k++) list = merge64(list, s_list[k][lane], lane);
+  }
+  if (w) return;
+  // a row without a finite maximum has no distribution
+  const float nan = __builtin_nanf("");
+  const bool fine = fabsf(sum.m) < __builtin_inff();
+  const float log_l = fine ? logf(sum.l) : nan;
+  if (a.entropy && lane == 0) a.entropy[row] = log_l - sum.s / sum.l;
+  if (lane < a.top) {
+    const size_t to = (size_t)row * a.top + lane;
+    a.top_ids[to] = list ? (int32_t)~(uint32_t)list : -1;
+    a.top_logprobs[to] = list ? value_of(list) - sum.m - log_l : nan;
+  }
+  for (uint32_t k = lane; k < a.given; k += 64) {
+    const size_t to = (size_t)row * a.given + k;
+    const int32_t t = a.tokens[to];
+    float p = 0.f;
+    if (t != -1) {
+      const bool in = (uint32_t)t < a.vocab;
+      if (!in) paged_err(a.err, PAGED_ERR_SCORE_TOKEN, row);
+      p = in ? L::up(x[t]) - sum.m - log_l : nan;
+    }
+    a.logprobs[to] = p;
+  }
+}
+
+#define DEF_LOGPROBS(TYPE, L)                                                                          \
+  extern "C" __global__ __launch_bounds__(THREADS) void smith_logprobs_##TYPE(ScoreArgs a) { \
+    logprobs_body<L>(a);                                                                               \
+  }
+DEF_LOGPROBS(f32, LogitsF32)
+DEF_LOGPROBS(f16, Logits16<_Float16>)
+DEF_LOGPROBS(bf16, Logits16<__bf16>)

@@ -87,6 +87,9 @@ struct Ctx {
   size_t pages_map_bytes = 0;
   void* pages_ws = nullptr;  // and the moves
   size_t pages_ws_bytes = 0;
+  void* score_ws = nullptr;  // partials of smith_logprobs
+  size_t score_ws_bytes = 0;
+  uint32_t* score_cnt = nullptr;  // and the splits of a row that are done
   bool capturing = false;
   // set while an entry point that must not allocate runs on the static
   // scratch (its name, for the error when a region is too small)
@@ -293,6 +296,7 @@ int check_paged_err(Ctx* c) {
       "smith_paged_fork or smith_paged_compact: request %u: its length is negative or longer than its block table; nothing was copied",
       "smith_paged_fork or smith_paged_compact: request %u: a page outside the pool; nothing was copied",
       "smith_paged_fork: the copies need more than the %u pages that nobody names; nothing was copied",
+      "smith_logprobs: row %u: a token outside the vocabulary",
   };
   return fail(c, what[code < sizeof what / sizeof what[0] ? code : 0], arg);
 }
@@ -1033,6 +1037,8 @@ void smith_destroy(void* ctx) {
   if (c->paged_cnt) (void)hipFree(c->paged_cnt);
   if (c->pages_map) (void)hipFree(c->pages_map);
   if (c->pages_ws) (void)hipFree(c->pages_ws);
+  if (c->score_ws) (void)hipFree(c->score_ws);
+  if (c->score_cnt) (void)hipFree(c->score_cnt);
   for (void* r : c->retired) (void)hipFree(r);
   for (auto& r : c->recs) {
     (void)hipEventDestroy(r.a);
@@ -2686,6 +2692,63 @@ int smith_paged_compact(void* ctx, uint32_t kv_type, const int32_t* lens, const 
   void* rargs[] = {&call.t, &call.w, &free_count, &new_tables};
   if (launch(c, "smith_pages_remap", dim3(n_req, split), dim3(PAGES_THREADS), rargs)) return -1;
   return pages_end(c, &call, n_pages / 2, n_kv_heads, pools, n_pools);
+}
+
+// ---------------- log probabilities ----------------
+// Workgroups that a call wants: rows of a text are cut until there are so many.
+constexpr uint32_t SCORE_TARGET = 1024;
+
+int smith_logprobs(void* ctx, uint32_t type, const void* logits, uint32_t ld, uint32_t rows, uint32_t vocab,
+                   const int32_t* tokens, uint32_t given, uint32_t top, float* logprobs, float* entropy,
+                   int32_t* top_ids, float* top_logprobs) {
+  Ctx* c = (Ctx*)ctx;
+  if (!c) return -1;
+  static const char fn[] = "smith_logprobs";
+  if (!kv_name(type)) return fail(c, "%s: unknown type of logits %u", fn, type);
+  if (!vocab || vocab > 0x7FFFFFFFu) return fail(c, "%s: a vocabulary of %u", fn, vocab);
+  if (ld < vocab) return fail(c, "%s: row stride %u for rows of %u logits", fn, ld, vocab);
+  if (rows > 0x7FFFFFFFu || given > 0x7FFFFFFFu) return fail(c, "%s: %u rows, %u tokens each", fn, rows, given);
+  if (top > SCORE_MAX_TOP || top > vocab)
+    return fail(c, "%s: %u top alternatives (up to %u, and the vocabulary)", fn, top, SCORE_MAX_TOP);
+  if (!rows) return 0;
+  if (!logits || (given && (!tokens || !logprobs)) || (top && (!top_ids || !top_logprobs)))
+    return fail(c, "%s: null buffer", fn);
+  const uint64_t e = type == SMITH_F32 ? 4 : 2, gb = 4ull * rows * given, kb = 4ull * rows * top;
+  if ((uintptr_t)logits % e) return fail(c, "%s: logits that are not aligned", fn);
+  const Range in[] = {{logits, e * ((uint64_t)(rows - 1) * ld + vocab)}, {tokens, gb}};
+  const Range out[] = {{logprobs, gb}, {entropy, entropy ? 4ull * rows : 0}, {top_ids, kb}, {top_logprobs, kb}};
+  for (int i = 0; i < 4; i++) {
+    for (const Range& r : in)
+      if (overlap(out[i], r)) return fail(c, "%s: an output overlaps an input", fn);
+    for (int k = 0; k < i; k++)
+      if (overlap(out[i], out[k])) return fail(c, "%s: two outputs overlap", fn);
+  }
+  if (set_device(c)) return -1;
+  // whole chunks of the workgroup to a split, as even as they go
+  const uint32_t chunk = SCORE_WAVE_CHUNK * (SCORE_THREADS / 64), chunks = (vocab + chunk - 1) / chunk;
+  const uint32_t want = std::min({SCORE_MAX_SPLITS, chunks, (SCORE_TARGET + rows - 1) / rows});
+  const uint32_t per = (chunks + want - 1) / want, splits = (chunks + per - 1) / per;
+  if (splits > 1) {
+    if (ensure(c, &c->score_ws, &c->score_ws_bytes, (size_t)rows * splits * (2 + top) * 8)) return -1;
+    if (!c->score_cnt) {
+      if (c->capturing) return fail(c, "%s: counters needed while capturing a graph; run the op once first", fn);
+      HIPCHK(c, hipMalloc((void**)&c->score_cnt, SCORE_TARGET * sizeof(uint32_t)));
+      c->allocated += SCORE_TARGET * sizeof(uint32_t);
+      if (zero_now(c, c->score_cnt, SCORE_TARGET * sizeof(uint32_t))) return -1;
+    }
+  }
+  char name[32];
+  snprintf(name, sizeof name, "smith_logprobs_%s", kv_name(type));
+  // a grid holds less than 2^32 threads
+  const uint32_t most = 1u << 23;
+  for (uint32_t r0 = 0; r0 < rows; r0 += most) {
+    const uint32_t n = std::min(rows - r0, most);
+    ScoreArgs a = {logits, tokens, logprobs, entropy, top_ids, top_logprobs, (uint64_t*)c->score_ws, c->score_cnt,
+                   c->paged_err_dev(), ld, vocab, given, top, splits, per * chunk, r0};
+    void* args[] = {&a};
+    if (launch(c, name, dim3(n * splits), dim3(SCORE_THREADS), args)) return -1;
+  }
+  return 0;
 }
 
 int smith_set_i32(void* ctx, int32_t* p, int32_t v) {

@@ -17,6 +17,7 @@ LLAMA_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_llama.hsaco")
 GEMM_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_gemm.hsaco")
 PAGED_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_paged.hsaco")
 PAGES_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_pages.hsaco")
+SCORE_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_score.hsaco")
 
 SHARED = 0
 PRIVATE = 1
@@ -128,6 +129,7 @@ SYMBOLS = {
                                 _U32, _P, _P, _P, _P]),
     "smith_paged_compact": (_INT, [_P, _U32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, ctypes.POINTER(_P), _U32, _U32,
                                    _U32, _P, _P, _P]),
+    "smith_logprobs": (_INT, [_P, _U32, _P, _U32, _U32, _U32, _P, _U32, _U32, _P, _P, _P, _P]),
     "smith_graph_begin": (_INT, [_P]),
     "smith_graph_end": (_P, [_P]),
     "smith_graph_launch": (_INT, [_P, _P]),
@@ -199,7 +201,7 @@ def shader_lib():
                                % (CODE_OBJECT_PATH, lib.smith_last_error(c).decode()))
         _library = lp
         for path in (LLAMA_CODE_OBJECT_PATH, GEMM_CODE_OBJECT_PATH, PAGED_CODE_OBJECT_PATH,
-                     PAGES_CODE_OBJECT_PATH):
+                     PAGES_CODE_OBJECT_PATH, SCORE_CODE_OBJECT_PATH):
             if not lib.smith_load_library(c, path.encode()):
                 raise RuntimeError("smith: failed to load code object at %s: %s"
                                    % (path, lib.smith_last_error(c).decode()))
