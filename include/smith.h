@@ -454,6 +454,34 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
                           const void* kpages, const void* vpages, uint32_t n_pages, uint32_t page_size, float* out,
                           uint32_t ld_out);
 
+/* smith_paged_attention of rows that see some of their keys: the row at position
+ * p those of p - window + 1 .. p, and of the first `sinks`.  window >= 1; windows
+ * and sinks longer than a request are fine.  Pages that no row of the call sees a
+ * key of may be gone: their entries in tables hold anything, and keys that a row
+ * does not see too.  For the rest as smith_paged_attention, also which kernel
+ * runs; the work is that of the keys that are seen. */
+int smith_paged_attention_window(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
+                                 const int32_t* row_start, const int32_t* lens, const int32_t* tables, uint32_t n_req,
+                                 uint32_t max_pages, uint32_t window, uint32_t sinks, uint32_t n_heads,
+                                 uint32_t n_kv_heads, uint32_t head_dim, float scale, const void* kpages,
+                                 const void* vpages, uint32_t n_pages, uint32_t page_size, float* out, uint32_t ld_out);
+/* smith_paged_attention of requests that have their first keys in common, whose
+ * keys and values are then read once for a group's rows together.  Group g is the
+ * requests group_start[g] .. group_start[g+1]-1 (n_groups + 1 ascending numbers
+ * from 0 to n_req, in device memory), and the first shared[g] keys of each are
+ * those that the block table of its first request names (as smith_paged_fork
+ * leaves them; a partly filled page may be a copy).  A request with rows has at
+ * least shared[g] keys before them; 0 shares nothing.  The results are those of
+ * smith_paged_attention but for f32 rounding.  A group that does not fit, or a
+ * request with fewer keys, is reported as there; nothing of such a request is
+ * written, of such a group or behind row starts that do not ascend the rows are
+ * undefined. */
+int smith_paged_attention_shared(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
+                                 const int32_t* row_start, const int32_t* lens, const int32_t* tables, uint32_t n_req,
+                                 uint32_t max_pages, const int32_t* group_start, const int32_t* shared, uint32_t n_groups,
+                                 uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale, const void* kpages,
+                                 const void* vpages, uint32_t n_pages, uint32_t page_size, float* out, uint32_t ld_out);
+
 /* ---- pages that requests share ----
  * Several continuations of one prompt name its full pages together; a page that
  * is partly filled belongs to one request, so that smith_paged_plan and

@@ -4,6 +4,7 @@
   smith_amd/lib/smith_llama.hsaco     (the GGUF decode-path kernels, same flags)
   smith_amd/lib/smith_gemm.hsaco      (the prefill MFMA GEMM, same flags)
   smith_amd/lib/smith_paged.hsaco     (the paged KV cache's kernels, same flags)
+  smith_amd/lib/smith_paged_{window,shared,own}.hsaco  (attention over parts of the keys, same flags)
   smith_amd/lib/smith_pages.hsaco     (fork and compact of its pages, same flags)
   smith_amd/lib/smith_score.hsaco     (log probabilities, same flags)
   smith_amd/lib/libsmith.so           hipcc -x hip: host code against libamdhip64 (+ static device scratch)
@@ -24,6 +25,7 @@ HSACO = os.path.join(LIBDIR, "smith_kernels.hsaco")
 HSACO_LLAMA = os.path.join(LIBDIR, "smith_llama.hsaco")
 HSACO_GEMM = os.path.join(LIBDIR, "smith_gemm.hsaco")
 HSACO_PAGED = os.path.join(LIBDIR, "smith_paged.hsaco")
+HSACO_PAGED_MORE = {n: os.path.join(LIBDIR, "smith_paged_%s.hsaco" % n) for n in ("window", "shared", "own")}
 HSACO_PAGES = os.path.join(LIBDIR, "smith_pages.hsaco")
 HSACO_SCORE = os.path.join(LIBDIR, "smith_score.hsaco")
 LIBSMITH = os.path.join(LIBDIR, "libsmith.so")
@@ -49,6 +51,7 @@ def _kernel_cmds():
              "-c", os.path.join(CSRC, src), "-o", dst]
             for src, dst in (("smith_kernels.hip", HSACO), ("llama_kernels.hip", HSACO_LLAMA),
                              ("gemm_kernels.hip", HSACO_GEMM), ("paged_kernels.hip", HSACO_PAGED),
+                             *(("paged_%s_kernels.hip" % n, dst) for n, dst in HSACO_PAGED_MORE.items()),
                              ("pages_kernels.hip", HSACO_PAGES), ("score_kernels.hip", HSACO_SCORE),
                              ("bench_floor.hip", HSACO_BENCH))]
 

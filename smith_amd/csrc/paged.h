@@ -9,6 +9,39 @@
 // attention: most splits of a block (their weights are kept in LDS, 16 columns of them)
 #define PAGED_SPLIT_MAX 128u
 
+// attention
+struct AttArgs {
+  const float* q;
+  const int32_t* row_start;
+  const int32_t* lens;
+  const int32_t* tables;
+  const void* kpages;
+  const void* vpages;
+  float* out;
+  float* parts;        // a split's partial: O [columns][head dim], then (m, l) of each column
+  uint32_t* counters;  // splits of a block that are done, by the index of its first partial; zero between calls
+  uint32_t* queue;     // items taken beyond each workgroup's first; zero between calls
+  uint64_t* err;
+  uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift;
+  uint32_t rows_blk, heads_blk, groups;  // rows to a block of columns, heads of each, blocks to a row's heads
+  float per_target;                     // KV heads / items wanted
+  float split_min;                      // least C
+  float q_factor;                       // scale log2 e = q_factor 2^c_exp, 0.36 < |q_factor| < 0.73
+  int32_t c_exp;
+};
+// and of the kernels whose rows do not see all keys, or not all at once
+struct ReachArgs : AttArgs {
+  uint32_t window, sinks;       // WINDOW
+  uint32_t most_keys;           // WINDOW: no block visits more
+  uint32_t n_groups;            // SHARED (n_req are the groups there)
+  uint32_t n_all;               // SHARED: requests
+  const int32_t* group_start;
+  const int32_t* shared;
+  int32_t* from;                // [requests] shared keys of each, written by SHARED, read by OWN
+  float* prior;                 // [max_rows][heads][head dim] O / l of the shared keys
+  float* prior_ml;              // [max_rows][heads][2]
+};
+
 // fork and compact: pools whose addresses go to a kernel at once, and in all
 #define PAGES_POOLS_LAUNCH 440u
 #define PAGES_MAX_POOLS 4096u
@@ -73,4 +106,6 @@ enum {
   PAGED_ERR_FORK_PAGE,        // the request
   PAGED_ERR_FORK_FREE,        // the free pages
   PAGED_ERR_SCORE_TOKEN,      // the row
+  PAGED_ERR_ATT_GROUP,        // the group
+  PAGED_ERR_ATT_SHARED,       // the request
 };

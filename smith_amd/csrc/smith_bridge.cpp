@@ -83,6 +83,8 @@ struct Ctx {
   void* paged_ws = nullptr;  // partials of smith_paged_attention
   size_t paged_ws_bytes = 0;
   uint32_t* paged_cnt = nullptr;  // and the splits of a block that are done
+  void* paged_prior = nullptr;    // what the shared keys give, of smith_paged_attention_shared
+  size_t paged_prior_bytes = 0;
   void* pages_map = nullptr;      // fork and compact: the state and the map of live pages (zero between calls)
   size_t pages_map_bytes = 0;
   void* pages_ws = nullptr;  // and the moves
@@ -297,6 +299,8 @@ int check_paged_err(Ctx* c) {
       "smith_paged_fork or smith_paged_compact: request %u: a page outside the pool; nothing was copied",
       "smith_paged_fork: the copies need more than the %u pages that nobody names; nothing was copied",
       "smith_logprobs: row %u: a token outside the vocabulary",
+      "smith_paged_attention_shared: group %u: its requests are no part of all of them in order, or its shared keys more than a block table's",
+      "smith_paged_attention_shared: request %u: more shared keys than it had before its rows",
   };
   return fail(c, what[code < sizeof what / sizeof what[0] ? code : 0], arg);
 }
@@ -1035,6 +1039,7 @@ void smith_destroy(void* ctx) {
   if (c->amx) (void)hipFree(c->amx);
   if (c->paged_ws) (void)hipFree(c->paged_ws);
   if (c->paged_cnt) (void)hipFree(c->paged_cnt);
+  if (c->paged_prior) (void)hipFree(c->paged_prior);
   if (c->pages_map) (void)hipFree(c->pages_map);
   if (c->pages_ws) (void)hipFree(c->pages_ws);
   if (c->score_ws) (void)hipFree(c->score_ws);
@@ -2443,6 +2448,123 @@ int smith_paged_append(void* ctx, uint32_t kv_type, const float* qkv, uint32_t l
   return 0;
 }
 
+// What the three attention calls have in common.
+struct AttCall {
+  const char* fn;
+  uint32_t kv_type;
+  const float* q;
+  uint32_t ld_q, max_rows;
+  const int32_t *row_start, *lens, *tables;
+  uint32_t n_req, max_pages, n_heads, n_kv_heads, head_dim;
+  float scale;
+  const void *kpages, *vpages;
+  uint32_t n_pages, page_size;
+  float* out;
+  uint32_t ld_out, shift;
+};
+
+static int check_attention(Ctx* c, AttCall& k, std::initializer_list<Range> more = {}) {
+  if (check_paged(c, k.fn, k.kv_type, k.n_heads, k.n_kv_heads, k.head_dim, k.kpages, k.vpages, k.n_pages, k.page_size, &k.shift))
+    return -1;
+  const uint64_t Wq = (uint64_t)k.n_heads * k.head_dim;
+  if (!k.n_req || k.n_req > PAGED_MAX_REQ) return fail(c, "%s: %u requests (1 .. %u)", k.fn, k.n_req, PAGED_MAX_REQ);
+  if (!k.max_pages || ((uint64_t)k.max_pages << k.shift) > 0x7FFFFFFFull)
+    return fail(c, "%s: block tables of %u pages of %u keys (at least one page, less than 2^31 keys)", k.fn, k.max_pages,
+                k.page_size);
+  if (!k.row_start && k.max_rows != k.n_req)
+    return fail(c, "%s: max_rows %u for one row of each of %u requests", k.fn, k.max_rows, k.n_req);
+  if (k.ld_q < Wq || k.ld_out < Wq)
+    return fail(c, "%s: row strides %u and %u for rows of %llu floats", k.fn, k.ld_q, k.ld_out, (unsigned long long)Wq);
+  if (k.max_rows > 0x7FFFFFFFu) return fail(c, "%s: max_rows %u", k.fn, k.max_rows);
+  if (!std::isfinite(k.scale)) return fail(c, "%s: scale %g", k.fn, (double)k.scale);
+  if (!k.max_rows) return 0;
+  if (!k.q || !k.lens || !k.tables || !k.out) return fail(c, "%s: null buffer", k.fn);
+  const Range o = {k.out, 4 * ((uint64_t)(k.max_rows - 1) * k.ld_out + Wq)};
+  if (overlap(o, {k.q, 4 * ((uint64_t)(k.max_rows - 1) * k.ld_q + Wq)})) return fail(c, "%s: out overlaps q", k.fn);
+  const uint64_t pool = pool_bytes(k.kv_type, k.n_kv_heads, k.head_dim, k.n_pages, k.page_size);
+  const Range in[] = {{k.row_start, k.row_start ? 4ull * k.n_req + 4 : 0}, {k.lens, 4ull * k.n_req},
+                      {k.tables, 4ull * k.n_req * k.max_pages}, {k.kpages, pool}, {k.vpages, pool}};
+  for (const Range& r : in)
+    if (overlap(o, r)) return fail(c, "%s: out overlaps an input", k.fn);
+  for (const Range& r : more)
+    if (overlap(o, r)) return fail(c, "%s: out overlaps an input", k.fn);
+  if (k.scale == 0.f) k.scale = 1.0f / sqrtf((float)k.head_dim);
+  return set_device(c);
+}
+
+// Where a request brings a row or so its columns (row, head) are few and its
+// keys the work: 16 columns to a workgroup, keys in registers.  Where the
+// columns fill most of two such tiles a workgroup shares the keys among four
+// waves' columns -- if there are enough of them for the waves of the card, which
+// its 64 or 128 columns to a workgroup otherwise leave idle.  Microseconds, the
+// first kernel's and the second's (32 heads on 8 of 128, f16 | bf16 | f32): a prompt
+// of 100 rows (3200 columns) 8.5, 13.5 | 8.8, 17.9 | 9.9, 16.8; of 200 (6400) 31.9,
+// 16.4 | 32.1, 21.9 | 35.3, 25.7; of 300 (9600) 18.5, 20.8 | 18.8, 26.9 | 22.9, 35.1;
+// of 400 23.6, 23.7 | 24.1, 31.5 | 32.6, 34.4; of 600 34.8, 31.6 | 36.1, 40.9 | 52.6,
+// 53.6; of 1000 62, 44 | 65, 53 | 110, 101; of 2000 179, 86 | 178, 113 | 387, 302; 256
+// rows (8192) behind 2000 keys 46.9, 42.3 | 48.5, 52.4 | 112, 97; behind 8000 keys 64
+// rows 51, 57 | 53, 68 | 112, 115, 128 rows 87, 75 | 88, 87 | 207, 186, 256 rows 150,
+// 94 | 154, 115 | 392, 312; 16 prompts of up to 200 rows 88, 40 | 91, 58 | 113, 71.
+// 8192 columns are right for several prompts and behind long caches; one prompt of 200
+// to 600 rows it gives the slower kernel, by up to 2x: what tells it from the others
+// is the lengths, which are on the device.  For the same reason max_rows and n_req
+// stand for the rows and the requests that bring some: 256 rows behind 7744 keys take
+// 101 us alone and 150 in a cache of 64 places.
+// The second loads 8 keys at once, of one page.  The first takes 16 keys as one
+// address, or looks them up one by one where pages are smaller.
+static bool many_columns(const AttCall& k) {
+  const uint32_t G = k.n_heads / k.n_kv_heads;
+  return k.row_start && k.shift >= 3 && (uint64_t)k.max_rows * G > 24ull * k.n_req && (uint64_t)k.max_rows * k.n_heads >= 8192;
+}
+
+// `n` requests (or groups) of k, by one of the two kernels of `of` (""; _window, _shared or _own)
+static int launch_attention(Ctx* c, const AttCall& k, const char* of, uint32_t n, bool many, ReachArgs* more) {
+  const uint32_t G = k.n_heads / k.n_kv_heads;
+  const bool small = !many && k.shift < 4;
+  const uint32_t CB = !many ? 16 : k.kv_type == SMITH_KV_F32 ? 64 : 128;
+  const uint32_t dims = k.head_dim <= 64 ? 64 : k.head_dim <= 96 ? 96 : 128;
+  const uint32_t target = 512;  // two workgroups to a CU
+  // Keys to a split at least.  A split of many columns leaves 64 KB and the join
+  // reads them again: 64 rows behind 8000 keys, 32 heads, in that kernel 58 us (f16) and
+  // 69 (bf16) with 512, 64 and 77 with 768, 74 and 84 with 384; 300 rows of a prompt 20.8
+  // uncut, 24.8 with 128.  f32 keys are eight times the work: 20 requests, half of them
+  // with chunks of up to 77 rows, 63 us with 256, 70 with 384, 80 with 512.
+  const float split_min = !many ? 128.f : k.kv_type == SMITH_KV_F32 ? 256.f : 512.f;
+  // a block that is cut has more than 5/4 C keys and so less than twice its keys / C
+  // splits: 2 W / C <= 2 target of them in all (and some for what f32 rounds)
+  const uint32_t max_parts = 2 * target + 16;
+  if (ensure(c, &c->paged_ws, &c->paged_ws_bytes, (size_t)max_parts * CB * (k.head_dim + 2) * sizeof(float))) return -1;
+  if (ensure_paged_counters(c)) return -1;
+  const uint32_t heads_blk = std::min(G, CB), RB = CB / heads_blk, groups = (G + CB - 1) / CB;
+  const uint64_t blocks = (uint64_t)groups * k.n_kv_heads * (k.row_start || n != k.n_req ? (uint64_t)n + k.max_rows / RB : n);
+  const uint64_t longest = ((uint64_t)k.max_pages << k.shift) / (uint32_t)split_min + 1;  // splits of one block
+  const uint32_t grid = (uint32_t)std::min<uint64_t>({(uint64_t)target, blocks + max_parts, blocks * longest});
+  // of attention_body: O and (m, l) of four waves; of attention_rows_body: two
+  // stages of K and V rows (64 of f16 / bf16 or 32 of f32: 256 bytes a head dim) and their marks;
+  // of both: the items' table
+  const uint32_t lds = (many ? 256 * 2 * (dims <= 64 ? 64 : 128) + 16 : 4 * 16 * (dims + 4) * 4 + 4 * 16 * 2 * 4) + 16 +
+                       (*of ? 24 : 20) * (n + 1);
+  int c_exp;
+  const float q_factor = (float)(frexp((double)k.scale, &c_exp) * (0.5 * 1.4426950408889634));
+  c_exp++;
+  AttArgs a = {k.q, k.row_start, k.lens, k.tables, k.kpages, k.vpages, k.out, (float*)c->paged_ws, c->paged_cnt,
+               c->paged_cnt + PAGED_COUNTERS, c->paged_err_dev(), k.ld_q, k.ld_out, k.max_rows, n, k.max_pages, k.n_kv_heads,
+               G, k.head_dim, k.n_pages, k.shift, RB, heads_blk, groups, (float)k.n_kv_heads / (float)target, split_min,
+               q_factor, c_exp};
+  char name[64];
+  snprintf(name, sizeof name, "smith_paged_attention%s_%s%s_d%u%s", of, many ? "rows_" : "", kv_name(k.kv_type), dims,
+           small ? "_s" : "");
+  void* args[] = {&a};
+  if (more) {
+    (AttArgs&)*more = a;
+    // WINDOW: the keys that a block visits, with those that fill tiles up
+    const uint64_t unit = many ? (k.kv_type == SMITH_KV_F32 ? 32 : 64) : k.kv_type == SMITH_KV_F32 ? 16 : 32;
+    more->most_keys = (uint32_t)std::min<uint64_t>(0x7FFFFFFFu, (uint64_t)more->window + more->sinks + RB + 3 * unit);
+    args[0] = more;
+  }
+  return launch(c, name, dim3(grid), dim3(256), args, lds);
+}
+
 int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
                           const int32_t* row_start, const int32_t* lens, const int32_t* tables, uint32_t n_req,
                           uint32_t max_pages, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,
@@ -2450,98 +2572,58 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
                           uint32_t ld_out) {
   Ctx* c = (Ctx*)ctx;
   if (!c) return -1;
-  static const char fn[] = "smith_paged_attention";
-  uint32_t shift;
-  if (check_paged(c, fn, kv_type, n_heads, n_kv_heads, head_dim, kpages, vpages, n_pages, page_size, &shift)) return -1;
-  const uint64_t Wq = (uint64_t)n_heads * head_dim;
-  if (!n_req || n_req > PAGED_MAX_REQ) return fail(c, "%s: %u requests (1 .. %u)", fn, n_req, PAGED_MAX_REQ);
-  if (!max_pages || ((uint64_t)max_pages << shift) > 0x7FFFFFFFull)
-    return fail(c, "%s: block tables of %u pages of %u keys (at least one page, less than 2^31 keys)", fn, max_pages,
-                page_size);
-  if (!row_start && max_rows != n_req)
-    return fail(c, "%s: max_rows %u for one row of each of %u requests", fn, max_rows, n_req);
-  if (ld_q < Wq || ld_out < Wq)
-    return fail(c, "%s: row strides %u and %u for rows of %llu floats", fn, ld_q, ld_out, (unsigned long long)Wq);
-  if (max_rows > 0x7FFFFFFFu) return fail(c, "%s: max_rows %u", fn, max_rows);
-  if (!std::isfinite(scale)) return fail(c, "%s: scale %g", fn, (double)scale);
+  AttCall k = {"smith_paged_attention", kv_type, q, ld_q, max_rows, row_start, lens, tables, n_req, max_pages, n_heads,
+               n_kv_heads, head_dim, scale, kpages, vpages, n_pages, page_size, out, ld_out, 0};
+  if (check_attention(c, k)) return -1;
   if (!max_rows) return 0;
-  if (!q || !lens || !tables || !out) return fail(c, "%s: null buffer", fn);
-  {
-    const Range o = {out, 4 * ((uint64_t)(max_rows - 1) * ld_out + Wq)};
-    if (overlap(o, {q, 4 * ((uint64_t)(max_rows - 1) * ld_q + Wq)})) return fail(c, "%s: out overlaps q", fn);
-    const uint64_t pool = pool_bytes(kv_type, n_kv_heads, head_dim, n_pages, page_size);
-    const Range in[] = {{row_start, row_start ? 4ull * n_req + 4 : 0}, {lens, 4ull * n_req},
-                        {tables, 4ull * n_req * max_pages}, {kpages, pool}, {vpages, pool}};
-    for (const Range& r : in)
-      if (overlap(o, r)) return fail(c, "%s: out overlaps an input", fn);
-  }
-  if (set_device(c)) return -1;
-  if (scale == 0.f) scale = 1.0f / sqrtf((float)head_dim);
-  // Where a request brings a row or so its columns (row, head) are few and its
-  // keys the work: 16 columns to a workgroup, keys in registers.  Where the
-  // columns fill most of two such tiles a workgroup shares the keys among four
-  // waves' columns -- if there are enough of them for the waves of the card, which
-  // its 64 or 128 columns to a workgroup otherwise leave idle.  Microseconds, the
-  // first kernel's and the second's (32 heads on 8 of 128, f16 | bf16 | f32): a prompt
-  // of 100 rows (3200 columns) 8.5, 13.5 | 8.8, 17.9 | 9.9, 16.8; of 200 (6400) 31.9,
-  // 16.4 | 32.1, 21.9 | 35.3, 25.7; of 300 (9600) 18.5, 20.8 | 18.8, 26.9 | 22.9, 35.1;
-  // of 400 23.6, 23.7 | 24.1, 31.5 | 32.6, 34.4; of 600 34.8, 31.6 | 36.1, 40.9 | 52.6,
-  // 53.6; of 1000 62, 44 | 65, 53 | 110, 101; of 2000 179, 86 | 178, 113 | 387, 302; 256
-  // rows (8192) behind 2000 keys 46.9, 42.3 | 48.5, 52.4 | 112, 97; behind 8000 keys 64
-  // rows 51, 57 | 53, 68 | 112, 115, 128 rows 87, 75 | 88, 87 | 207, 186, 256 rows 150,
-  // 94 | 154, 115 | 392, 312; 16 prompts of up to 200 rows 88, 40 | 91, 58 | 113, 71.
-  // 8192 columns are right for several prompts and behind long caches; one prompt of 200
-  // to 600 rows it gives the slower kernel, by up to 2x: what tells it from the others
-  // is the lengths, which are on the device.  For the same reason max_rows and n_req
-  // stand for the rows and the requests that bring some: 256 rows behind 7744 keys take
-  // 101 us alone and 150 in a cache of 64 places.
-  // The second loads 8 keys at once, of one page.  The first takes 16 keys as one
-  // address, or looks them up one by one where pages are smaller.
-  const uint32_t G = n_heads / n_kv_heads;
-  const bool many = row_start && shift >= 3 && (uint64_t)max_rows * G > 24ull * n_req &&
-                    (uint64_t)max_rows * n_heads >= 8192;
-  const bool small = !many && shift < 4;
-  const uint32_t CB = !many ? 16 : kv_type == SMITH_KV_F32 ? 64 : 128, dims = head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : 128;
-  const uint32_t target = 512;  // two workgroups to a CU
-  // Keys to a split at least.  A split of many columns leaves 64 KB and the join
-  // reads them again: 64 rows behind 8000 keys, 32 heads, in that kernel 58 us (f16) and
-  // 69 (bf16) with 512, 64 and 77 with 768, 74 and 84 with 384; 300 rows of a prompt 20.8
-  // uncut, 24.8 with 128.  f32 keys are eight times the work: 20 requests, half of them
-  // with chunks of up to 77 rows, 63 us with 256, 70 with 384, 80 with 512.
-  const float split_min = !many ? 128.f : kv_type == SMITH_KV_F32 ? 256.f : 512.f;
-  // a block that is cut has more than 5/4 C keys and so less than twice its keys / C
-  // splits: 2 W / C <= 2 target of them in all (and some for what f32 rounds)
-  const uint32_t max_parts = 2 * target + 16;
-  if (ensure(c, &c->paged_ws, &c->paged_ws_bytes, (size_t)max_parts * CB * (head_dim + 2) * sizeof(float))) return -1;
-  if (ensure_paged_counters(c)) return -1;
-  const uint32_t heads_blk = std::min(G, CB), RB = CB / heads_blk, groups = (G + CB - 1) / CB;
-  const uint64_t blocks = (uint64_t)groups * n_kv_heads * (row_start ? (uint64_t)n_req + max_rows / RB : n_req);
-  const uint64_t longest = ((uint64_t)max_pages << shift) / (uint32_t)split_min + 1;  // splits of one block
-  const uint32_t grid = (uint32_t)std::min<uint64_t>({(uint64_t)target, blocks + max_parts, blocks * longest});
-  // of attention_body: O and (m, l) of four waves; of attention_rows_body: two
-  // stages of K and V rows (64 of f16 / bf16 or 32 of f32: 256 bytes a head dim) and their marks
-  const uint32_t lds = (many ? 256 * 2 * (dims <= 64 ? 64 : 128) + 16 : 4 * 16 * (dims + 4) * 4 + 4 * 16 * 2 * 4) + 16 + 20 * (n_req + 1);
-  int c_exp;
-  const float q_factor = (float)(frexp((double)scale, &c_exp) * (0.5 * 1.4426950408889634));
-  c_exp++;
-  struct {
-    const float* q;
-    const int32_t *row_start, *lens, *tables;
-    const void *kpages, *vpages;
-    float *out, *parts;
-    uint32_t *counters, *queue;
-    uint64_t* err;
-    uint32_t ld_q, ld_out, max_rows, n_req, max_pages, nKV, G, hd, n_pages, shift, rows_blk, heads_blk, groups;
-    float per_target, split_min, q_factor;
-    int32_t c_exp;
-  } a = {q, row_start, lens, tables, kpages, vpages, out, (float*)c->paged_ws, c->paged_cnt, c->paged_cnt + PAGED_COUNTERS,
-         c->paged_err_dev(),
-         ld_q, ld_out, max_rows, n_req, max_pages, n_kv_heads, G, head_dim, n_pages, shift, RB, heads_blk, groups,
-         (float)n_kv_heads / (float)target, split_min, q_factor, c_exp};
-  char name[64];
-  snprintf(name, sizeof name, "smith_paged_attention_%s%s_d%u%s", many ? "rows_" : "", kv_name(kv_type), dims, small ? "_s" : "");
-  void* args[] = {&a};
-  return launch(c, name, dim3(grid), dim3(256), args, lds);
+  return launch_attention(c, k, "", n_req, many_columns(k), nullptr);
+}
+
+int smith_paged_attention_window(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
+                                 const int32_t* row_start, const int32_t* lens, const int32_t* tables, uint32_t n_req,
+                                 uint32_t max_pages, uint32_t window, uint32_t sinks, uint32_t n_heads,
+                                 uint32_t n_kv_heads, uint32_t head_dim, float scale, const void* kpages,
+                                 const void* vpages, uint32_t n_pages, uint32_t page_size, float* out, uint32_t ld_out) {
+  Ctx* c = (Ctx*)ctx;
+  if (!c) return -1;
+  AttCall k = {"smith_paged_attention_window", kv_type, q, ld_q, max_rows, row_start, lens, tables, n_req, max_pages,
+               n_heads, n_kv_heads, head_dim, scale, kpages, vpages, n_pages, page_size, out, ld_out, 0};
+  if (check_attention(c, k)) return -1;
+  if (!window) return fail(c, "%s: a window of 0 keys (a row sees its own)", k.fn);
+  if (!max_rows) return 0;
+  ReachArgs more = {};
+  more.window = std::min(window, 0x7FFFFFFFu);  // as long as a request can be
+  more.sinks = std::min(sinks, 0x7FFFFFFFu);
+  return launch_attention(c, k, "_window", n_req, many_columns(k), &more);
+}
+
+int smith_paged_attention_shared(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
+                                 const int32_t* row_start, const int32_t* lens, const int32_t* tables, uint32_t n_req,
+                                 uint32_t max_pages, const int32_t* group_start, const int32_t* shared, uint32_t n_groups,
+                                 uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale, const void* kpages,
+                                 const void* vpages, uint32_t n_pages, uint32_t page_size, float* out, uint32_t ld_out) {
+  Ctx* c = (Ctx*)ctx;
+  if (!c) return -1;
+  AttCall k = {"smith_paged_attention_shared", kv_type, q, ld_q, max_rows, row_start, lens, tables, n_req, max_pages,
+               n_heads, n_kv_heads, head_dim, scale, kpages, vpages, n_pages, page_size, out, ld_out, 0};
+  if (check_attention(c, k, {{group_start, 4ull * n_groups + 4}, {shared, 4ull * n_groups}})) return -1;
+  if (!n_groups || n_groups > n_req) return fail(c, "%s: %u groups of %u requests", k.fn, n_groups, n_req);
+  if (!max_rows) return 0;
+  if (!group_start || !shared) return fail(c, "%s: null buffer", k.fn);
+  // of each column what its shared keys give, and of each request how many they are
+  const size_t H = n_heads, floats = (size_t)max_rows * H * (head_dim + 2);
+  if (ensure(c, &c->paged_prior, &c->paged_prior_bytes, (floats + n_req) * 4)) return -1;
+  ReachArgs more = {};
+  more.n_groups = n_groups;
+  more.n_all = n_req;
+  more.group_start = group_start;
+  more.shared = shared;
+  more.prior = (float*)c->paged_prior;
+  more.prior_ml = more.prior + (size_t)max_rows * H * head_dim;
+  more.from = (int32_t*)(more.prior + floats);
+  const bool many = k.shift >= 3 && (uint64_t)max_rows * (n_heads / n_kv_heads) >= 48ull * n_groups;
+  if (launch_attention(c, k, "_shared", n_groups, many, &more)) return -1;
+  return launch_attention(c, k, "_own", n_req, many_columns(k), &more);
 }
 
 // The state and map of fork and compact: as ensure(), and zero.

@@ -16,6 +16,7 @@ CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_kernels.hsaco")
 LLAMA_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_llama.hsaco")
 GEMM_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_gemm.hsaco")
 PAGED_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_paged.hsaco")
+PAGED_MORE_CODE_OBJECT_PATHS = [os.path.join(_HERE, "lib", "smith_paged_%s.hsaco" % n) for n in ("window", "shared", "own")]
 PAGES_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_pages.hsaco")
 SCORE_CODE_OBJECT_PATH = os.path.join(_HERE, "lib", "smith_score.hsaco")
 
@@ -125,6 +126,10 @@ SYMBOLS = {
                                   _U32, _U32, _P, _U32]),
     "smith_paged_attention": (_INT, [_P, _U32, _P, _U32, _U32, _P, _P, _P, _U32, _U32, _U32, _U32, _U32,
                                      ctypes.c_float, _P, _P, _U32, _U32, _P, _U32]),
+    "smith_paged_attention_window": (_INT, [_P, _U32, _P, _U32, _U32, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _U32,
+                                            ctypes.c_float, _P, _P, _U32, _U32, _P, _U32]),
+    "smith_paged_attention_shared": (_INT, [_P, _U32, _P, _U32, _U32, _P, _P, _P, _U32, _U32, _P, _P, _U32, _U32, _U32, _U32,
+                                            ctypes.c_float, _P, _P, _U32, _U32, _P, _U32]),
     "smith_paged_fork": (_INT, [_P, _U32, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, ctypes.POINTER(_P), _U32, _U32,
                                 _U32, _P, _P, _P, _P]),
     "smith_paged_compact": (_INT, [_P, _U32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, ctypes.POINTER(_P), _U32, _U32,
@@ -201,7 +206,7 @@ def shader_lib():
                                % (CODE_OBJECT_PATH, lib.smith_last_error(c).decode()))
         _library = lp
         for path in (LLAMA_CODE_OBJECT_PATH, GEMM_CODE_OBJECT_PATH, PAGED_CODE_OBJECT_PATH,
-                     PAGES_CODE_OBJECT_PATH, SCORE_CODE_OBJECT_PATH):
+                     *PAGED_MORE_CODE_OBJECT_PATHS, PAGES_CODE_OBJECT_PATH, SCORE_CODE_OBJECT_PATH):
             if not lib.smith_load_library(c, path.encode()):
                 raise RuntimeError("smith: failed to load code object at %s: %s"
                                    % (path, lib.smith_last_error(c).decode()))

@@ -29,6 +29,7 @@ from . import tensor as T
 KV_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 ROPE_NONE, ROPE_ROW, ROPE_HEAD = 0, 1, 2
 MAX_REQUESTS = 4096  # of one step
+MOST_KEYS = 2 ** 31 - 1  # of a request
 
 
 def _want(t, shape, dtype, what):
@@ -81,11 +82,17 @@ def pagedAppend(qkv, slots, positions, numHeads, kPages, vPages, rope=ROPE_NONE,
     return q
 
 
-def pagedAttention(q, lens, tables, kPages, vPages, rowStart=None, scale=0.0, out=None):
+def pagedAttention(q, lens, tables, kPages, vPages, rowStart=None, scale=0.0, out=None, window=0, sinks=0,
+                   groupStart=None, shared=None):
     """Causal attention of rows q [rows, numHeads * headDim] over the pages
     (smith_paged_attention): request b's rows are rowStart[b] .. rowStart[b+1]-1,
     or row b alone without rowStart.  Returns out (a new tensor if None is given,
-    whose rows behind the last one are then undefined)."""
+    whose rows behind the last one are then undefined).
+
+    window > 0: a row sees the last `window` keys up to its own and the first
+    `sinks` (smith_paged_attention_window).  groupStart [n + 1], shared [n] i32: the
+    requests groupStart[g] .. groupStart[g+1]-1 have their first shared[g] keys in
+    common, which are read once for all of them (smith_paged_attention_shared)."""
     nPages, nKV, P, hd = _pools(kPages, vPages, "pagedAttention")
     rows, width = q.shape
     n = lens.shape[0]
@@ -95,13 +102,25 @@ def pagedAttention(q, lens, tables, kPages, vPages, rowStart=None, scale=0.0, ou
     _want(tables, [n, tables.shape[-1]], "i32", "pagedAttention: tables")
     if rowStart is not None:
         _want(rowStart, [n + 1], "i32", "pagedAttention: rowStart")
+    if window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError("pagedAttention: a window of %d keys and %d sinks" % (window, sinks))
+    name, reach = "smith_paged_attention", ()
+    if groupStart is not None or shared is not None:
+        if groupStart is None or shared is None or window:
+            raise ValueError("pagedAttention: shared keys take groupStart and shared, and no window")
+        groups = shared.shape[0]
+        _want(shared, [groups], "i32", "pagedAttention: shared")
+        _want(groupStart, [groups + 1], "i32", "pagedAttention: groupStart")
+        name, reach = "smith_paged_attention_shared", (groupStart.buffer, shared.buffer, groups)
+    elif window:
+        name, reach = "smith_paged_attention_window", (min(window, MOST_KEYS), min(sinks, MOST_KEYS))
     if out is None:
         out = T.create([rows, width])
     _want(out, [rows, width], "f32", "pagedAttention: out")
-    device.check(device.lib.smith_paged_attention(
+    device.check(getattr(device.lib, name)(
         device.ops_ctx(), KV_TYPES[kPages.dtype], q.buffer, width, rows,
-        rowStart.buffer if rowStart is not None else None, lens.buffer, tables.buffer, n, tables.shape[1], width // hd,
-        nKV, hd, scale, kPages.buffer, vPages.buffer, nPages, P, out.buffer, width), "pagedAttention")
+        rowStart.buffer if rowStart is not None else None, lens.buffer, tables.buffer, n, tables.shape[1], *reach,
+        width // hd, nKV, hd, scale, kPages.buffer, vPages.buffer, nPages, P, out.buffer, width), "pagedAttention")
     return out
 
 

@@ -48,3 +48,46 @@ def compact(lens, tables, n_pages, P, free, window=0, sinks=0):
         tables[b, j] = to.get(q, q) if kept(j, P, int(lens[b]), window, sinks) else -1
     free[:n_pages - n] = np.arange(n_pages - 1, n - 1, -1)
     return tables, free, n_pages - n, moves
+
+
+def attention(q, row_start, lens, tables, k, v, seen, scale=None):
+    """(out, magnitude, largest score sum, keys), as paged_reference.attention, of rows that
+    see the keys for which seen(b, position, key numbers) holds: pools k, v of f64 values."""
+    H, D = q.shape[1:]
+    G, P = H // k.shape[1], k.shape[2]
+    scale = D ** -0.5 if not scale else scale
+    out, mag, big, keys = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(len(q))
+    for b, n in enumerate(lens):
+        r0, r1 = row_start[b], row_start[b + 1]
+        for r in range(r0, r1):
+            at = n - (r1 - r0) + (r - r0)
+            t = np.arange(at + 1)
+            t = t[seen(b, at, t)]
+            keys[r] = len(t)
+            if not len(t):
+                continue
+            page = tables[b][t // P]
+            kk, vv = k[page, :, t % P], v[page, :, t % P]  # [keys, kv heads, dim]
+            for h in range(H):
+                kt, vt = kk[:, h // G], vv[:, h // G]
+                s = scale * (kt @ q[r, h])
+                p = np.exp(s - s.max())
+                out[r, h] = p @ vt / p.sum()
+                mag[r, h] = p @ np.abs(vt) / p.sum()
+                big[r, h] = abs(scale) * (np.abs(kt) @ np.abs(q[r, h])).max()
+    return out, mag, big, keys
+
+
+def check_attention(got, want, D):
+    """The bound of an output (one of f32, f16 or bf16 pages): a score is a sum of D
+    products of q (kept to 2^-22 of its row's largest element) and k in f32: off by at
+    most (D + 8) 2^-24 + 2^-21 of B = scale sum |q k|; its weight by twice that, and by
+    2^-21 for the exponential and the weight's own split; the sums over n keys by n half
+    steps, each relative to sum p |v| / sum p; a join of two such sums by 2^-21."""
+    out, mag, big, keys = want
+    rel = 2 * ((D + 8) * 2.0 ** -24 + 2.0 ** -21) * big + 2.0 ** -20 + keys[:, None] * 2.0 ** -23 + 2.0 ** -21
+    off = np.abs(got.astype(np.float64).reshape(out.shape) - out)
+    assert np.all(off <= mag * rel[..., None]), (off / (mag * rel[..., None] + 1e-300)).max()
+    norm = np.linalg.norm(out)
+    if norm:
+        assert np.linalg.norm(off) <= 1e-5 * norm, np.linalg.norm(off) / norm
