@@ -473,9 +473,9 @@ int smith_paged_attention_window(void* ctx, uint32_t kv_type, const float* q, ui
  * leaves them; a partly filled page may be a copy).  A request with rows has at
  * least shared[g] keys before them; 0 shares nothing.  The results are those of
  * smith_paged_attention but for f32 rounding.  A group that does not fit, or a
- * request with fewer keys, is reported as there; nothing of such a request is
- * written, of such a group or behind row starts that do not ascend the rows are
- * undefined. */
+ * request with fewer keys, is reported as there, and the rows of such are undefined,
+ * as they are where row starts do not ascend.  Where max_pages has no room for
+ * many keys each request reads all of its own. */
 int smith_paged_attention_shared(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
                                  const int32_t* row_start, const int32_t* lens, const int32_t* tables, uint32_t n_req,
                                  uint32_t max_pages, const int32_t* group_start, const int32_t* shared, uint32_t n_groups,

@@ -29,6 +29,11 @@ struct AttArgs {
   float q_factor;                       // scale log2 e = q_factor 2^c_exp, 0.36 < |q_factor| < 0.73
   int32_t c_exp;
 };
+// a request's group: its shared keys, its first partial, splits of its blocks, first row, blocks
+struct SharedOf {
+  int32_t keys;
+  uint32_t part, splits, row0, blocks;
+};
 // and of the kernels whose rows do not see all keys, or not all at once
 struct ReachArgs : AttArgs {
   uint32_t window, sinks;       // WINDOW
@@ -37,9 +42,13 @@ struct ReachArgs : AttArgs {
   uint32_t n_all;               // SHARED: requests
   const int32_t* group_start;
   const int32_t* shared;
-  int32_t* from;                // [requests] shared keys of each, written by SHARED, read by OWN
-  float* prior;                 // [max_rows][heads][head dim] O / l of the shared keys
-  float* prior_ml;              // [max_rows][heads][2]
+  SharedOf* from;               // [requests], written by SHARED, read by OWN
+  float* prior;                 // [max_rows][heads][head dim] O of shared keys that are not cut
+  float* prior_ml;              // [max_rows][heads][2] and m, l
+  // OWN: SHARED's parts, columns of each, rows_blk, heads_blk and groups
+  const float* s_parts;
+  uint32_t s_columns, s_rows_blk, s_heads_blk, s_groups;
+  uint32_t whole;  // OWN: all of a request's keys are its own
 };
 
 // fork and compact: pools whose addresses go to a kernel at once, and in all

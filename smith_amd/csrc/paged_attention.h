@@ -345,10 +345,10 @@ struct Tile32 {
 //   ALL     all of them
 //   WINDOW  the first `sinks` and those above p - window
 //   SHARED  a group's columns against its first shared[g] keys, of which all see all;
-//           (O / l, m, l) of each column goes to the scratch
-//   OWN     a request's own keys behind those, joined with what SHARED left:
-//           with w1 = l1 2^(m1 - M), w2 = 2^(m2 - M), M = max(m1, m2)
-//             out = (w1 O1 + w2 O2) / (w1 + w2 l2)
+//           (O, m, l) of each column and split stays in the scratch
+//   OWN     a request's own keys behind those, joined with what SHARED left: with
+//           weights w = 2^(m - M), M = max m, of its own and of each split
+//             out = sum w O / sum w l
 // For the others than ALL the keys that a block of rows visits are numbered without
 // those that none of them sees, in whole tiles: key t is key t of the request, or
 // for t >= `first` key t + gap.
@@ -435,7 +435,7 @@ __device__ __forceinline__ void request(const Args<R>& a, uint32_t b, bool tell,
     len = 0;
   }
   if constexpr (R == OWN) {
-    const int32_t f = a.from[b];
+    const int32_t f = a.whole ? 0 : a.from[b].keys;
     if (n && f && (f < 0 || f > l - (int32_t)n)) {
       if (tell && f > 0) paged_err(a.err, PAGED_ERR_ATT_SHARED, b);
       n = 0;
@@ -473,7 +473,10 @@ struct Items {
   float inv_c;
 
   static __device__ __forceinline__ uint32_t splits(uint32_t keys, float inv_c) {  // of at most about 5/4 C keys
-    const uint32_t s = (uint32_t)((float)keys * inv_c * 0.8f + 0.999f);
+    // (WINDOW: of less than twice C.  Blocks visit nearly the same number of keys, and a cut
+    // that gives more items than there are workgroups only makes a second round of them: a
+    // window of 500, 16 requests of 30 rows, 32 heads on 8 of 128, f16, 36.2 and 19.5 us.)
+    const uint32_t s = (uint32_t)(R == WINDOW ? (float)keys * inv_c + 0.001f : (float)keys * inv_c * 0.8f + 0.999f);
     return s < 1 ? 1u : s > PAGED_SPLIT_MAX ? PAGED_SPLIT_MAX : s;
   }
   // keys that its blocks visit, at most and about
@@ -591,7 +594,7 @@ __device__ __forceinline__ void find_items(const Args<R>& a, uint32_t* lds, Item
   }
   t.total += total_long;
   put_head();
-  if (blockIdx.x >= t.total) return;
+  if (R != SHARED && blockIdx.x >= t.total) return;
   for (uint32_t k = 0; k < per; k++) {
     const uint32_t b = tid * per + k;
     if (b >= a.n_req) break;
@@ -790,30 +793,71 @@ __device__ __forceinline__ bool last_split(const AttArgs& a, const Item<R>& I) {
   return s_last;
 }
 
-// The numbers of a column: where they go.  o of W dims from d0 on, sum l, maximum m.
-template <Reach R, int W, class V>
-__device__ __forceinline__ V finished(const Args<R>& a, const Item<R>& I, uint32_t col, uint32_t d0, V o, float l, float m) {
-  if constexpr (R == OWN) {
-    const uint32_t H = a.nKV * a.G;
-    const float* ml = a.prior_ml + I.at(col, 2 * H, 2);
-    const float* p = a.prior + I.at(col, H * a.hd, a.hd) + d0;
-    const float m1 = ml[0], l1 = ml[1], M = fmaxf(m, m1);
-    const float w1 = m1 == -__builtin_inff() ? 0.f : l1 * __builtin_amdgcn_exp2f(m1 - M);
-    const float w2 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - M);
-    const float sum = __builtin_fmaf(w2, l, w1), inv = I.keys || l1 != 0.f ? 1.0f / sum : 0.f;
-#pragma unroll
-    for (int d = 0; d < W; d++) o[d] = __builtin_fmaf(w2, o[d], w1 * p[d]) * inv;
-  } else {
-    const float inv = I.keys ? 1.0f / l : 0.f;
-#pragma unroll
-    for (int d = 0; d < W; d++) o[d] *= inv;
+// OWN: what the shared keys give a column, splits' partials or one alone.
+template <Reach R>
+struct Prior {
+  const float *o, *ml;  // the first's
+  size_t stride;        // to the next split's
+  __device__ __forceinline__ Prior(const Args<R>& a, const Item<R>& I, const SharedOf& f, uint32_t col) {
+    const uint32_t row = I.row_of(col), head = I.head0 + col - row * I.heads, kvh = head / a.G, h = head - kvh * a.G;
+    const uint32_t r = I.r0 + I.row0 + row - f.row0, rowblk = r / a.s_rows_blk, hgroup = h / a.s_columns;
+    const uint32_t left = a.G - hgroup * a.s_columns, heads = left < a.s_heads_blk ? left : a.s_heads_blk;
+    const uint32_t c = (r - rowblk * a.s_rows_blk) * heads + h - hgroup * a.s_columns, blk = rowblk * a.s_groups + hgroup;
+    stride = (size_t)a.nKV * a.s_columns * (a.hd + 2);
+    const size_t part = f.part + (size_t)(f.blocks - 1 - blk) * f.splits * a.nKV + kvh;
+    const float* p = a.s_parts + part * a.s_columns * (a.hd + 2);
+    if (f.splits > 1) {
+      o = p + c * a.hd;
+      ml = p + a.s_columns * a.hd + c * 2;
+    } else {
+      const size_t at = I.at(col, a.nKV * a.G, 1);
+      o = a.prior + at * a.hd;
+      ml = a.prior_ml + at * 2;
+    }
   }
-  return o;
+};
+// Splits w, w + by, .. of a column's prior as if their keys were among those seen:
+// into its m, its sum l and its O, of which load(dims of a split, x) takes this lane's.
+// The lanes of a column are those that differ in lane / 16; l is counted once.
+template <int N, class LOAD, class ADD>
+__device__ __forceinline__ void add_prior(const float* o, const float* ml, size_t stride, uint32_t splits, uint32_t w,
+                                          uint32_t by, bool lead, float& m, float& l, LOAD load, ADD add) {
+  constexpr uint32_t BATCH = N > 16 ? 4 : 8;
+  for (uint32_t s0 = w; s0 < splits; s0 += BATCH * by) {
+    float x[BATCH][N], pm[BATCH], pl[BATCH];
+#pragma unroll
+    for (uint32_t j = 0; j < BATCH; j++) {
+      const size_t at = (s0 + j * by < splits ? s0 + j * by : s0) * stride;
+      pm[j] = ml[at];
+      pl[j] = ml[at + 1];
+      load(o + at, x[j]);
+    }
+    float M = m;
+#pragma unroll
+    for (uint32_t j = 0; j < BATCH; j++) M = fmaxf(M, pm[j]);  // (one behind the last is the batch's first again)
+    const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - M);
+    float p[BATCH];
+    l *= f;
+#pragma unroll
+    for (uint32_t j = 0; j < BATCH; j++) {
+      p[j] = s0 + j * by >= splits || pm[j] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(pm[j] - M);
+      if (lead) l = __builtin_fmaf(p[j], pl[j], l);
+    }
+    m = M;
+    add(f, p, x);
+  }
 }
+
 template <Reach R>
 __device__ __forceinline__ float* place(const Args<R>& a, const Item<R>& I, uint32_t col) {
   if constexpr (R == SHARED) return a.prior + I.at(col, a.nKV * a.G * a.hd, a.hd);
   else return a.out + I.at(col, a.ld_out, a.hd);
+}
+// of a split's partial; SHARED's are read by the launch behind it
+template <Reach R>
+__device__ __forceinline__ void put_part(float* p, float a, float b) {
+  if constexpr (R == SHARED) *(f32x2*)p = (f32x2){a, b};
+  else put2(p, a, b);
 }
 // SHARED: and a column's m and l
 template <Reach R>
@@ -824,12 +868,6 @@ __device__ __forceinline__ void keep_ml(const Args<R>& a, const Item<R>& I, uint
     to[1] = l;
   }
 }
-template <int W>
-struct Dims {
-  float v[W];
-  __device__ __forceinline__ float& operator[](int d) { return v[d]; }
-};
-
 template <uint32_t N_>
 struct Count {
   static constexpr uint32_t N = N_;
@@ -898,20 +936,10 @@ __device__ __forceinline__ void join_16(const Args<R>& a, const Item<R>& I, floa
       if (s0 >= ns) break;
       load(e, s0);
     }
-    const float l = s_ml[64 + k] + s_ml[80 + k] + s_ml[96 + k] + s_ml[112 + k];
-    if constexpr (R == ALL) {
-      const float inv = 1.0f / l;
-      float* y = a.out + I.at(k, a.ld_out, hd) + d;
-      y[0] = o.x * inv;
-      y[1] = o.y * inv;
-    } else {
-      const float m = fmaxf(fmaxf(s_ml[k], s_ml[16 + k]), fmaxf(s_ml[32 + k], s_ml[48 + k]));
-      const Dims<2> z = finished<R, 2>(a, I, k, d, Dims<2>{{o.x, o.y}}, l, m);
-      float* y = place<R>(a, I, k) + d;
-      y[0] = z.v[0];
-      y[1] = z.v[1];
-      if (d == 0) keep_ml<R>(a, I, k, m, l);
-    }
+    const float inv = 1.0f / (s_ml[64 + k] + s_ml[80 + k] + s_ml[96 + k] + s_ml[112 + k]);
+    float* y = a.out + I.at(k, a.ld_out, hd) + d;
+    y[0] = o.x * inv;
+    y[1] = o.y * inv;
   }
 }
 
@@ -947,8 +975,6 @@ __device__ __forceinline__ void join_many(const Args<R>& a, const Item<R>& I, ui
     s[tid] = mx;
     __syncthreads();
     for (uint32_t k = 0; k < groups; k++) mx = fmaxf(mx, s[(k << lw) + c]);
-    __shared__ float s_mx[R == ALL ? 1 : 128];
-    if (R != ALL && tid < width) s_mx[tid] = mx;
     for (uint32_t k = group; k < ns; k += groups) {
       const float m = s_m[(k << lw) + c], f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mx);
       s_m[(k << lw) + c] = f;
@@ -962,12 +988,7 @@ __device__ __forceinline__ void join_many(const Args<R>& a, const Item<R>& I, ui
       const uint32_t k = small_quotient(e, hd);
       float tot = 0.f;
       for (uint32_t g = 0; g < groups; g++) tot += s[(g << lw) + k];
-      if constexpr (R == ALL) {
-        store4(a.out + I.at(c0 + k, a.ld_out, hd) + (e - k * hd), o * (1.0f / tot));
-      } else {
-        store4(place<R>(a, I, c0 + k) + (e - k * hd), finished<R, 4>(a, I, c0 + k, e - k * hd, o, tot, s_mx[k]));
-        if (e == k * hd) keep_ml<R>(a, I, c0 + k, s_mx[k], tot);
-      }
+      store4(a.out + I.at(c0 + k, a.ld_out, hd) + (e - k * hd), o * (1.0f / tot));
     };
     // four dims at a time, all loads of 8 such in flight where there are few splits,
     // of 8 splits where there are many; what is behind the last split or dim is
@@ -1072,16 +1093,39 @@ __device__ __forceinline__ const Args<R>& again() {
   asm volatile("" : "+s"(p));
   return *(const Args<R>*)p;
 }
-// SHARED: the shared keys of each request, for the call that follows
-template <Reach R>
-__device__ __forceinline__ void tell_requests(const Args<R>& a) {
-  if constexpr (R == SHARED)
+// SHARED: each request's group, for the call that follows
+template <bool SORT, Reach R>
+__device__ __forceinline__ void tell_requests(const Args<R>& a, const Items<SORT, R>& t) {
+  if constexpr (R == SHARED) {
+    if (a.n_req <= 64) __syncthreads();  // each wave has written the table for itself
     for (uint32_t g = blockIdx.x; g < a.n_req; g += gridDim.x) {
       const int32_t g0 = a.group_start[g], g1 = a.group_start[g + 1], l = a.shared[g];
       if (g0 < 0 || g1 < g0 || (uint32_t)g1 > a.n_all) continue;
       const bool fits = l >= 0 && (uint64_t)(uint32_t)l <= ((uint64_t)a.max_pages << a.shift);
-      for (uint32_t b = (uint32_t)g0 + threadIdx.x; b < (uint32_t)g1; b += 256) a.from[b] = fits ? l : -1;
+      const uint32_t n = t.row[g + 1] - t.row[g];
+      const SharedOf f = {fits ? l : -1, t.part[g], t.splits(t.len[g], t.inv_c), t.row[g], div_up(n, a.rows_blk) * a.groups};
+      for (uint32_t b = (uint32_t)g0 + threadIdx.x; b < (uint32_t)g1; b += 256) a.from[b] = f;
     }
+  }
+}
+// OWN of whole requests: nobody reads the groups, but what is wrong with them is told
+template <Reach R>
+__device__ __forceinline__ void check_groups(const Args<R>& a) {
+  if constexpr (R == OWN) {
+    if (!a.whole || blockIdx.x + 1 != gridDim.x) return;
+    for (uint32_t g = threadIdx.x; g < a.n_groups; g += 256) {
+      const int32_t g0 = a.group_start[g], g1 = a.group_start[g + 1], l = a.shared[g];
+      if (g0 < 0 || g1 < g0 || (uint32_t)g1 > a.n_req || (g == 0 && g0) || (g + 1 == a.n_groups && (uint32_t)g1 != a.n_req) ||
+          l < 0 || (uint64_t)(uint32_t)l > ((uint64_t)a.max_pages << a.shift)) {
+        paged_err(a.err, PAGED_ERR_ATT_GROUP, g);
+        continue;
+      }
+      for (int32_t b = g0; l && b < g1; b++) {
+        const int32_t n = a.row_start ? a.row_start[b + 1] - a.row_start[b] : 1;
+        if (n > 0 && l > a.lens[b] - n) paged_err(a.err, PAGED_ERR_ATT_SHARED, (uint32_t)b);
+      }
+    }
+  }
 }
 // a request's block table (SHARED: that of the group's first)
 template <Reach R>
@@ -1113,15 +1157,18 @@ __device__ __forceinline__ void attention_body(const Args<R>& args) {
   float* s_ml = s_o + OFLOATS;  // [4 waves][16 columns][m, l]
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t ln = lane & 15, lg = lane >> 4;
-  tell_requests<R>(args);
   Items<false, R> items;
   find_items<false, R>(args, (uint32_t*)(s_ml + 4 * 16 * 2), items);
+  tell_requests<false, R>(args, items);
 
   for (Turn turn(items.total, false); turn.item < items.total; turn.next(again<R>(), items.total)) {
     const Args<R>& a = again<R>();
     const uint32_t P = 1u << a.shift, hd = a.hd;
     const Item<R> I(a, items, turn.item, CB, TK);
     const uint32_t k0 = I.k0, k1 = I.k1, kvh = I.kvh;
+    SharedOf of;
+    if constexpr (R == OWN)
+      if (!a.whole) of = a.from[I.b];
     f32x4 q_raw[TILE::QRAW];
     TILE::load_q(a.q + I.at(ln < I.ncols ? ln : 0, a.ld_q, hd), lg, hd, q_raw);
 
@@ -1277,6 +1324,40 @@ __device__ __forceinline__ void attention_body(const Args<R>& args) {
     for (int i = 0; i < 4; i++)
 #pragma unroll
       for (int d = 0; d < DPL; d++) s_o[(w * 16 + ln) * OS + (4 * lg + i) * DPL + d] = O[d][i];
+    if constexpr (R == OWN) {
+      // four columns to a wave, 16 lanes each; of few columns the prior's splits go to
+      // several waves in turn.  A wave adds its share to what it has just written.
+      const uint32_t few = I.ncols <= 4 ? 4 : I.ncols <= 8 ? 2 : 1, c = w / few * 4 + lg;
+      if (!z.whole && I.split == 0 && c < I.ncols) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (ln * DPL < z.hd) {
+          const Prior<R> prior(z, I, of, c);
+          float *so = s_o + (w * 16 + c) * OS + ln * DPL, *sml = s_ml + (w * 16 + c) * 2, y[DPL], pm = sml[0], pl = sml[1];
+#pragma unroll
+          for (int d = 0; d < DPL; d++) y[d] = so[d];
+          add_prior<DPL>(prior.o + first_dim<DPL>(ln, z.hd), prior.ml, prior.stride, uniform(of.splits), w % few, few, true, pm, pl,
+                         [&](const float* o, float(&x)[DPL]) {
+                           const Words<DPL> v = *(const Words<DPL>*)o;
+#pragma unroll
+                           for (int d = 0; d < DPL; d++) x[d] = __uint_as_float(v.w[d]);
+                         },
+                         [&](float f, const auto& p, const auto& x) {
+#pragma unroll
+                           for (int d = 0; d < DPL; d++) {
+                             y[d] *= f;
+#pragma unroll
+                             for (uint32_t j = 0; j < sizeof(p) / 4; j++) y[d] = __builtin_fmaf(p[j], x[j][d], y[d]);
+                           }
+                         });
+#pragma unroll
+          for (int d = 0; d < DPL; d++) so[d] = y[d];
+          if (ln == 0) {
+            sml[0] = pm;
+            sml[1] = pl;
+          }
+        }
+      }
+    }
     __syncthreads();
     const uint32_t col = tid >> 4, at = (tid & 15) * DPL;
     float mx = s_ml[col * 2];
@@ -1297,32 +1378,22 @@ __device__ __forceinline__ void attention_body(const Args<R>& args) {
     if (col < I.ncols && at < z.hd) {
       const uint32_t d0 = first_dim<DPL>(tid & 15, z.hd);
       if (I.ns == 1) {
+        const float inv = R == SHARED ? 1.f : I.keys ? 1.0f / sum : 0.f;
+        float* y = place<R>(z, I, col) + d0;
         Words<DPL> x;
-        float* y;
-        if constexpr (R == ALL) {
-          const float inv = I.keys ? 1.0f / sum : 0.f;
-          y = z.out + I.at(col, z.ld_out, z.hd) + d0;
 #pragma unroll
-          for (int d = 0; d < DPL; d++) x.w[d] = __float_as_uint(o[d] * inv);
-        } else {
-          Dims<DPL> v;
-#pragma unroll
-          for (int d = 0; d < DPL; d++) v[d] = o[d];
-          v = finished<R, DPL>(z, I, col, d0, v, sum, mx);
-          y = place<R>(z, I, col) + d0;
-#pragma unroll
-          for (int d = 0; d < DPL; d++) x.w[d] = __float_as_uint(v[d]);
-          if (d0 == 0) keep_ml<R>(z, I, col, mx, sum);
-        }
+        for (int d = 0; d < DPL; d++) x.w[d] = __float_as_uint(o[d] * inv);
+        if (d0 == 0) keep_ml<R>(z, I, col, mx, sum);
         *(Words<DPL>*)y = x;
       } else {
 #pragma unroll
-        for (int d = 0; d < DPL; d += 2) put2(mine + col * z.hd + d0 + d, o[d], o[d + 1]);
-        if (d0 == 0) put2(mine + CB * z.hd + col * 2, mx, sum);
+        for (int d = 0; d < DPL; d += 2) put_part<R>(mine + col * z.hd + d0 + d, o[d], o[d + 1]);
+        if (d0 == 0) put_part<R>(mine + CB * z.hd + col * 2, mx, sum);
       }
     }
-    if (I.ns > 1) join_16<R>(z, I, s_o);
+    if (R != SHARED && I.ns > 1) join_16<R>(z, I, s_o);
   }
+  check_groups<R>(again<R>());
 }
 
 // ---------------------------------------------------------------------------
@@ -1378,12 +1449,12 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t r) {
 template <int DPL>
 constexpr uint32_t LINE = DPL <= 4 ? 4 : 8;
 
-template <class MM_, int DPL>
+template <class MM_, int DPL, int CT_ = 2>
 struct Rows16 {
   typedef MM_ MM;
   typedef Tile16<MM, DPL> TILE;
   typedef typename MM::T T;
-  static constexpr int CT = 2, KT = 64, NJ = KT / 16, TERMS = MM::TERMS;
+  static constexpr int CT = CT_, KT = 64, NJ = KT / 16, TERMS = MM::TERMS;
   static constexpr uint32_t CHUNKS = 2 * LINE<DPL>, ROWB = 32 * LINE<DPL>;
   // scores of the CT tiles' columns against the stage's keys
   template <class BETWEEN>
@@ -1537,15 +1608,18 @@ __device__ __forceinline__ void attention_rows_body(const Args<R>& args) {
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t ln = lane & 15, lg = lane >> 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  tell_requests<R>(args);
   Items<true, R> items;
   find_items<true, R>(args, s_odd + 4, items);
+  tell_requests<true, R>(args, items);
 
   for (Turn turn(items.total, true); turn.item < items.total; turn.next(again<R>(), items.total)) {
     const Args<R>& a = again<R>();
     const uint32_t P = 1u << a.shift, hd = a.hd;
     const Item<R> I(a, items, turn.item, CB, KT);
     const uint32_t k0 = I.k0, k1 = I.k1;
+    SharedOf of;
+    if constexpr (R == OWN)
+      if (!a.whole) of = a.from[I.b];
     // ---- this wave's share of a stage: KT / 4 rows of K and of V, 8 or 16, a page to 8 ----
     constexpr uint32_t SHARE = KT / 4, RPI = 1024 / ROWB, PARTS = SHARE / 8, INSTR = 8 / RPI;  // rows, instructions to 8 rows
     constexpr uint32_t AHEAD = 64 / PARTS;
@@ -1705,35 +1779,53 @@ __device__ __forceinline__ void attention_rows_body(const Args<R>& args) {
 #pragma unroll
     for (int t = 0; t < CT; t++) {
       const uint32_t col = (w * CT + t) * 16 + ln;
+      if constexpr (R == OWN) {
+        if (!z.whole && I.split == 0 && col < I.ncols) {
+          const Prior<R> prior(z, I, of, col);
+          add_prior<4 * DPL>(prior.o, prior.ml, prior.stride, uniform(of.splits), 0, 1, lg == 0, m[t], l[t],
+                             [&](const float* o, float(&x)[4 * DPL]) {
+#pragma unroll
+                               for (int d = 0; d < DPL; d++) {
+                                 const f32x4 v = load8(o + (16 * d + 4 * lg < z.hd ? 16 * d + 4 * lg : 0));
+#pragma unroll
+                                 for (int i = 0; i < 4; i++) x[4 * d + i] = v[i];
+                               }
+                             },
+                             [&](float f, const auto& p, const auto& x) {
+#pragma unroll
+                               for (int d = 0; d < DPL; d++)
+#pragma unroll
+                                 for (int i = 0; i < 4; i++) {
+                                   float o = O[t][d][i] * f;
+#pragma unroll
+                                   for (uint32_t j = 0; j < sizeof(p) / 4; j++) o = __builtin_fmaf(p[j], x[j][4 * d + i], o);
+                                   O[t][d][i] = o;
+                                 }
+                             });
+        }
+      }
       l[t] = add_xor32(add_xor16(l[t]));
       if (col >= I.ncols) continue;
       if (I.ns == 1) {
-        if constexpr (R == ALL) {
-          const float inv = I.keys ? 1.0f / l[t] : 0.f;
-          float* y = z.out + I.at(col, z.ld_out, z.hd) + 4 * lg;
+        const float inv = R == SHARED ? 1.f : I.keys ? 1.0f / l[t] : 0.f;
+        float* y = place<R>(z, I, col) + 4 * lg;
 #pragma unroll
-          for (int d = 0; d < DPL; d++)
-            if (16 * d + 4 * lg < z.hd) store4(y + 16 * d, O[t][d] * inv);
-        } else {
-          float* y = place<R>(z, I, col) + 4 * lg;
-#pragma unroll
-          for (int d = 0; d < DPL; d++)
-            if (16 * d + 4 * lg < z.hd)
-              store4(y + 16 * d, finished<R, 4>(z, I, col, 16 * d + 4 * lg, O[t][d], l[t], m[t]));
-          if (lg == 0) keep_ml<R>(z, I, col, m[t], l[t]);
-        }
+        for (int d = 0; d < DPL; d++)
+          if (16 * d + 4 * lg < z.hd) store4(y + 16 * d, O[t][d] * inv);
+        if (lg == 0) keep_ml<R>(z, I, col, m[t], l[t]);
       } else {
 #pragma unroll
         for (int d = 0; d < DPL; d++)
           if (16 * d + 4 * lg < z.hd) {
-            put2(mine + col * z.hd + 16 * d + 4 * lg, O[t][d][0], O[t][d][1]);
-            put2(mine + col * z.hd + 16 * d + 4 * lg + 2, O[t][d][2], O[t][d][3]);
+            put_part<R>(mine + col * z.hd + 16 * d + 4 * lg, O[t][d][0], O[t][d][1]);
+            put_part<R>(mine + col * z.hd + 16 * d + 4 * lg + 2, O[t][d][2], O[t][d][3]);
           }
-        if (lg == 0) put2(mine + CB * z.hd + col * 2, m[t], l[t]);
+        if (lg == 0) put_part<R>(mine + CB * z.hd + col * 2, m[t], l[t]);
       }
     }
-    if (I.ns > 1) join_many<R>(z, I, CB, (float*)lds, REGION);
+    if (R != SHARED && I.ns > 1) join_many<R>(z, I, CB, (float*)lds, REGION);
   }
+  check_groups<R>(again<R>());
 }
 
 #define DEF_ATTENTION(NAME, REACH, BODY, ...)                             \
@@ -1771,3 +1863,19 @@ typedef Rows16<MmBf16, 8> RowsBf16d128;
   DEF_ATTENTIONS(OF, REACH, bf16, 64, 4, TileBf16d64, RowsBf16d64)              \
   DEF_ATTENTIONS(OF, REACH, bf16, 96, 6, TileBf16d96, RowsBf16d96)              \
   DEF_ATTENTIONS(OF, REACH, bf16, 128, 8, TileBf16d128, RowsBf16d128)
+// The others' blocks of many columns have 64, a tile to a wave.  Two cost them more than
+// the products that share an operand save: shorter items fill the card better.  32
+// heads on 8 of 128 dims, f16 | bf16, 128 columns and 64: a window of 2048, 1500 rows
+// 132, 127 | 170, 146 us, 300 rows 55, 42 | 68, 46; 64 rows on 1000 shared keys 25.5,
+// 20.8 | 30.4, 22.0, 128 on 16000 103, 101 | 125, 117.
+#define PACK(...) __VA_ARGS__
+#define DEF_PART_ATTENTIONS(OF, REACH)                                                          \
+  DEF_ATTENTIONS(OF, REACH, f32, 64, 4, Tile32<4>, Rows32<4>)                                   \
+  DEF_ATTENTIONS(OF, REACH, f32, 96, 6, Tile32<6>, Rows32<6>)                                   \
+  DEF_ATTENTIONS(OF, REACH, f32, 128, 8, Tile32<8>, Rows32<8>)                                  \
+  DEF_ATTENTIONS(OF, REACH, f16, 64, 4, TileF16d64, PACK(Rows16<MmF16, 4, 1>))                  \
+  DEF_ATTENTIONS(OF, REACH, f16, 96, 6, TileF16d96, PACK(Rows16<MmF16, 6, 1>))                  \
+  DEF_ATTENTIONS(OF, REACH, f16, 128, 8, TileF16d128, PACK(Rows16<MmF16, 8, 1>))                \
+  DEF_ATTENTIONS(OF, REACH, bf16, 64, 4, TileBf16d64, PACK(Rows16<MmBf16, 4, 1>))               \
+  DEF_ATTENTIONS(OF, REACH, bf16, 96, 6, TileBf16d96, PACK(Rows16<MmBf16, 6, 1>))               \
+  DEF_ATTENTIONS(OF, REACH, bf16, 128, 8, TileBf16d128, PACK(Rows16<MmBf16, 8, 1>))

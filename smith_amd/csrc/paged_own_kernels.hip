@@ -2,4 +2,4 @@
 // (smith_paged_own.hsaco): each request's own keys, joined with the shared ones.
 #include "paged_attention.h"
 
-DEF_ALL_ATTENTIONS(_own, OWN)
+DEF_PART_ATTENTIONS(_own, OWN)

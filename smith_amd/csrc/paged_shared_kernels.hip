@@ -3,4 +3,4 @@
 // common, once for all their columns.
 #include "paged_attention.h"
 
-DEF_ALL_ATTENTIONS(_shared, SHARED)
+DEF_PART_ATTENTIONS(_shared, SHARED)

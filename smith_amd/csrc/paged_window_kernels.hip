@@ -2,4 +2,4 @@
 // (smith_paged_window.hsaco): rows see the first keys and a window of the last.
 #include "paged_attention.h"
 
-DEF_ALL_ATTENTIONS(_window, WINDOW)
+DEF_PART_ATTENTIONS(_window, WINDOW)

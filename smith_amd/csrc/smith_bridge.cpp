@@ -2517,22 +2517,34 @@ static bool many_columns(const AttCall& k) {
   return k.row_start && k.shift >= 3 && (uint64_t)k.max_rows * G > 24ull * k.n_req && (uint64_t)k.max_rows * k.n_heads >= 8192;
 }
 
-// `n` requests (or groups) of k, by one of the two kernels of `of` (""; _window, _shared or _own)
-static int launch_attention(Ctx* c, const AttCall& k, const char* of, uint32_t n, bool many, ReachArgs* more) {
+constexpr uint32_t ATT_TARGET = 512;  // items wanted: two workgroups to a CU
+// a block that is cut has more than 5/4 C keys and so less than twice its keys / C
+// splits: 2 W / C <= 2 target of them in all (and some for what f32 rounds)
+constexpr uint32_t ATT_MAX_PARTS = 2 * ATT_TARGET + 16;
+
+// `n` requests (or groups) of k, by the kernel of `of` ("", _window, _shared or _own) whose blocks have CB columns
+static int launch_attention(Ctx* c, const AttCall& k, const char* of, uint32_t n, uint32_t CB, ReachArgs* more) {
   const uint32_t G = k.n_heads / k.n_kv_heads;
-  const bool small = !many && k.shift < 4;
-  const uint32_t CB = !many ? 16 : k.kv_type == SMITH_KV_F32 ? 64 : 128;
+  const bool many = CB > 16, small = !many && k.shift < 4;
   const uint32_t dims = k.head_dim <= 64 ? 64 : k.head_dim <= 96 ? 96 : 128;
-  const uint32_t target = 512;  // two workgroups to a CU
+  const uint32_t target = ATT_TARGET;
   // Keys to a split at least.  A split of many columns leaves 64 KB and the join
   // reads them again: 64 rows behind 8000 keys, 32 heads, in that kernel 58 us (f16) and
   // 69 (bf16) with 512, 64 and 77 with 768, 74 and 84 with 384; 300 rows of a prompt 20.8
   // uncut, 24.8 with 128.  f32 keys are eight times the work: 20 requests, half of them
   // with chunks of up to 77 rows, 63 us with 256, 70 with 384, 80 with 512.
-  const float split_min = !many ? 128.f : k.kv_type == SMITH_KV_F32 ? 256.f : 512.f;
-  // a block that is cut has more than 5/4 C keys and so less than twice its keys / C
-  // splits: 2 W / C <= 2 target of them in all (and some for what f32 rounds)
-  const uint32_t max_parts = 2 * target + 16;
+  // The others' blocks of 64 columns leave half of that, and those of shared keys no
+  // join: 4 requests behind 700 f32 keys 13.8 us with 64, 14.8 with 128; 3 of a window
+  // of 512 8.9 and 9.7; 64 requests behind 6001 f16 keys 40.5 with 128, 59 with 512; 16
+  // rows of a window of 2048 (blocks of 16) 20.4 with 128.  Requests' own keys: 64
+  // requests of 1 to 300 22 us with 128, 14.5 with 256 (one item each).
+  const bool f32 = k.kv_type == SMITH_KV_F32;
+  const float split_min = !*of ? !many ? 128.f : f32 ? 256.f : 512.f
+                          : !strcmp(of, "_own")    ? 256.f
+                          : !strcmp(of, "_shared") ? f32 ? 64.f : 128.f
+                          : !many                  ? f32 ? 64.f : 128.f
+                                                   : f32 ? 128.f : 256.f;
+  const uint32_t max_parts = ATT_MAX_PARTS;
   if (ensure(c, &c->paged_ws, &c->paged_ws_bytes, (size_t)max_parts * CB * (k.head_dim + 2) * sizeof(float))) return -1;
   if (ensure_paged_counters(c)) return -1;
   const uint32_t heads_blk = std::min(G, CB), RB = CB / heads_blk, groups = (G + CB - 1) / CB;
@@ -2557,6 +2569,7 @@ static int launch_attention(Ctx* c, const AttCall& k, const char* of, uint32_t n
   void* args[] = {&a};
   if (more) {
     (AttArgs&)*more = a;
+    if (!strcmp(of, "_shared")) more->parts = (float*)more->s_parts;  // they stay until the own keys are through
     // WINDOW: the keys that a block visits, with those that fill tiles up
     const uint64_t unit = many ? (k.kv_type == SMITH_KV_F32 ? 32 : 64) : k.kv_type == SMITH_KV_F32 ? 16 : 32;
     more->most_keys = (uint32_t)std::min<uint64_t>(0x7FFFFFFFu, (uint64_t)more->window + more->sinks + RB + 3 * unit);
@@ -2576,7 +2589,7 @@ int smith_paged_attention(void* ctx, uint32_t kv_type, const float* q, uint32_t 
                n_kv_heads, head_dim, scale, kpages, vpages, n_pages, page_size, out, ld_out, 0};
   if (check_attention(c, k)) return -1;
   if (!max_rows) return 0;
-  return launch_attention(c, k, "", n_req, many_columns(k), nullptr);
+  return launch_attention(c, k, "", n_req, !many_columns(k) ? 16 : kv_type == SMITH_KV_F32 ? 64 : 128, nullptr);
 }
 
 int smith_paged_attention_window(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
@@ -2594,8 +2607,20 @@ int smith_paged_attention_window(void* ctx, uint32_t kv_type, const float* q, ui
   ReachArgs more = {};
   more.window = std::min(window, 0x7FFFFFFFu);  // as long as a request can be
   more.sinks = std::min(sinks, 0x7FFFFFFFu);
-  return launch_attention(c, k, "_window", n_req, many_columns(k), &more);
+  // Blocks of 64 columns pay where the rows' windows are enough work for them.
+  // Microseconds, 16 and 64 columns (32 heads on 8 of 128 unless said, f16 | f32): a window
+  // of 2048, 64 rows of a prompt 26, 28 | 42, 46; 128 rows 35, 31 | 66, 62; 200 rows 46, 35
+  // | 105, 95; 300 rows 70, 42 | 152, 121; 1500 rows 271, 129 | 600, 505; 16 heads on 4 of 64,
+  // 200 rows 23, 21 | 36, 37; 1500 rows 85, 53 | 162, 181; windows of 500, 16 requests of 30
+  // rows 20, 25 | 37, 50, 4 of 500 rows 81, 52 | 135, 146; of 2000, 8 of 100 rows 78, 50 |
+  // 150, 167; of 1024, 600 rows 72, 51 | 137, 172.
+  const uint64_t seen = std::min<uint64_t>((uint64_t)more.window + more.sinks, (uint64_t)max_pages << k.shift);
+  const bool many = row_start && k.shift >= 3 && (uint64_t)max_rows * (n_heads / n_kv_heads) > 24ull * n_req &&
+                    (uint64_t)max_rows * n_heads * seen >= (kv_type == SMITH_KV_F32 ? 64ull << 20 : 8ull << 20);
+  return launch_attention(c, k, "_window", n_req, many ? 64 : 16, &more);
 }
+
+constexpr uint64_t SHARED_ROOM = 48ull << 20;
 
 int smith_paged_attention_shared(void* ctx, uint32_t kv_type, const float* q, uint32_t ld_q, uint32_t max_rows,
                                  const int32_t* row_start, const int32_t* lens, const int32_t* tables, uint32_t n_req,
@@ -2610,20 +2635,38 @@ int smith_paged_attention_shared(void* ctx, uint32_t kv_type, const float* q, ui
   if (!n_groups || n_groups > n_req) return fail(c, "%s: %u groups of %u requests", k.fn, n_groups, n_req);
   if (!max_rows) return 0;
   if (!group_start || !shared) return fail(c, "%s: null buffer", k.fn);
-  // of each column what its shared keys give, and of each request how many they are
-  const size_t H = n_heads, floats = (size_t)max_rows * H * (head_dim + 2);
-  if (ensure(c, &c->paged_prior, &c->paged_prior_bytes, (floats + n_req) * 4)) return -1;
   ReachArgs more = {};
   more.n_groups = n_groups;
   more.n_all = n_req;
   more.group_start = group_start;
   more.shared = shared;
+  // Where the block tables have no room for more keys than are read in the time of a
+  // launch each request reads its own: 4 requests behind 700 f32 keys of 4 heads of 64
+  // 10.5 us, apart 14; behind 1000 f16 keys of 8 heads of 128 11.2, 16.8 (17 MB), 8 requests
+  // behind 1200 13, 17 (40 MB).
+  const uint64_t room = pool_bytes(kv_type, n_kv_heads, head_dim, n_req, 1) * 2 * ((uint64_t)max_pages << k.shift);
+  more.whole = room <= SHARED_ROOM;
+  if (more.whole) return launch_attention(c, k, "_own", n_req, many_columns(k) ? 64 : 16, &more);
+  // of each column what its shared keys give, and of each request how many they are
+  const size_t H = n_heads, floats = (size_t)max_rows * H * (head_dim + 2), parts = (size_t)ATT_MAX_PARTS * 64 * (head_dim + 2);
+  if (ensure(c, &c->paged_prior, &c->paged_prior_bytes, (floats + parts) * 4 + n_req * sizeof(SharedOf))) return -1;
   more.prior = (float*)c->paged_prior;
   more.prior_ml = more.prior + (size_t)max_rows * H * head_dim;
-  more.from = (int32_t*)(more.prior + floats);
-  const bool many = k.shift >= 3 && (uint64_t)max_rows * (n_heads / n_kv_heads) >= 48ull * n_groups;
-  if (launch_attention(c, k, "_shared", n_groups, many, &more)) return -1;
-  return launch_attention(c, k, "_own", n_req, many_columns(k), &more);
+  more.from = (SharedOf*)(more.prior + floats + parts);
+  more.s_parts = more.prior + floats;
+  // Blocks of 16 columns or of 64, by the columns of a KV head and group, about.
+  // Microseconds with the own keys, 1 group unless said (32 heads on 8 of 128, f16 | f32),
+  // 16 and 64: 32 columns behind 2000 keys 17.2, 18.1 | 20, 28; 48 behind 3000 19.9, 19.2
+  // | 26, 30; 64 behind 4000 21.8, 20.5 | 33, 32; 256 behind 1000 21.8, 20.8 | 32, 33; 512 behind
+  // 16000 173, 101 | 395, 363; 20 groups of 32 behind 2000 60, 54 | 88, 101.
+  const uint64_t columns = (uint64_t)max_rows * (n_heads / n_kv_heads) / n_groups;
+  const uint32_t CB = k.shift < 3 || columns < (kv_type == SMITH_KV_F32 ? 64 : 48) ? 16 : 64;
+  if (launch_attention(c, k, "_shared", n_groups, CB, &more)) return -1;
+  more.s_columns = CB;
+  more.s_rows_blk = more.rows_blk;
+  more.s_heads_blk = more.heads_blk;
+  more.s_groups = more.groups;
+  return launch_attention(c, k, "_own", n_req, many_columns(k) ? 64 : 16, &more);
 }
 
 // The state and map of fork and compact: as ensure(), and zero.

@@ -12,7 +12,14 @@ pytestmark = pytest.mark.gpu
 TYPES = ["f32", "f16", "bf16"]
 
 
-def case(seed, dtype, H, nKV, D, P, widths, shared, own, added, q_std=2.0):
+# keys that the block tables have room for, so that the shared keys are computed apart: 48 MB and more
+def wide(tables, nKV, D, dtype, P):
+    keys = (48 << 20) // (2 * nKV * D * (4 if dtype == "f32" else 2)) // len(tables)
+    more = max(0, keys // P + 1 - tables.shape[1])
+    return np.concatenate([tables, np.full((len(tables), more), 2 ** 31 - 1, np.int32)], 1)
+
+
+def case(seed, dtype, H, nKV, D, P, widths, shared, own, added, q_std=2.0, apart=True):
     """Groups of widths[g] requests, the first shared[g] keys of each the same (a
     partly filled page a copy), own[b] keys behind them, the last added[b] of rows."""
     rs = np.random.RandomState(seed)
@@ -39,6 +46,8 @@ def case(seed, dtype, H, nKV, D, P, widths, shared, own, added, q_std=2.0):
         if b != first and part:
             for pool in (k, v):
                 pool[tables[b, full], :, :part] = pool[tables[first, full], :, :part]
+    if apart:
+        tables = wide(tables, nKV, D, dtype, P)
     q = (rs.standard_normal((int(added.sum()), H, D)) * q_std).astype(np.float32)
     row_start = np.concatenate([[0], np.cumsum(added)]).astype(np.int32)
     return q, row_start, lens, tables, k, v, start.astype(np.int32), shared.astype(np.int32)
@@ -70,22 +79,24 @@ def check(got, c, dtype, scale=None, seen=everything):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shared", [0, 1, 7, 15, 16, 17, 31, 64, 65, 100, 128, 300, 1000])
 @pytest.mark.parametrize("P", [4, 16, 64])
-def test_one_group(dtype, shared, P):
+@pytest.mark.parametrize("apart", [True, False])
+def test_one_group(dtype, shared, P, apart):
     own = np.array([1, 2, 16, 33, 60])
-    c = case(shared + P, dtype, 4, 2, 32, P, [5], shared, own, 1)
+    c = case(shared + P, dtype, 4, 2, 32, P, [5], shared, own, 1, apart=apart)
     check(run(*c, False), c, dtype)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("H,nKV,D,P", [(1, 1, 8, 1), (9, 3, 64, 8), (10, 2, 80, 32), (12, 4, 96, 16), (20, 1, 128, 128), (33, 1, 40, 2)])
 @pytest.mark.parametrize("ragged", [False, True])
-def test_heads_pages_and_groups(dtype, H, nKV, D, P, ragged):
+@pytest.mark.parametrize("apart", [True, False])
+def test_heads_pages_and_groups(dtype, H, nKV, D, P, ragged, apart):
     """Groups of one and of many requests, with and without shared keys, requests that sit out."""
     rs = np.random.RandomState(H)
     widths = [1, 7, 2, 1, 12]
     own = rs.randint(4, 50, 23)
     added = rs.randint(0, 5, 23) if ragged else 1
-    c = case(H + D, dtype, H, nKV, D, P, widths, [40, 133, 0, 0, 70], own, added)
+    c = case(H + D, dtype, H, nKV, D, P, widths, [40, 133, 0, 0, 70], own, added, apart=apart)
     check(run(*c, ragged), c, dtype)
 
 
@@ -207,8 +218,10 @@ def test_strides_and_rows_behind_the_last(ragged):
     ("short", "request 1: more shared keys", [1]), ("negative", "group 0: ", [0, 1, 2]), ("long", "group 0: ", [0, 1, 2]),
     ("start", "group 0: ", [0, 1, 2, 3, 4]), ("order", "group ", [0, 1, 2, 3, 4]), ("end", "group 1: ", [3, 4]), ("len", "request 4: its length", [4]),
     ("page", "request 0: a page outside", [0, 1, 2])])
-def test_leaves_out_what_does_not_fit(bad, message, lost):
-    c = q, row_start, lens, tables, k, v, start, shared = case(5, "f16", 4, 2, 32, 16, [3, 2], [40, 20], [5, 6, 7, 8, 9], 1)
+@pytest.mark.parametrize("apart", [True, False])
+def test_leaves_out_what_does_not_fit(bad, message, lost, apart):
+    c = q, row_start, lens, tables, k, v, start, shared = case(5, "f16", 4, 2, 32, 16, [3, 2], [40, 20], [5, 6, 7, 8, 9], 1,
+                                                               apart=apart)
     lens, start, shared, now = lens.copy(), start.copy(), shared.copy(), tables.copy()
     if bad == "short":
         lens[1] = 40
@@ -226,13 +239,15 @@ def test_leaves_out_what_does_not_fit(bad, message, lost):
         lens[4] = -1
     else:
         now[0, 1] = k.shape[0]
+        if not apart:
+            message = "a page outside"
     out = R.upload(np.full((5, 128), 5, np.float32))
     S.pagedAttention(R.upload(q.reshape(5, -1)), i32(lens), i32(now), R.upload(k), R.upload(v), None, 0.0, out,
                      groupStart=i32(start), shared=i32(shared))
     assert message in sync_error()
     device.sync()
     got = out.data
-    if bad in ("short", "len"):
+    if bad == "len":
         assert (got[lost] == 5).all()
     rest = [b for b in range(5) if b not in lost]
     want = P_.attention(q.astype(np.float64), row_start, c[2], tables, R.value(k, "f16"), R.value(v, "f16"), everything)
