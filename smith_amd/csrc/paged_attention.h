@@ -1127,11 +1127,11 @@ __device__ __forceinline__ void check_groups(const Args<R>& a) {
     }
   }
 }
-// a request's block table (SHARED: that of the group's first)
+// the request whose block table item b reads (SHARED: the group's first)
 template <Reach R>
-__device__ __forceinline__ const int32_t* table_of(const Args<R>& a, uint32_t b) {
+__device__ __forceinline__ uint32_t request_of(const Args<R>& a, uint32_t b) {
   if constexpr (R == SHARED) b = uniform((uint32_t)a.group_start[b]);
-  return a.tables + (size_t)b * a.max_pages;
+  return b;
 }
 
 // One tile of 16 columns to a workgroup.  Its four waves take the keys in turn, TK
@@ -1174,7 +1174,7 @@ __device__ __forceinline__ void attention_body(const Args<R>& args) {
 
     // ---- this wave's keys, a tile's loads in flight before it is needed ----
     TILE tile;
-    const int32_t* table = table_of<R>(a, I.b);
+    const int32_t* table = a.tables + (size_t)request_of<R>(a, I.b) * a.max_pages;
     const size_t head_len = (size_t)hd << a.shift;  // values of a page's KV head
     uint32_t bad = 0;
     auto page_of = [&](uint32_t t) {  // of key t < k1
@@ -1310,7 +1310,7 @@ __device__ __forceinline__ void attention_body(const Args<R>& args) {
       if (more) load_v(t0 + 4 * TK);
     }
     const Args<R>& z = again<R>();
-    if (bad) paged_err(z.err, PAGED_ERR_ATT_PAGE, I.b);
+    if (bad) paged_err(z.err, PAGED_ERR_ATT_PAGE, request_of<R>(z, I.b));
     turn.take(z, items.total);
 
     // ---- join the waves ----
@@ -1623,7 +1623,7 @@ __device__ __forceinline__ void attention_rows_body(const Args<R>& args) {
     // ---- this wave's share of a stage: KT / 4 rows of K and of V, 8 or 16, a page to 8 ----
     constexpr uint32_t SHARE = KT / 4, RPI = 1024 / ROWB, PARTS = SHARE / 8, INSTR = 8 / RPI;  // rows, instructions to 8 rows
     constexpr uint32_t AHEAD = 64 / PARTS;
-    const int32_t* table = table_of<R>(a, I.b);
+    const int32_t* table = a.tables + (size_t)request_of<R>(a, I.b) * a.max_pages;
     const size_t head_len = (size_t)hd << a.shift;
     uint32_t bad = 0, pages = 0, ahead = AHEAD;  // lane PARTS x + h: page of this wave's h-th 8 rows x stages on
     const size_t page_bytes = a.nKV * head_len * sizeof(T);
@@ -1771,7 +1771,7 @@ __device__ __forceinline__ void attention_rows_body(const Args<R>& args) {
       ROWS::add_pv(v, hn, hg, S, c, shift, l, O);
     }
     const Args<R>& z = again<R>();
-    if (bad) paged_err(z.err, PAGED_ERR_ATT_PAGE, I.b);
+    if (bad) paged_err(z.err, PAGED_ERR_ATT_PAGE, request_of<R>(z, I.b));
     turn.take(z, items.total);
 
     // ---- out, or a partial ----

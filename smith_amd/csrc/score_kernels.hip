@@ -10,11 +10,15 @@
 // ordered as a whole number, above the complement of its place, so that keys are
 // all different and the larger one is the larger value or, of equal ones, the
 // lower place.  A wave keeps the 64 best of its elements sorted over its lanes;
-// an element goes in if it is above the k-th, which after a few thousand elements
-// is rare, so that the pass costs a comparison with the maximum of 16.  Lists are
+// an element goes in if it is above the k-th of each of the workgroup's waves, which
+// after a few thousand elements is rare, so that the pass costs a comparison with
+// the maximum of 16.  Lists are
 // joined by bitonic merges: the result does not depend on who comes first.
 //
-// Bound by memory: the logits are read once.
+// Bound by memory where few are wanted of long f32 rows: 900 of 131072, 472 MB, 85 us
+// without top ones (5.5 TB/s; a large copy: 4.8), 91 with 8, 140 with 64; of bf16 logits
+// by the operations, 49, 72 and 138.  Short rows by the first lists and their merges: one
+// row of 32000 4.8 us without top ones, 9.0 with 5, 13.3 with 64.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -28,6 +32,8 @@ typedef uint32_t u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
 #define LOG2E 1.44269504088896341f
 #define THREADS SCORE_THREADS
 #define WAVES (SCORE_THREADS / 64)
+#define MANY 12                   // lanes whose elements go into a list together
+#define FEW 24                    // of so many top ones one element of each lane tells the others from nearly all
 #define PER 16                    // elements of a thread to a chunk
 #define CHUNK SCORE_WAVE_CHUNK    // of a wave
 
@@ -65,36 +71,59 @@ __device__ __forceinline__ float value_of(uint64_t key) {
   const uint32_t u = (uint32_t)(key >> 32);
   return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
 }
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t k, int d) {
-  return ((uint64_t)(uint32_t)__shfl_xor((int)(k >> 32), d) << 32) | (uint32_t)__shfl_xor((int)k, d);
+// lane ^ D's, without an LDS round trip: DPP within 16 lanes, swaps of rows and halves
+template <int D>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  if constexpr (D == 1) return dpp_u32<0xB1>(v);
+  if constexpr (D == 2) return dpp_u32<0x4E>(v);
+  if constexpr (D == 3) return dpp_u32<0x1B>(v);
+  if constexpr (D == 7) return dpp_u32<0x141>(v);   // half-row mirror
+  if constexpr (D == 15) return dpp_u32<0x140>(v);  // row mirror
+  if constexpr (D == 4) return lane_xor<7>(lane_xor<3>(v));
+  if constexpr (D == 8) return lane_xor<15>(lane_xor<7>(v));
+  if constexpr (D == 16) {
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? p[0] : p[1];
+  }
+  if constexpr (D == 32) {
+    const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? p[0] : p[1];
+  }
+  if constexpr (D == 63) return lane_xor<32>(lane_xor<16>(lane_xor<15>(v)));
+}
+template <int D>
+__device__ __forceinline__ uint64_t lane_xor64(uint64_t k) {
+  return ((uint64_t)lane_xor<D>((uint32_t)(k >> 32)) << 32) | lane_xor<D>((uint32_t)k);
 }
 __device__ __forceinline__ uint64_t readlane64(uint64_t k, uint32_t lane) {
   return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), (int)lane) << 32) |
          (uint32_t)__builtin_amdgcn_readlane((int)k, (int)lane);
 }
 // the larger (or smaller) of a lane's key and its partner's
-__device__ __forceinline__ uint64_t exchange(uint64_t k, int d, bool larger) {
-  const uint64_t o = shfl_xor64(k, d);
+template <int D>
+__device__ __forceinline__ uint64_t exchange(uint64_t k, bool larger) {
+  const uint64_t o = lane_xor64<D>(k);
   return (o > k) == larger ? o : k;
 }
-// a bitonic sequence over the lanes, sorted: the largest in lane 0
-__device__ __forceinline__ uint64_t sort_bitonic(uint64_t k, uint32_t lane) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) k = exchange(k, d, !(lane & d));
+// bitonic sequences of 2 D lanes each, sorted: the largest first, or last where `up`
+template <int D>
+__device__ __forceinline__ uint64_t sort_bitonic(uint64_t k, uint32_t lane, bool up) {
+  k = exchange<D>(k, !(lane & D) != up);
+  if constexpr (D > 1) k = sort_bitonic<D / 2>(k, lane, up);
   return k;
 }
 __device__ __forceinline__ uint64_t sort64(uint64_t k, uint32_t lane) {
-#pragma unroll
-  for (int n = 2; n <= 32; n <<= 1)
-#pragma unroll
-    for (int d = n >> 1; d; d >>= 1) k = exchange(k, d, !(lane & d) == !(lane & n));
-  return sort_bitonic(k, lane);
+  k = sort_bitonic<1>(k, lane, lane & 2);
+  k = sort_bitonic<2>(k, lane, lane & 4);
+  k = sort_bitonic<4>(k, lane, lane & 8);
+  k = sort_bitonic<8>(k, lane, lane & 16);
+  k = sort_bitonic<16>(k, lane, lane & 32);
+  return sort_bitonic<32>(k, lane, false);
 }
 // the 64 largest of two sorted lists, sorted
 __device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b, uint32_t lane) {
-  const uint64_t o = ((uint64_t)(uint32_t)__shfl((int)(b >> 32), (int)(63 - lane)) << 32) |
-                     (uint32_t)__shfl((int)b, (int)(63 - lane));
-  return sort_bitonic(a > o ? a : o, lane);
+  const uint64_t o = lane_xor64<63>(b);
+  return sort_bitonic<32>(a > o ? a : o, lane, false);
 }
 // key c (the same in all lanes) into a sorted list
 __device__ __forceinline__ uint64_t insert(uint64_t list, uint64_t c, uint32_t lane) {
@@ -113,9 +142,9 @@ __device__ __forceinline__ Sums moved(Sums a, float M) {  // to a maximum that i
   return {M, f * a.l, some ? f * (f == 0.f ? 0.f : __builtin_fmaf(d, a.l, a.s)) : 0.f};
 }
 __device__ __forceinline__ Sums over_lanes(Sums a) {
-  float M = a.m;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
+  float M = max16_lanes(a.m);
+  M = fmaxf(M, __uint_as_float(lane_xor<16>(__float_as_uint(M))));
+  M = fmaxf(M, __uint_as_float(lane_xor<32>(__float_as_uint(M))));
   a = moved(a, M);
   return {M, sum64_lanes(a.l), sum64_lanes(a.s)};
 }
@@ -138,58 +167,75 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
   __shared__ uint64_t s_list[WAVES][64];
   __shared__ Sums s_sums[WAVES];
   __shared__ uint32_t s_last;
+  __shared__ uint64_t s_least;  // the highest of the waves' k-th: no lower element is one of the row's k
   const uint32_t tid = threadIdx.x, lane = tid & 63, w = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t row = a.row0 + blockIdx.x / a.splits, split = blockIdx.x % a.splits;
   const T* x = (const T*)a.logits + (size_t)row * a.ld;
   // this split's chunks, to the waves in turn
   const uint32_t begin = split * a.per_split, end = a.vocab - begin < a.per_split ? a.vocab : begin + a.per_split;
 
+  if (tid == 0) s_least = 0;
+  if (a.top) __syncthreads();
   Sums sum = {-__builtin_inff(), 0.f, 0.f};
-  uint64_t list = 0, least = 0;  // sorted over the lanes; its k-th
+  uint64_t list = 0, least = 0;  // sorted over the lanes; the highest k-th that the wave knows of
   float least_value = -__builtin_inff();
+  auto place = [&](uint32_t at, uint32_t i) { return at + i / L::WIDTH * 64 * L::WIDTH + lane * L::WIDTH + i % L::WIDTH; };
   auto load = [&](uint32_t at, float (&v)[PER]) {
     if (at + CHUNK <= end) {
 #pragma unroll
       for (uint32_t k = 0; k < LOADS; k++) L::load(x + at + k * 64 * L::WIDTH + lane * L::WIDTH, v + k * L::WIDTH);
     } else {
 #pragma unroll
-      for (uint32_t i = 0; i < PER; i++) {
-        const uint32_t e = at + i / L::WIDTH * 64 * L::WIDTH + lane * L::WIDTH + i % L::WIDTH;
-        v[i] = e < end ? L::up(x[e]) : -__builtin_inff();  // weighs nothing
-      }
+      for (uint32_t i = 0; i < PER; i++)
+        v[i] = place(at, i) < end ? L::up(x[place(at, i)]) : -__builtin_inff();  // weighs nothing
     }
   };
-  // the chunk's elements above the list's k-th
-  auto pick = [&](uint32_t at, const float (&v)[PER]) {
+  // The chunk's elements above the k-th of any of the waves' lists.  While many lanes
+  // have some, the best of each lane goes in, sorted first; the others one by one, slot
+  // by slot (an element of each lane).
+  auto pick = [&](uint32_t at, const float (&v)[PER], bool many) {
     uint64_t below = ~0ull;  // the lane's elements from this key on are through
-    for (;;) {
+    auto key = [&](uint32_t i) {  // 0: none, or no number
+      // (worked out anew for each use: kept, the 16 keys cost half of the waves)
+      float x = v[i];
+      asm volatile("" : "+v"(x));
+      const uint64_t k = key_of(x, place(at, i));
+      return x == x && k < below && k > least ? k : 0ull;
+    };
+    auto raise = [&] {
+      const uint64_t k = readlane64(list, a.top - 1);
+      least = k > least ? k : least;
+      least_value = least ? value_of(least) : -__builtin_inff();
+    };
+    while (many) {
       uint64_t best = 0;
 #pragma unroll
       for (uint32_t i = 0; i < PER; i++) {
-        const uint32_t e = at + i / L::WIDTH * 64 * L::WIDTH + lane * L::WIDTH + i % L::WIDTH;
-        const uint64_t k = key_of(v[i], e);
-        if (v[i] == v[i] && e < end && k < below && k > best) best = k;
+        const uint64_t k = key(i);
+        best = k > best ? k : best;
       }
-      if (best <= least) best = 0;
-      uint64_t there = __ballot(best != 0);
-      if (!there) break;
-      if (__popcll(there) > 12) {
-        list = merge64(list, sort64(best, lane), lane);
-        least = readlane64(list, a.top - 1);
-      } else {
-        do {
-          const uint32_t from = (uint32_t)__ffsll((unsigned long long)there) - 1;
-          there &= there - 1;
-          const uint64_t c = readlane64(best, from);
-          if (c > least) {
-            list = insert(list, c, lane);
-            least = readlane64(list, a.top - 1);
-          }
-        } while (there);
-      }
-      below = best ? best : 0;
+      many = __popcll(__ballot(best != 0)) > MANY;
+      if (!many) break;
+      list = merge64(list, sort64(best, lane), lane);
+      raise();
+      below = best;
+      if (a.top <= FEW) break;
     }
-    least_value = least ? value_of(least) : -__builtin_inff();
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) {
+      if (!__any(v[i] >= least_value)) continue;
+      const uint64_t k = key(i);
+      uint64_t there = __ballot(k != 0);
+      while (there) {
+        const uint64_t c = readlane64(k, (uint32_t)__ffsll((unsigned long long)there) - 1);
+        there &= there - 1;
+        if (c > least) {
+          list = insert(list, c, lane);
+          raise();
+        }
+      }
+    }
+    if (lane == 0) __hip_atomic_fetch_max(&s_least, least, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   };
   float v[PER], next[PER];
   uint32_t at = begin + w * CHUNK;
@@ -208,7 +254,22 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
       sum.l += e;
       sum.s = __builtin_fmaf(e, fmaxf(d, -1000.f), sum.s);  // 0 of -inf
     }
-    if (a.top && __any(least ? mx > least_value : true)) pick(at, v);
+    if (a.top && __any(mx >= least_value || !least)) {
+      const uint64_t others = __hip_atomic_load(&s_least, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      const uint64_t known = readlane64(others, 0);
+      if (known > least) {
+        least = known;
+        least_value = value_of(least);
+      }
+      const uint64_t some = __ballot(mx >= least_value || !least);
+      if (some) {
+        if (at + CHUNK > end)
+#pragma unroll
+          for (uint32_t i = 0; i < PER; i++)
+            if (place(at, i) >= end) v[i] = __builtin_nanf("");  // no element
+        pick(at, v, __popcll(some) > MANY);
+      }
+    }
     if (more)
 #pragma unroll
       for (uint32_t i = 0; i < PER; i++) v[i] = next[i];
@@ -224,12 +285,17 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
     const Sums p = moved(sum, M), q = moved(b, M);
     sum = {M, p.l + q.l, p.s + q.s};
   };
-  if (w == 0) {
-    for (uint32_t k = 1; k < WAVES; k++) {
-      if (a.top) list = merge64(list, s_list[k][lane], lane);
-      join(s_sums[k]);
-    }
-  }
+  // lists of the waves into wave 0's
+  auto gather = [&] {
+    static_assert(WAVES == 4, "two levels");
+    if (!(w & 1)) list = merge64(list, s_list[w + 1][lane], lane);
+    if (w == 2) s_list[2][lane] = list;
+    __syncthreads();
+    if (w == 0) list = merge64(list, s_list[2][lane], lane);
+  };
+  if (a.top) gather();
+  if (w == 0)
+    for (uint32_t k = 1; k < WAVES; k++) join(s_sums[k]);
   if (a.splits > 1) {
     // per split: (m, l), (s, -), the keys
     const size_t stride = a.top + 2;
@@ -253,8 +319,17 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
     if (!s_last) return;
     list = 0;
     if (a.top) {
-      for (uint32_t k = w; k < a.splits; k += WAVES)
-        list = merge64(list, lane < a.top ? get64(all + k * stride + 2 + lane) : 0ull, lane);
+      constexpr uint32_t BATCH = 8;  // loads under way
+      for (uint32_t k0 = w; k0 < a.splits; k0 += WAVES * BATCH) {
+        uint64_t x[BATCH];
+#pragma unroll
+        for (uint32_t j = 0; j < BATCH; j++)
+          x[j] = lane < a.top && k0 + j * WAVES < a.splits ? get64(all + (k0 + j * WAVES) * stride + 2 + lane) : 0ull;
+        if (k0 == w) list = x[0];
+#pragma unroll
+        for (uint32_t j = 0; j < BATCH; j++)
+          if (k0 + j * WAVES < a.splits && (j || k0 != w)) list = merge64(list, x[j], lane);
+      }
       s_list[w][lane] = list;
     }
     sum = {-__builtin_inff(), 0.f, 0.f};
@@ -264,8 +339,7 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
     }
     sum = over_lanes(sum);
     __syncthreads();
-    if (w == 0 && a.top)
-      for (uint32_t k = 1; k < WAVES; k++) list = merge64(list, s_list[k][lane], lane);
+    if (a.top) gather();
   }
   if (w) return;
   // a row without a finite maximum has no distribution
