@@ -29,6 +29,8 @@ import numpy as np
 
 from . import device
 from .paged import ROPE_ROW
+from .score import MAX_TOP, logProbs
+from .tensor import Tensor, tensor
 
 # SMITH_DECODE_GRAPH=0 runs every decode step eagerly (kernel-level profilers
 # that cannot trace graph replays); results are identical.
@@ -258,10 +260,11 @@ class _Engine:
             self.row_logits = DeviceArray((min(step, max(64, ROW_LOGITS_BYTES // (vocab * 4) // 64 * 64)), vocab))
         return self.row_logits
 
-    def paged_step(self, model, tokens, cache):
+    def paged_step(self, model, tokens, cache, take):
         """Rows of several requests (tokens[b]: request b's) through every layer on
-        a PagedCache; the logits of each request's last row, in order.  Whatever
-        raises, the cache is as it was."""
+        a PagedCache, then take(device rows of logits, their number) for each
+        request's last row, in order, some at a time.  Whatever raises, the cache is as
+        it was."""
         cfg, vocab = self.cfg, self.cfg["vocabSize"]
         added = [len(t) for t in tokens]
         M = sum(added)
@@ -271,16 +274,18 @@ class _Engine:
         if flat and not 0 <= min(flat) <= max(flat) < vocab:
             raise ValueError("paged step: a token outside the vocabulary of %d" % vocab)
         cache.check_model(cfg)
-        out, before = self._row_logits(), cache.state()
+        out = self._row_logits()
+        cache.make_room(added)
+        before = cache.state()
         try:
-            return self._paged_rows(model, flat, added, cache, cache.plan(added), out)
+            self._paged_rows(model, flat, added, cache, cache.plan(added), out, take)
         except BaseException:
             cache.restore(before)  # no keys of this step: it can be tried again
             raise
 
-    def _paged_rows(self, model, flat, added, cache, plan, out):
+    def _paged_rows(self, model, flat, added, cache, plan, out, take):
         cfg, ctx, eps = self.cfg, device.ops_ctx(), model["normEps"]
-        dim, vocab, H, ld, M = cfg["dim"], cfg["vocabSize"], cfg["numHeads"], self.qkv_ld, len(flat)
+        dim, H, ld, M = cfg["dim"], cfg["numHeads"], self.qkv_ld, len(flat)
         self.embed(model, flat)
         x, x2, qkv, attn, h = self.x.ptr, self.x2.ptr, self.qkv.ptr, self.attn.ptr, self.h.ptr
         rope = model["rope"]
@@ -298,35 +303,52 @@ class _Engine:
             rows = x2
             for i, r in enumerate(last):
                 device.check(device.lib.smith_copy_d2d(ctx, x2, i * dim * 4, x, int(r) * dim * 4, dim * 4), "last rows")
-        logits = np.empty((len(last), vocab), np.float32)
         for b0 in range(0, len(last), out.shape[0]):
             b1 = min(len(last), b0 + out.shape[0])
             self._lm_head_rows_at(model, rows + b0 * dim * 4, b1 - b0, out.ptr)
-            device.download_into(logits[b0:b1], out.ptr)
-        return logits
+            take(out.ptr, b1 - b0)
 
-    def prefill(self, model, tokens, caches, all_logits=False):
+    def score_rows(self, ptr, rows, tokens, top):
+        """logProbs of device rows of logits, as host arrays; tokens [rows] or None."""
+        made = []
+        try:
+            given = None
+            if tokens is not None:
+                given = tensor(np.asarray(tokens, np.int32), dtype="i32")
+                made.append(given)
+            r = logProbs(Tensor([rows, self.cfg["vocabSize"]], "f32", buffer=ptr), given, top)
+            made += r.values()
+            return {name: t.data for name, t in r.items()}
+        finally:
+            for t in made:
+                t.release()
+
+    def prefill(self, model, tokens, caches, all_logits=False, take=None):
         """Prompt rows in chunks of <= 256 (attention keeps a chunk's keys in
-        LDS); returns the logits of every row if asked, else of the last."""
+        LDS); returns the logits of every row if asked, else of the last.  take: of every
+        row, left on the device, some rows at a time for take(device rows, their number)."""
         n = len(tokens)
         if all_logits and not n:
             raise ValueError("prefill of an empty prompt: there are no logits to return")
         step, dim, vocab = _chunk_rows(self.cfg), self.cfg["dim"], self.cfg["vocabSize"]
         logits = np.empty((n, vocab), np.float32) if all_logits else None
-        if all_logits:
+        if all_logits or take:
             block = self._row_logits().shape[0]
         for r0 in range(0, n, step):
             r1 = min(n, r0 + step)
             self.embed(model, tokens[r0:r1])
             self.set_pos(r0)
             self.layers(model, caches, r1 - r0)
-            if all_logits:
+            if all_logits or take:
                 for b0 in range(r0, r1, block):
                     b1 = min(r1, b0 + block)
                     self.lm_head_rows(model, b0 - r0, b1 - b0, self.row_logits.ptr)
-                    device.download_into(logits[b0:b1], self.row_logits.ptr)
+                    if take:
+                        take(self.row_logits.ptr, b1 - b0)
+                    else:
+                        device.download_into(logits[b0:b1], self.row_logits.ptr)
         last = (n - 1) % step
-        if not all_logits:
+        if not all_logits and not take:
             self.lm_head(model, self.x.ptr + last * dim * 4)
         for c in caches:
             c["len"] = n
@@ -369,12 +391,7 @@ def forwardLlamaCachedDecode(model, tokenId, position, caches):
     return {"logits": e.logits.numpy()[None, :].copy()}
 
 
-def forwardPagedStep(model, tokens, cache):
-    """One step of several requests on a PagedCache (paged.py): tokens[b] are the
-    new tokens of request b, any number of them -- a prompt, a chunk of one, the
-    last token that was generated, none -- up to 256 in all.  Returns {'logits':
-    [n, vocab] (host), 'requests': the n requests that had tokens}: the logits
-    behind each one's last token."""
+def _paged_tokens(model, tokens, cache):
     e = _engine(model)
     tokens = [list(t) for t in tokens]
     if len(tokens) != cache.requests:
@@ -382,7 +399,67 @@ def forwardPagedStep(model, tokens, cache):
     for n, t in zip(cache.lens, tokens):
         if t:
             _check_rope_range(e.cfg, int(n) + len(t) - 1)
-    return {"logits": e.paged_step(model, tokens, cache), "requests": [b for b, t in enumerate(tokens) if t]}
+    return e, tokens
+
+
+def forwardPagedStep(model, tokens, cache):
+    """One step of several requests on a PagedCache (paged.py): tokens[b] are the
+    new tokens of request b, any number of them -- a prompt, a chunk of one, the
+    last token that was generated, none -- up to 256 in all.  Returns {'logits':
+    [n, vocab] (host), 'requests': the n requests that had tokens}: the logits
+    behind each one's last token."""
+    e, tokens = _paged_tokens(model, tokens, cache)
+    logits = []
+
+    def take(ptr, rows):
+        logits.append(device.download_into(np.empty((rows, e.cfg["vocabSize"]), np.float32), ptr))
+    e.paged_step(model, tokens, cache, take)
+    return {"logits": np.concatenate(logits), "requests": [b for b, t in enumerate(tokens) if t]}
+
+
+def scorePagedStep(model, tokens, cache, top=8):
+    """forwardPagedStep whose logits stay on the device: {'topIds', 'topLogprobs'
+    [n, top], 'entropy' [n], 'requests'}, the likeliest tokens behind each request's
+    last one, the likeliest first, and the entropy of that distribution (logProbs)."""
+    e, tokens = _paged_tokens(model, tokens, cache)
+    _check_top(e, top, 1)
+    parts = []
+    e.paged_step(model, tokens, cache, lambda ptr, rows: parts.append(e.score_rows(ptr, rows, None, top)))
+    out = {name: np.concatenate([p[name] for p in parts]) for name in ("topIds", "topLogprobs", "entropy")}
+    return dict(out, requests=[b for b, t in enumerate(tokens) if t])
+
+
+def scoreTokens(model, tokenIds, top=0):
+    """What the model says of a text: of each of its tokens but the first the log
+    probability behind those before it, the entropy there and the top alternatives:
+    {'logprobs', 'entropy' [n - 1], 'topIds', 'topLogprobs' [n - 1, top]} (host).  The
+    logits stay on the device."""
+    e, tokens = _engine(model), [int(t) for t in tokenIds]
+    if len(tokens) < 2 or len(tokens) - 1 > e.cfg["maxSeqLen"]:
+        raise ValueError("score: a text of %d tokens (2 .. %d)" % (len(tokens), e.cfg["maxSeqLen"] + 1))
+    if not 0 <= min(tokens) <= max(tokens) < e.cfg["vocabSize"]:
+        raise ValueError("score: a token outside the vocabulary of %d" % e.cfg["vocabSize"])
+    _check_rope_range(e.cfg, len(tokens) - 2)
+    _check_top(e, top, 0)
+    caches, parts, at = createGGUFCache(e.cfg), [], [1]
+
+    def take(ptr, rows):
+        part = e.score_rows(ptr, rows, tokens[at[0]:at[0] + rows], top)
+        parts.append(part)
+        at[0] += rows
+    try:
+        e.prefill(model, tokens[:-1], caches, take=take)
+    finally:
+        for c in caches:
+            for name in ("k", "v"):
+                device.release_buffer(c[name].ptr)
+    out = {name: np.concatenate([p[name] for p in parts]) for name in ("logprobs", "entropy", "topIds", "topLogprobs")}
+    return dict(out, logprobs=out["logprobs"][:, 0])
+
+
+def _check_top(e, top, least):
+    if not least <= top <= min(MAX_TOP, e.cfg["vocabSize"]):
+        raise ValueError("score: %d top alternatives (%d .. %d)" % (top, least, min(MAX_TOP, e.cfg["vocabSize"])))
 
 
 # --- host sampling (generate.js:11-70), used when temperature > 0 or a

@@ -22,7 +22,7 @@ import numpy as np
 from . import device
 from . import gguf as G
 from .gguf_cache import (createGGUFCache, forwardLlamaCachedDecode, forwardLlamaCachedPrefill, forwardPagedStep,
-                         generateGGUF, resetCache)
+                         generateGGUF, resetCache, scorePagedStep, scoreTokens)
 from .paged import createPagedCache
 
 LLAMA_MAP = {
@@ -473,7 +473,8 @@ def loadGGUF(path):
         return GGUFModel(model=model, config=config, metadata=parsed["metadata"], loaded=loaded, skipped=skipped,
                          forward=unsupported, createCache=lambda: createGGUFCache(model["config"]),
                          forwardPrefill=unsupported, forwardDecode=unsupported, generate=unsupported,
-                         createPagedCache=unsupported, forwardPagedStep=unsupported, resetCache=resetCache)
+                         createPagedCache=unsupported, forwardPagedStep=unsupported, scorePagedStep=unsupported,
+                         score=unsupported, resetCache=resetCache)
     model = createGGUFModel(config)
     res = loadWeights(parsed, model)
     return GGUFModel(
@@ -484,8 +485,10 @@ def loadGGUF(path):
         forwardDecode=lambda tokenId, position, caches: forwardLlamaCachedDecode(model, tokenId, position, caches),
         generate=lambda promptIds, genConfig=None, callbacks=None: generateGGUF(model, promptIds, genConfig or {},
                                                                                callbacks or {}),
-        createPagedCache=lambda requests, pages, pageSize=16, dtype="f16": createPagedCache(
-            model["config"], requests, pages, pageSize, dtype),
+        createPagedCache=lambda requests, pages, pageSize=16, dtype="f16", window=0, sinks=0: createPagedCache(
+            model["config"], requests, pages, pageSize, dtype, window, sinks),
         forwardPagedStep=lambda tokens, cache: forwardPagedStep(model, tokens, cache),
+        scorePagedStep=lambda tokens, cache, top=8: scorePagedStep(model, tokens, cache, top),
+        score=lambda tokenIds, top=0: scoreTokens(model, tokenIds, top),
         resetCache=resetCache,
     )

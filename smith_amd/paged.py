@@ -19,7 +19,9 @@ on Tensors (one call into libsmith.so each, include/smith.h states what each
 reads and writes).  PagedCache keeps the pools, tables and lengths of a model's
 requests on the device; forwardPagedStep of a loaded GGUF model runs on it.
 """
+import collections
 import ctypes
+import itertools
 
 import numpy as np
 
@@ -177,13 +179,22 @@ def _release(tensors):
         t.release()
 
 
+# Keys and values of a layer's shared keys that are read once instead of once a
+# request, in bytes, from which the launch that computes them apart is worth its time
+# (6 us a layer, in which the card reads 30 MB).
+SHARED_BYTES = 32 << 20
+
+
 class PagedCache:
     """The paged cache of a model's requests: per layer the pools k and v, and on
     the device the block tables [requests, maxPages], lengths and free list, which
     the host mirrors in `lens` and `freeCount`.  A request is its number, 0 ..
-    requests - 1; it takes pages as it grows and gives them back with release()."""
+    requests - 1; it takes pages as it grows and gives them back with release().
+    fork() lets requests go on from others on shared pages.  With a window a row
+    sees the last `window` keys up to its own and the first `sinks`, and pages that no
+    later row sees are given back when others are needed, or by trim()."""
 
-    def __init__(self, config, requests, pages, pageSize=16, dtype="f16"):
+    def __init__(self, config, requests, pages, pageSize=16, dtype="f16", window=0, sinks=0):
         if dtype not in KV_TYPES:
             raise ValueError("createPagedCache: pages of %s (f32, f16 or bf16)" % dtype)
         if not 1 <= requests <= MAX_REQUESTS:
@@ -194,11 +205,18 @@ class PagedCache:
             raise ValueError("createPagedCache: %d pages of %d keys" % (pages, pageSize))
         if config["headDim"] % 8 or not 8 <= config["headDim"] <= 128:
             raise ValueError("createPagedCache: heads of %d dims (8, 16 .. 128)" % config["headDim"])
+        if window < 0 or sinks < 0 or (sinks and not window):
+            raise ValueError("createPagedCache: a window of %d keys and %d sinks" % (window, sinks))
         self.requests, self.pages, self.pageSize, self.dtype = requests, pages, pageSize, dtype
+        self.window, self.sinks = min(window, MOST_KEYS), min(sinks, MOST_KEYS)
         self.maxPages = -(-config["maxSeqLen"] // pageSize)
         self.lens = np.zeros(requests, np.int32)
         self.freeCount = pages
         self.layers, self._rows, self._turn, self._tensors = [], None, 0, []
+        # from the first fork on: of each request a number for each of its pages (None: given
+        # back), and how many requests name it; what they share, host and device
+        self._ids, self._named, self._next_id = None, collections.Counter(), 0
+        self._groups, self._group_tensors, self._spare = [], None, None
         try:
             self._allocate(config)
         except BaseException:
@@ -230,6 +248,15 @@ class PagedCache:
     def _there(self):
         if not self._tensors:
             raise ValueError("paged cache: it was freed")
+
+    def _pages(self, n):
+        return -(-int(n) // self.pageSize)
+
+    def make_room(self, added):
+        """Gives back what the window has passed, if the rows `added` need it."""
+        new = sum(self._pages(n + a) - self._pages(n) for n, a in zip(self.lens, added))
+        if self.window and new > self.freeCount:
+            self.trim()
 
     def plan(self, added):
         """The step in which request b brings added[b] rows: {rowStart, lens, slots,
@@ -265,8 +292,19 @@ class PagedCache:
             self._row_start.buffer, self._lens[b].buffer, slots.buffer, positions.buffer, self._count[b].buffer),
             "paged step")
         self._turn, self.lens, self.freeCount = b, lens.astype(np.int32), self.freeCount - new
+        if self._ids is not None:
+            for r in np.nonzero(added)[0]:
+                self._name(r)
         return {"rowStart": self._row_start, "lens": self._lens[b], "slots": slots, "positions": positions,
                 "tables": self._tables}
+
+    def _name(self, r):
+        """Numbers for the pages that request r has and had not."""
+        ids = self._ids[r]
+        while len(ids) < self._pages(self.lens[r]):
+            ids.append(self._next_id)
+            self._named[self._next_id] = 1
+            self._next_id += 1
 
     def state(self):
         """For restore()."""
@@ -276,6 +314,180 @@ class PagedCache:
         """Back to a state() from before the last plan(), if nothing was released
         since: what that step read on the device is still there."""
         self._turn, self.lens, self.freeCount = state
+        if self._ids is not None:
+            for ids, n in zip(self._ids, self.lens):
+                while len(ids) > self._pages(n):
+                    del self._named[ids.pop()]
+
+    # --- requests that go on from others ---
+    def _kept(self, j, n):
+        """Whether page j of a request of n keys has a sink or one that a later row sees."""
+        P = self.pageSize
+        return not self.window or j * P < self.sinks or (j + 1) * P + self.window > n + 1
+
+    def _seen(self, ids, n):
+        """A copy of a request's numbers of pages, None for those that its window has passed."""
+        return [x if self._kept(j, int(n)) else None for j, x in enumerate(ids)] if self.window else ids.copy()
+
+    @staticmethod
+    def _count_names(ids):
+        named = collections.Counter(itertools.chain.from_iterable(ids))
+        named.pop(None, None)
+        return named
+
+    def fork(self, parents):
+        """Request b goes on from request parents[b] as it was: itself, another, or -1,
+        none.  Full pages are shared; a partly filled one stays with the first request
+        that goes on from its own, and is copied for the others.  Nothing happens
+        (ValueError) if there are too few pages for the copies."""
+        self._there()
+        parents = np.asarray(parents)
+        if parents.shape != (self.requests,) or parents.dtype.kind not in "iu" or not (
+                (parents >= -1) & (parents < self.requests)).all():
+            raise ValueError("paged fork: parents are %d numbers of requests or -1" % self.requests)
+        if self._ids is None:
+            self._ids = [[] for _ in range(self.requests)]
+            for r in range(self.requests):
+                self._name(r)
+        ids, seen, next_id = [], set(), self._next_id
+        lens = np.where(parents >= 0, self.lens[parents], 0).astype(np.int32)
+        for p, n in zip(parents, lens):
+            mine = self._seen(self._ids[p], n) if p >= 0 else []
+            if p in seen and n % self.pageSize:
+                mine[-1], next_id = next_id, next_id + 1
+            seen.add(p)
+            ids.append(mine)
+        named = self._count_names(ids)
+        if len(named) > self.pages:
+            raise ValueError("paged fork: %d pages, there are %d" % (len(named), self.pages))
+        tables, free, todo = self._spares()
+        a, b = self._turn, 1 - self._turn
+        todo.set_data(parents)
+        pools = [layer[name].buffer for layer in self.layers for name in ("k", "v")]
+        shape = self.layers[0]["k"].shape if self.layers else [0, 1, 0, 8]
+        device.check(device.lib.smith_paged_fork(
+            device.ops_ctx(), KV_TYPES[self.dtype], self._lens[a].buffer, self._tables.buffer, todo.buffer, self.requests,
+            self.maxPages, self.window, self.sinks, shape[1], shape[3], (ctypes.c_void_p * len(pools))(*pools), len(pools),
+            self.pages, self.pageSize, self._lens[b].buffer, tables.buffer, free.buffer, self._count[b].buffer), "paged fork")
+        self._turn, self.lens, self.freeCount = b, lens, self.pages - len(named)
+        self._spare = (self._tables, self._free, todo)
+        self._tables, self._free = tables, free
+        self._ids, self._named, self._next_id = ids, named, next_id
+        self._find_groups()
+
+    def _spares(self):
+        """Tables, a free list and parents for a fork to write and read (and what
+        _find_groups writes): there before it begins."""
+        if self._spare is None:
+            got, n = [], self.requests
+            try:
+                for shape in ([n, self.maxPages], [self.pages], [n], [n + 1], [n]):
+                    got.append(T.create(shape, "i32"))
+            except BaseException:
+                _release(got)
+                raise
+            self._tensors += got
+            self._spare, self._group_tensors = tuple(got[:3]), tuple(got[3:])
+        return self._spare
+
+    def _find_groups(self):
+        """Runs of requests whose first pages are the same ones: [first, behind the last,
+        pages], a request that shares none by itself."""
+        groups = []
+        for r, ids in enumerate(() if self.window else self._ids):
+            if groups:
+                first, _, most = groups[-1]
+                same, of = 0, self._ids[first]
+                if most and ids[:most] == of[:most]:
+                    same = most
+                else:
+                    while same < min(len(ids), len(of)) and ids[same] == of[same]:
+                        same += 1
+                # (a run is not cut to less than half of what it shares for one more)
+                if same and (r == first + 1 or same * 2 > most):
+                    groups[-1] = [first, r + 1, min(most, same) if most else same]
+                    continue
+            groups.append([r, r + 1, 0])
+        if self.window or len(groups) == self.requests:
+            self._groups = []
+            return
+        start, shared = np.full(self.requests + 1, self.requests), np.zeros(self.requests, np.int64)
+        start[:len(groups)] = [g[0] for g in groups]
+        shared[:len(groups)] = [g[2] * self.pageSize for g in groups]
+        self._group_tensors[0].set_data(start)
+        self._group_tensors[1].set_data(shared)
+        self._groups = groups
+
+    def _read_twice(self):
+        """Bytes of a layer's shared keys and values that are read more than once if each
+        request reads its own."""
+        if not self._groups:
+            return 0
+        k = self.layers[0]["k"]
+        size = 2 * k.shape[1] * k.shape[3] * (4 if self.dtype == "f32" else 2)
+        return size * sum((b - a - 1) * n * self.pageSize for a, b, n in self._groups)
+
+    def trim(self):
+        """Gives back the pages that the window has passed."""
+        self.fork(np.arange(self.requests))
+
+    def compact(self):
+        """Moves the pages that requests have to the pools' low end; their number."""
+        self._there()
+        tables, free, _ = self._spares()
+        a, b = self._turn, 1 - self._turn
+        pools = [layer[name].buffer for layer in self.layers for name in ("k", "v")]
+        shape = self.layers[0]["k"].shape if self.layers else [0, 1, 0, 8]
+        device.check(device.lib.smith_paged_compact(
+            device.ops_ctx(), KV_TYPES[self.dtype], self._lens[a].buffer, self._tables.buffer, self.requests, self.maxPages,
+            self.window if self._ids is not None else 0, self.sinks if self._ids is not None else 0, shape[1], shape[3],
+            (ctypes.c_void_p * len(pools))(*pools), len(pools), self.pages, self.pageSize, tables.buffer, free.buffer,
+            self._count[b].buffer), "paged compact")
+        # the lengths are those of this turn: only the count is new
+        device.check(device.lib.smith_copy_d2d(device.ops_ctx(), self._count[a].buffer, 0, self._count[b].buffer, 0, 4),
+                     "paged compact")
+        self._spare = (self._tables, self._free, self._spare[2])
+        self._tables, self._free = tables, free
+        if self._ids is not None and self.window:  # pages that the window had passed are free now
+            self._ids = [self._seen(ids, n) for ids, n in zip(self._ids, self.lens)]
+            self._named = self._count_names(self._ids)
+            self.freeCount = self.pages - len(self._named)
+        return self.pages - self.freeCount
+
+    def resize(self, pages):
+        """Pools of `pages` pages, as many as the requests have at least (compact() says how
+        many that is); the device holds the old and the new ones for a while."""
+        live = self.compact()
+        if pages < max(1, live) or pages * self.pageSize >= 1 << 31:
+            raise ValueError("paged cache: %d pages for the %d that its requests have" % (pages, live))
+        got = []
+        try:
+            for layer in self.layers:
+                for name in ("k", "v"):
+                    got.append(T.create([pages] + layer[name].shape[1:], self.dtype))
+            got.append(T.tensor(np.arange(pages - 1, -1, -1), dtype="i32"))
+            got.append(T.create([pages], "i32"))
+            ctx = device.ops_ctx()
+            for old, new in zip([layer[name] for layer in self.layers for name in ("k", "v")], got):
+                if live:
+                    device.check(device.lib.smith_copy_d2d(ctx, new.buffer, 0, old.buffer, 0, old.nbytes // self.pages * live),
+                                 "paged cache")
+            device.sync()  # the old pools are read until here
+            device.check(device.lib.smith_set_i32(ctx, self._count[self._turn].buffer, pages - live), "paged cache")
+        except BaseException:
+            _release(got)
+            raise
+        spare_tables, _, todo = self._spare
+        gone = [layer.pop(name) for layer in self.layers for name in ("k", "v")] + [self._free, self._spare[1]]
+        for layer in self.layers:
+            layer["k"], layer["v"] = got.pop(0), got.pop(0)
+        self._free, spare_free = got
+        self._spare = (spare_tables, spare_free, todo)
+        drop = {id(t) for t in gone}
+        self._tensors = [t for t in self._tensors if id(t) not in drop]
+        self._tensors += [layer[name] for layer in self.layers for name in ("k", "v")] + got
+        _release(gone)
+        self.pages, self.freeCount = pages, pages - live
 
     def append(self, layer, plan, qkv, ld, rows, numHeads, rope, cos, sin, ropeLen):
         """A layer's rows [q | k | v] (device pointer, row stride ld floats) into its
@@ -291,19 +503,35 @@ class PagedCache:
         """A layer's attention of the step's rows into out [rows, numHeads * headDim]."""
         self._there()
         k, v = self.layers[layer]["k"], self.layers[layer]["v"]
-        device.check(device.lib.smith_paged_attention(
+        name, reach = "smith_paged_attention", ()
+        if self.window:
+            name, reach = "smith_paged_attention_window", (self.window, self.sinks)
+        elif self._read_twice() >= SHARED_BYTES:
+            name = "smith_paged_attention_shared"
+            reach = (*(t.buffer for t in self._group_tensors), len(self._groups))
+        device.check(getattr(device.lib, name)(
             device.ops_ctx(), KV_TYPES[self.dtype], q, ld, rows, plan["rowStart"].buffer, plan["lens"].buffer,
-            plan["tables"].buffer, self.requests, self.maxPages, numHeads, k.shape[1], k.shape[3], 0.0, k.buffer,
+            plan["tables"].buffer, self.requests, self.maxPages, *reach, numHeads, k.shape[1], k.shape[3], 0.0, k.buffer,
             v.buffer, self.pages, self.pageSize, out, numHeads * k.shape[3]), "paged attention")
 
     def release(self, request):
-        """The request's pages back to the free list; its number is free for another."""
+        """The request's pages back to the free list, but for those that others share;
+        its number is free for another."""
         self._there()
         if not 0 <= request < self.requests:
             raise ValueError("paged cache: request %d of %d" % (request, self.requests))
-        n = -(-int(self.lens[request]) // self.pageSize)
+        n = self._pages(self.lens[request])
         if not n:
             return
+        if self._ids is not None:
+            if any(x is None or self._named[x] > 1 for x in self._ids[request]):
+                parents = np.arange(self.requests)
+                parents[request] = -1
+                return self.fork(parents)
+            for x in self._ids[request]:
+                del self._named[x]
+            self._ids[request] = []
+            self._find_groups()
         ctx, a = device.ops_ctx(), self._turn
         device.check(device.lib.smith_copy_d2d(ctx, self._free.buffer, 4 * self.freeCount, self._tables.buffer,
                                                4 * request * self.maxPages, 4 * n), "paged cache")
@@ -316,9 +544,11 @@ class PagedCache:
         """Gives the device memory back; the cache is not used after it."""
         _release(self._tensors + list((self._rows or {}).values()))
         self.layers, self._rows, self._tensors = [], None, []
+        self._spare = self._group_tensors = None
 
 
-def createPagedCache(config, requests, pages, pageSize=16, dtype="f16"):
+def createPagedCache(config, requests, pages, pageSize=16, dtype="f16", window=0, sinks=0):
     """A PagedCache for a model of this config (GGUFModel.config's fields of
-    createGGUFCache): pools of `pages` pages of pageSize keys per layer."""
-    return PagedCache(config, requests, pages, pageSize, dtype)
+    createGGUFCache): pools of `pages` pages of pageSize keys per layer, whose rows
+    see all keys, or the last `window` and the first `sinks`."""
+    return PagedCache(config, requests, pages, pageSize, dtype, window, sinks)
