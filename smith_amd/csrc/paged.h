@@ -55,6 +55,9 @@ struct ReachArgs : AttArgs {
 #define PAGES_POOLS_LAUNCH 440u
 #define PAGES_MAX_POOLS 4096u
 #define PAGES_THREADS 256u
+// a fork in one workgroup: most requests and pages
+#define PAGES_SMALL_REQ 1024u
+#define PAGES_SMALL_PAGES 65536u
 
 // a request's table as the calls see it
 struct PagesTables {

@@ -236,6 +236,132 @@ extern "C" __global__ __launch_bounds__(PAGES_THREADS) void smith_pages_fork(Tab
   });
 }
 
+// mark and fork in one launch of one workgroup, the map in LDS, for few requests and
+// pages: what mark's workgroups spread over the card is then less than a launch takes.
+// A thread to a request, then the entries of all tables one after another, a request
+// found by bisection, then a lane to a page.  Bound by latency: parent, length, entry.
+#define SMALL_THREADS 1024u
+extern "C" __global__ __launch_bounds__(SMALL_THREADS) void smith_pages_fork_small(Tables t, Work w, int32_t* __restrict__ new_lens,
+                                                                                  int32_t* __restrict__ new_tables,
+                                                                                  int32_t* __restrict__ free_pages,
+                                                                                  int32_t* __restrict__ free_count,
+                                                                                  uint64_t* __restrict__ err) {
+  constexpr uint32_t WAVES = SMALL_THREADS / 64, REQ = PAGES_SMALL_REQ, WORDS = PAGES_SMALL_PAGES / 32;
+  static_assert(REQ == SMALL_THREADS && WORDS == 2 * SMALL_THREADS, "a thread to a request, and to two words");
+  __shared__ uint32_t s_map[WORDS], s_before[WORDS], s_start[REQ + 1], s_first[REQ], s_who[REQ], s_wave[WAVES], s_bad;
+  __shared__ int32_t s_parent[REQ], s_len[REQ];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = 1u << t.shift;
+  // sum over the threads before this one, and over all
+  auto scan = [&](uint32_t v, uint32_t& total) {
+    const uint32_t upto = scan64_lanes(v);
+    __syncthreads();
+    if (lane == 63) s_wave[wave] = upto;
+    __syncthreads();
+    uint32_t before = upto - v;
+    total = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < WAVES; k++) {
+      if (k < wave) before += s_wave[k];
+      total += s_wave[k];
+    }
+    return before;
+  };
+  int32_t p = -1, len = 0;
+  if (tid < t.n_req) p = t.parents[tid];
+  s_map[tid] = s_map[tid + SMALL_THREADS] = 0;
+  s_first[tid] = ~0u;
+  if (tid == 0) s_bad = 0;
+  __syncthreads();
+  if (p != -1) {
+    if (p < -1 || (uint32_t)p >= t.n_req) {
+      paged_err(err, PAGED_ERR_FORK_PARENT, tid);
+      s_bad = 1;
+      p = -1;
+    } else {
+      len = t.lens[p];
+      if (!fits(t, len)) {
+        paged_err(err, PAGED_ERR_FORK_LENGTH, (uint32_t)p);
+        s_bad = 1;
+        len = 0;
+      }
+      atomicMin(&s_first[p], tid);
+    }
+  }
+  s_parent[tid] = p;
+  s_len[tid] = len;
+  const uint32_t pages = pages_of(t, len);
+  uint32_t entries;
+  s_start[tid] = scan(pages, entries);
+  if (tid == 0) s_start[REQ] = entries;
+  __syncthreads();
+  const bool copy = p >= 0 && s_first[p] != tid && (len & (int32_t)(P - 1));
+  if (tid < t.n_req) new_lens[tid] = len;
+  constexpr uint32_t BATCH = 4;
+  for (uint32_t e0 = tid; e0 < entries; e0 += BATCH * SMALL_THREADS) {
+    int32_t page[BATCH];
+    uint32_t of[BATCH], j[BATCH];
+    bool kept[BATCH];
+#pragma unroll
+    for (uint32_t k = 0; k < BATCH; k++) {
+      const uint32_t e = e0 + k * SMALL_THREADS < entries ? e0 + k * SMALL_THREADS : entries - 1;
+      // the last request that starts at or before e (those without pages start there too)
+      uint32_t lo = 0;
+#pragma unroll
+      for (uint32_t step = REQ / 2; step; step >>= 1)
+        if (s_start[lo + step] <= e) lo += step;
+      of[k] = lo;
+      j[k] = e - s_start[lo];
+      kept[k] = is_kept(t, j[k], (uint32_t)s_len[lo]);
+      page[k] = kept[k] ? t.tables[(size_t)s_parent[lo] * t.max_pages + j[k]] : -1;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < BATCH; k++) {
+      if (e0 + k * SMALL_THREADS >= entries) continue;
+      if (kept[k]) {
+        if ((uint32_t)page[k] >= t.n_pages) {
+          paged_err(err, PAGED_ERR_FORK_PAGE, (uint32_t)s_parent[of[k]]);
+          s_bad = 1;
+          continue;
+        }
+        atomicOr(&s_map[(uint32_t)page[k] >> 5], 1u << (page[k] & 31));
+      }
+      // the last entry of a request that copies is written below
+      const int32_t n = s_len[of[k]];
+      if (s_first[s_parent[of[k]]] == of[k] || !(n & (int32_t)(P - 1)) || j[k] != (uint32_t)n >> t.shift)
+        new_tables[(size_t)of[k] * t.max_pages + j[k]] = page[k];
+    }
+  }
+  uint32_t need, lives;
+  const uint32_t at = scan(copy, need);
+  if (copy) s_who[at] = tid;
+  const uint32_t x0 = s_map[2 * tid], x1 = s_map[2 * tid + 1];
+  const uint32_t before = scan((uint32_t)(__popc(x0) + __popc(x1)), lives), frees = t.n_pages - lives;
+  s_before[2 * tid] = before;
+  s_before[2 * tid + 1] = before + (uint32_t)__popc(x0);
+  __syncthreads();
+  const bool bad = s_bad || need > frees;
+  if (tid == 0) {
+    if (!s_bad && bad) paged_err(err, PAGED_ERR_FORK_FREE, frees);
+    free_count[0] = bad ? 0 : (int32_t)(frees - need);
+    w.state[1] = bad ? 0 : need;
+  }
+  if (bad) return;
+  for (uint32_t page = tid; page < t.n_pages; page += SMALL_THREADS) {
+    const uint32_t bits = s_map[page >> 5], bit = page & 31;
+    if (bits >> bit & 1) continue;
+    const uint32_t rank = page - s_before[page >> 5] - (uint32_t)__popc(bits & ((1u << bit) - 1));  // free pages before it
+    if (rank >= need) {
+      free_pages[frees - 1 - rank] = (int32_t)page;
+      continue;
+    }
+    const uint32_t b = s_who[rank], n = (uint32_t)s_len[b], j = n >> t.shift;
+    w.src[rank] = (uint32_t)t.tables[(size_t)s_parent[b] * t.max_pages + j];
+    w.dst[rank] = page;
+    w.keys[rank] = n & (P - 1);
+    new_tables[(size_t)b * t.max_pages + j] = (int32_t)page;
+  }
+}
+
 // The moves of a compaction: of n live pages, those at n and above go to the free
 // ones below n, lowest to lowest.  A page that is read is never written.
 extern "C" __global__ __launch_bounds__(PAGES_THREADS) void smith_pages_line(Work w, uint32_t n_pages,

@@ -2681,6 +2681,10 @@ static int ensure_pages_map(Ctx* c, const char* fn, size_t need) {
 
 // Pools of more than so many times 8192 pages get a launch that counts them
 constexpr uint32_t PAGES_COUNT_BLOCKS = 32;
+// Entries of all block tables, used or not, that one workgroup looks through: 8 requests
+// on 700 keys (368 entries) 9.6 us, 13.1 by the card; 160 of 1000 (16320) 15.0, 23.6; 400
+// of 1200 (30800) 21, 27; 256 of 3000 (53504) 32, 35; 120 of 8000 (64080) 38, 28.
+constexpr uint64_t PAGES_SMALL_ENTRIES = 3 << 14;
 
 // What fork and compact have in common: checks, scratch and the first launch.
 struct PagesCall {
@@ -2688,6 +2692,7 @@ struct PagesCall {
   PagesWork w;
   uint32_t row16, blocks;  // 16-byte units of a key, workgroups of 256 words
   uint64_t page16;         // 16-byte units of a page
+  bool small;
 };
 
 static int pages_begin(Ctx* c, const char* fn, PagesCall* call, uint32_t kv_type, const int32_t* lens, const int32_t* tables,
@@ -2752,6 +2757,12 @@ static int pages_begin(Ctx* c, const char* fn, PagesCall* call, uint32_t kv_type
   call->row16 = head_dim * (kv_type == SMITH_KV_F32 ? 4 : 2) / 16;
   call->page16 = pool / n_pages / 16;
   call->blocks = blocks;
+  // A fork whose tables have room for few entries is one workgroup's work.
+  call->small = fork && n_req <= PAGES_SMALL_REQ && n_pages <= PAGES_SMALL_PAGES && (uint64_t)n_req * max_pages <= PAGES_SMALL_ENTRIES;
+  if (call->small) {
+    call->w.words = 0;  // it has a map of its own
+    return 0;
+  }
   // a request's entries over as many workgroups as fill the card, 256 entries each at least
   const uint32_t split = std::max<uint32_t>(1, std::min<uint32_t>(2048 / n_req, (max_pages + PAGES_THREADS - 1) / PAGES_THREADS));
   uint64_t* perr = c->paged_err_dev();
@@ -2796,7 +2807,9 @@ int smith_paged_fork(void* ctx, uint32_t kv_type, const int32_t* lens, const int
     return -1;
   uint64_t* perr = c->paged_err_dev();
   void* args[] = {&call.t, &call.w, &new_lens, &new_tables, &free_pages, &free_count, &perr};
-  if (launch(c, "smith_pages_fork", dim3(call.blocks), dim3(PAGES_THREADS), args)) return -1;
+  if (call.small ? launch(c, "smith_pages_fork_small", dim3(1), dim3(1024), args)
+                 : launch(c, "smith_pages_fork", dim3(call.blocks), dim3(PAGES_THREADS), args))
+    return -1;
   return pages_end(c, &call, n_req, n_kv_heads, pools, n_pools);
 }
 

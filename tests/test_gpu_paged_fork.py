@@ -50,6 +50,12 @@ def state(seed, n, P, longest, spare=5, share=0.6):
     return rs, lens.astype(np.int32), tables.astype(np.int32), n_pages
 
 
+def widened(tables):
+    """With room for more entries than one workgroup looks through."""
+    n, w = tables.shape
+    return np.concatenate([tables, np.full((n, max(0, (3 << 14) // n + 1 - w)), 2 ** 30, np.int32)], 1)
+
+
 def pools_of(rs, count, n_pages, kv, P, D, dtype):
     return [R.stored(rs.standard_normal((n_pages, kv, P, D)).astype(np.float32), dtype) for _ in range(count)]
 
@@ -77,11 +83,14 @@ def parents_of(rs, n, how):
 
 @pytest.mark.parametrize("n,P,longest,dtype,kv,D,count", [
     (1, 16, 40, "f16", 2, 16, 1), (2, 1, 7, "f32", 1, 8, 2), (5, 4, 30, "bf16", 3, 24, 4), (24, 16, 200, "f32", 2, 128, 3),
-    (64, 8, 100, "f16", 1, 8, 2), (65, 32, 100, "bf16", 2, 40, 2), (257, 2, 40, "f16", 1, 8, 1), (700, 16, 90, "f32", 1, 8, 1),
+    (64, 8, 100, "f16", 1, 8, 2), (1024, 8, 60, "f16", 1, 8, 1), (1025, 8, 60, "f16", 1, 8, 1), (65, 32, 100, "bf16", 2, 40, 2), (257, 2, 40, "f16", 1, 8, 1), (700, 16, 90, "f32", 1, 8, 1),
     (4096, 16, 33, "f16", 1, 8, 1), (3, 128, 5000, "f16", 8, 128, 2), (2, 16, 9000, "f32", 1, 8, 1)])
 @pytest.mark.parametrize("how", ["same", "one", "none", "swap", "any"])
-def test_fork(n, P, longest, dtype, kv, D, count, how):
+@pytest.mark.parametrize("wide", [False, True])
+def test_fork(n, P, longest, dtype, kv, D, count, how, wide):
     rs, lens, tables, n_pages = state(n + P, n, P, longest, 5 + n)
+    if wide:
+        tables = widened(tables)
     parents = parents_of(rs, n, how).astype(np.int32)
     pools = pools_of(rs, count, n_pages, kv, P, D, dtype)
     marks = np.full(tables.shape, -77, np.int32)
@@ -105,8 +114,11 @@ def test_fork(n, P, longest, dtype, kv, D, count, how):
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 5), (7, 0), (16, 4), (17, 16), (40, 17), (1000, 3), (2 ** 31, 2 ** 31)])
 @pytest.mark.parametrize("P", [1, 4, 16])
-def test_fork_leaves_what_a_window_sees(window, sinks, P):
+@pytest.mark.parametrize("wide", [False, True])
+def test_fork_leaves_what_a_window_sees(window, sinks, P, wide):
     rs, lens, tables, n_pages = state(window % 97 + P, 12, P, 120, 20)
+    if wide:
+        tables = widened(tables)
     pools = pools_of(rs, 2, n_pages, 2, P, 8, "f16")
     # pages that no later row sees were dropped before, too
     for b in range(12):
@@ -151,7 +163,7 @@ def test_compact(n, P, longest, dtype, kv, D, spare, window, sinks):
         x.release()
 
 
-@pytest.mark.parametrize("n_pages,n", [(40000, 6), (300000, 40), (1 << 20, 3), (1 << 20, 2000)])
+@pytest.mark.parametrize("n_pages,n", [(40000, 6), (65536, 30), (65537, 30), (300000, 40), (1 << 20, 3), (1 << 20, 2000)])
 def test_large_pools(n_pages, n):
     """Pools whose pages are counted by a launch of their own, and smaller ones."""
     rs = np.random.RandomState(n)
@@ -207,13 +219,14 @@ def test_more_pools_than_one_launch_takes():
     assert np.array_equal(out[1].data, want[1]) and out[3].data[0] == want[3]
 
 
-def test_a_graph_of_forks_and_compactions():
+@pytest.mark.parametrize("wide", [False, True])
+def test_a_graph_of_forks_and_compactions(wide):
     """Both captured in one graph, replayed on other requests with eager calls between."""
     ctx = device.ops_ctx()
     P, n = 4, 9
     states = [state(40 + k, n, P, 60, 30) for k in range(5)]
     n_pages = max(s[3] for s in states)
-    width = max(s[2].shape[1] for s in states)
+    width = (3 << 14) // n + 1 if wide else max(s[2].shape[1] for s in states)
     rs = np.random.RandomState(1)
     pool = R.upload(pools_of(rs, 1, n_pages, 2, P, 16, "f32")[0], "f32")
     lens, tables, parents = S.zeros([n], "i32"), S.zeros([n, width], "i32"), S.zeros([n], "i32")
@@ -277,7 +290,7 @@ def test_a_graph_of_forks_and_compactions():
     ("parent", "request 2: its parent"), ("parent_low", "request 2: its parent"), ("negative", "request 1: its length"),
     ("long", "request 1: its length"), ("page", "request 1: a page outside"), ("page_low", "request 1: a page outside"),
     ("free", "more than the 0 pages")])
-@pytest.mark.parametrize("call", ["fork", "compact"])
+@pytest.mark.parametrize("call", ["fork", "wide fork", "compact"])
 def test_what_does_not_fit_copies_nothing(call, what, message):
     P, n_pages = 4, 7
     lens, parents = np.array([6, 9, 0, 4], np.int32), np.array([1, 0, 1, 3], np.int32)
@@ -288,19 +301,21 @@ def test_what_does_not_fit_copies_nothing(call, what, message):
         parents[2] = -2
     elif what == "negative":
         lens[1] = -1
-    elif what == "long":
-        lens[1] = 13
     elif what.startswith("page"):
         tables[1, 1] = 7 if what == "page" else -1
-    else:
+    elif what == "free":
         lens[3], tables[3, 1] = 8, 6
     if call == "compact" and (what.startswith("parent") or what == "free"):
         return  # it has no parents and copies nothing
+    if call == "wide fork":
+        tables = widened(tables)
+    if what == "long":
+        lens[1] = tables.shape[1] * P + 1
     rs = np.random.RandomState(0)
     host = pools_of(rs, 1, n_pages, 2, P, 8, "f32")[0]
     pool, t = R.upload(host), i32(tables)
     for _ in range(2):
-        if call == "fork":
+        if call != "compact":
             new = S.pagedFork(i32(lens), t, i32(parents), [pool])
         else:
             new = S.pagedCompact(i32(lens), t, [pool])
