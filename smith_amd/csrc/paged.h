@@ -29,10 +29,11 @@ struct AttArgs {
   float q_factor;                       // scale log2 e = q_factor 2^c_exp, 0.36 < |q_factor| < 0.73
   int32_t c_exp;
 };
-// a request's group: its shared keys, its first partial, splits of its blocks, first row, blocks
+// a request's group: its shared keys (-1: it does not fit), its first partial, splits of
+// its blocks, first row, rows, blocks
 struct SharedOf {
   int32_t keys;
-  uint32_t part, splits, row0, blocks;
+  uint32_t part, splits, row0, rows, blocks;
 };
 // and of the kernels whose rows do not see all keys, or not all at once
 struct ReachArgs : AttArgs {

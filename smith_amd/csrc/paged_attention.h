@@ -389,8 +389,9 @@ __device__ __forceinline__ float2 get2(const float* p) {
 // Request b's first row, rows and length; no rows if they do not fit, or if
 // row_start does not end in the rows there are.
 // (SHARED: group b's, and its shared keys.)  from: OWN, the shared keys before them.
+// False if they do not fit.
 template <Reach R>
-__device__ __forceinline__ void request(const Args<R>& a, uint32_t b, bool tell, uint32_t& r0, uint32_t& n, uint32_t& len,
+__device__ __forceinline__ bool request(const Args<R>& a, uint32_t b, bool tell, uint32_t& r0, uint32_t& n, uint32_t& len,
                                         uint32_t& from) {
   from = 0;
   if constexpr (R == SHARED) {
@@ -410,7 +411,7 @@ __device__ __forceinline__ void request(const Args<R>& a, uint32_t b, bool tell,
     r0 = (uint32_t)s;
     n = fits ? (uint32_t)(e - s) : 0u;
     len = fits ? (uint32_t)l : 0u;
-    return;
+    return fits;
   }
   int32_t s = (int32_t)b, e = s + 1;
   if (a.row_start) {
@@ -435,14 +436,21 @@ __device__ __forceinline__ void request(const Args<R>& a, uint32_t b, bool tell,
     len = 0;
   }
   if constexpr (R == OWN) {
-    const int32_t f = a.whole ? 0 : a.from[b].keys;
-    if (n && f && (f < 0 || f > l - (int32_t)n)) {
-      if (tell && f > 0) paged_err(a.err, PAGED_ERR_ATT_SHARED, b);
-      n = 0;
-      len = 0;
+    if (n && !a.whole) {
+      // its rows are rows of its group: what SHARED left of them is there
+      const SharedOf f = a.from[b];
+      const bool enough = f.keys == 0 || f.keys <= l - (int32_t)n;
+      const bool inside = r0 >= f.row0 && r0 - f.row0 <= f.rows && n <= f.rows - (r0 - f.row0);
+      if (f.keys < 0 || (f.keys && !(enough && inside))) {
+        if (tell && f.keys > 0) paged_err(a.err, enough ? PAGED_ERR_ATT_LENGTH : PAGED_ERR_ATT_SHARED, b);
+        n = 0;
+        len = 0;
+        return false;
+      }
+      from = (uint32_t)f.keys;
     }
-    from = n ? (uint32_t)f : 0u;
   }
+  return fits;
 }
 
 // The items of a call, from what each workgroup works out in LDS.  Which comes when
@@ -1099,11 +1107,11 @@ __device__ __forceinline__ void tell_requests(const Args<R>& a, const Items<SORT
   if constexpr (R == SHARED) {
     if (a.n_req <= 64) __syncthreads();  // each wave has written the table for itself
     for (uint32_t g = blockIdx.x; g < a.n_req; g += gridDim.x) {
-      const int32_t g0 = a.group_start[g], g1 = a.group_start[g + 1], l = a.shared[g];
+      const int32_t g0 = a.group_start[g], g1 = a.group_start[g + 1];
       if (g0 < 0 || g1 < g0 || (uint32_t)g1 > a.n_all) continue;
-      const bool fits = l >= 0 && (uint64_t)(uint32_t)l <= ((uint64_t)a.max_pages << a.shift);
-      const uint32_t n = t.row[g + 1] - t.row[g];
-      const SharedOf f = {fits ? l : -1, t.part[g], t.splits(t.len[g], t.inv_c), t.row[g], div_up(n, a.rows_blk) * a.groups};
+      uint32_t r0, n, len, from;
+      const bool fits = request<R>(a, g, false, r0, n, len, from);
+      const SharedOf f = {fits ? (int32_t)len : -1, t.part[g], t.splits(len, t.inv_c), r0, n, div_up(n, a.rows_blk) * a.groups};
       for (uint32_t b = (uint32_t)g0 + threadIdx.x; b < (uint32_t)g1; b += 256) a.from[b] = f;
     }
   }
@@ -1328,7 +1336,7 @@ __device__ __forceinline__ void attention_body(const Args<R>& args) {
       // four columns to a wave, 16 lanes each; of few columns the prior's splits go to
       // several waves in turn.  A wave adds its share to what it has just written.
       const uint32_t few = I.ncols <= 4 ? 4 : I.ncols <= 8 ? 2 : 1, c = w / few * 4 + lg;
-      if (!z.whole && I.split == 0 && c < I.ncols) {
+      if (!z.whole && of.keys && I.split == 0 && c < I.ncols) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (ln * DPL < z.hd) {
           const Prior<R> prior(z, I, of, c);
@@ -1780,7 +1788,7 @@ __device__ __forceinline__ void attention_rows_body(const Args<R>& args) {
     for (int t = 0; t < CT; t++) {
       const uint32_t col = (w * CT + t) * 16 + ln;
       if constexpr (R == OWN) {
-        if (!z.whole && I.split == 0 && col < I.ncols) {
+        if (!z.whole && of.keys && I.split == 0 && col < I.ncols) {
           const Prior<R> prior(z, I, of, col);
           add_prior<4 * DPL>(prior.o, prior.ml, prior.stride, uniform(of.splits), 0, 1, lg == 0, m[t], l[t],
                              [&](const float* o, float(&x)[4 * DPL]) {

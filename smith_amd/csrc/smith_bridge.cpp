@@ -2555,7 +2555,7 @@ static int launch_attention(Ctx* c, const AttCall& k, const char* of, uint32_t n
   // stages of K and V rows (64 of f16 / bf16 or 32 of f32: 256 bytes a head dim) and their marks;
   // of both: the items' table
   const uint32_t lds = (many ? 256 * 2 * (dims <= 64 ? 64 : 128) + 16 : 4 * 16 * (dims + 4) * 4 + 4 * 16 * 2 * 4) + 16 +
-                       (*of ? 24 : 20) * (n + 1);
+                       (strcmp(of, "_own") ? 20 : 24) * (n + 1);
   int c_exp;
   const float q_factor = (float)(frexp((double)k.scale, &c_exp) * (0.5 * 1.4426950408889634));
   c_exp++;
@@ -2646,7 +2646,8 @@ int smith_paged_attention_shared(void* ctx, uint32_t kv_type, const float* q, ui
   // behind 1200 13, 17 (40 MB).
   const uint64_t room = pool_bytes(kv_type, n_kv_heads, head_dim, n_req, 1) * 2 * ((uint64_t)max_pages << k.shift);
   more.whole = room <= SHARED_ROOM;
-  if (more.whole) return launch_attention(c, k, "_own", n_req, many_columns(k) ? 64 : 16, &more);
+  const uint32_t own = many_columns(k) && n_req <= 4000 ? 64 : 16;  // of more the items' table has no room in LDS beside the stages
+  if (more.whole) return launch_attention(c, k, "_own", n_req, own, &more);
   // of each column what its shared keys give, and of each request how many they are
   const size_t H = n_heads, floats = (size_t)max_rows * H * (head_dim + 2), parts = (size_t)ATT_MAX_PARTS * 64 * (head_dim + 2);
   if (ensure(c, &c->paged_prior, &c->paged_prior_bytes, (floats + parts) * 4 + n_req * sizeof(SharedOf))) return -1;
@@ -2666,7 +2667,7 @@ int smith_paged_attention_shared(void* ctx, uint32_t kv_type, const float* q, ui
   more.s_rows_blk = more.rows_blk;
   more.s_heads_blk = more.heads_blk;
   more.s_groups = more.groups;
-  return launch_attention(c, k, "_own", n_req, many_columns(k) ? 64 : 16, &more);
+  return launch_attention(c, k, "_own", n_req, own, &more);
 }
 
 // The state and map of fork and compact: as ensure(), and zero.

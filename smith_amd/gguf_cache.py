@@ -441,18 +441,12 @@ def scoreTokens(model, tokenIds, top=0):
         raise ValueError("score: a token outside the vocabulary of %d" % e.cfg["vocabSize"])
     _check_rope_range(e.cfg, len(tokens) - 2)
     _check_top(e, top, 0)
-    caches, parts, at = createGGUFCache(e.cfg), [], [1]
+    caches, parts, at = _kept_caches(model, e.cfg), [], [1]
 
     def take(ptr, rows):
-        part = e.score_rows(ptr, rows, tokens[at[0]:at[0] + rows], top)
-        parts.append(part)
+        parts.append(e.score_rows(ptr, rows, tokens[at[0]:at[0] + rows], top))
         at[0] += rows
-    try:
-        e.prefill(model, tokens[:-1], caches, take=take)
-    finally:
-        for c in caches:
-            for name in ("k", "v"):
-                device.release_buffer(c[name].ptr)
+    e.prefill(model, tokens[:-1], caches, take=take)
     out = {name: np.concatenate([p[name] for p in parts]) for name in ("logprobs", "entropy", "topIds", "topLogprobs")}
     return dict(out, logprobs=out["logprobs"][:, 0])
 
@@ -499,6 +493,15 @@ def _sample(logits, generated, cfg, rng):
     return min(idx, lg.size - 1)
 
 
+def _kept_caches(model, cfg):
+    """The caches of generate and score, empty."""
+    caches = model.get("_gen_caches")
+    if caches is None:
+        caches = model["_gen_caches"] = createGGUFCache(cfg)
+    resetCache(caches)
+    return caches
+
+
 def generateGGUF(model, promptIds, config=None, callbacks=None):
     """gguf_cache.js:309-371: prefill, then one token per step; returns
     [...prompt, ...generated]."""
@@ -516,10 +519,7 @@ def generateGGUF(model, promptIds, config=None, callbacks=None):
     n = len(prompt)
     last_pos = min(n + cfg["maxTokens"] - 2, mcfg["maxSeqLen"] - 1)
     _check_rope_range(mcfg, max(n - 1, last_pos))
-    caches = model.get("_gen_caches")
-    if caches is None:
-        caches = model["_gen_caches"] = createGGUFCache(mcfg)
-    resetCache(caches)
+    caches = _kept_caches(model, mcfg)
     greedy = cfg["temperature"] == 0 and cfg["repetitionPenalty"] <= 1
     rng = np.random.default_rng(config.get("seed"))
 

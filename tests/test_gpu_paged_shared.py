@@ -133,6 +133,35 @@ def test_many_requests(dtype, n, groups):
     check(run(*c, False), c, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,groups", [(4096, 4096), (4096, 3), (4000, 200)])
+def test_most_requests_with_many_columns(dtype, n, groups):
+    """By the kernels of many columns where their tables fit beside the stages."""
+    rs = np.random.RandomState(groups)
+    widths = np.full(groups, n // groups)
+    widths[:n % groups] += 1
+    c = case(n + groups, dtype, 8, 1, 8, 8, widths, rs.randint(0, 20, groups), rs.randint(4, 9, n), 4)
+    check(run(*c, True), c, dtype)
+
+
+@pytest.mark.parametrize("room", [0, room_for_many(4, 2, 4)])
+@pytest.mark.parametrize("starts", [[0, 5, 3, 8, 9], [0, 3, 9, 4, 6], [3, 1, 9, 4, 9], [9, 0, 9, 0, 9], [0, 9, 9, 2, 2], [-1, 4, 5, 7, 9]])
+@pytest.mark.parametrize("apart", [True, False])
+def test_row_start_out_of_order_stays_inside(starts, room, apart):
+    """Starts that go back and forth: no request reads what its group did not leave, and
+    the calls after it are right."""
+    c = q, row_start, lens, tables, k, v, start, shared = case(6, "f16", 4, 2, 32, 16, [2, 2], [40, 30], [20, 20, 20, 20],
+                                                               [3, 2, 2, 2], apart=apart)
+    rows = max(room, len(q))
+    hq = np.zeros((rows, 128), np.float32)
+    hq[:len(q)] = q.reshape(len(q), -1)
+    S.pagedAttention(R.upload(hq), i32(lens), i32(tables), R.upload(k), R.upload(v), i32(starts), 0.0, None,
+                     groupStart=i32(start), shared=i32(shared))
+    assert "smith_paged_attention" in sync_error()
+    device.sync()
+    check(run(*c, True, room), c, "f16")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("where", ["shared", "own"])
 @pytest.mark.parametrize("ragged", [False, True])

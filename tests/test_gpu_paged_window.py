@@ -98,6 +98,12 @@ def test_many_requests(dtype, n):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_most_requests_with_many_columns(dtype):
+    rs = np.random.RandomState(2)
+    one(5, dtype, 8, 1, 8, 8, rs.randint(4, 40, 4096), [4] * 4096, 300, 2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("ragged,room", [(False, 0), (True, 0), (True, room_for_many(6, 2, 4))])
 @pytest.mark.parametrize("junk", [np.nan, np.inf, -np.inf])
 def test_ignores_what_a_row_does_not_see(dtype, ragged, room, junk):
