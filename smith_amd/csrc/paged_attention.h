@@ -1,6 +1,7 @@
 // paged_attention.h -- attention over the pages of the paged cache: what its
-// kernels are made of (gfx950).  paged_kernels.hip and paged_band_kernels.hip
-// instantiate them.
+// kernels are made of (gfx950).  paged_kernels.hip instantiates those over all keys,
+// paged_window_kernels.hip, paged_shared_kernels.hip and paged_own_kernels.hip those
+// over some of them.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

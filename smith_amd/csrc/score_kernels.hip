@@ -15,10 +15,10 @@
 // the maximum of 16.  Lists are
 // joined by bitonic merges: the result does not depend on who comes first.
 //
-// Bound by memory where few are wanted of long f32 rows: 900 of 131072, 472 MB, 85 us
-// without top ones (5.5 TB/s; a large copy: 4.8), 91 with 8, 140 with 64; of bf16 logits
-// by the operations, 49, 72 and 138.  Short rows by the first lists and their merges: one
-// row of 32000 4.8 us without top ones, 9.0 with 5, 13.3 with 64.
+// Bound by memory where few are wanted of long f32 rows: 900 of 131072, 472 MB, 83 us
+// without top ones (5.7 TB/s; a large copy: 5.2), 90 with 8, 138 with 64; of bf16 logits
+// by the operations, 48, 70 and 136.  Short rows by the first lists and their merges: one
+// row of 32000 4.6 us without top ones, 8.9 with 8, 13.0 with 64.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -174,6 +174,13 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
   // this split's chunks, to the waves in turn
   const uint32_t begin = split * a.per_split, end = a.vocab - begin < a.per_split ? a.vocab : begin + a.per_split;
 
+  // the first 64 given tokens and their logits, on their way while the row is read
+  int32_t token = -1;
+  float given = 0.f;
+  if (w == 0 && lane < a.given) {
+    token = a.tokens[(size_t)row * a.given + lane];
+    if ((uint32_t)token < a.vocab) given = L::up(x[token]);
+  }
   if (tid == 0) s_least = 0;
   if (a.top) __syncthreads();
   Sums sum = {-__builtin_inff(), 0.f, 0.f};
@@ -216,7 +223,8 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
       }
       many = __popcll(__ballot(best != 0)) > MANY;
       if (!many) break;
-      list = merge64(list, sort64(best, lane), lane);
+      const uint64_t sorted = sort64(best, lane);
+      list = readlane64(list, 0) ? merge64(list, sorted, lane) : sorted;
       raise();
       below = best;
       if (a.top <= FEW) break;
@@ -354,12 +362,15 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
   }
   for (uint32_t k = lane; k < a.given; k += 64) {
     const size_t to = (size_t)row * a.given + k;
-    const int32_t t = a.tokens[to];
+    if (k >= 64) {
+      token = a.tokens[to];
+      if ((uint32_t)token < a.vocab) given = L::up(x[token]);
+    }
     float p = 0.f;
-    if (t != -1) {
-      const bool in = (uint32_t)t < a.vocab;
+    if (token != -1) {
+      const bool in = (uint32_t)token < a.vocab;
       if (!in) paged_err(a.err, PAGED_ERR_SCORE_TOKEN, row);
-      p = in ? L::up(x[t]) - sum.m - log_l : nan;
+      p = in ? given - sum.m - log_l : nan;
     }
     a.logprobs[to] = p;
   }
