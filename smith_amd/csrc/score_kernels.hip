@@ -32,8 +32,12 @@ typedef uint32_t u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
 #define LOG2E 1.44269504088896341f
 #define THREADS SCORE_THREADS
 #define WAVES (SCORE_THREADS / 64)
-#define MANY 12                   // lanes whose elements go into a list together
-#define FEW 24                    // of so many top ones one element of each lane tells the others from nearly all
+// Lanes whose elements go into a list together, sorted first (900 rows of 131072 f32, top
+// 64, 138 us, 150 with 6, 138 with 24; 256 rows of 32000, top 20, 22.1, 22.5 and 22.6)
+#define MANY 12
+// Top ones for which one sorted round is enough, the rest of a chunk going in one by one (57
+// rows of 50003, top 20: 14.2 us, 15.1 with rounds while they are many; top 64: 23 and 18)
+#define FEW 24
 #define PER 16                    // elements of a thread to a chunk
 #define CHUNK SCORE_WAVE_CHUNK    // of a wave
 
