@@ -9,6 +9,12 @@
 // attention: most splits of a block (their weights are kept in LDS, 16 columns of them)
 #define PAGED_SPLIT_MAX 128u
 
+// items wanted of a call, two workgroups to a CU, and partials at most: a block that is
+// cut has more than 5/4 C keys and so less than twice its keys / C splits, 2 W / C <= 2
+// target of them in all (and some for what f32 rounds)
+#define PAGED_TARGET 512u
+#define PAGED_MAX_PARTS (2u * PAGED_TARGET + 16u)
+
 // attention
 struct AttArgs {
   const float* q;

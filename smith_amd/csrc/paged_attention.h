@@ -441,8 +441,14 @@ __device__ __forceinline__ bool request(const Args<R>& a, uint32_t b, bool tell,
       // its rows are rows of its group: what SHARED left of them is there
       const SharedOf f = a.from[b];
       const bool enough = f.keys == 0 || f.keys <= l - (int32_t)n;
+      // (of requests that no group has, or two, f may be anything: its partials are some
+      // of those there is room for)
       const bool inside = r0 >= f.row0 && r0 - f.row0 <= f.rows && n <= f.rows - (r0 - f.row0);
-      if (f.keys < 0 || (f.keys && !(enough && inside))) {
+      const bool there = f.splits <= 1 ||
+                         (f.splits <= PAGED_SPLIT_MAX && f.rows <= a.max_rows && f.blocks <= PAGED_MAX_PARTS &&
+                          div_up(f.rows, a.s_rows_blk) * (uint64_t)a.s_groups <= f.blocks &&
+                          f.part + (uint64_t)f.blocks * f.splits * a.nKV <= PAGED_MAX_PARTS);
+      if (f.keys < 0 || (f.keys && !(enough && inside && there))) {
         if (tell && f.keys > 0) paged_err(a.err, enough ? PAGED_ERR_ATT_LENGTH : PAGED_ERR_ATT_SHARED, b);
         n = 0;
         len = 0;

@@ -2517,17 +2517,12 @@ static bool many_columns(const AttCall& k) {
   return k.row_start && k.shift >= 3 && (uint64_t)k.max_rows * G > 24ull * k.n_req && (uint64_t)k.max_rows * k.n_heads >= 8192;
 }
 
-constexpr uint32_t ATT_TARGET = 512;  // items wanted: two workgroups to a CU
-// a block that is cut has more than 5/4 C keys and so less than twice its keys / C
-// splits: 2 W / C <= 2 target of them in all (and some for what f32 rounds)
-constexpr uint32_t ATT_MAX_PARTS = 2 * ATT_TARGET + 16;
-
 // `n` requests (or groups) of k, by the kernel of `of` ("", _window, _shared or _own) whose blocks have CB columns
 static int launch_attention(Ctx* c, const AttCall& k, const char* of, uint32_t n, uint32_t CB, ReachArgs* more) {
   const uint32_t G = k.n_heads / k.n_kv_heads;
   const bool many = CB > 16, small = !many && k.shift < 4;
   const uint32_t dims = k.head_dim <= 64 ? 64 : k.head_dim <= 96 ? 96 : 128;
-  const uint32_t target = ATT_TARGET;
+  const uint32_t target = PAGED_TARGET;
   // Keys to a split at least.  A split of many columns leaves 64 KB and the join
   // reads them again: 64 rows behind 8000 keys, 32 heads, in that kernel 58 us (f16) and
   // 69 (bf16) with 512, 64 and 77 with 768, 74 and 84 with 384; 300 rows of a prompt 20.8
@@ -2544,7 +2539,7 @@ static int launch_attention(Ctx* c, const AttCall& k, const char* of, uint32_t n
                           : !strcmp(of, "_shared") ? f32 ? 64.f : 128.f
                           : !many                  ? f32 ? 64.f : 128.f
                                                    : f32 ? 128.f : 256.f;
-  const uint32_t max_parts = ATT_MAX_PARTS;
+  const uint32_t max_parts = PAGED_MAX_PARTS;
   if (ensure(c, &c->paged_ws, &c->paged_ws_bytes, (size_t)max_parts * CB * (k.head_dim + 2) * sizeof(float))) return -1;
   if (ensure_paged_counters(c)) return -1;
   const uint32_t heads_blk = std::min(G, CB), RB = CB / heads_blk, groups = (G + CB - 1) / CB;
@@ -2649,7 +2644,7 @@ int smith_paged_attention_shared(void* ctx, uint32_t kv_type, const float* q, ui
   const uint32_t own = many_columns(k) && n_req <= 4000 ? 64 : 16;  // of more the items' table has no room in LDS beside the stages
   if (more.whole) return launch_attention(c, k, "_own", n_req, own, &more);
   // of each column what its shared keys give, and of each request how many they are
-  const size_t H = n_heads, floats = (size_t)max_rows * H * (head_dim + 2), parts = (size_t)ATT_MAX_PARTS * 64 * (head_dim + 2);
+  const size_t H = n_heads, floats = (size_t)max_rows * H * (head_dim + 2), parts = (size_t)PAGED_MAX_PARTS * 64 * (head_dim + 2);
   if (ensure(c, &c->paged_prior, &c->paged_prior_bytes, (floats + parts) * 4 + n_req * sizeof(SharedOf))) return -1;
   more.prior = (float*)c->paged_prior;
   more.prior_ml = more.prior + (size_t)max_rows * H * head_dim;

@@ -162,6 +162,24 @@ def test_row_start_out_of_order_stays_inside(starts, room, apart):
     check(run(*c, True, room), c, "f16")
 
 
+@pytest.mark.parametrize("room", [0, room_for_many(4, 2, 9)])
+@pytest.mark.parametrize("starts", [[0, 3, -1, 9], [0, 6, 2, 9], [0, 9, 0, 9], [4, 9, 9, 9], [0, -5, 2 ** 31 - 1, 9]])
+@pytest.mark.parametrize("apart", [True, False])
+def test_groups_that_leave_out_or_repeat_requests_stay_inside(starts, room, apart):
+    """Requests of no group, and of two, behind a call whose shared keys were cut."""
+    c = q, row_start, lens, tables, k, v, start, shared = case(8, "f16", 4, 2, 32, 16, [2, 5, 2], [900, 40, 30], 20,
+                                                               [3, 2, 2, 2, 1, 0, 4, 5, 1], apart=apart)
+    check(run(*c, True, room), c, "f16")
+    rows = max(room, len(q))
+    hq = np.zeros((rows, 128), np.float32)
+    hq[:len(q)] = q.reshape(len(q), -1)
+    S.pagedAttention(R.upload(hq), i32(lens), i32(tables), R.upload(k), R.upload(v), i32(row_start), 0.0, None,
+                     groupStart=i32(starts), shared=i32([30, 40, 30]))
+    assert "smith_paged_attention_shared: group" in sync_error()
+    device.sync()
+    check(run(*c, True, room), c, "f16")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("where", ["shared", "own"])
 @pytest.mark.parametrize("ragged", [False, True])
