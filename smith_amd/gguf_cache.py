@@ -409,12 +409,14 @@ def forwardPagedStep(model, tokens, cache):
     [n, vocab] (host), 'requests': the n requests that had tokens}: the logits
     behind each one's last token."""
     e, tokens = _paged_tokens(model, tokens, cache)
-    logits = []
+    requests, at = [b for b, t in enumerate(tokens) if t], [0]
+    logits = np.empty((len(requests), e.cfg["vocabSize"]), np.float32)
 
     def take(ptr, rows):
-        logits.append(device.download_into(np.empty((rows, e.cfg["vocabSize"]), np.float32), ptr))
+        device.download_into(logits[at[0]:at[0] + rows], ptr)
+        at[0] += rows
     e.paged_step(model, tokens, cache, take)
-    return {"logits": np.concatenate(logits), "requests": [b for b, t in enumerate(tokens) if t]}
+    return {"logits": logits, "requests": requests}
 
 
 def scorePagedStep(model, tokens, cache, top=8):

@@ -34,6 +34,13 @@ MAX_REQUESTS = 4096  # of one step
 MOST_KEYS = 2 ** 31 - 1  # of a request
 
 
+def _window(window, sinks, what):
+    """Both as they fit the calls: no request is longer."""
+    if window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError("%s: a window of %d keys and %d sinks" % (what, window, sinks))
+    return min(window, MOST_KEYS), min(sinks, MOST_KEYS)
+
+
 def _want(t, shape, dtype, what):
     if list(t.shape) != list(shape) or t.dtype != dtype:
         raise ValueError("%s: %s %s wanted, got %s %s" % (what, dtype, list(shape), t.dtype, list(t.shape)))
@@ -104,8 +111,7 @@ def pagedAttention(q, lens, tables, kPages, vPages, rowStart=None, scale=0.0, ou
     _want(tables, [n, tables.shape[-1]], "i32", "pagedAttention: tables")
     if rowStart is not None:
         _want(rowStart, [n + 1], "i32", "pagedAttention: rowStart")
-    if window < 0 or sinks < 0 or (sinks and not window):
-        raise ValueError("pagedAttention: a window of %d keys and %d sinks" % (window, sinks))
+    window, sinks = _window(window, sinks, "pagedAttention")
     name, reach = "smith_paged_attention", ()
     if groupStart is not None or shared is not None:
         if groupStart is None or shared is None or window:
@@ -115,7 +121,7 @@ def pagedAttention(q, lens, tables, kPages, vPages, rowStart=None, scale=0.0, ou
         _want(groupStart, [groups + 1], "i32", "pagedAttention: groupStart")
         name, reach = "smith_paged_attention_shared", (groupStart.buffer, shared.buffer, groups)
     elif window:
-        name, reach = "smith_paged_attention_window", (min(window, MOST_KEYS), min(sinks, MOST_KEYS))
+        name, reach = "smith_paged_attention_window", (window, sinks)
     if out is None:
         out = T.create([rows, width])
     _want(out, [rows, width], "f32", "pagedAttention: out")
@@ -146,6 +152,7 @@ def pagedFork(lens, tables, parents, pools, window=0, sinks=0, newTables=None):
     _want(lens, [n], "i32", "pagedFork: lens")
     _want(parents, [n], "i32", "pagedFork: parents")
     _want(tables, [n, tables.shape[-1]], "i32", "pagedFork: tables")
+    window, sinks = _window(window, sinks, "pagedFork")
     shape, dtype, pointers = _all_pools(pools, "pagedFork")
     if newTables is None:
         newTables = T.create(tables.shape, "i32")
@@ -165,6 +172,7 @@ def pagedCompact(lens, tables, pools, window=0, sinks=0):
     n = lens.shape[0]
     _want(lens, [n], "i32", "pagedCompact: lens")
     _want(tables, [n, tables.shape[-1]], "i32", "pagedCompact: tables")
+    window, sinks = _window(window, sinks, "pagedCompact")
     shape, dtype, pointers = _all_pools(pools, "pagedCompact")
     new = {"freePages": T.create([shape[0]], "i32"), "freeCount": T.create([1], "i32")}
     device.check(device.lib.smith_paged_compact(
@@ -205,10 +213,8 @@ class PagedCache:
             raise ValueError("createPagedCache: %d pages of %d keys" % (pages, pageSize))
         if config["headDim"] % 8 or not 8 <= config["headDim"] <= 128:
             raise ValueError("createPagedCache: heads of %d dims (8, 16 .. 128)" % config["headDim"])
-        if window < 0 or sinks < 0 or (sinks and not window):
-            raise ValueError("createPagedCache: a window of %d keys and %d sinks" % (window, sinks))
         self.requests, self.pages, self.pageSize, self.dtype = requests, pages, pageSize, dtype
-        self.window, self.sinks = min(window, MOST_KEYS), min(sinks, MOST_KEYS)
+        self.window, self.sinks = _window(window, sinks, "createPagedCache")
         self.maxPages = -(-config["maxSeqLen"] // pageSize)
         self.lens = np.zeros(requests, np.int32)
         self.freeCount = pages
@@ -217,6 +223,7 @@ class PagedCache:
         # back), and how many requests name it; what they share, host and device
         self._ids, self._named, self._next_id = None, collections.Counter(), 0
         self._groups, self._group_tensors, self._spare = [], None, None
+        self._read_twice = 0  # bytes of a layer's shared keys and values, once for each further request
         try:
             self._allocate(config)
         except BaseException:
@@ -408,8 +415,8 @@ class PagedCache:
                     groups[-1] = [first, r + 1, min(most, same) if most else same]
                     continue
             groups.append([r, r + 1, 0])
+        self._groups, self._read_twice = [], 0
         if self.window or len(groups) == self.requests:
-            self._groups = []
             return
         start, shared = np.full(self.requests + 1, self.requests), np.zeros(self.requests, np.int64)
         start[:len(groups)] = [g[0] for g in groups]
@@ -417,15 +424,9 @@ class PagedCache:
         self._group_tensors[0].set_data(start)
         self._group_tensors[1].set_data(shared)
         self._groups = groups
-
-    def _read_twice(self):
-        """Bytes of a layer's shared keys and values that are read more than once if each
-        request reads its own."""
-        if not self._groups:
-            return 0
-        k = self.layers[0]["k"]
-        size = 2 * k.shape[1] * k.shape[3] * (4 if self.dtype == "f32" else 2)
-        return size * sum((b - a - 1) * n * self.pageSize for a, b, n in self._groups)
+        k = self.layers[0]["k"] if self.layers else None
+        size = 2 * k.shape[1] * k.shape[3] * (4 if self.dtype == "f32" else 2) if k else 0
+        self._read_twice = size * sum((b - a - 1) * n * self.pageSize for a, b, n in groups)
 
     def trim(self):
         """Gives back the pages that the window has passed."""
@@ -506,7 +507,7 @@ class PagedCache:
         name, reach = "smith_paged_attention", ()
         if self.window:
             name, reach = "smith_paged_attention_window", (self.window, self.sinks)
-        elif self._read_twice() >= SHARED_BYTES:
+        elif self._groups and self._read_twice >= SHARED_BYTES:
             name = "smith_paged_attention_shared"
             reach = (*(t.buffer for t in self._group_tensors), len(self._groups))
         device.check(getattr(device.lib, name)(

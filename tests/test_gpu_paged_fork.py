@@ -426,3 +426,18 @@ def test_a_free_list_that_is_too_short():
         S.pagedFork(lens, t, i32([0]), [pool, S.zeros([9, 1, 4, 8], "f32")])
     with pytest.raises(ValueError, match="pools are"):
         S.pagedCompact(lens, t, [])
+    for call, args in ((S.pagedFork, (lens, t, i32([0]), [pool])), (S.pagedCompact, (lens, t, [pool]))):
+        for window, sinks in ((-1, 0), (0, 1), (3, -1)):
+            with pytest.raises(ValueError, match="a window of %d keys and %d sinks" % (window, sinks)):
+                call(*args, window, sinks)
+
+
+def test_a_window_longer_than_any_request():
+    """More than fits 32 bits is no window of 0."""
+    rs, lens, tables, n_pages = state(3, 5, 4, 40, 3)
+    pool = R.upload(pools_of(rs, 1, n_pages, 1, 4, 8, "f16")[0], "f16")
+    got = [S.pagedFork(i32(lens), i32(tables), i32(np.arange(5)), [pool], window, sinks, i32(tables))
+           for window, sinks in ((0, 0), (2 ** 32 + 1, 2 ** 32))]
+    device.sync()
+    for name in ("lens", "tables", "freeCount"):
+        assert np.array_equal(got[0][name].data, got[1][name].data)
