@@ -18,7 +18,7 @@
 // Bound by memory where few are wanted of long f32 rows: 900 of 131072, 472 MB, 83 us
 // without top ones (5.7 TB/s; a large copy: 5.2), 90 with 8, 138 with 64; of bf16 logits
 // by the operations, 48, 70 and 136.  Short rows by the first lists and their merges: one
-// row of 32000 4.6 us without top ones, 8.9 with 8, 13.0 with 64.
+// row of 32000 4.8 us without top ones, 8.6 with 8, 12.8 with 64.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -83,8 +83,11 @@ __device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
   if constexpr (D == 3) return dpp_u32<0x1B>(v);
   if constexpr (D == 7) return dpp_u32<0x141>(v);   // half-row mirror
   if constexpr (D == 15) return dpp_u32<0x140>(v);  // row mirror
-  if constexpr (D == 4) return lane_xor<7>(lane_xor<3>(v));
-  if constexpr (D == 8) return lane_xor<15>(lane_xor<7>(v));
+  if constexpr (D == 4) {  // lane + 4 to the lower half of 8, lane - 4 to the upper
+    const int lower = __builtin_amdgcn_update_dpp((int)v, (int)v, 0x104, 0xF, 0x5, false);
+    return (uint32_t)__builtin_amdgcn_update_dpp(lower, (int)v, 0x114, 0xF, 0xA, false);
+  }
+  if constexpr (D == 8) return dpp_u32<0x128>(v);  // rotated within 16
   if constexpr (D == 16) {
     const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     return threadIdx.x & 16 ? p[0] : p[1];
@@ -93,6 +96,7 @@ __device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
     const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return threadIdx.x & 32 ? p[0] : p[1];
   }
+  if constexpr (D == 31) return lane_xor<16>(lane_xor<15>(v));
   if constexpr (D == 63) return lane_xor<32>(lane_xor<16>(lane_xor<15>(v)));
 }
 template <int D>
@@ -103,31 +107,41 @@ __device__ __forceinline__ uint64_t readlane64(uint64_t k, uint32_t lane) {
   return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), (int)lane) << 32) |
          (uint32_t)__builtin_amdgcn_readlane((int)k, (int)lane);
 }
-// the larger (or smaller) of a lane's key and its partner's
-template <int D>
-__device__ __forceinline__ uint64_t exchange(uint64_t k, bool larger) {
-  const uint64_t o = lane_xor64<D>(k);
-  return (o > k) == larger ? o : k;
+// the larger of a lane's key and its partner's where lane & HALF is 0, the smaller elsewhere
+template <int PARTNER, int HALF>
+__device__ __forceinline__ uint64_t exchange(uint64_t k) {
+  constexpr uint64_t upper = HALF == 1 ? 0xAAAAAAAAAAAAAAAA : HALF == 2 ? 0xCCCCCCCCCCCCCCCC : HALF == 4 ? 0xF0F0F0F0F0F0F0F0
+                             : HALF == 8 ? 0xFF00FF00FF00FF00 : HALF == 16 ? 0xFFFF0000FFFF0000 : 0xFFFFFFFF00000000;
+  const uint64_t o = lane_xor64<PARTNER>(k);
+  return __builtin_amdgcn_inverse_ballot_w64(__builtin_amdgcn_ballot_w64(o > k) ^ upper) ? o : k;
 }
-// bitonic sequences of 2 D lanes each, sorted: the largest first, or last where `up`
+// bitonic sequences of 2 D lanes each, sorted, the largest first
 template <int D>
-__device__ __forceinline__ uint64_t sort_bitonic(uint64_t k, uint32_t lane, bool up) {
-  k = exchange<D>(k, !(lane & D) != up);
-  if constexpr (D > 1) k = sort_bitonic<D / 2>(k, lane, up);
+__device__ __forceinline__ uint64_t sort_bitonic(uint64_t k) {
+  k = exchange<D, D>(k);
+  if constexpr (D > 1) k = sort_bitonic<D / 2>(k);
   return k;
 }
-__device__ __forceinline__ uint64_t sort64(uint64_t k, uint32_t lane) {
-  k = sort_bitonic<1>(k, lane, lane & 2);
-  k = sort_bitonic<2>(k, lane, lane & 4);
-  k = sort_bitonic<4>(k, lane, lane & 8);
-  k = sort_bitonic<8>(k, lane, lane & 16);
-  k = sort_bitonic<16>(k, lane, lane & 32);
-  return sort_bitonic<32>(k, lane, false);
+// two sorted sequences of D lanes each into one: after an exchange with the mirror lane
+// both halves are bitonic
+template <int D>
+__device__ __forceinline__ uint64_t sort_halves(uint64_t k) {
+  k = exchange<2 * D - 1, D>(k);
+  if constexpr (D > 1) k = sort_bitonic<D / 2>(k);
+  return k;
+}
+__device__ __forceinline__ uint64_t sort64(uint64_t k) {
+  k = sort_halves<1>(k);
+  k = sort_halves<2>(k);
+  k = sort_halves<4>(k);
+  k = sort_halves<8>(k);
+  k = sort_halves<16>(k);
+  return sort_halves<32>(k);
 }
 // the 64 largest of two sorted lists, sorted
-__device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b, uint32_t lane) {
+__device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b) {
   const uint64_t o = lane_xor64<63>(b);
-  return sort_bitonic<32>(a > o ? a : o, lane, false);
+  return sort_bitonic<32>(a > o ? a : o);
 }
 // key c (the same in all lanes) into a sorted list
 __device__ __forceinline__ uint64_t insert(uint64_t list, uint64_t c, uint32_t lane) {
@@ -227,8 +241,8 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
       }
       many = __popcll(__ballot(best != 0)) > MANY;
       if (!many) break;
-      const uint64_t sorted = sort64(best, lane);
-      list = readlane64(list, 0) ? merge64(list, sorted, lane) : sorted;
+      const uint64_t sorted = sort64(best);
+      list = readlane64(list, 0) ? merge64(list, sorted) : sorted;
       raise();
       below = best;
       if (a.top <= FEW) break;
@@ -300,10 +314,10 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
   // lists of the waves into wave 0's
   auto gather = [&] {
     static_assert(WAVES == 4, "two levels");
-    if (!(w & 1)) list = merge64(list, s_list[w + 1][lane], lane);
+    if (!(w & 1)) list = merge64(list, s_list[w + 1][lane]);
     if (w == 2) s_list[2][lane] = list;
     __syncthreads();
-    if (w == 0) list = merge64(list, s_list[2][lane], lane);
+    if (w == 0) list = merge64(list, s_list[2][lane]);
   };
   if (a.top) gather();
   if (w == 0)
@@ -340,7 +354,7 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
         if (k0 == w) list = x[0];
 #pragma unroll
         for (uint32_t j = 0; j < BATCH; j++)
-          if (k0 + j * WAVES < a.splits && (j || k0 != w)) list = merge64(list, x[j], lane);
+          if (k0 + j * WAVES < a.splits && (j || k0 != w)) list = merge64(list, x[j]);
       }
       s_list[w][lane] = list;
     }
