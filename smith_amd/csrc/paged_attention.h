@@ -441,14 +441,8 @@ __device__ __forceinline__ bool request(const Args<R>& a, uint32_t b, bool tell,
       // its rows are rows of its group: what SHARED left of them is there
       const SharedOf f = a.from[b];
       const bool enough = f.keys == 0 || f.keys <= l - (int32_t)n;
-      // (of requests that no group has, or two, f may be anything: its partials are some
-      // of those there is room for)
       const bool inside = r0 >= f.row0 && r0 - f.row0 <= f.rows && n <= f.rows - (r0 - f.row0);
-      const bool there = f.splits <= 1 ||
-                         (f.splits <= PAGED_SPLIT_MAX && f.rows <= a.max_rows && f.blocks <= PAGED_MAX_PARTS &&
-                          div_up(f.rows, a.s_rows_blk) * (uint64_t)a.s_groups <= f.blocks &&
-                          f.part + (uint64_t)f.blocks * f.splits * a.nKV <= PAGED_MAX_PARTS);
-      if (f.keys < 0 || (f.keys && !(enough && inside && there))) {
+      if (f.keys < 0 || (f.keys && !(enough && inside))) {
         if (tell && f.keys > 0) paged_err(a.err, enough ? PAGED_ERR_ATT_LENGTH : PAGED_ERR_ATT_SHARED, b);
         n = 0;
         len = 0;
@@ -812,6 +806,14 @@ __device__ __forceinline__ bool last_split(const AttArgs& a, const Item<R>& I) {
   return s_last;
 }
 
+// OWN: what SHARED says of a request.  Of one that no group has, or two, that is anything;
+// its partials are some of those there is room for (here and below).
+template <Reach R>
+__device__ __forceinline__ SharedOf shared_of(const Args<R>& a, uint32_t b) {
+  SharedOf f = a.from[b];
+  if (f.splits > PAGED_SPLIT_MAX || f.splits * a.nKV > PAGED_MAX_PARTS) f.splits = 0;
+  return f;
+}
 // OWN: what the shared keys give a column, splits' partials or one alone.
 template <Reach R>
 struct Prior {
@@ -823,9 +825,9 @@ struct Prior {
     const uint32_t left = a.G - hgroup * a.s_columns, heads = left < a.s_heads_blk ? left : a.s_heads_blk;
     const uint32_t c = (r - rowblk * a.s_rows_blk) * heads + h - hgroup * a.s_columns, blk = rowblk * a.s_groups + hgroup;
     stride = (size_t)a.nKV * a.s_columns * (a.hd + 2);
-    const size_t part = f.part + (size_t)(f.blocks - 1 - blk) * f.splits * a.nKV + kvh;
-    const float* p = a.s_parts + part * a.s_columns * (a.hd + 2);
     if (f.splits > 1) {
+      const uint32_t part = f.part + (f.blocks - 1 - blk) * f.splits * a.nKV + kvh, most = PAGED_MAX_PARTS - 1 - (f.splits - 1) * a.nKV;
+      const float* p = a.s_parts + (size_t)(part < most ? part : most) * a.s_columns * (a.hd + 2);
       o = p + c * a.hd;
       ml = p + a.s_columns * a.hd + c * 2;
     } else {
@@ -1187,7 +1189,7 @@ __device__ __forceinline__ void attention_body(const Args<R>& args) {
     const uint32_t k0 = I.k0, k1 = I.k1, kvh = I.kvh;
     SharedOf of;
     if constexpr (R == OWN)
-      if (!a.whole) of = a.from[I.b];
+      if (!a.whole) of = shared_of<R>(a, I.b);
     f32x4 q_raw[TILE::QRAW];
     TILE::load_q(a.q + I.at(ln < I.ncols ? ln : 0, a.ld_q, hd), lg, hd, q_raw);
 
@@ -1638,7 +1640,7 @@ __device__ __forceinline__ void attention_rows_body(const Args<R>& args) {
     const uint32_t k0 = I.k0, k1 = I.k1;
     SharedOf of;
     if constexpr (R == OWN)
-      if (!a.whole) of = a.from[I.b];
+      if (!a.whole) of = shared_of<R>(a, I.b);
     // ---- this wave's share of a stage: KT / 4 rows of K and of V, 8 or 16, a page to 8 ----
     constexpr uint32_t SHARE = KT / 4, RPI = 1024 / ROWB, PARTS = SHARE / 8, INSTR = 8 / RPI;  // rows, instructions to 8 rows
     constexpr uint32_t AHEAD = 64 / PARTS;
