@@ -88,6 +88,7 @@ class _Engine:
         self.tok_in = DeviceArray((R,), np.int32)
         self.graph = None
         self.graph_caches = None
+        self.embeds = 0  # how often rows of tokens were put into x
         hd = cfg["headDim"]
         self.use_act = (all(b[k].has_act for b in model["blocks"] for k in ("qkv", "outProj", "gateUp", "ffnDown"))
                         and dim % 32 == 0 and ffn % 32 == 0 and hd % 8 == 0 and cfg["numHeads"] * hd == dim)
@@ -228,6 +229,7 @@ class _Engine:
 
     def embed(self, model, tokens):
         t = np.ascontiguousarray(tokens, dtype=np.int32)
+        self.embeds += 1
         device.upload(self.tok_in.ptr, t)
         a0, g0 = self._act0(model) if len(t) == 1 else (None, None)
         device.check(device.lib.smith_embed(device.ops_ctx(), model["embedding"].ptr, self.tok_in.ptr, self.x.ptr,
@@ -443,7 +445,8 @@ def scoreTokens(model, tokenIds, top=0):
         raise ValueError("score: a token outside the vocabulary of %d" % e.cfg["vocabSize"])
     _check_rope_range(e.cfg, len(tokens) - 2)
     _check_top(e, top, 0)
-    caches, parts, at = _kept_caches(model, e.cfg), [], [1]
+    # caches of its own: generate may be under way, and this be called by its onToken
+    caches, parts, at = _kept_caches(model, e.cfg, "_score_caches"), [], [1]
 
     def take(ptr, rows):
         parts.append(e.score_rows(ptr, rows, tokens[at[0]:at[0] + rows], top))
@@ -495,11 +498,11 @@ def _sample(logits, generated, cfg, rng):
     return min(idx, lg.size - 1)
 
 
-def _kept_caches(model, cfg):
-    """The caches of generate and score, empty."""
-    caches = model.get("_gen_caches")
+def _kept_caches(model, cfg, name):
+    """The caches that generate, or score, keeps under this name, empty."""
+    caches = model.get(name)
     if caches is None:
-        caches = model["_gen_caches"] = createGGUFCache(cfg)
+        caches = model[name] = createGGUFCache(cfg)
     resetCache(caches)
     return caches
 
@@ -521,7 +524,7 @@ def generateGGUF(model, promptIds, config=None, callbacks=None):
     n = len(prompt)
     last_pos = min(n + cfg["maxTokens"] - 2, mcfg["maxSeqLen"] - 1)
     _check_rope_range(mcfg, max(n - 1, last_pos))
-    caches = _kept_caches(model, mcfg)
+    caches = _kept_caches(model, mcfg, "_gen_caches")
     greedy = cfg["temperature"] == 0 and cfg["repetitionPenalty"] <= 1
     rng = np.random.default_rng(config.get("seed"))
 
@@ -530,6 +533,17 @@ def generateGGUF(model, promptIds, config=None, callbacks=None):
         device.check(device.lib.smith_set_i32(device.ops_ctx(), e.count.ptr, 0), "count")
         e.set_pos(n - 1)
         e.greedy_step(model)  # token 1; pos -> n; x = E[token]
+
+        def stops(tok, i):
+            """onToken's answer; a callback that scored a text or made a step left its
+            own row and position behind, so the step's input is put there again."""
+            mine = e.embeds
+            if on_token(tok, i):
+                return True
+            if e.embeds != mine:
+                e.embed(model, [tok])
+                e.set_pos(n + i - 1)
+            return False
         steps = 0
         for i in range(1, cfg["maxTokens"]):
             if n + i - 1 >= mcfg["maxSeqLen"]:
@@ -541,7 +555,7 @@ def generateGGUF(model, promptIds, config=None, callbacks=None):
             generated.append(tok)
             if eos is not None and tok == eos:
                 return generated
-            if on_token and on_token(tok, 1):
+            if on_token and stops(tok, 1):
                 return generated
         graph = None
         for i in range(1, steps + 1):
@@ -557,7 +571,7 @@ def generateGGUF(model, promptIds, config=None, callbacks=None):
                 generated.append(tok)
                 if eos is not None and tok == eos:
                     break
-                if on_token and on_token(tok, i + 1):
+                if on_token and stops(tok, i + 1):
                     break
         if not sync_each:
             generated.extend(int(t) for t in e.tokens.numpy()[:steps + 1])
