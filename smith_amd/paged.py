@@ -261,8 +261,10 @@ class PagedCache:
 
     def make_room(self, added):
         """Gives back what the window has passed, if the rows `added` need it."""
-        new = sum(self._pages(n + a) - self._pages(n) for n, a in zip(self.lens, added))
-        if self.window and new > self.freeCount:
+        if not self.window:
+            return
+        lens = self.lens.astype(np.int64)
+        if int((-(-(lens + added) // self.pageSize) - -(-lens // self.pageSize)).sum()) > self.freeCount:
             self.trim()
 
     def plan(self, added):
