@@ -489,7 +489,8 @@ int smith_paged_attention_shared(void* ctx, uint32_t kv_type, const float* q, ui
  * key: of tables[b] the first ceil(lens[b] / page_size) entries count.  With
  * window > 0 those that neither hold one of the first `sinks` keys nor one of
  * the last window - 1 (what a later row of smith_paged_attention_window sees) do
- * not: they may hold anything, become -1 in new_tables, and their pages are free.
+ * not, but for a partly filled last page, in which the next key has its place:
+ * they may hold anything, become -1 in new_tables, and their pages are free.
  *
  * smith_paged_fork: request b goes on from request parents[b] as it was before
  * the call (itself; another; -1: it ends and has no keys).  new_lens [n_req] and
@@ -533,7 +534,7 @@ int smith_paged_compact(void* ctx, uint32_t kv_type, const int32_t* lens, const 
  * top_ids those of its largest elements that are numbers, -1 behind them).
  * Outputs overlap no input and each other.  Enqueued, and can be captured once it
  * has run with the same sizes.  A token outside the vocabulary gets NaN, and the
- * next synchronising call returns -1 with the first such row in smith_last_error. */
+ * next synchronising call returns -1 with one such row in smith_last_error. */
 #define SMITH_F32 SMITH_KV_F32
 #define SMITH_F16 SMITH_KV_F16
 #define SMITH_BF16 SMITH_KV_BF16
