@@ -796,7 +796,7 @@ template <Reach R>
 __device__ __forceinline__ bool last_split(const AttArgs& a, const Item<R>& I) {
   __shared__ uint32_t s_last;
   uint32_t* done = a.counters + (I.part - I.split * a.nKV);
-  __builtin_amdgcn_s_waitcnt(0);
+  stores_done();
   __syncthreads();
   if (threadIdx.x == 0) {
     s_last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == I.ns - 1;

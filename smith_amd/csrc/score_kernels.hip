@@ -334,7 +334,7 @@ __device__ __forceinline__ void logprobs_body(const ScoreArgs& a) {
         put64(mine + 1, two(sum.s, 0.f));
       }
     }
-    __builtin_amdgcn_s_waitcnt(0);
+    stores_done();
     __syncthreads();
     if (tid == 0) {
       uint32_t* done = a.counters + (row - a.row0);
