@@ -99,7 +99,8 @@ def test_window_accuracy(dtype, D, kind, q_std):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("win,sinks,H,nKV,D,P", [
     (5, 3, 6, 2, 24, 8), (16, 0, 9, 3, 64, 16), (40, 17, 6, 2, 80, 16), (64, 100, 12, 4, 96, 32), (90, 1, 6, 2, 128, 8),
-    (333, 20, 20, 1, 104, 128), (5000, 4, 6, 2, 72, 16), (33, 33, 33, 1, 40, 64)])
+    (333, 20, 20, 1, 104, 128), (5000, 4, 6, 2, 72, 16), (33, 33, 33, 1, 40, 64),
+    (50, 9, 70, 1, 32, 16)])
 def test_window_rows(dtype, win, sinks, H, nKV, D, P):
     window(win + P, dtype, H, nKV, D, P, [150, 30, 64, 400, 9], [80, 1, 20, 70, 0], win, sinks, "rows")
 
@@ -244,10 +245,29 @@ def test_shared_accuracy(dtype, D, kind, apart, q_std):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("H,nKV,D,P", [(6, 2, 24, 8), (9, 3, 72, 32), (10, 2, 80, 8), (12, 4, 104, 128), (20, 1, 120, 16), (33, 1, 40, 64)])
+@pytest.mark.parametrize("H,nKV,D,P", [(6, 2, 24, 8), (9, 3, 72, 32), (10, 2, 80, 8), (12, 4, 104, 128), (20, 1, 120, 16), (33, 1, 40, 64),
+                                       (70, 1, 32, 16)])
 @pytest.mark.parametrize("apart", [True, False])
 def test_chunks_behind_shared_keys(dtype, H, nKV, D, P, apart):
     shared(H + D, dtype, H, nKV, D, P, "chunks", apart)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,nKV,D", [(70, 1, 32), (140, 2, 16), (12, 1, 64), (100, 4, 72)])
+def test_one_row_each_with_more_heads_than_a_block_has_columns(dtype, H, nKV, D):
+    """Blocks of 64 columns for the shared keys, of 16 for the own ones."""
+    shared(H, dtype, H, nKV, D, 16, "wide", True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_most_groups_by_the_kernel_of_many_columns(dtype):
+    """The items' table of 4096 groups beside the stages."""
+    rs = np.random.RandomState(4)
+    n, H, D = 4096, 8, 8
+    c = shared_case(3, dtype, H, 1, D, 8, np.ones(n, int), rs.randint(0, 20, n), rs.randint(1, 9, n), 1)
+    got = attend(*c[:6], ["_shared_rows_%s_d64" % dtype, "_own_%s_d64_s" % dtype], 64 * n // H, groupStart=c[6], shared=c[7])
+    q, row_start, lens, tables, k, v = c[:6]
+    check(got, P_.attention(q.astype(np.float64), row_start, lens, tables, R.value(k, dtype), R.value(v, dtype), everything), D)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
