@@ -8,6 +8,11 @@
 // Bound by memory: 192 requests of up to 500 own bf16 keys behind shared ones (208 MB)
 // 65 us; 64 of up to 300 f16 keys 15 us.  Of few keys in all (`whole`) it is the whole
 // call, and reads shared keys as each request's own.
+//
+// The kernels of many rows and 128 dims keep 33 registers (f32) or 13 (f16, bf16) in
+// scratch where they add four splits at once, behind the loop over the keys: 4 requests
+// of 813 rows in all 29 us (f16), 30 (bf16), 55 (f32), beside 240, 298 and 1145 for
+// the 8000 shared keys before them.
 #include "paged_attention.h"
 
 DEF_PART_ATTENTIONS(_own, OWN)

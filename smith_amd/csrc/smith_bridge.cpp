@@ -2638,7 +2638,8 @@ int smith_paged_attention_shared(void* ctx, uint32_t kv_type, const float* q, ui
   // Where the block tables have no room for more keys than are read in the time of a
   // launch each request reads its own: 4 requests behind 700 f32 keys of 4 heads of 64
   // 10.5 us, apart 14; behind 1000 f16 keys of 8 heads of 128 11.2, 16.8 (17 MB), 8 requests
-  // behind 1200 13, 17 (40 MB).
+  // behind 1200 13, 17 (40 MB).  Tables wider than their content count as they are: the
+  // 4 requests in tables of 8192 keys (64 MB) are computed apart.
   const uint64_t room = pool_bytes(kv_type, n_kv_heads, head_dim, n_req, 1) * 2 * ((uint64_t)max_pages << k.shift);
   more.whole = room <= SHARED_ROOM;
   const uint32_t own = many_columns(k) && n_req <= 4000 ? 64 : 16;  // of more the items' table has no room in LDS beside the stages
@@ -2679,7 +2680,9 @@ static int ensure_pages_map(Ctx* c, const char* fn, size_t need) {
 constexpr uint32_t PAGES_COUNT_BLOCKS = 32;
 // Entries of all block tables, used or not, that one workgroup looks through: 8 requests
 // on 700 keys (368 entries) 9.6 us, 13.1 by the card; 160 of 1000 (16320) 15.0, 23.6; 400
-// of 1200 (30800) 21, 27; 256 of 3000 (53504) 32, 35; 120 of 8000 (64080) 38, 28.
+// of 1200 (30800) 21, 27; 256 of 3000 (53504) 32, 35; 120 of 8000 (64080) 38, 28.  The
+// entries in use are known on the device alone: the 160 in tables of 8192 keys (81920)
+// go by the card, 23.4 us.
 constexpr uint64_t PAGES_SMALL_ENTRIES = 3 << 14;
 
 // What fork and compact have in common: checks, scratch and the first launch.
